@@ -1,5 +1,5 @@
-"""ctypes binding of libggemm_vark.so (declarations in include/ggemm_vark.h,
-include/ggemm_persistent.h and include/ggemm_quant.h)."""
+"""ctypes binding of libggemm_vark.so (declarations in include/ggemm_vark.h, include/ggemm_persistent.h,
+include/ggemm_quant.h and include/ggemm_moe.h)."""
 from __future__ import annotations
 
 import ctypes
@@ -77,10 +77,20 @@ QUANT_EXPORTS = (
     "ggemm_quant_mxfp8_grouped",
 )
 
+MOE_EXPORTS = (
+    "ggemm_moe_route",
+    "ggemm_moe_route_backward",
+    "ggemm_moe_plan",
+    "ggemm_moe_plan_workspace",
+    "ggemm_moe_dispatch",
+    "ggemm_moe_combine",
+    "ggemm_moe_combine_backward",
+)
+
 # GGEMM_VARK_ABI_VERSION of include/ggemm_vark.h that these bindings are written for. Some exports
 # changed signature between versions (ggemm_vark_wgrad_fp8_out and ggemm_vark_wgrad_mxfp8 took
 # M_total from version 3 on), so a library of another version is refused at load.
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 ERRORS = {
     0: "GGEMM_OK", -1: "GGEMM_E_NULL", -2: "GGEMM_E_SHAPE", -3: "GGEMM_E_STRIDE",
@@ -182,6 +192,18 @@ def load():
     lib.ggemm_quant_fp8_tensorwise_transpose_delayed_dev.restype = ctypes.c_int
     lib.ggemm_quant_mxfp8_grouped.argtypes = [vp, i32, i64, i32, i64, vp, i32, i32, vp, i64, i64, vp, i64, vp, vp]
     lib.ggemm_quant_mxfp8_grouped.restype = ctypes.c_int
+    f32 = ctypes.c_float
+    lib.ggemm_moe_route.argtypes = [vp, i32, i64, i32, i64, i32, i32, vp, i32, i32, i32, i32, f32, vp, vp, vp]
+    lib.ggemm_moe_route_backward.argtypes = [vp, vp, i32, i64, i32, i64, i32, i32, i32, f32, vp, vp, vp]
+    lib.ggemm_moe_plan.argtypes = [vp, i64, i32, vp, vp, vp, vp]
+    lib.ggemm_moe_dispatch.argtypes = [vp, i64, i64, i64, i32, vp, vp, i32, vp, i64, i64, vp]
+    lib.ggemm_moe_combine.argtypes = [vp, i32, i64, i64, vp, i64, i32, vp, vp, i64, i32, vp, i64, vp]
+    lib.ggemm_moe_combine_backward.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, i32, vp, vp, i32, i32, vp, i64, vp,
+                                               vp]
+    for name in MOE_EXPORTS:
+        getattr(lib, name).restype = ctypes.c_int
+    lib.ggemm_moe_plan_workspace.argtypes = [i64, i32]
+    lib.ggemm_moe_plan_workspace.restype = ctypes.c_int64
     _lib = lib
     return lib
 

@@ -2,7 +2,8 @@
 
 * ``lib/libggemm_vark.so`` -- the extern "C" launcher library: the variable-K wgrad kernels
   (tensorwise, K=32-MFMA, MXFP8; include/ggemm_vark.h), the persistent fwd/dgrad grouped GEMM
-  (include/ggemm_persistent.h) and the FP8 quantization producer (include/ggemm_quant.h).
+  (include/ggemm_persistent.h), the FP8 quantization producer (include/ggemm_quant.h), and expert
+  routing with the rows' way to the experts and back (include/ggemm_moe.h).
 * ``lib/variable_k_wgrad.co`` -- the drop-in code object exporting only
   ``_grouped_variable_k_gemm_kernel`` with the reference kernarg layout.
 * ``lib/persistent_e4m3.co`` / ``lib/persistent_e5m2.co`` -- drop-in code objects exporting only
@@ -22,6 +23,8 @@ CO_PATH = os.path.join(LIB_DIR, "variable_k_wgrad.co")
 PERSISTENT_CO_PATHS = {"e4m3": os.path.join(LIB_DIR, "persistent_e4m3.co"),
                        "e5m2": os.path.join(LIB_DIR, "persistent_e5m2.co")}
 ARCH = "gfx950"
+LIB_SOURCES = [os.path.join(CSRC, f) for f in ("vark_capi.hip", "persistent_capi.hip", "quant_capi.hip",
+                                               "moe_capi.hip")]
 
 # Packed-FP32 VALU ops are disabled for all device code (they are left to no hand-written use).
 DEVICE_FLAGS = ["-O3", "-std=c++17", f"--offload-arch={ARCH}",
@@ -59,8 +62,7 @@ def build_so(verbose: bool = False) -> str:
     generate_wide_asm()
     os.makedirs(LIB_DIR, exist_ok=True)
     tmp = SO_PATH + ".tmp"
-    _run([hipcc(), *DEVICE_FLAGS, "-fPIC", "-shared", os.path.join(CSRC, "vark_capi.hip"),
-          os.path.join(CSRC, "persistent_capi.hip"), os.path.join(CSRC, "quant_capi.hip"), "-o", tmp], verbose)
+    _run([hipcc(), *DEVICE_FLAGS, "-fPIC", "-shared", *LIB_SOURCES, "-o", tmp], verbose)
     os.replace(tmp, SO_PATH)
     return SO_PATH
 
@@ -112,8 +114,7 @@ def build_host_sanitized(verbose: bool = False) -> dict:
     host = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined",
             "-Xarch_host", "-fno-omit-frame-pointer", "-Xarch_host", "-fno-sanitize-recover=undefined"]
     _run([hipcc(), *DEVICE_FLAGS, "-g", "-fPIC", "-shared", "-shared-libsan", *host,
-          os.path.join(CSRC, "vark_capi.hip"), os.path.join(CSRC, "persistent_capi.hip"),
-          os.path.join(CSRC, "quant_capi.hip"), "-o", lib + ".tmp"], verbose)
+          *LIB_SOURCES, "-o", lib + ".tmp"], verbose)
     os.replace(lib + ".tmp", lib)
     clang = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin", "clang")
     oracle_c = os.path.join(os.path.dirname(PKG_DIR), "oracle", "vark_oracle.c")

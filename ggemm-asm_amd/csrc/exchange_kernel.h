@@ -1,0 +1,361 @@
+// Rows of tokens into expert order and back, for gfx950: the order itself (a stable counting sort of the
+// choices by expert), the copy of each token's row to its experts' rows, and the weighted sum back, with
+// its gradients.
+//
+// All but the sort are streams of rows, bound by HBM. They go by token: a token's row is read once and
+// written to its rows (or its rows read and summed in registers), so no inverse of the order is kept, no
+// two waves write one element and no sum depends on the order in which waves run.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace ggemm {
+namespace ex {
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kMaxGroups = 2047;
+constexpr int kPlanBlocks = 256;             // workgroups of a plan, at most
+constexpr int kPlanEntries = 512;            // choices that a workgroup takes, at least
+constexpr int kPlanAlone = 2048;             // choices that one workgroup orders by itself
+typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------------------------ the order
+
+struct PlanArgs {
+  const int* experts;
+  int64_t n;
+  int G;
+  int per;                 // choices per workgroup, a multiple of kThreads
+  int64_t* group_offs;
+  int* slots;
+  int* hist;               // [workgroups][G]: choices of each expert (plan_count_kernel)
+};
+
+__device__ __forceinline__ int group_of(const PlanArgs& a, int64_t i) {
+  const int e = a.experts[i];
+  return e >= 0 && e < a.G ? e : -1;
+}
+
+__global__ __launch_bounds__(kThreads) void plan_count_kernel(PlanArgs a) {
+  extern __shared__ int s_cnt[];
+  for (int g = threadIdx.x; g < a.G; g += kThreads) s_cnt[g] = 0;
+  __syncthreads();
+  const int64_t lo = (int64_t)blockIdx.x * a.per, end = min(lo + a.per, a.n);
+  for (int64_t i = lo + threadIdx.x; i < end; i += kThreads) {
+    const int g = group_of(a, i);
+    if (g >= 0) atomicAdd(&s_cnt[g], 1);
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < a.G; g += kThreads) a.hist[(int64_t)blockIdx.x * a.G + g] = s_cnt[g];
+}
+
+// Rows of this workgroup's choices: first row of the expert (a scan over the experts' totals), plus its
+// choices in the workgroups before, in the waves before, and in the wave before. A wave takes consecutive
+// choices, 64 at a time; lanes of one expert find each other by a ballot for each bit of its number.
+inline int plan_lds(int G) { return 4 * ((kWaves + 2) * G + kWaves); }
+
+__global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
+  extern __shared__ int s_pl[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = a.G;
+  int* s_wave = s_pl;                        // [kWaves][G]: counts, then each wave's next row
+  int* s_all = s_pl + kWaves * G;            // [G]: choices of each expert
+  int* s_before = s_all + G;                 // [G]: those in the workgroups before this one
+  int* s_scan = s_before + G;                // [kWaves]
+  for (int g = tid; g < (kWaves + 2) * G; g += kThreads) s_pl[g] = 0;
+  __syncthreads();
+  const int64_t lo = (int64_t)blockIdx.x * a.per, end = min(lo + a.per, a.n);
+  const int each = a.per / kWaves;           // a multiple of 64
+  const int64_t wlo = lo + wave * each, wend = min(wlo + each, end);
+  for (int64_t i = wlo + lane; i < wend; i += 64) {
+    const int g = group_of(a, i);
+    if (g >= 0) atomicAdd(&s_wave[wave * G + g], 1);
+  }
+  const int blocks = gridDim.x;
+  if (blocks > 1) {
+    const int parts = max(1, kThreads / G);  // threads that share an expert's column
+    for (int u = tid; u < G * parts; u += kThreads) {
+      const int g = u % G;
+      int before = 0, all = 0;
+      for (int b = u / G; b < blocks; b += parts) {
+        const int c = a.hist[(int64_t)b * G + g];
+        all += c;
+        before += b < (int)blockIdx.x ? c : 0;
+      }
+      atomicAdd(&s_all[g], all);
+      atomicAdd(&s_before[g], before);
+    }
+  }
+  __syncthreads();
+  const int span = (G + kThreads - 1) / kThreads, g0 = min(tid * span, G), g1 = min(g0 + span, G);
+  int sum = 0;
+  for (int g = g0; g < g1; ++g) {
+    if (blocks == 1)
+      for (int w = 0; w < kWaves; ++w) s_all[g] += s_wave[w * G + g];
+    sum += s_all[g];
+  }
+  int incl = sum;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(incl, d, 64);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 63) s_scan[wave] = incl;
+  __syncthreads();
+  int run = incl - sum;
+  for (int w = 0; w < wave; ++w) run += s_scan[w];
+  for (int g = g0; g < g1; ++g) {
+    if (blockIdx.x == 0) a.group_offs[g] = run;
+    int start = run + s_before[g];
+    for (int w = 0; w < kWaves; ++w) {
+      const int c = s_wave[w * G + g];
+      s_wave[w * G + g] = start;
+      start += c;
+    }
+    run += s_all[g];
+  }
+  if (blockIdx.x == 0 && tid == kThreads - 1) a.group_offs[G] = run;
+  __syncthreads();
+  const int bits = 32 - __builtin_clz(G);    // of expert numbers below G
+  int* next = s_wave + wave * G;
+  for (int64_t i = wlo; i < wend; i += 64) {
+    const bool in = i + lane < wend;
+    const int g = in ? group_of(a, i + lane) : -1;
+    uint64_t same = __ballot(g >= 0);
+    for (int b = 0; b < bits; ++b) {
+      const bool bit = (g >> b) & 1;
+      const uint64_t with = __ballot(bit);
+      same &= bit ? with : ~with;
+    }
+    int row = -1;
+    if (g >= 0) row = next[g] + __popcll(same & ((1ull << lane) - 1));
+    if (in) a.slots[i + lane] = row;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (g >= 0 && __builtin_ctzll(same) == lane) next[g] = row + __popcll(same);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+
+// ------------------------------------------------------------------------------------ the rows
+
+struct CopyArgs {
+  const uint8_t* x;
+  int64_t bytes, x_stride, T;   // bytes of a row
+  int k;
+  const int* slots;
+  const int64_t* group_offs;
+  int G;
+  uint8_t* rows;
+  int64_t rows_stride, M;
+};
+
+template <int kBytes> struct Word;
+template <> struct Word<16> { typedef v4u type; };
+template <> struct Word<4> { typedef uint32_t type; };
+template <> struct Word<2> { typedef uint16_t type; };
+template <> struct Word<1> { typedef uint8_t type; };
+
+// Rows from the end of the last group to M become zero, dealt to the grid's waves.
+template <typename W>
+__device__ __forceinline__ void clear_rows(uint8_t* rows, int64_t stride, int64_t bytes, const int64_t* group_offs,
+                                           int G, int64_t M, int64_t wave, int64_t waves, int lane) {
+  int64_t r = group_offs[G];
+  r = (r < 0 ? 0 : r) + wave;
+  for (; r < M; r += waves)
+    for (int64_t c = lane * (int64_t)sizeof(W); c < bytes; c += 64 * sizeof(W)) *(W*)(rows + r * stride + c) = W{};
+}
+
+// A wave per token: kUnroll words of the row in each lane, stored k times.
+template <int kBytes>
+__global__ __launch_bounds__(kThreads) void dispatch_kernel(CopyArgs a) {
+  using W = typename Word<kBytes>::type;
+  constexpr int kUnroll = 4;
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t waves = (int64_t)gridDim.x * kWaves;
+  for (int64_t t = wave; t < a.T; t += waves) {
+    const uint8_t* src = a.x + t * a.x_stride;
+    const int* slots = a.slots + t * a.k;
+    for (int64_t c0 = lane * kBytes; c0 < a.bytes; c0 += 64 * kBytes * kUnroll) {
+      W v[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (c0 + 64 * kBytes * u < a.bytes) v[u] = *(const W*)(src + c0 + 64 * kBytes * u);
+      for (int j = 0; j < a.k; ++j) {
+        const int s = slots[j];
+        if (s < 0 || s >= a.M) continue;
+        uint8_t* dst = a.rows + s * a.rows_stride;
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+          if (c0 + 64 * kBytes * u < a.bytes) *(W*)(dst + c0 + 64 * kBytes * u) = v[u];
+      }
+    }
+  }
+  clear_rows<W>(a.rows, a.rows_stride, a.bytes, a.group_offs, a.G, a.M, wave, waves, lane);
+}
+
+// N elements of a row in fp32.
+template <typename T, int N>
+struct Vec {
+  float f[N];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (N == 1) {
+      if constexpr (sizeof(T) == 2) f[0] = __uint_as_float((uint32_t)*(const uint16_t*)p << 16);
+      else f[0] = *(const float*)p;
+    } else {
+      const v4u w = *(const v4u*)p;
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          f[2 * i] = __uint_as_float(w[i] << 16);
+          f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+      }
+    }
+  }
+  static __device__ __forceinline__ uint32_t bf16(float v) {
+    const uint32_t u = __float_as_uint(v);
+    return (u & 0x7fffffffu) > 0x7f800000u ? 0x7fc0u : (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (N == 1) {
+      if constexpr (sizeof(T) == 2) *(uint16_t*)p = (uint16_t)bf16(f[0]);
+      else *(float*)p = f[0];
+    } else {
+      v4u w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = sizeof(T) == 2 ? bf16(f[2 * i]) | bf16(f[2 * i + 1]) << 16 : __float_as_uint(f[i]);
+      *(v4u*)p = w;
+    }
+  }
+};
+
+struct CombineArgs {
+  const void* y;
+  int64_t y_stride, M;
+  const int* slots;
+  int64_t T;
+  int k;
+  const float* weights;
+  const void* residual;
+  int64_t residual_stride;
+  int H;
+  void* out;
+  int64_t out_stride;
+};
+
+// A wave per token, N elements of the row per lane and step; the rows of four choices are loaded before
+// the first is added.
+template <typename T, int N>
+__global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t waves = (int64_t)gridDim.x * kWaves;
+  for (int64_t t = wave; t < a.T; t += waves) {
+    const int* slots = a.slots + t * a.k;
+    for (int c = lane * N; c < a.H; c += 64 * N) {
+      float acc[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] = 0.f;
+      for (int j0 = 0; j0 < a.k; j0 += 4) {
+        Vec<T, N> v[4];
+        float w[4];
+        bool use[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int s = j0 + j < a.k ? slots[j0 + j] : -1;
+          use[j] = s >= 0 && s < a.M;
+          if (use[j]) {
+            v[j].load((const T*)a.y + s * a.y_stride + c);
+            w[j] = a.weights ? a.weights[t * a.k + j0 + j] : 1.f;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (use[j]) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[i] = fmaf(w[j], v[j].f[i], acc[i]);
+          }
+      }
+      Vec<T, N> r;
+      if (a.residual) {
+        r.load((const T*)a.residual + t * a.residual_stride + c);
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.f[i] += acc[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.f[i] = acc[i];
+      }
+      r.store((T*)a.out + t * a.out_stride + c);
+    }
+  }
+}
+
+struct CombineBackArgs {
+  const void* dout;
+  int64_t dout_stride;
+  const void* y;
+  int64_t y_stride, M;
+  const int* slots;
+  int64_t T;
+  int k;
+  const float* weights;
+  const int64_t* group_offs;
+  int G, H;
+  void* dy;
+  int64_t dy_stride;
+  float* dweights;
+};
+
+// A wave per token; the token's gradient is read again for each choice (from cache).
+template <typename T, int N>
+__global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineBackArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t waves = (int64_t)gridDim.x * kWaves;
+  for (int64_t t = wave; t < a.T; t += waves) {
+    const T* dout = (const T*)a.dout + t * a.dout_stride;
+    for (int j = 0; j < a.k; ++j) {
+      const int s = a.slots[t * a.k + j];
+      const bool use = s >= 0 && s < a.M;
+      float dot = 0.f;
+      if (use) {
+        const float w = a.weights ? a.weights[t * a.k + j] : 1.f;
+        for (int c = lane * N; c < a.H; c += 64 * N) {
+          Vec<T, N> d, y;
+          d.load(dout + c);
+          if (a.dweights) {
+            y.load((const T*)a.y + s * a.y_stride + c);
+#pragma unroll
+            for (int i = 0; i < N; ++i) dot = fmaf(d.f[i], y.f[i], dot);
+          }
+          if (a.dy) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) d.f[i] *= w;
+            d.store((T*)a.dy + s * a.dy_stride + c);
+          }
+        }
+      }
+      if (a.dweights) {
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d, 64);
+        if (lane == 0) a.dweights[t * a.k + j] = dot;
+      }
+    }
+  }
+  if (a.dy) {
+    if constexpr (N > 1)
+      clear_rows<v4u>((uint8_t*)a.dy, a.dy_stride * sizeof(T), (int64_t)a.H * sizeof(T), a.group_offs, a.G, a.M, wave,
+                      waves, lane);
+    else
+      clear_rows<T>((uint8_t*)a.dy, a.dy_stride * sizeof(T), (int64_t)a.H * sizeof(T), a.group_offs, a.G, a.M, wave,
+                    waves, lane);
+  }
+}
+
+}  // namespace ex
+}  // namespace ggemm

@@ -17,7 +17,7 @@
 extern "C" {
 #endif
 
-#define GGEMM_VARK_ABI_VERSION 10
+#define GGEMM_VARK_ABI_VERSION 11
 
 enum {
   GGEMM_OK = 0,
