@@ -8,6 +8,7 @@ include/ggemm_persistent.h. Modules:
 
 * ``vark``       -- variable-K wgrad torch ops over the C ABI (mirror of the reference's oracle op)
 * ``persistent`` -- fwd/dgrad grouped GEMM torch op over the C ABI (same)
+* ``product``    -- the fwd grouped GEMM with bias, activation and residual, and their gradient, over the C ABI
 * ``quant``      -- FP8 quantization producer (per-tensor and MX with group padding) over the C ABI
 * ``moe``        -- routing tokens to experts, their rows into expert order and back, over the C ABI
 * ``autograd``   -- the FP8 grouped linear layer (forward, dgrad, wgrad) as a torch autograd op
@@ -20,6 +21,7 @@ from ._lib import GGemmError, bf16_kernel, launch_geometry, library_path, load a
 from .autograd import FP8DelayedScaling, FP8WeightCache, GroupedLinearFP8, grouped_linear_fp8  # noqa: F401
 from .moe import DispatchPlan, combine_tokens, dispatch_tokens, plan_dispatch, route_experts  # noqa: F401
 from .persistent import grouped_gemm_fp8_tensorwise  # noqa: F401
+from .product import bias_act_backward, grouped_gemm_fp8_bias_act  # noqa: F401
 from .quant import (amax, padded_rows, quantize_fp8_tensorwise, quantize_fp8_tensorwise_delayed,  # noqa: F401
                     quantize_fp8_tensorwise_transpose, quantize_fp8_tensorwise_transpose_delayed,
                     quantize_mxfp8_grouped)

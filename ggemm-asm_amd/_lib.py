@@ -1,5 +1,5 @@
 """ctypes binding of libggemm_vark.so (declarations in include/ggemm_vark.h, include/ggemm_persistent.h,
-include/ggemm_quant.h and include/ggemm_moe.h)."""
+include/ggemm_quant.h, include/ggemm_moe.h and include/ggemm_product.h)."""
 from __future__ import annotations
 
 import ctypes
@@ -85,6 +85,12 @@ MOE_EXPORTS = (
     "ggemm_moe_dispatch",
     "ggemm_moe_combine",
     "ggemm_moe_combine_backward",
+)
+
+PRODUCT_EXPORTS = (
+    "ggemm_product_fp8_bias_act",
+    "ggemm_product_act_backward",
+    "ggemm_product_act_workspace",
 )
 
 # GGEMM_VARK_ABI_VERSION of include/ggemm_vark.h that these bindings are written for. Some exports
@@ -200,10 +206,14 @@ def load():
     lib.ggemm_moe_combine.argtypes = [vp, i32, i64, i64, vp, i64, i32, vp, vp, i64, i32, vp, i64, vp]
     lib.ggemm_moe_combine_backward.argtypes = [vp, i32, i64, vp, i64, i64, vp, i64, i32, vp, vp, i32, i32, vp, i64, vp,
                                                vp]
-    for name in MOE_EXPORTS:
+    lib.ggemm_product_fp8_bias_act.argtypes = [vp] * 7 + [i32, vp, vp] + [i32] * 10 + [f32, f32, f32, i64, i32, vp]
+    lib.ggemm_product_act_backward.argtypes = [vp, vp, vp] + [i32] * 5 + [f32, f32, f32, i64, vp, i32, vp, vp, vp]
+    for name in MOE_EXPORTS + PRODUCT_EXPORTS:
         getattr(lib, name).restype = ctypes.c_int
     lib.ggemm_moe_plan_workspace.argtypes = [i64, i32]
     lib.ggemm_moe_plan_workspace.restype = ctypes.c_int64
+    lib.ggemm_product_act_workspace.argtypes = [i64, i32, i32]
+    lib.ggemm_product_act_workspace.restype = ctypes.c_int64
     _lib = lib
     return lib
 

@@ -1,0 +1,140 @@
+// Epilogue of the grouped FP8 products with bias, activation and residual:
+//
+//   z = alpha acc + bias[g];  out = act(z) + residual   (fp32, rounded once to bf16)
+//
+// for the kernels whose waves hold C as blocks of 16 x 16 from v_mfma_f32_16x16x128 (mid_gemm.h,
+// persistent_kernel.h): lane 16 q + s holds row s, columns 4 q .. 4 q + 3 of a block, so the gate and the
+// value of a swiglu pair (columns 2 i, 2 i + 1) are neighbours in one lane, and its output is half as
+// wide as the product.
+#pragma once
+
+#include "vark_kernel.h"
+
+namespace ggemm {
+namespace epi {
+
+constexpr int kNone = 0, kSilu = 1, kGelu = 2, kSwiglu = 3;
+
+struct Args {
+  uint16_t* pre;           // z in bf16, or null
+  int stride_pre;
+  const void* bias;        // [G, N] fp32 or bf16, or null
+  int bias_f32;
+  const uint16_t* residual;
+  int stride_res;
+  float slope, limit, shift;
+};
+
+// 1 / (1 + e^-x). The hardware's exp2 and reciprocal, each within an ulp; the rounding of x log2(e) adds
+// |x| 2^-24: against the 2^-8 of the bf16 results, and 2e-7 in the fp32 sums of the bias' gradient.
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896f));
+}
+__device__ __forceinline__ float gelu_cdf(float x) { return 0.5f * (1.f + erff(x * 0.707106781186548f)); }
+
+// NaN stays NaN in both (a comparison with it is false).
+__device__ __forceinline__ float at_most(float x, float m) { return x > m ? m : x; }
+__device__ __forceinline__ float within(float x, float m) { return x > m ? m : x < -m ? -m : x; }
+
+__device__ __forceinline__ float swiglu(float g, float u, const Args& e) {
+  g = at_most(g, e.limit);
+  return g * sigmoid(e.slope * g) * (within(u, e.limit) + e.shift);
+}
+
+__device__ __forceinline__ float from_bf16(uint32_t low) { return __uint_as_float(low << 16); }
+
+__device__ __forceinline__ v4f load_bias(const Args& e, int64_t i) {
+  if (e.bias == nullptr) return v4f{0.f, 0.f, 0.f, 0.f};
+  if (e.bias_f32) return *(const v4f*)((const float*)e.bias + i);
+  const v2i w = *(const v2i*)((const uint16_t*)e.bias + i);
+  return v4f{from_bf16(w[0]), __uint_as_float(w[0] & 0xffff0000u), from_bf16(w[1]), __uint_as_float(w[1] & 0xffff0000u)};
+}
+
+__device__ __forceinline__ int pack(float a, float b) {
+  return (int)(f32_to_bf16_rne(a) | (f32_to_bf16_rne(b) << 16));
+}
+
+// LDS that a wave stages 32 rows of NB blocks in, rows 16 bytes apart so that 16 of them start on different banks.
+template <int NB>
+constexpr int kRegion = 32 * (32 * NB + 16);
+
+// 32 staged rows of kChunks 16-byte chunks to dst (row 0), the first `rows` of them; chunk c is stored where c < chunks.
+template <int kChunks>
+__device__ __forceinline__ void store_rows(const GG_LDS uint8_t* reg, uint16_t* dst, int64_t stride, int rows,
+                                           int chunks, int lane) {
+  constexpr int kPitch = 16 * kChunks + 16;
+#pragma unroll
+  for (int k = 0; k < (32 * kChunks + 63) / 64; ++k) {
+    const int f = 64 * k + lane, r = f / kChunks, c = f - r * kChunks;
+    if (r < rows && r < 32 && c < chunks) store_c16(dst + r * stride + 8 * c, *(const GG_LDS v4i*)(reg + r * kPitch + 16 * c));
+  }
+}
+
+// A wave's block of 16 MB x 16 NB: rows row0 .. of the launch (the first `rows` of them exist), columns n0 .. of
+// group g's product. reg: this wave's kRegion<NB> bytes of LDS.
+template <int kAct, int MB, int NB>
+__device__ __forceinline__ void store(const v4f (&acc)[MB][NB], float alpha, const Args& e, uint16_t* out,
+                                      int stride_out, int g, int N, int64_t row0, int rows, int n0,
+                                      GG_LDS uint8_t* reg, int lane) {
+  static_assert(MB % 2 == 0, "two blocks of rows per pass");
+  constexpr bool kGated = kAct == kSwiglu;
+  const int q = lane >> 4, s = lane & 15;
+  const int blocks = min(NB, (N - n0 + 15) / 16);      // N is a multiple of 16; none past it
+  v4f bias[NB];
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+    bias[j] = j < blocks ? load_bias(e, (int64_t)g * N + n0 + 16 * j + 4 * q) : v4f{0.f, 0.f, 0.f, 0.f};
+  constexpr int kOutChunks = kGated ? NB : 2 * NB;
+  const int o0 = kGated ? n0 / 2 : n0;
+#pragma unroll
+  for (int p = 0; p < MB / 2; ++p) {
+    const int64_t prow = row0 + 32 * p;
+    const int prows = rows - 32 * p;
+    if (prows <= 0) return;                            // uniform in the wave
+    if (e.pre != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          const v4f z = acc[2 * p + i][j] * alpha + bias[j];
+          *(GG_LDS v2i*)(reg + (16 * i + s) * (32 * NB + 16) + 32 * j + 8 * q) = v2i{pack(z[0], z[1]), pack(z[2], z[3])};
+        }
+      store_rows<2 * NB>(reg, e.pre + prow * e.stride_pre + n0, e.stride_pre, prows, 2 * blocks, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = 16 * i + s;
+      const uint16_t* res = e.residual != nullptr && r < prows ? e.residual + (prow + r) * e.stride_res + o0 : nullptr;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const v4f z = acc[2 * p + i][j] * alpha + bias[j];
+        GG_LDS uint8_t* at = reg + r * (16 * kOutChunks + 16);
+        if constexpr (kGated) {
+          float x = swiglu(z[0], z[1], e), y = swiglu(z[2], z[3], e);
+          if (res != nullptr && j < blocks) {
+            const uint32_t w = *(const uint32_t*)(res + 8 * j + 2 * q);
+            x += from_bf16(w);
+            y += __uint_as_float(w & 0xffff0000u);
+          }
+          *(GG_LDS int*)(at + 16 * j + 4 * q) = pack(x, y);
+        } else {
+          v4f x = z;
+          if constexpr (kAct == kSilu || kAct == kGelu) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) x[c] = z[c] * (kAct == kSilu ? sigmoid(z[c]) : gelu_cdf(z[c]));
+          }
+          if (res != nullptr && j < blocks) {
+            const v2i w = *(const v2i*)(res + 16 * j + 4 * q);
+            x += v4f{from_bf16(w[0]), __uint_as_float(w[0] & 0xffff0000u), from_bf16(w[1]),
+                     __uint_as_float(w[1] & 0xffff0000u)};
+          }
+          *(GG_LDS v2i*)(at + 32 * j + 8 * q) = v2i{pack(x[0], x[1]), pack(x[2], x[3])};
+        }
+      }
+    }
+    store_rows<kOutChunks>(reg, out + prow * stride_out + o0, stride_out, prows, kGated ? blocks : 2 * blocks, lane);
+  }
+}
+
+}  // namespace epi
+}  // namespace ggemm

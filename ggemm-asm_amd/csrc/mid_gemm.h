@@ -14,6 +14,7 @@
 // bits. Waves: 1 x 4 of 64 x 32 (BM = 64) or 2 x 2 of 64 x 64 (BM = 128).
 #pragma once
 
+#include "fused_epilogue.h"
 #include "mid_common.h"
 #include "persistent_kernel.h"
 
@@ -35,8 +36,9 @@ struct GemmCfg {
   static constexpr int BandN = 8;                            // column tiles of a band, rows tiles walked inside
 };
 
-template <bool kAE5M2, int kBM>
-__device__ __forceinline__ void gemm_body(const nt::Args& a, GG_LDS uint8_t* lds) {
+// kEpi: 0 for C as it is, else 1 + the activation of an epilogue with bias and residual (e, fused_epilogue.h).
+template <bool kAE5M2, int kBM, int kEpi = 0>
+__device__ __forceinline__ void gemm_body(const nt::Args& a, GG_LDS uint8_t* lds, const epi::Args& e = {}) {
   using C = GemmCfg<kBM>;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -146,6 +148,13 @@ __device__ __forceinline__ void gemm_body(const nt::Args& a, GG_LDS uint8_t* lds
   // last stage's barrier, so none reads it any more
   const float alpha = *a.a_scale * *a.b_scale;
   constexpr int kCols = 16 * C::NB;
+  if constexpr (kEpi != 0) {
+    static_assert(4 * epi::kRegion<C::NB> <= C::Slot, "epilogue staging fits a slot");
+    epi::store<kEpi - 1, C::MB, C::NB>(acc, alpha, e, a.c, a.stride_cm, 4 * gl + gx, a.N,
+                                        (int64_t)row_base + m0 + 64 * wm, rows - 64 * wm, n0 + kCols * wn,
+                                        lds + cur * C::Slot + wave * epi::kRegion<C::NB>, lane);
+    return;
+  }
   store_bf16<C::NB>(acc, alpha, lds + cur * C::Slot + wave * (64 * 2 * kCols),
                     a.c + (int64_t)(row_base + m0 + 64 * wm) * a.stride_cm + n0 + kCols * wn, a.stride_cm,
                     rows - 64 * wm, cols - kCols * wn, lane);

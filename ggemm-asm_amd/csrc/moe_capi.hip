@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/ggemm_moe.h"
 #include "capi_common.h"

@@ -36,6 +36,7 @@
 //    of equal tile counts (every tile costs ceil(K/128) stages) and alternate rounds of 32 tiles.
 #pragma once
 
+#include "fused_epilogue.h"
 #include "vark_kernel.h"
 
 namespace ggemm {
@@ -264,8 +265,9 @@ __device__ __forceinline__ Tile tile_of(const GG_LDS int* s_pre, const GG_LDS in
   return T;
 }
 
-template <bool kAE5M2, int kTN>
-__device__ __forceinline__ void persistent_body(const Args& a, GG_LDS uint8_t* lds) {
+// kEpi: 0 for C as it is, else 1 + the activation of an epilogue with bias and residual (e, fused_epilogue.h).
+template <bool kAE5M2, int kTN, int kEpi = 0>
+__device__ __forceinline__ void persistent_body(const Args& a, GG_LDS uint8_t* lds, const epi::Args& e = {}) {
   using C = Cfg<kTN>;
   using C2 = Cfg2<kTN>;
   constexpr int NB = C::NB;
@@ -422,6 +424,16 @@ __device__ __forceinline__ void persistent_body(const Args& a, GG_LDS uint8_t* l
     asm volatile("" : "+v"(el));
     uint16_t* cbase = a.c + (int64_t)T.row_base * a.stride_cm;
     const int m_end = T.m0 + T.rows;
+    if constexpr (kEpi != 0) {
+      static_assert(kWaves * epi::kRegion<NB> <= C2::kSlot, "epilogue staging fits a slot");
+      const int wrow = wm * kWaveM, wcol = T.n0 + wn * C::WaveN;
+      if (wcol < a.N)
+        epi::store<kEpi - 1, kMB, NB>(acc, alpha, e, a.c, a.stride_cm, T.g, a.N, (int64_t)T.row_base + T.m0 + wrow,
+                                       T.rows - wrow, wcol, lds + (cur ^ 1) * C2::kSlot + wave * epi::kRegion<NB>, el);
+      t = t_next;
+      T = N;
+      continue;
+    }
     if constexpr (kPairEpi<kTN>) {
       epilogue_pairs<NB>(acc, alpha, lds + (cur ^ 1) * C2::kSlot, cbase, a.stride_cm, T.m0, m_end, T.n0, a.N, wm, wn,
                          s16, q, el);
@@ -478,8 +490,8 @@ __device__ void poison_out(const Args& a) {
     for (int n = threadIdx.x; n < a.N; n += (int)pkt->workgroup_size_x) a.c[r * a.stride_cm + (int64_t)n * a.stride_cn] = 0x7fc0u;
 }
 
-template <bool kAE5M2>
-__device__ __forceinline__ void persistent_entry(const Args& a, GG_LDS uint8_t* dyn) {
+template <bool kAE5M2, int kEpi = 0>
+__device__ __forceinline__ void persistent_entry(const Args& a, GG_LDS uint8_t* dyn, const epi::Args& e = {}) {
   __shared__ __attribute__((aligned(1024))) uint8_t static_lds[kStaticLdsBytes];
   if (a.G <= 0 || a.G > kMaxGroups || a.K <= 0 || a.N <= 0) return;
   GG_LDS uint8_t* st = (GG_LDS uint8_t*)static_lds;
@@ -493,9 +505,9 @@ __device__ __forceinline__ void persistent_entry(const Args& a, GG_LDS uint8_t* 
     return;
   }
   if (wide_tiles(a.N, false))
-    persistent_body<kAE5M2, 384>(a, st);
+    persistent_body<kAE5M2, 384, kEpi>(a, st, e);
   else
-    persistent_body<kAE5M2, 320>(a, st);
+    persistent_body<kAE5M2, 320, kEpi>(a, st, e);
 }
 
 }  // namespace nt

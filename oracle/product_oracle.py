@@ -1,0 +1,76 @@
+"""64-bit reference of the grouped product with bias, activation and residual, and of its gradient (torch float64 on
+the CPU, test infrastructure)."""
+from __future__ import annotations
+
+import math
+
+import torch
+
+
+def act(z, activation, slope=1.0, limit=math.inf, shift=0.0):
+    if activation == "swiglu":
+        g, u = z[:, 0::2], z[:, 1::2]
+        g = torch.where(g > limit, torch.full_like(g, limit), g)
+        u = torch.where(u > limit, torch.full_like(u, limit), torch.where(u < -limit, torch.full_like(u, -limit), u))
+        return g * torch.sigmoid(slope * g) * (u + shift)
+    if activation == "silu":
+        return z * torch.sigmoid(z)
+    if activation == "gelu":
+        return 0.5 * z * (1 + torch.erf(z * math.sqrt(0.5)))
+    return z
+
+
+def act_grad(z, activation, slope=1.0, limit=math.inf, shift=0.0):
+    """d act / dz by the formula: for swiglu [M, N], the factor of each column's own output gradient."""
+    if activation == "swiglu":
+        z0, z1 = z[:, 0::2], z[:, 1::2]
+        g, u = z0.clamp(max=limit), z1.clamp(-limit, limit)
+        s = torch.sigmoid(slope * g)
+        dg = torch.where(z0 > limit, 0.0, (u + shift) * s * (1 + slope * g * (1 - s)))
+        du = torch.where(z1.abs() > limit, 0.0, g * s)
+        return torch.stack((dg, du), 2).reshape(z.shape)
+    if activation == "silu":
+        s = torch.sigmoid(z)
+        return s * (1 + z * (1 - s))
+    if activation == "gelu":
+        return 0.5 * (1 + torch.erf(z * math.sqrt(0.5))) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    return torch.ones_like(z)
+
+
+def product(a, b, scale, offs, bias, activation, residual, **options):
+    """(z, out, bound) float64: the value before the activation, the result (rows of no group NaN), and how far the
+    kernels' z may be off: the matrix cores drop bits 2^-8 below the largest product of each 64 (the bound of
+    ``vark_oracle.fp8_mfma_error_bound``, with the product of the two largest factors for the largest product), block
+    sums and the bias add in fp32."""
+    a, b = a.double(), b.double()
+    M, (N, K) = a.shape[0], b.shape[1:]
+
+    def tops(t):                                      # the largest magnitude of each 64 along K
+        pad = torch.nn.functional.pad(t.abs(), (0, -K % 64))
+        return pad.view(t.shape[0], pad.shape[1] // 64, 64).amax(2)
+
+    z = torch.full((M, N), math.nan, dtype=torch.float64)
+    size = torch.zeros((M, N), dtype=torch.float64)
+    for g, (lo, hi) in enumerate(zip(offs, offs[1:])):
+        z[lo:hi] = scale * (a[lo:hi] @ b[g].t())
+        size[lo:hi] = scale * (2.0 ** -8 * tops(a[lo:hi]) @ tops(b[g]).t()
+                               + (K / 16 + 4) * 2.0 ** -24 * a[lo:hi].abs() @ b[g].abs().t())
+        if bias is not None:
+            z[lo:hi] += bias[g].double()
+            size[lo:hi] += 2.0 ** -23 * (bias[g].double().abs() + z[lo:hi].abs())
+    out = act(z, activation, **options)
+    return z, out if residual is None else out + residual.double(), size
+
+
+def backward(dout, pre, offs, activation, **options):
+    """(dpre, dbias, size): rows of no group zero; size the sum of the magnitudes of dbias' terms."""
+    d = dout.double()
+    d = d.repeat_interleave(2, 1) if activation == "swiglu" else d
+    full = d if activation is None else d * act_grad(pre.double(), activation, **options)
+    dpre = torch.zeros_like(full)
+    G = len(offs) - 1
+    dbias, size = (torch.zeros((G, full.shape[1]), dtype=torch.float64) for _ in range(2))
+    for g, (lo, hi) in enumerate(zip(offs, offs[1:])):
+        dpre[lo:hi] = full[lo:hi]
+        dbias[g], size[g] = full[lo:hi].sum(0), full[lo:hi].abs().sum(0)
+    return dpre, dbias, size

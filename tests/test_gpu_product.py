@@ -1,0 +1,188 @@
+"""The grouped FP8 product with bias, activation and residual, and the gradient of bias and activation, on the GPU
+against the 64-bit oracle.
+
+Tolerances. z has the error of the matrix cores' fp8 sums (the oracle's bound, pinned by the products' own tests); an activation carries that error on by its slope, at most 1.2 times
+the gate's reach, and adds a few ulps of exp2, reciprocal or erf (16 units of 2^-23 of the value and of z). The result
+is rounded once to bf16: 2^-8. Gradients: the same ulps against the size of the factor, and in dbias the rounding
+of a sum of `rows` terms, (rows / 64 + 16) 2^-24 of their magnitudes beside each term's 32 2^-23.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import product_oracle as orx
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -23
+BF = 2.0 ** -8
+GATE = dict(slope=1.702, limit=7.0, shift=1.0)
+ACTS = [(None, {}), ("silu", {}), ("gelu", {}), ("swiglu", {}), ("swiglu", GATE)]
+
+
+def _inputs(M, N, K, lens, seed, std=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    a = (torch.randn((M, K), generator=gen) * 4).to(torch.float8_e4m3fn)
+    b = (torch.randn((len(lens), N, K), generator=gen) * 4).to(torch.float8_e4m3fn)
+    sa, sb = 0.25, 0.25 * std / math.sqrt(K)
+    offs = [0]
+    for n in lens:
+        offs.append(offs[-1] + n)
+    return a, b, sa, sb, offs, gen
+
+
+def _strided(t, pad):
+    """t on the GPU, its rows `pad` elements apart more than they are long."""
+    wide = torch.zeros(tuple(t.shape[:-1]) + (t.shape[-1] + pad,), dtype=torch.uint8 if t.element_size() == 1 else t.dtype,
+                       device="cuda")
+    src = t.view(torch.uint8) if t.element_size() == 1 else t
+    wide[..., :t.shape[-1]] = src.cuda()
+    return (wide.view(t.dtype) if t.element_size() == 1 else wide)[..., :t.shape[-1]]
+
+
+def _check(out, pre, z, ref, size, activation, options, extra):
+    live = ~torch.isnan(z).any(1)
+    dz = size[live]
+    if pre is not None:
+        assert ((pre[live] - z[live]).abs() <= dz + 1.01 * BF * z[live].abs() + 1e-30).all()
+    if activation == "swiglu":
+        zz = z[live].abs() + 1
+        reach = torch.maximum(zz[:, 0::2], zz[:, 1::2]) + options.get("shift", 0.0)
+        err = 1.2 * options.get("slope", 1.0) * (dz[:, 0::2] + dz[:, 1::2]) * reach + 16 * U * reach * reach
+    else:
+        err = 1.2 * dz + 16 * U * (z[live].abs() + 1) if activation else dz
+    got, want = out[live], ref[live]
+    bad = (got - want).abs() > err + 1.01 * BF * want.abs() + 4 * U * extra[live] + 1e-30
+    assert not bad.any(), ((got - want).abs()[bad].max(), bad.nonzero()[:3])
+
+
+# one row; groups empty, of one row and ragged; a tile and its edges; features below a tile, off its grid and over several
+SHAPES = [(1, 16, 16, [0, 1, 0]), (4, 320, 2880, [1, 0, 1, 1, 0, 1]), (70, 48, 144, [0, 33, 1, 0, 36]),
+          (300, 400, 272, [65, 0, 128, 100]), (257, 1040, 128, [257]), (64, 5760, 1424, [3] * 20),
+          (5003, 336, 240, [1200, 0, 1, 3700, 99]), (4100, 2048, 160, [700] * 5 + [597])]
+
+
+@pytest.mark.parametrize("M,N,K,lens", SHAPES)
+@pytest.mark.parametrize("activation,options", ACTS)
+@pytest.mark.parametrize("bias,residual,keep", [(None, False, True), (torch.float32, True, False), (torch.bfloat16, False, False),
+                                                (torch.bfloat16, True, True)])
+def test_product(pkg, M, N, K, lens, activation, options, bias, residual, keep):
+    a, b, sa, sb, offs, gen = _inputs(M, N, K, lens, M + N)
+    width = N // 2 if activation == "swiglu" else N
+    bv = None if bias is None else torch.randn((len(lens), N), generator=gen).to(bias)
+    res = torch.randn((M, width), generator=gen).to(torch.bfloat16) if residual else None
+    pad = 16 if keep else 0
+    dev = dict(device="cuda")
+    args = (_strided(a, pad), _strided(b, pad), torch.tensor(sa, **dev), torch.tensor(sb, **dev), torch.tensor(offs, **dev),
+            None if bv is None else bv.cuda(), activation, None if res is None else _strided(res, pad))
+    got = pkg.grouped_gemm_fp8_bias_act(*args, keep_preact=keep, zero_tail=True, **options)
+    out, pre = got if keep else (got, None)
+    assert out.dtype == torch.bfloat16 and tuple(out.shape) == (M, width)
+    z, ref, size = orx.product(a, b, sa * sb, offs, bv, activation, res, **options)
+    _check(out.cpu().double(), None if pre is None else pre.cpu().double(), z, ref, size, activation, options,
+           torch.zeros_like(ref) if res is None else res.double().abs())
+    end = offs[-1]
+    assert not out[end:].any() and (pre is None or not pre[end:].any())
+    again = pkg.grouped_gemm_fp8_bias_act(*args, keep_preact=keep, zero_tail=True, **options)
+    assert torch.equal(out, again[0] if keep else again)
+
+
+def test_more_groups_than_the_small_tiles_take(pkg):
+    """300 groups: the launch goes to the persistent kernel whatever its rows."""
+    lens = [1, 0, 2] * 100
+    a, b, sa, sb, offs, gen = _inputs(sum(lens), 352, 96, lens, 9)
+    bias = torch.randn((300, 352), generator=gen)
+    for activation, options in ACTS:
+        out, pre = pkg.grouped_gemm_fp8_bias_act(a.cuda(), b.cuda(), torch.tensor(sa).cuda(), torch.tensor(sb).cuda(),
+                                                 torch.tensor(offs).cuda(), bias.cuda(), activation, keep_preact=True, **options)
+        z, ref, size = orx.product(a, b, sa * sb, offs, bias, activation, None, **options)
+        _check(out.cpu().double(), pre.cpu().double(), z, ref, size, activation, options, torch.zeros_like(ref))
+
+
+@pytest.mark.parametrize("activation,options", ACTS)
+def test_clamped_and_extreme_values(pkg, activation, options):
+    """z far outside the activations' bends and the clamp: nothing overflows on the way."""
+    a, b, sa, sb, offs, _ = _inputs(40, 64, 64, [40], 5, std=200.0)
+    out, pre = pkg.grouped_gemm_fp8_bias_act(a.cuda(), b.cuda(), torch.tensor(sa).cuda(), torch.tensor(sb).cuda(),
+                                             torch.tensor(offs).cuda(), None, activation, keep_preact=True, **options)
+    z, ref, size = orx.product(a, b, sa * sb, offs, None, activation, None, **options)
+    assert torch.isfinite(out).all() and z.abs().max() > 300
+    _check(out.cpu().double(), pre.cpu().double(), z, ref, size, activation, options, torch.zeros_like(ref))
+
+
+def test_nan_and_infinite_bias(pkg):
+    """NaN stays NaN through the clamp, and only in its own columns."""
+    a, b, sa, sb, offs, _ = _inputs(20, 64, 32, [20], 6)
+    bias = torch.zeros((1, 64))
+    bias[0, 10], bias[0, 21], bias[0, 40] = math.nan, math.nan, math.inf
+    for activation, options in ACTS:
+        out = pkg.grouped_gemm_fp8_bias_act(a.cuda(), b.cuda(), torch.tensor(sa).cuda(), torch.tensor(sb).cuda(),
+                                            torch.tensor(offs).cuda(), bias.cuda(), activation, **options).cpu()
+        _, ref, _ = orx.product(a, b, sa * sb, offs, bias, activation, None, **options)
+        assert torch.equal(torch.isnan(out), torch.isnan(ref)), activation
+        fin = torch.isfinite(ref)
+        assert torch.equal(torch.isfinite(out), fin)
+
+
+def test_empty_and_offsets_past_the_rows(pkg):
+    a, b, sa, sb, offs, _ = _inputs(100, 64, 32, [30, 70], 8)
+    one = torch.tensor(1.0).cuda()
+    out = pkg.grouped_gemm_fp8_bias_act(a[:0].cuda(), b.cuda(), one, one, torch.tensor([0, 0, 0]).cuda(), None, "swiglu")
+    assert tuple(out.shape) == (0, 32)
+    cut = pkg.grouped_gemm_fp8_bias_act(a[:50].cuda(), b.cuda(), one, one, torch.tensor([0, 30, 10 ** 12]).cuda())
+    full = pkg.grouped_gemm_fp8_bias_act(a.cuda(), b.cuda(), one, one, torch.tensor(offs).cuda())
+    assert torch.equal(cut, full[:50])
+    with pytest.raises(pkg.GGemmError):
+        pkg.grouped_gemm_fp8_bias_act(a.cuda(), b.cuda(), one, one, torch.tensor([0, 50, 40]).cuda(), validate=True)
+
+
+BACK = [(1, 16, [1]), (7, 48, [0, 3, 0, 2]), (100, 2064, [33, 1, 60]), (1000, 320, [0, 999]), (2500, 5760, [400, 0, 1, 2000, 50]),
+        (40000, 64, [13000, 27000]), (600, 32, [2] * 300)]
+
+
+@pytest.mark.parametrize("M,N,lens", BACK)
+@pytest.mark.parametrize("activation,options", ACTS)
+def test_gradient(pkg, M, N, lens, activation, options):
+    gen = torch.Generator().manual_seed(M + N)
+    width = N // 2 if activation == "swiglu" else N
+    pre = (torch.randn((M, N), generator=gen) * 4).to(torch.bfloat16)
+    dout = torch.randn((M, width), generator=gen).to(torch.bfloat16)
+    offs = [0]
+    for n in lens:
+        offs.append(offs[-1] + n)
+    dev_offs = torch.tensor(offs).cuda()
+    dpre, dbias = pkg.bias_act_backward(_strided(dout, 8), _strided(pre, 8), dev_offs, activation, **options)
+    ref, rbias, size = orx.backward(dout, pre, offs, activation, **options)
+    # each factor's error against its largest term
+    term = dout.double().abs()
+    term = term.repeat_interleave(2, 1) if activation == "swiglu" else term
+    other = pre.double().abs()
+    if activation == "swiglu":
+        other = torch.maximum(other[:, 0::2], other[:, 1::2]).repeat_interleave(2, 1)
+    term = term * (other + 2) ** 2 if activation == "swiglu" else term * (other + 2)
+    if activation is None:
+        assert torch.equal(dpre.cpu(), dout)
+    else:
+        end = offs[-1]
+        assert ((dpre.cpu().double() - ref).abs() <= 1.01 * BF * ref.abs() + 32 * U * term + 1e-30).all()
+        assert not dpre[end:].any()
+    for g, (lo, hi) in enumerate(zip(offs, offs[1:])):
+        tol = 32 * U * term[lo:hi].sum(0) + ((hi - lo) / 64 + 16) * 2.0 ** -24 * size[g]
+        assert ((dbias[g].cpu().double() - rbias[g]).abs() <= tol).all()
+    same, none = pkg.bias_act_backward(dout.cuda(), pre.cuda(), dev_offs, activation, bias_grad=False, **options)
+    assert none is None and torch.equal(same, dpre)
+    assert torch.equal(pkg.bias_act_backward(dout.cuda(), pre.cuda(), dev_offs, activation, **options)[1], dbias)
+
+
+def test_gradient_of_no_rows_and_odd_offsets(pkg):
+    one = torch.ones((6, 16), dtype=torch.bfloat16, device="cuda")
+    _, dbias = pkg.bias_act_backward(one[:0], one[:0], torch.tensor([0, 0, 0]).cuda(), "silu")
+    assert tuple(dbias.shape) == (2, 16) and not dbias.any()
+    # offsets that begin late, fall and leave the rows: rows belong to the first group that holds them
+    offs = torch.tensor([1, 4, 2, 99]).cuda()
+    dpre, dbias = pkg.bias_act_backward(one, None, offs)
+    assert dbias[:, 0].tolist() == [3.0, 0.0, 2.0]
+    zero = torch.zeros_like(one)
+    dpre, _ = pkg.bias_act_backward(one, zero, offs, "silu")
+    assert dpre[:, 0].tolist() == [0.0, 0.5, 0.5, 0.5, 0.5, 0.5]
