@@ -12,13 +12,16 @@ include/ggemm_persistent.h. Modules:
 * ``quant``      -- FP8 quantization producer (per-tensor and MX with group padding) over the C ABI
 * ``moe``        -- routing tokens to experts, their rows into expert order and back, over the C ABI
 * ``autograd``   -- the FP8 grouped linear layer (forward, dgrad, wgrad) as a torch autograd op
+* ``layer``      -- a whole MoE layer from router logits to the combined tokens
 * ``harness``    -- code-object launch paths mirroring the reference's hipModule harness
 * ``inputs``     -- seeded generators for the measured configurations
 * ``build``      -- in-tree hipcc build of the library and the drop-in code objects
 """
 from . import build, inputs  # noqa: F401
 from ._lib import GGemmError, bf16_kernel, launch_geometry, library_path, load as load_library  # noqa: F401
-from .autograd import FP8DelayedScaling, FP8WeightCache, GroupedLinearFP8, grouped_linear_fp8  # noqa: F401
+from .autograd import (FP8DelayedScaling, FP8WeightCache, GroupedLinearActFP8, GroupedLinearFP8,  # noqa: F401
+                       grouped_linear_fp8)
+from .layer import moe_layer_fp8  # noqa: F401
 from .moe import DispatchPlan, combine_tokens, dispatch_tokens, plan_dispatch, route_experts  # noqa: F401
 from .persistent import grouped_gemm_fp8_tensorwise  # noqa: F401
 from .product import bias_act_backward, grouped_gemm_fp8_bias_act  # noqa: F401

@@ -29,6 +29,9 @@ the autograd wiring left to the framework (Primus-Turbo, not vendored).
 * ``scaling=FP8DelayedScaling()``: x, w and dy are quantized with delayed scaling (the largest
   amax of their previous calls, recorded on the device in the quantizing pass itself), which drops
   the standalone amax passes; values beyond the historical range saturate at +-fmax.
+* ``bias=``, ``activation=``: the expert's bias (bf16 / fp32 [G, N]) and activation in the forward product's
+  epilogue (``grouped_gemm_fp8_bias_act``); the value before the activation is kept in bf16, and backward begins with
+  ``bias_act_backward``, whose result is what is quantized as dy.
 There is no CPU path: the tensors must live on a gfx950 GPU.
 """
 from __future__ import annotations
@@ -38,6 +41,7 @@ import weakref
 import torch
 
 from .persistent import grouped_gemm_fp8_tensorwise
+from .product import bias_act_backward, grouped_gemm_fp8_bias_act
 from .quant import (quantize_fp8_tensorwise, quantize_fp8_tensorwise_delayed, quantize_fp8_tensorwise_transpose,
                     quantize_fp8_tensorwise_transpose_delayed)
 from .vark import grouped_gemm_fp8_tensorwise_variable_k, weight_grad_fp8
@@ -176,67 +180,109 @@ class FP8DelayedScaling:
         return qw, qwt, scale
 
 
+def _forward_operands(ctx, x, w, group_offs, main_grad, weight_cache, scaling):
+    """(qx, qw, sx, sw) of the forward product; keeps what ``_backward_products`` needs but the tensors."""
+    if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2]:
+        raise ValueError("x must be [M, K] and w [G, N, K]")
+    if w.shape[0] != group_offs.numel() - 1:
+        raise ValueError("w holds one weight per group")
+    # operand rows start on 128-byte lines (padded buffers): K-major rows of K = 2880 bytes
+    # would otherwise straddle lines and cost the GEMMs 1.5 line requests per row segment
+    if scaling is not None:
+        qx, sx = scaling.quantize("x", x.contiguous(), "e4m3")
+    else:
+        qx, sx, _ = quantize_fp8_tensorwise(x.contiguous(), "e4m3", row_align=_LINE)
+    if weight_cache is not None:
+        qw, qwt, sw = weight_cache.get(w, ctx.needs_input_grad[0], scaling)
+    else:
+        qw, qwt, sw = _quantize_weight(w, ctx.needs_input_grad[0], scaling)
+    ctx.main_grad = main_grad
+    ctx.scaling = scaling
+    ctx.x_dtype, ctx.w_dtype = x.dtype, w.dtype
+    return qx, qw, qwt, sx, sw
+
+
+def _backward_products(ctx, dy, qx, sx, qwt, sw, group_offs):
+    """(dx, dw) of the linear part, dw None where it went into main_grad."""
+    if ctx.scaling is not None:
+        qdy, sdy = ctx.scaling.quantize("dy", dy.contiguous(), "e5m2")
+    else:
+        qdy, sdy, _ = quantize_fp8_tensorwise(dy.contiguous(), "e5m2", row_align=_LINE)
+    dx = dw = None
+    if ctx.needs_input_grad[0]:
+        # dx[r] = dy[r] @ w[g]: B[g] = w[g]^T, [N_out = K, K_red = N] K-major
+        dx = grouped_gemm_fp8_tensorwise(qdy, qwt, sdy, sw, group_offs, zero_tail=True)
+        dx = dx.to(ctx.x_dtype)
+    if ctx.needs_input_grad[1] or ctx.main_grad is not None:
+        if ctx.main_grad is not None:
+            grouped_gemm_fp8_tensorwise_variable_k(qx, qdy, sx, sdy, group_offs, out=ctx.main_grad,
+                                                   accumulate=True)
+        else:
+            # written as [G, N, K]: a [G, K, N] result handed on as a transposed view is copied
+            # into the parameter's layout by autograd, 300 us beside the GEMM's 250 for
+            # [4, 5760, 2880] and 16384 tokens
+            dw = weight_grad_fp8(qdy, qx, sdy, sx, group_offs).to(ctx.w_dtype)
+    return dx, dw
+
+
 class GroupedLinearFP8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, group_offs, main_grad, weight_cache=None, scaling=None):
-        if x.dim() != 2 or w.dim() != 3 or x.shape[1] != w.shape[2]:
-            raise ValueError("x must be [M, K] and w [G, N, K]")
-        if w.shape[0] != group_offs.numel() - 1:
-            raise ValueError("w holds one weight per group")
-        # operand rows start on 128-byte lines (padded buffers): K-major rows of K = 2880 bytes
-        # would otherwise straddle lines and cost the GEMMs 1.5 line requests per row segment
-        if scaling is not None:
-            qx, sx = scaling.quantize("x", x.contiguous(), "e4m3")
-        else:
-            qx, sx, _ = quantize_fp8_tensorwise(x.contiguous(), "e4m3", row_align=_LINE)
-        if weight_cache is not None:
-            qw, qwt, sw = weight_cache.get(w, ctx.needs_input_grad[0], scaling)
-        else:
-            qw, qwt, sw = _quantize_weight(w, ctx.needs_input_grad[0], scaling)
+        qx, qw, qwt, sx, sw = _forward_operands(ctx, x, w, group_offs, main_grad, weight_cache, scaling)
         # rows past offs[G] (tokens the routing dropped) come out as exact zeros
         out = grouped_gemm_fp8_tensorwise(qx, qw, sx, sw, group_offs, zero_tail=True)
         ctx.save_for_backward(qx, sx, qwt, sw, group_offs)
-        ctx.main_grad = main_grad
-        ctx.scaling = scaling
-        ctx.x_dtype, ctx.w_dtype = x.dtype, w.dtype
         return out
 
     @staticmethod
     def backward(ctx, dy):
-        qx, sx, qwt, sw, group_offs = ctx.saved_tensors
-        if ctx.scaling is not None:
-            qdy, sdy = ctx.scaling.quantize("dy", dy.contiguous(), "e5m2")
-        else:
-            qdy, sdy, _ = quantize_fp8_tensorwise(dy.contiguous(), "e5m2", row_align=_LINE)
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            # dx[r] = dy[r] @ w[g]: B[g] = w[g]^T, [N_out = K, K_red = N] K-major
-            dx = grouped_gemm_fp8_tensorwise(qdy, qwt, sdy, sw, group_offs, zero_tail=True)
-            dx = dx.to(ctx.x_dtype)
-        if ctx.needs_input_grad[1] or ctx.main_grad is not None:
-            if ctx.main_grad is not None:
-                grouped_gemm_fp8_tensorwise_variable_k(qx, qdy, sx, sdy, group_offs, out=ctx.main_grad,
-                                                       accumulate=True)
-            else:
-                # written as [G, N, K]: a [G, K, N] result handed on as a transposed view is copied
-                # into the parameter's layout by autograd, 300 us beside the GEMM's 250 for
-                # [4, 5760, 2880] and 16384 tokens
-                dw = weight_grad_fp8(qdy, qx, sdy, sx, group_offs).to(ctx.w_dtype)
+        dx, dw = _backward_products(ctx, dy, *ctx.saved_tensors)
         return dx, dw, None, None, None, None
+
+
+class GroupedLinearActFP8(torch.autograd.Function):
+    """The same with bias and activation in the forward product's epilogue."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias, group_offs, main_grad, weight_cache, scaling, activation, options):
+        qx, qw, qwt, sx, sw = _forward_operands(ctx, x, w, group_offs, main_grad, weight_cache, scaling)
+        keep = activation is not None and any(ctx.needs_input_grad)
+        got = grouped_gemm_fp8_bias_act(qx, qw, sx, sw, group_offs, bias, activation, keep_preact=keep, zero_tail=True,
+                                        **options)
+        out, pre = got if keep else (got, None)
+        ctx.save_for_backward(qx, sx, qwt, sw, group_offs, pre)
+        ctx.act = activation, options
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        *saved, pre = ctx.saved_tensors
+        activation, options = ctx.act
+        dy, db = bias_act_backward(dout, pre, saved[-1], activation, bias_grad=ctx.needs_input_grad[2], **options)
+        dx, dw = _backward_products(ctx, dy, *saved)
+        return dx, dw, None if db is None else db.to(ctx.bias_dtype), None, None, None, None, None, None
 
 
 def grouped_linear_fp8(x: torch.Tensor, w: torch.Tensor, group_offs: torch.Tensor,
                        main_grad: torch.Tensor | None = None,
                        weight_cache: FP8WeightCache | None = None,
-                       scaling: FP8DelayedScaling | None = None) -> torch.Tensor:
-    """FP8 grouped linear layer: ``out[r] = x[r] @ w[g]^T`` for the rows of group g, bf16 out.
+                       scaling: FP8DelayedScaling | None = None, *, bias: torch.Tensor | None = None,
+                       activation: str | None = None, slope: float = 1.0, limit: float | None = None,
+                       shift: float = 0.0) -> torch.Tensor:
+    """FP8 grouped linear layer: ``out[r] = act(x[r] @ w[g]^T + bias[g])`` for the rows of group g, bf16 out.
 
     x: bf16 / fp32 [M, K] (rows grouped by expert); w: bf16 / fp32 [G, N, K]; group_offs: int64
     [G+1] on the device. Backward gives dx [M, K] and dw [G, N, K]; with ``main_grad`` (fp32
     [G, K, N], the wgrad kernel's orientation) the weight gradient is added into it instead. With
     ``weight_cache`` the weight's fp8 copy is reused while the weight is unchanged. With ``scaling``
-    (one FP8DelayedScaling per layer) x, w and dy take delayed scaling (module docstring)."""
+    (one FP8DelayedScaling per layer) x, w and dy take delayed scaling (module docstring). bias: bf16 / fp32 [G, N],
+    with a gradient of its type; ``activation`` and its options as for ``grouped_gemm_fp8_bias_act`` ("swiglu" halves
+    the width)."""
     if main_grad is not None:
         if main_grad.dtype != torch.float32 or tuple(main_grad.shape) != (w.shape[0], w.shape[2], w.shape[1]):
             raise ValueError(f"main_grad must be fp32 [G, K, N] = {[w.shape[0], w.shape[2], w.shape[1]]}")
-    return GroupedLinearFP8.apply(x, w, group_offs, main_grad, weight_cache, scaling)
+    if bias is None and activation is None:
+        return GroupedLinearFP8.apply(x, w, group_offs, main_grad, weight_cache, scaling)
+    options = {"slope": slope, "limit": limit, "shift": shift}
+    return GroupedLinearActFP8.apply(x, w, bias, group_offs, main_grad, weight_cache, scaling, activation, options)
