@@ -124,7 +124,9 @@ __device__ __forceinline__ void grad8(const v4i& z8, const v4i& d8, const epi::A
         const float s = epi::sigmoid(z[i]);
         out[i] = d[i] * (s + z[i] * s * (1.f - s));
       } else if constexpr (kAct == epi::kGelu) {
-        out[i] = d[i] * (epi::gelu_cdf(z[i]) + z[i] * expf(-0.5f * z[i] * z[i]) * 0.398942280401433f);
+        float gauss;
+        const float cdf = epi::normal_cdf(z[i], &gauss);
+        out[i] = d[i] * (cdf + z[i] * gauss * 0.398942280401433f);
       } else {
         out[i] = d[i];
       }
@@ -178,9 +180,10 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
       grad8<kAct>(z[u], d[u], a.act, x);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] += x[i];
-      if (a.dpre != nullptr)
+      if (a.dpre != nullptr) {
         store_c16(a.dpre + (r + u) * a.stride_dpre + n,
                   v4i{epi::pack(x[0], x[1]), epi::pack(x[2], x[3]), epi::pack(x[4], x[5]), epi::pack(x[6], x[7])});
+      }
     }
   }
   if (a.dbias != nullptr) {
@@ -190,15 +193,29 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
   }
 }
 
-// dbias[g, n] over the group's units; grid (columns / kThreads, G).
+// dbias[g, n] over the group's units; grid (columns / 64, G): a wave takes 64 columns and every kWaves-th unit, eight
+// of them in flight, and the waves' sums are added in their order.
 __global__ __launch_bounds__(kThreads) void bias_sum_kernel(Args a) {
   __shared__ Table t;
+  __shared__ float s_sum[kThreads];
   group_table(a, t);
-  const int n = blockIdx.x * kThreads + threadIdx.x, g = blockIdx.y;
-  if (n >= a.N) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = blockIdx.x * 64 + lane, g = blockIdx.y;
   float s = 0.f;
-  for (int u = t.pre[g]; u < t.pre[g + 1]; ++u) s += a.partial[(int64_t)u * a.N + n];
-  a.dbias[(int64_t)g * a.N + n] = s;
+  if (n < a.N)
+    for (int u = t.pre[g] + wave; u < t.pre[g + 1]; u += 8 * kWaves) {
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = u + i * kWaves < t.pre[g + 1] ? a.partial[(int64_t)(u + i * kWaves) * a.N + n] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += p[i];
+    }
+  s_sum[threadIdx.x] = s;
+  __syncthreads();
+  if (wave == 0 && n < a.N) {
+    for (int w = 1; w < kWaves; ++w) s += s_sum[64 * w + lane];
+    a.dbias[(int64_t)g * a.N + n] = s;
+  }
 }
 
 }  // namespace ag

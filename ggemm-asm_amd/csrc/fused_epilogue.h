@@ -30,7 +30,25 @@ struct Args {
 __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896f));
 }
-__device__ __forceinline__ float gelu_cdf(float x) { return 0.5f * (1.f + erff(x * 0.707106781186548f)); }
+// The normal distribution's cdf and e^(-x^2 / 2), by Hastings' rational approximation of the error function (Abramowitz
+// and Stegun, Handbook of Mathematical Functions, 7.1.26; absolute error 1.5e-7): erfc(y) = t (a1 + t (a2 + t (a3 +
+// t (a4 + t a5)))) e^(-y^2), t = 1 / (1 + p y), y = |x| / sqrt 2. Half of erfc is the cdf of -|x|, so small values of the
+// negative side keep their relative accuracy. A third of the instructions of erff, which takes two branches.
+__device__ __forceinline__ float normal_cdf(float x, float* gauss) {
+  const float y = fabsf(x) * 0.707106781186548f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, y, 1.f));
+  float p = fmaf(t, 1.061405429f, -1.453152027f);
+  p = fmaf(t, p, 1.421413741f);
+  p = fmaf(t, p, -0.284496736f);
+  p = fmaf(t, p, 0.254829592f);
+  *gauss = __builtin_amdgcn_exp2f(x * x * -0.721347520444482f);
+  const float below = 0.5f * t * p * *gauss;
+  return x > 0.f ? 1.f - below : below;
+}
+__device__ __forceinline__ float gelu_cdf(float x) {
+  float gauss;
+  return normal_cdf(x, &gauss);
+}
 
 // NaN stays NaN in both (a comparison with it is false).
 __device__ __forceinline__ float at_most(float x, float m) { return x > m ? m : x; }
@@ -50,8 +68,12 @@ __device__ __forceinline__ v4f load_bias(const Args& e, int64_t i) {
   return v4f{from_bf16(w[0]), __uint_as_float(w[0] & 0xffff0000u), from_bf16(w[1]), __uint_as_float(w[1] & 0xffff0000u)};
 }
 
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef __bf16 v2b __attribute__((ext_vector_type(2)));
+
+// Two values rounded to nearest even, one v_cvt_pk_bf16_f32.
 __device__ __forceinline__ int pack(float a, float b) {
-  return (int)(f32_to_bf16_rne(a) | (f32_to_bf16_rne(b) << 16));
+  return __builtin_bit_cast(int, __builtin_convertvector(v2f{a, b}, v2b));
 }
 
 // LDS that a wave stages 32 rows of NB blocks in, rows 16 bytes apart so that 16 of them start on different banks.
@@ -91,6 +113,20 @@ __device__ __forceinline__ void store(const v4f (&acc)[MB][NB], float alpha, con
     const int64_t prow = row0 + 32 * p;
     const int prows = rows - 32 * p;
     if (prows <= 0) return;                            // uniform in the wave
+    // the pass's residual, in flight while z is staged
+    v2i res[2][NB];
+    if (e.residual != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          res[i][j] = v2i{0, 0};
+          if (16 * i + s >= prows || j >= blocks) continue;
+          const uint16_t* at = e.residual + (prow + 16 * i + s) * e.stride_res + o0 + (kGated ? 8 * j + 2 * q : 16 * j + 4 * q);
+          if constexpr (kGated) res[i][j][0] = *(const int*)at;
+          else res[i][j] = *(const v2i*)at;
+        }
+    }
     if (e.pre != nullptr) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -104,15 +140,14 @@ __device__ __forceinline__ void store(const v4f (&acc)[MB][NB], float alpha, con
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = 16 * i + s;
-      const uint16_t* res = e.residual != nullptr && r < prows ? e.residual + (prow + r) * e.stride_res + o0 : nullptr;
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         const v4f z = acc[2 * p + i][j] * alpha + bias[j];
         GG_LDS uint8_t* at = reg + r * (16 * kOutChunks + 16);
         if constexpr (kGated) {
           float x = swiglu(z[0], z[1], e), y = swiglu(z[2], z[3], e);
-          if (res != nullptr && j < blocks) {
-            const uint32_t w = *(const uint32_t*)(res + 8 * j + 2 * q);
+          if (e.residual != nullptr) {
+            const uint32_t w = res[i][j][0];
             x += from_bf16(w);
             y += __uint_as_float(w & 0xffff0000u);
           }
@@ -123,8 +158,8 @@ __device__ __forceinline__ void store(const v4f (&acc)[MB][NB], float alpha, con
 #pragma unroll
             for (int c = 0; c < 4; ++c) x[c] = z[c] * (kAct == kSilu ? sigmoid(z[c]) : gelu_cdf(z[c]));
           }
-          if (res != nullptr && j < blocks) {
-            const v2i w = *(const v2i*)(res + 16 * j + 4 * q);
+          if (e.residual != nullptr) {
+            const v2i w = res[i][j];
             x += v4f{from_bf16(w[0]), __uint_as_float(w[0] & 0xffff0000u), from_bf16(w[1]),
                      __uint_as_float(w[1] & 0xffff0000u)};
           }

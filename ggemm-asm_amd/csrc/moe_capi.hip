@@ -58,6 +58,11 @@ int with_layout(int E, F f) {
 int common_bytes(uint64_t all) { return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : all % 2 == 0 ? 2 : 1; }
 uint64_t bits(const void* p) { return (uint64_t)reinterpret_cast<uintptr_t>(p); }
 
+// Whether a lane's V elements of every row are one aligned access (of at most 16 bytes each).
+bool one_load(int V, int item, int E, int64_t stride, const void* p) {
+  return E % V == 0 && stride % V == 0 && aligned(p, (uintptr_t)std::min(V * item, 16));
+}
+
 // Workgroups of four waves, a wave per row, at most eight to a CU.
 int row_grid(int64_t rows, int cus) {
   return (int)std::max<int64_t>(1, std::min<int64_t>((rows + ex::kWaves - 1) / ex::kWaves, (int64_t)cus * 8));
@@ -97,12 +102,14 @@ int ggemm_moe_route(const void* logits, int32_t dtype, int64_t T, int32_t E, int
   rc = device_cus(&cus);
   if (rc) return rc;
   if (T == 0) return GGEMM_OK;
-  const rt::Args a{logits, T,          stride,      E,     top_k,   score, bias, num_groups, top_groups, group_best,
-                   renormalize, scale, weights, experts};
+  rt::Args a{logits, T, stride, E, top_k, score, bias, num_groups, top_groups, group_best, renormalize, scale, weights,
+             experts, false};
+  const int item = dtype == GGEMM_IN_BF16 ? 2 : 4;
   return with_layout(E, [&](auto l, auto v) {
     constexpr int L = decltype(l)::value, V = decltype(v)::value;
     const dim3 grid((uint32_t)((T + rt::kThreads / L - 1) / (rt::kThreads / L)));
     const int lds = rt::route_lds(L, E, top_k, num_groups);
+    a.vec = one_load(V, item, E, stride, logits);
     if (dtype == GGEMM_IN_BF16)
       hipLaunchKernelGGL((rt::route_kernel<uint16_t, L, V>), grid, dim3(rt::kThreads), lds, (hipStream_t)stream, a);
     else
@@ -123,11 +130,14 @@ int ggemm_moe_route_backward(const float* dweights, const void* logits, int32_t 
   rc = device_cus(&cus);
   if (rc) return rc;
   if (T == 0) return GGEMM_OK;
-  const rt::BackArgs a{dweights, logits, T, stride, E, top_k, score, renormalize, scale, experts, dlogits};
+  rt::BackArgs a{dweights, logits, T, stride, E, top_k, score, renormalize, scale, experts, dlogits, false, false};
+  const int item = dtype == GGEMM_IN_BF16 ? 2 : 4;
   return with_layout(E, [&](auto l, auto v) {
     constexpr int L = decltype(l)::value, V = decltype(v)::value;
     const dim3 grid((uint32_t)((T + rt::kThreads / L - 1) / (rt::kThreads / L)));
     const int lds = rt::route_back_lds(L, E, top_k);
+    a.vec = one_load(V, item, E, stride, logits);
+    a.vec_out = one_load(V, item, E, E, dlogits);
     if (dtype == GGEMM_IN_BF16)
       hipLaunchKernelGGL((rt::route_backward_kernel<uint16_t, L, V>), grid, dim3(rt::kThreads), lds,
                          (hipStream_t)stream, a);

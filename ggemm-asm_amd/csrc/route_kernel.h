@@ -33,6 +33,7 @@ struct Args {
   float scale;
   float* weights;
   int* experts;
+  bool vec;                       // a lane's logits are one aligned load
 };
 
 struct BackArgs {
@@ -43,14 +44,14 @@ struct BackArgs {
   float scale;
   const int* experts;
   void* dlogits;
+  bool vec, vec_out;              // a lane's logits, and its part of dlogits, are one aligned access
 };
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
 __device__ __forceinline__ void from_f32(float f, float* p) { *p = f; }
 __device__ __forceinline__ void from_f32(float f, uint16_t* p) {
-  const uint32_t u = __float_as_uint(f);
-  *p = (uint16_t)((u & 0x7fffffffu) > 0x7f800000u ? 0x7fc0u : (u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+  *p = __builtin_bit_cast(uint16_t, (__bf16)f);
 }
 
 // Floats as unsigned integers of the same order: -inf is kDead, zeros are equal, NaN is the largest.
@@ -96,12 +97,43 @@ __device__ __forceinline__ float sum_f32(float x) {
   }));
 }
 
-// Logits of the lane's V experts e0 .. e0 + V - 1 (-inf past E).
+// The two largest keys of groups of `lanes` lanes (a power of two), in each of their lanes.
+template <int L, int kStep = 0>
+__device__ __forceinline__ void merge_best(uint32_t& b0, uint32_t& b1, int lanes) {
+  if constexpr ((1 << kStep) < L) {
+    if ((1 << kStep) >= lanes) return;               // the same for the whole launch
+    const uint32_t o0 = partner<kStep>(b0), o1 = partner<kStep>(b1);
+    b1 = max(max(b1, o1), min(b0, o0));
+    b0 = max(b0, o0);
+    merge_best<L, kStep + 1>(b0, b1, lanes);
+  }
+}
+
+// Logits of the lane's V experts e0 .. e0 + V - 1 (-inf past E). vec: E is a multiple of V and every row starts on a
+// multiple of V elements, so a lane's logits are one load.
 template <typename T, int V>
-__device__ __forceinline__ void load_logits(const T* row, int e0, int E, float (&x)[V]) {
+__device__ __forceinline__ void load_logits(const T* row, int e0, int E, bool vec, float (&x)[V]) {
+  if (V > 1 && vec) {
+    struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Pack {
+      T v[V];
+    };
+    if (e0 < E) {
+      const Pack p = *(const Pack*)(row + e0);
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v] = to_f32(p.v[v]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v] = -INFINITY;
+    }
+    return;
+  }
 #pragma unroll
   for (int v = 0; v < V; ++v) x[v] = e0 + v < E ? to_f32(row[e0 + v]) : -INFINITY;
 }
+
+// Orders this wave's LDS accesses for the compiler (the hardware runs them in order): what the lanes of a token
+// hand each other never leaves their wave.
+__device__ __forceinline__ void lds_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // max and sum of exp(l - max) over a token's logits; the max of a token with every expert masked as 0.
 template <int L, int V>
@@ -137,7 +169,7 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
   float* s_val = (float*)s_rt + kTokens * a.k + tok * a.k;
 
   float x[V];
-  load_logits<T, V>((const T*)a.logits + (real ? t : 0) * a.stride, l * V, a.E, x);
+  load_logits<T, V>((const T*)a.logits + (real ? t : 0) * a.stride, l * V, a.E, a.vec, x);
   // p[v]: the score where keys or weights need it, else the logit
   const bool by_logit = a.bias == nullptr && a.groups <= 1;
   const bool scored = a.score == 1 || !a.renorm || !by_logit;
@@ -154,40 +186,63 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
     key[v] = e >= a.E ? 0u : x[v] == -INFINITY ? kDead : key_of(f);
   }
 
+  const int lane = tid & 63, seg = lane / L * L;
   if (a.groups > 1) {
-    const int gs = a.E / a.groups;
-    uint32_t* s_key = s_rt + 2 * kTokens * a.k + tok * a.E;
-    uint32_t* s_grp = s_rt + kTokens * (2 * a.k + a.E) + tok * a.groups;
-    uint32_t* s_keep = s_rt + kTokens * (2 * a.k + a.E + a.groups) + tok * a.groups;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (l * V + v < a.E) s_key[l * V + v] = key[v];
-    __syncthreads();
-    for (int g = l; g < a.groups; g += L) {
+    const int gs = a.E / a.groups, lg = gs / V;
+    if (gs % V == 0 && (lg & (lg - 1)) == 0) {
+      // a group is the V experts each of lg = 1, 2, 4 .. lanes: their two largest keys merged over those lanes,
+      // then every group's value read from its first lane
       uint32_t b0 = 0, b1 = 0;
-      for (int i = 0; i < gs; ++i) {
-        const uint32_t k = s_key[g * gs + i];
-        b1 = max(b1, min(b0, k));
-        b0 = max(b0, k);
-      }
-      s_grp[g] = a.group_best == 2 ? key_of(value_of(b0) + value_of(b1)) : b0;
-    }
-    __syncthreads();
-    for (int g = l; g < a.groups; g += L) {
-      const uint32_t mine = s_grp[g];
-      int before = 0;
-      for (int h = 0; h < a.groups; ++h) before += s_grp[h] > mine || (s_grp[h] == mine && h < g);
-      s_keep[g] = before < a.top_groups;
-    }
-    __syncthreads();
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int e = l * V + v;
-      if (e < a.E && !s_keep[e / gs]) key[v] = kDead;
+      for (int v = 0; v < V; ++v) {
+        b1 = max(b1, min(b0, key[v]));
+        b0 = max(b0, key[v]);
+      }
+      merge_best<L>(b0, b1, lg);
+      const uint32_t mine = a.group_best == 2 ? key_of(value_of(b0) + value_of(b1)) : b0;
+      const int group = l / lg;
+      int before = 0;
+      for (int h = 0; h < a.groups; ++h) {
+        const uint32_t other = L == 64 ? (uint32_t)__builtin_amdgcn_readlane((int)mine, h * lg)
+                                       : (uint32_t)__shfl((int)mine, seg + h * lg, 64);
+        before += other > mine || (other == mine && h < group);
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (key[v] != 0 && before >= a.top_groups) key[v] = kDead;
+    } else {
+      uint32_t* s_key = s_rt + 2 * kTokens * a.k + tok * a.E;
+      uint32_t* s_grp = s_rt + kTokens * (2 * a.k + a.E) + tok * a.groups;
+      uint32_t* s_keep = s_rt + kTokens * (2 * a.k + a.E + a.groups) + tok * a.groups;
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (l * V + v < a.E) s_key[l * V + v] = key[v];
+      lds_order();
+      for (int g = l; g < a.groups; g += L) {
+        uint32_t b0 = 0, b1 = 0;
+        for (int i = 0; i < gs; ++i) {
+          const uint32_t k = s_key[g * gs + i];
+          b1 = max(b1, min(b0, k));
+          b0 = max(b0, k);
+        }
+        s_grp[g] = a.group_best == 2 ? key_of(value_of(b0) + value_of(b1)) : b0;
+      }
+      lds_order();
+      for (int g = l; g < a.groups; g += L) {
+        const uint32_t mine = s_grp[g];
+        int before = 0;
+        for (int h = 0; h < a.groups; ++h) before += s_grp[h] > mine || (s_grp[h] == mine && h < g);
+        s_keep[g] = before < a.top_groups;
+      }
+      lds_order();
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int e = l * V + v;
+        if (e < a.E && !s_keep[e / gs]) key[v] = kDead;
+      }
     }
   }
 
-  const int lane = tid & 63, seg = lane / L * L;
   for (int j = 0; j < a.k; ++j) {
     uint32_t best = key[0];
 #pragma unroll
@@ -209,26 +264,28 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
         }
     }
   }
-  __syncthreads();
-  if (!real) return;
-
-  float base = 0.f, total = 1.f;
+  lds_order();
+  // weights: lane l takes places l, l + L, .. of the token; max and sum over the lanes
   const bool over_taken = a.score == 0 && a.renorm;
+  float base = 0.f, total = 1.f;
+  if (over_taken) {
+    base = -INFINITY;
+    for (int j = l; j < a.k; j += L) base = s_idx[j] >= 0 ? fmaxf(base, s_val[j]) : base;
+    base = max_f32<L>(base);
+  }
   if (a.renorm) {
     total = 0.f;
-    if (over_taken) {
-      base = -INFINITY;
-      for (int j = 0; j < a.k; ++j) base = s_idx[j] >= 0 ? fmaxf(base, s_val[j]) : base;
-      for (int j = 0; j < a.k; ++j) total += s_idx[j] >= 0 ? expf(s_val[j] - base) : 0.f;
-    } else {
-      for (int j = 0; j < a.k; ++j) total += s_val[j];
-      total = total < 1e-20f ? 1e-20f : total;
+    for (int j = l; j < a.k; j += L) {
+      if (over_taken) s_val[j] = s_idx[j] >= 0 ? expf(s_val[j] - base) : 0.f;
+      total += s_val[j];
     }
+    total = sum_f32<L>(total);
+    if (!over_taken && total < 1e-20f) total = 1e-20f;
   }
+  if (!real) return;
   for (int j = l; j < a.k; j += L) {
     const int e = s_idx[j];
-    const float q = (over_taken ? expf(s_val[j] - base) : s_val[j]) / total;
-    a.weights[t * a.k + j] = e >= 0 ? q * a.scale : 0.f;
+    a.weights[t * a.k + j] = e >= 0 ? s_val[j] / total * a.scale : 0.f;
     a.experts[t * a.k + j] = e;
   }
 }
@@ -236,7 +293,8 @@ __global__ __launch_bounds__(kThreads) void route_kernel(Args a) {
 // dlogits, one token to L lanes again. Per taken expert d = scale * dweight; with renormalised weights
 // d -= sum_i d_i q_i (q = weight / scale), and sigmoid divides by the sum of scores. Then
 //   softmax of the taken: d q;  softmax of all: d p [taken] - p sum_i d_i p_i;  sigmoid: d p (1 - p).
-// The taken experts' terms are put into a row of LDS and the row is written whole.
+// Bound by writing the row, of which k values are not zero but for a softmax of all: the taken experts' terms are put
+// into a row of LDS, which the lanes write whole. Only a softmax of all reads the other experts' logits.
 inline int route_back_lds(int L, int E, int k) { return kThreads / L * 4 * (E + 3 * k); }
 
 template <typename T, int L, int V>
@@ -254,63 +312,73 @@ __global__ __launch_bounds__(kThreads) void route_backward_kernel(BackArgs a) {
   const bool over_all = a.score == 0 && !a.renorm;
 
   float x[V], m = 0.f, sum = 1.f;
-  load_logits<T, V>(row, l * V, a.E, x);
-  if (over_all) softmax_stats<L, V>(x, &m, &sum);
-  for (int e = l; e < a.E; e += L) s_row[e] = 0.f;
+  if (over_all) {
+    load_logits<T, V>(row, l * V, a.E, a.vec, x);
+    softmax_stats<L, V>(x, &m, &sum);
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (l * V + v < a.E) s_row[l * V + v] = 0.f;
+  float base = -INFINITY;
   for (int j = l; j < a.k; j += L) {
     int e = real ? a.experts[t * a.k + j] : -1;
     e = e >= 0 && e < a.E ? e : -1;
-    const float lj = e >= 0 ? to_f32(row[e]) : 0.f;
+    const float lj = e >= 0 ? to_f32(row[e]) : -INFINITY;
     s_idx[j] = e;
-    s_val[j] = e < 0 ? 0.f : a.score == 1 ? sigmoid(lj) : over_all ? expf(lj - m) / sum : lj;
+    s_val[j] = lj;
     s_d[j] = e >= 0 ? a.dweights[t * a.k + j] * a.scale : 0.f;
+    base = fmaxf(base, lj);
   }
-  __syncthreads();
-
-  float base = 0.f, total = 1.f, dot = 0.f;
+  lds_order();
+  base = max_f32<L>(base);
+  // s_val becomes the score, or with a softmax of the taken its numerator
+  float total = 0.f, dot = 0.f;
+  for (int j = l; j < a.k; j += L) {
+    const float p = s_idx[j] < 0      ? 0.f
+                    : a.score == 1    ? sigmoid(s_val[j])
+                    : over_all        ? expf(s_val[j] - m) / sum
+                                      : expf(s_val[j] - base);
+    s_val[j] = p;
+    total += p;
+    dot += s_d[j] * p;
+  }
+  total = sum_f32<L>(total);
+  dot = sum_f32<L>(dot);
   if (a.renorm) {
-    total = 0.f;
-    if (a.score == 0) {
-      base = -INFINITY;
-      for (int j = 0; j < a.k; ++j) base = s_idx[j] >= 0 ? fmaxf(base, s_val[j]) : base;
-      for (int j = 0; j < a.k; ++j) total += s_idx[j] >= 0 ? expf(s_val[j] - base) : 0.f;
-      for (int j = 0; j < a.k; ++j) dot += s_idx[j] >= 0 ? s_d[j] * (expf(s_val[j] - base) / total) : 0.f;
-    } else {
-      for (int j = 0; j < a.k; ++j) total += s_val[j];
-      const bool small = total < 1e-20f;             // the sum's floor: the weights are p / 1e-20
-      total = small ? 1e-20f : total;
-      if (!small)
-        for (int j = 0; j < a.k; ++j) dot += s_d[j] * (s_val[j] / total);
-    }
-  } else if (over_all) {
-    for (int j = 0; j < a.k; ++j) dot += s_d[j] * s_val[j];
+    const bool small = a.score == 1 && total < 1e-20f;   // the sum's floor: the weights are p / 1e-20
+    total = small ? 1e-20f : total;
+    dot = small ? 0.f : dot / total;
   }
   for (int j = l; j < a.k; j += L) {
     const int e = s_idx[j];
     if (e < 0) continue;
-    float g;
-    if (a.score == 1) {
-      const float p = s_val[j], not_p = sigmoid(-to_f32(row[e]));
-      g = (s_d[j] - dot) / total * p * not_p;
-    } else if (a.renorm) {
-      g = (s_d[j] - dot) * (expf(s_val[j] - base) / total);
-    } else {
-      g = s_d[j] * s_val[j];
-    }
-    s_row[e] = g;
+    const float p = s_val[j], d = s_d[j];
+    s_row[e] = over_all      ? d * p
+               : a.score == 0 ? (d - dot) * (p / total)
+                              : (a.renorm ? (d - dot) / total : d) * p * sigmoid(-to_f32(row[e]));
   }
-  __syncthreads();
+  lds_order();
   if (!real) return;
-  T* out = (T*)a.dlogits + t * a.E;
-  if (over_all) {
+  float g[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int e = l * V + v;
-      if (e < a.E) from_f32(x[v] == -INFINITY ? 0.f : s_row[e] - dot * (expf(x[v] - m) / sum), out + e);
-    }
-  } else {
-    for (int e = l; e < a.E; e += L) from_f32(s_row[e], out + e);
+  for (int v = 0; v < V; ++v) {
+    const int e = l * V + v;
+    g[v] = e < a.E ? s_row[e] : 0.f;
+    if (over_all) g[v] = e < a.E && x[v] == -INFINITY ? 0.f : g[v] - dot * (expf(x[v] - m) / sum);
   }
+  T* out = (T*)a.dlogits + t * a.E + l * V;
+  if (V > 1 && a.vec_out) {
+    struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Pack {
+      T v[V];
+    } p;
+#pragma unroll
+    for (int v = 0; v < V; ++v) from_f32(g[v], &p.v[v]);
+    if (l * V < a.E) *(Pack*)out = p;
+    return;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+    if (l * V + v < a.E) from_f32(g[v], out + v);
 }
 
 }  // namespace rt

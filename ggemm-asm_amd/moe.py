@@ -71,10 +71,13 @@ class _Route(torch.autograd.Function):
         ctx.save_for_backward(logits, experts)
         ctx.args = score, renormalize, scale
         ctx.mark_non_differentiable(experts)
+        ctx.set_materialize_grads(False)              # no zeros made for the experts, which have no gradient
         return weights, experts
 
     @staticmethod
     def backward(ctx, dweights, _):
+        if dweights is None:
+            return (None,) * 9
         logits, experts = ctx.saved_tensors
         score, renormalize, scale = ctx.args
         T, E = logits.shape
