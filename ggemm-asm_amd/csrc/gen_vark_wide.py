@@ -1016,6 +1016,9 @@ SGPR_K = dict(SGPR, RECA=SGPR["CM0"], RECB=SGPR["CN0"], HALF="s89")
 class GenK(Gen):
     """The K-major pipeline; the bf16 epilogue (and vm model) is the wgrad kernels'."""
 
+    def tile_start(self):
+        pass
+
     def wait_oldest(self):
         s, OP, c = SGPR_K, self.OP, self.cfg
         self.emit(f"s_sub_u32 {s['NEED']}, {OP['vmt']}, {OP['q0']}")
@@ -1204,6 +1207,7 @@ class GenK(Gen):
         e(f"s_addc_u32 {s['BR1']}, {OP['bRT_hi']}, 0")
         e(f"s_mov_b32 {s['RECA']}, {OP['recAT']}")
         e(f"s_mov_b32 {s['RECB']}, {OP['recBT']}")
+        self.tile_start()
         e("s_barrier")   # the previous tile's epilogue is done with its staging slot
         e(f"s_min_u32 {s['LIMTOP']}, {s['S']}, {KSLOTS}")
         top, topdone = self.label("top"), self.label("topdone")
@@ -1244,13 +1248,265 @@ class GenK(Gen):
         e(f"s_cselect_b32 {OP['nis']}, {s['IDX']}, 0")
 
 
+# ---------------------------------------------------------------- products with an epilogue
+#
+# The K-major forward tile with bias and activation (product_wide.h): z = alpha acc + bias, then
+#   bias      z rounded to bf16 is C;
+#   gate      swiglu of neighbouring columns (z0, z1), (z2, z3) .., half as wide as the tile: v = min(z0, limit)
+#             sigmoid(slope v) (clamp(z1, limit) + shift);
+#   gatekeep  both, z into a second tensor.
+# A lane's accumulators 4 g .. 4 g + 3 of a block are four neighbouring columns of one row (32 j + 8 g + 4 h + r, h = l /
+# 32), so a pair never leaves its lane. The tile's bias comes as one load per wave at the tile's start, 160 columns of
+# fp32 or bf16 in lanes 0-39, and is handed to all lanes through LDS in the epilogue. A wave stages 32 rows x 160
+# columns of z, and 80 of the result, in rows padded to an odd number of 16-byte chunks, and stores them as chunks.
+# Per SIMD and tile the activation is 160 pairs of 13 vector operations and an exp2 and a reciprocal at a quarter of
+# the rate each, about 12 thousand cycles beside the tile's 90 thousand, and nothing overlaps them: one wave holds
+# the SIMD's registers. 131072 rows x 5760 x 2880 take @@GATE@@ us so, @@KEEP@@ with z kept; without an epilogue 1690.
+ZPITCH, OPITCH = 336, 176            # bytes of a staged row of z (160 bf16) and of the result (80)
+OREGION = 32 * ZPITCH                # a wave's staged result, after its z; 16 KiB together
+BIAS_OFF = 4 * 16384                 # the waves' bias, 1 KiB each
+
+
+class KEConfig(KConfig):
+    def __init__(self, mode):
+        super().__init__(256, 320, False)
+        self.mode, self.name = mode, f"pe256x320_{mode}"
+        self.keep_z, self.gate = mode != "gate", mode != "bias"
+        self.e_stores = self.bm * (10 * self.keep_z + 5 * self.gate)
+        self.vbias = self.epi_x - 4                     # four registers, loaded at the tile's start
+        self.vgpr_clobber = list(range(self.vbias, 256))
+        ops = [o for o in self.operands if o[0] not in ("ew_base", "ew_s", "rb_even", "rb_odd", "gb")]
+        ops += [(n, "v") for n in ("vboff", "b_lo", "b_hi", "brec", "bf32")]
+        if self.gate:
+            ops += [(n, "v") for n in ("nslope", "limit", "shift")]
+        if mode == "gatekeep":
+            ops += [(n, "v") for n in ("zT_lo", "zT_hi", "zrecT", "zm2", "sw_z")]
+        self.operands = ops
+        self.op = {name: f"%{i}" for i, (name, _) in enumerate(ops)}
+        assert BIAS_OFF + 4096 <= self.slot and OREGION + 32 * OPITCH == 16384
+        assert self.vbias % 2 == 0 and self.vop0 + 72 <= self.vacc0
+
+
+KECONFIGS = (KEConfig("bias"), KEConfig("gate"), KEConfig("gatekeep"))
+
+
+class GenKE(GenK):
+    def wait_oldest(self):
+        """As GenK's, the counts within vmcnt's 63 (a stricter wait is safe)."""
+        s, OP, c = SGPR_K, self.OP, self.cfg
+        self.emit(f"s_sub_u32 {s['NEED']}, {OP['vmt']}, {OP['q0']}")
+        self.emit(f"s_mov_b32 {OP['q0']}, {OP['q1']}")
+        self.emit(f"s_mov_b32 {OP['q1']}, {OP['q2']}")
+        self.emit(f"s_sub_u32 {OP['np']}, {OP['np']}, 1")
+        counts = sorted({min(n, 63) for n in (c.e_stores + c.loads, c.e_stores, c.loads)}, reverse=True)
+        done = self.label("wdone")
+        tgt = {n: self.label(f"w{n}_") for n in counts}
+        for n in counts:
+            self.emit(f"s_cmp_ge_u32 {s['NEED']}, {n}")
+            self.emit(f"s_cbranch_scc1 {tgt[n]}")
+        self.emit("s_waitcnt vmcnt(0)")
+        self.emit(f"s_branch {done}")
+        for n in counts:
+            self.emit(f"{tgt[n]}:")
+            self.emit(f"s_waitcnt vmcnt({n})")
+            self.emit(f"s_branch {done}")
+        self.emit(f"{done}:")
+
+    def tile_start(self):
+        """The wave's bias: 160 columns, four to a lane (lanes past 39 and no bias at all read zeros). Older than every
+        load of the tile that is still to be issued, so at most one stage's loads are younger in the epilogue."""
+        s, OP, e, c = SGPR_K, self.OP, self.emit, self.cfg
+        half, done = self.label("b16"), self.label("bdone")
+        e(f"v_readfirstlane_b32 {s['RC0']}, {OP['b_lo']}")
+        e(f"v_readfirstlane_b32 {s['RC1']}, {OP['b_hi']}")
+        e(f"v_readfirstlane_b32 {s['RC2']}, {OP['brec']}")
+        e(f"v_readfirstlane_b32 {s['T']}, {OP['bf32']}")
+        e(f"s_mov_b32 {s['RC3']}, 0x{WORD3:x}")
+        e("s_nop 4")
+        e(f"s_and_b32 {s['RC1']}, {s['RC1']}, 0xffff")
+        e(f"s_cmp_eq_u32 {s['T']}, 0")
+        e(f"s_cbranch_scc1 {half}")
+        e(f"buffer_load_dwordx4 v[{c.vbias}:{c.vbias + 3}], {OP['vboff']}, {s['RC']}, 0 offen")
+        e(f"s_branch {done}")
+        e(f"{half}:")
+        e(f"buffer_load_dwordx2 v[{c.vbias}:{c.vbias + 1}], {OP['vboff']}, {s['RC']}, 0 offen")
+        e(f"{done}:")
+        e(f"s_add_u32 {OP['vmt']}, {OP['vmt']}, 1")
+
+    def epilogue(self):
+        s, OP, e, c = SGPR_K, self.OP, self.emit, self.cfg
+        v0 = c.vop0                                    # the 72 operand registers are free here
+        bset, data = (v0, v0 + 16), v0 + 16            # bias of a block, two sets; read-back data (over the second)
+        z, ex, pk = v0 + 32, v0 + 36, v0 + 38          # z of four columns, exponentials, packed results
+        lane = {n: v0 + 56 + k for k, n in enumerate(("zw", "ow", "ba", "zr0", "zr1", "or0", "or1", "zg0", "zg1", "og0",
+                                                      "og1"))}
+        ln, t0, t1 = (v0 + 67 + k for k in range(3))
+        assert data + 40 <= v0 + 56 and v0 + 70 <= c.vacc0
+        L = {n: f"v{r}" for n, r in lane.items()}
+        limit, nlimit, nslope, shift = s["K"], s["LIM"], s["NEED"], s["LIMTOP"]   # free after the last stage
+        zres, zm2, swz = s["RL"], s["RR0"], s["RR1"]
+        e("s_nop 7")
+        e("s_nop 7")
+        e("s_nop 7")
+        e("s_barrier")                                 # every wave is past its reads of the last stage's slot
+        self.gate_values(limit, nlimit, nslope, shift)
+        if c.mode == "gatekeep":
+            for d, n in (("RL0", "zT_lo"), ("RL1", "zT_hi"), ("RL2", "zrecT"), ("RR0", "zm2"), ("RR1", "sw_z")):
+                e(f"v_readfirstlane_b32 {s[d]}, {OP[n]}")
+            e(f"s_mov_b32 {s['RL3']}, 0x{WORD3:x}")
+            e("s_nop 4")
+            e(f"s_and_b32 {s['RL1']}, {s['RL1']}, 0xffff")
+        elif c.mode == "bias":                         # z is the result
+            zres, zm2, swz = s["RC"], OP["cm2"], OP["sw_epi"]
+        self.c_resource()
+        # this wave's LDS: EPI its staged rows, T2 its bias
+        e(f"s_add_u32 {s['T']}, {OP['lds_base']}, {s['CS']}")
+        e(f"s_lshl_b32 {s['EPI']}, {OP['w1k']}, 4")
+        e(f"s_add_u32 {s['EPI']}, {s['EPI']}, {s['T']}")
+        e(f"s_add_u32 {s['T2']}, {s['T']}, {OP['w1k']}")
+        e(f"s_add_u32 {s['T2']}, {s['T2']}, {BIAS_OFF}")
+        e(f"v_mbcnt_lo_u32_b32 v{ln}, -1, 0")
+        e(f"v_mbcnt_hi_u32_b32 v{ln}, -1, v{ln}")
+        # the bias, one stage's loads younger at most, as fp32 into LDS
+        f32, ready = self.label("bf"), self.label("bready")
+        b = c.vbias
+        e(f"v_readfirstlane_b32 {s['T']}, {OP['bf32']}")
+        e(f"v_lshlrev_b32 v{t0}, 4, v{ln}")
+        e(f"v_add_u32 v{t0}, {s['T2']}, v{t0}")
+        e(f"s_waitcnt vmcnt({c.loads})")
+        e(f"s_cmp_eq_u32 {s['T']}, 0")
+        e(f"s_cbranch_scc0 {f32}")
+        e(f"v_and_b32 v{b + 3}, 0xffff0000, v{b + 1}")
+        e(f"v_lshlrev_b32 v{b + 2}, 16, v{b + 1}")
+        e(f"v_and_b32 v{b + 1}, 0xffff0000, v{b}")
+        e(f"v_lshlrev_b32 v{b}, 16, v{b}")
+        e(f"{f32}:")
+        e(f"ds_write_b128 v{t0}, v[{b}:{b + 3}]")
+        # lane bases: staging writes at row l % 32, half l / 32; read-backs of 16 (z) or 8 chunks a row and of the
+        # rows' last 4 or 2; the same rows and chunks in memory
+        e(f"v_and_b32 v{t0}, 31, v{ln}")
+        e(f"v_lshrrev_b32 v{t1}, 5, v{ln}")
+        e(f"v_lshl_add_u32 {L['ba']}, v{t1}, 4, {s['T2']}")
+        e(f"v_mul_u32_u24 {L['zw']}, {ZPITCH}, v{t0}")
+        e(f"v_lshl_add_u32 {L['zw']}, v{t1}, 3, {L['zw']}")
+        e(f"v_add_u32 {L['zw']}, {s['EPI']}, {L['zw']}")
+        e(f"v_mul_u32_u24 {L['ow']}, {OPITCH}, v{t0}")
+        e(f"v_lshl_add_u32 {L['ow']}, v{t1}, 2, {L['ow']}")
+        e(f"v_add_u32 {L['ow']}, {s['EPI']}, {L['ow']}")
+        for on, pitch, stride, wide in ((c.keep_z, ZPITCH, zm2, (("z", 0, 4, 0), ("z", 1, 2, 256))),
+                                        (c.gate, OPITCH, OP["cm2"], (("o", 0, 3, 0), ("o", 1, 1, 128)))):
+            for n, k, shift_, first in wide if on else ():
+                # row l >> shift, chunk l % 2^shift, from byte `first` of the row
+                rd, mem = L[f"{n}r{k}"], L[f"{n}g{k}"]
+                e(f"v_lshrrev_b32 v{t0}, {shift_}, v{ln}")
+                e(f"v_and_b32 v{t1}, {(1 << shift_) - 1}, v{ln}")
+                e(f"v_lshlrev_b32 v{t1}, 4, v{t1}")
+                if first:
+                    e(f"v_add_u32 v{t1}, {first}, v{t1}")
+                e(f"v_mul_u32_u24 {rd}, {pitch}, v{t0}")
+                e(f"v_add3_u32 {rd}, {rd}, v{t1}, {s['EPI']}")
+                e(f"v_mul_lo_u32 {mem}, v{t0}, {stride}")
+                e(f"v_add_u32 {mem}, {mem}, v{t1}")
+
+        def bias_reads(j, dst):
+            for g in range(4):
+                e(f"ds_read_b128 v[{dst + 4 * g}:{dst + 4 * g + 3}], {L['ba']} offset:{128 * j + 32 * g}")
+
+        def columns(i, j, g, bias):
+            """Four columns of block (i, j): z, the pairs' results, both staged."""
+            kind, base = c.acc(i, j)
+            for r in range(4):
+                src = f"v{base + 4 * g + r}"
+                if kind == "a":
+                    e(f"v_accvgpr_read_b32 v{z + r}, a{base + 4 * g + r}")
+                    src = f"v{z + r}"
+                e(f"v_fma_f32 v{z + r}, {src}, {OP['alpha']}, v{bias + 4 * g + r}")
+            if c.keep_z:
+                e(f"v_cvt_pk_bf16_f32 v{pk}, v{z}, v{z + 1}")
+                e(f"v_cvt_pk_bf16_f32 v{pk + 1}, v{z + 2}, v{z + 3}")
+                e(f"ds_write_b64 {L['zw']}, v[{pk}:{pk + 1}] offset:{64 * j + 16 * g}")
+            if not c.gate:
+                return
+            # a transcendental's result is read two instructions later at the earliest
+            for r in (0, 2):
+                e(f"v_minimum3_f32 v{z + r}, v{z + r}, {limit}, {limit}")
+            for r in (0, 2):
+                e(f"v_mul_f32 v{ex + r // 2}, {nslope}, v{z + r}")
+            for r in (1, 3):
+                e(f"v_minimum3_f32 v{z + r}, v{z + r}, {limit}, {limit}")
+            for k in (0, 1):
+                e(f"v_exp_f32 v{ex + k}, v{ex + k}")
+            for r in (1, 3):
+                e(f"v_maximum3_f32 v{z + r}, v{z + r}, {nlimit}, {nlimit}")
+            for k in (0, 1):
+                e(f"v_add_f32 v{ex + k}, 1.0, v{ex + k}")
+            for r in (1, 3):
+                e(f"v_add_f32 v{z + r}, {shift}, v{z + r}")
+            for k in (0, 1):
+                e(f"v_rcp_f32 v{ex + k}, v{ex + k}")
+            for r in (0, 2):
+                e(f"v_mul_f32 v{z + r}, v{z + r}, v{z + r + 1}")
+            for r in (0, 2):
+                e(f"v_mul_f32 v{z + r}, v{z + r}, v{ex + r // 2}")
+            e(f"v_cvt_pk_bf16_f32 v{pk + 2}, v{z}, v{z + 2}")
+            e(f"ds_write_b32 {L['ow']}, v{pk + 2} offset:{OREGION + 32 * j + 8 * g}")
+
+        def read_back(n, i, first, res, stride, wave, region):
+            """Staged rows 32 i .. + 31 to memory: (instructions, rows of one, bytes of a staged row)."""
+            parts = ((0, 8, 4), (1, 2, 16)) if n == "z" else ((0, 4, 8), (1, 1, 32))
+            pitch = ZPITCH if n == "z" else OPITCH
+            d, steps = first, []
+            for k, count, rows in parts:
+                for q in range(count):
+                    e(f"ds_read_b128 v[{d}:{d + 3}], {L[f'{n}r{k}']} offset:{region + rows * q * pitch}")
+                    steps.append((d, k, rows * q))
+                    d += 4
+            e("s_waitcnt lgkmcnt(0)")
+            for d, k, row in steps:
+                e(f"s_mul_i32 {s['T']}, {stride}, {32 * i + row}")
+                e(f"s_add_u32 {s['T']}, {s['T']}, {wave}")
+                e(f"v_add_u32 {c.vt2}, {s['T']}, {L[f'{n}g{k}']}")
+                e(f"buffer_store_dwordx4 v[{d}:{d + 3}], {c.vt2}, {res}, 0 offen" + STORE_HINT[n])
+
+        writes = 4 * (c.keep_z + c.gate)               # of a block, younger than the next block's bias
+        bias_reads(0, bset[0])
+        for i in range(c.bm):
+            for j in range(c.bn):
+                e(f"s_waitcnt lgkmcnt({writes if j else 0})")
+                if j + 1 < c.bn:
+                    bias_reads(j + 1, bset[(j + 1) % 2])
+                for g in range(4):
+                    columns(i, j, g, bset[j % 2])
+            if i + 1 < c.bm:
+                bias_reads(0, bset[0])
+            if c.keep_z:
+                read_back("z", i, data, zres, zm2, swz, 0)
+            if c.gate:
+                read_back("o", i, data, s["RC"], OP["cm2"], OP["sw_epi"], OREGION)
+        e(f"s_add_u32 {OP['vmt']}, {OP['vmt']}, {c.e_stores}")
+
+    def gate_values(self, limit, nlimit, nslope, shift):
+        s, OP, e = SGPR_K, self.OP, self.emit
+        if not self.cfg.gate:
+            return
+        e(f"v_readfirstlane_b32 {limit}, {OP['limit']}")
+        e(f"v_readfirstlane_b32 {nslope}, {OP['nslope']}")
+        e(f"v_readfirstlane_b32 {shift}, {OP['shift']}")
+        e("s_nop 1")
+        e(f"s_xor_b32 {nlimit}, {limit}, 0x80000000")
+
+
+STORE_HINT = {"z": " nt", "o": " nt"}
+
+
 def render():
     out = ["// Generated by gen_vark_wide.py; do not edit. Per-tile bodies of the wide-tile FP8 grouped",
-           "// wgrad kernels (vark_wide.h) and of the wide persistent fwd / dgrad kernel (persistent_wide.h):",
+           "// wgrad kernels (vark_wide.h) and of the wide persistent fwd / dgrad kernel (persistent_wide.h, with an",
+           "// epilogue product_wide.h):",
            "// gfx950 assembly, one inline asm statement per tile shape."]
     total = 0
-    for c in CONFIGS + SWAPPED_CONFIGS + KCONFIGS:
-        g = GenK(c) if isinstance(c, KConfig) else Gen(c)
+    for c in CONFIGS + SWAPPED_CONFIGS + KCONFIGS + KECONFIGS:
+        g = GenKE(c) if isinstance(c, KEConfig) else GenK(c) if isinstance(c, KConfig) else Gen(c)
         g.tile()
         total += len(g.lines)
         text = "\\n\\t".join(g.lines)

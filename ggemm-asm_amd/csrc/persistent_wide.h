@@ -28,6 +28,7 @@
 // lines; the line the two wave halves share goes through a joint pass).
 #pragma once
 
+#include "fused_epilogue.h"
 #include "persistent_kernel.h"
 #include "vark_wide.h"
 
@@ -45,16 +46,25 @@ constexpr int kNL = kTM * kKS / 4096, kNR = kTN * kKS / 4096;   // LDS-DMA instr
 static_assert(kLdsBytes <= 160 * 1024, "gfx950 LDS");
 static_assert(GGEMM_WIDE_NOPERANDS_pk256x320_e4m3 == 60 && GGEMM_WIDE_NOPERANDS_pk256x320_e5m2 == 60,
               "operand list of vark_wide_asm.inc");
+static_assert(GGEMM_WIDE_NOPERANDS_pe256x320_bias == 60 && GGEMM_WIDE_NOPERANDS_pe256x320_gate == 63 &&
+                  GGEMM_WIDE_NOPERANDS_pe256x320_gatekeep == 68,
+              "operand lists of vark_wide_asm.inc");
 static_assert(8 * kNT <= kSlot, "the group scan's scratch fits slot 1");
+
+// What a tile's assembly ends with: C as it is, or the epilogues of products with bias and activation
+// (gen_vark_wide.py): z = alpha acc + bias is C; swiglu of z's pairs of columns is C; the same, with z kept.
+constexpr int kPlain = 0, kBias = 1, kGate = 2, kGateKeep = 3;
 
 // Shapes the wide kernel takes (the host also checks strides and bases as for every launch).
 __host__ __device__ constexpr bool fits(int N, int K) { return N % kTN == 0 && K % 64 == 0 && K > 0; }
 
 }  // namespace pw
 
-template <bool kAE5M2>
-__device__ __forceinline__ void persistent_wide_body(const nt::Args& a, GG_LDS uint8_t* lds) {
+template <bool kAE5M2, int kMode = pw::kPlain>
+__device__ __forceinline__ void persistent_wide_body(const nt::Args& a, GG_LDS uint8_t* lds, const epi::Args& ep = {}) {
   using namespace pw;
+  static_assert(kMode == kPlain || !kAE5M2, "epilogues of the forward's format");
+  constexpr bool kGated = kMode == kGate || kMode == kGateKeep;
   GG_LDS int* s_pre = (GG_LDS int*)(lds + kPreOff);
   GG_LDS int* s_offs = (GG_LDS int*)(lds + kOffsOff);
   GG_LDS int64_t* s_scan = (GG_LDS int64_t*)(lds + kSlot);   // slot 1: no stage is issued before the scan ends
@@ -105,7 +115,7 @@ __device__ __forceinline__ void persistent_wide_body(const nt::Args& a, GG_LDS u
   const int rb_even = er * 128 + 16 * (ec ^ es);
   const int rb_odd = (8 + er) * 128 + 16 * (ec ^ (es ^ 4));
   const int gb = (er * a.stride_cm + 8 * ec) * 2;
-  const uint32_t sw_epi = (uint32_t)(128 * wm * a.stride_cm + 160 * wn) * 2u;
+  const uint32_t sw_epi = (uint32_t)(128 * wm * a.stride_cm + (kGated ? 80 : 160) * wn) * 2u;
   const uint32_t alpha_bits = __builtin_amdgcn_readfirstlane(__float_as_uint(*a.a_scale * *a.b_scale));
   const uint32_t cm2 = (uint32_t)a.stride_cm * 2u;
   const uint32_t w1k = (uint32_t)wave * 1024u;
@@ -129,11 +139,12 @@ __device__ __forceinline__ void persistent_wide_body(const nt::Args& a, GG_LDS u
     const uint32_t rat = (uint32_t)((T.rows - 1) * a.stride_am), rbt = (uint32_t)((kTN - 1) * a.stride_bn);
     const uint32_t ran = (uint32_t)((N.rows - 1) * a.stride_am);
     const uint32_t kln = has_next ? klen : 0u;
-    const uint16_t* ct = a.c + (int64_t)(T.row_base + T.m0) * a.stride_cm + T.n0;
-    const uint32_t crec = (uint32_t)(((int64_t)T.rows * a.stride_cm - T.n0) * 2);
+    const int c0n = kGated ? T.n0 / 2 : T.n0;          // first column of C
+    const uint16_t* ct = a.c + (int64_t)(T.row_base + T.m0) * a.stride_cm + c0n;
+    const uint32_t crec = (uint32_t)(((int64_t)T.rows * a.stride_cm - c0n) * 2);
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-#define GGEMM_PW_OPERANDS                                                                                       \
+#define GGEMM_PW_TILE_OPERANDS                                                                                  \
   : "+s"(c0), "+s"(nis), "+s"(vmt), "+s"(q0), "+s"(q1), "+s"(q2), "+s"(np)                                        \
   : "s"(lds_base), "s"(w1k), "s"(lo32(blt)), "s"(hi32(blt)), "s"(lo32(brt)), "s"(hi32(brt)), "s"(klen), "s"(rat), \
     "s"(rbt), "s"(lo32(bln)), "s"(hi32(bln)), "s"(lo32(brn)), "s"(hi32(brn)), "s"(kln), "s"(ran), "s"(rbt),        \
@@ -141,13 +152,39 @@ __device__ __forceinline__ void persistent_wide_body(const nt::Args& a, GG_LDS u
     "v"(voffl[1]), "v"(voffl[2]), "v"(voffl[3]), "v"(voffl[4]), "v"(voffl[5]), "v"(voffl[6]), "v"(voffl[7]),     \
     "v"(voffr[0]), "v"(voffr[1]), "v"(voffr[2]), "v"(voffr[3]), "v"(voffr[4]), "v"(voffr[5]), "v"(voffr[6]),     \
     "v"(voffr[7]), "v"(voffr[8]), "v"(voffr[9]), "v"(rd[0][0][0]), "v"(rd[0][0][1]), "v"(rd[0][1][0]),           \
-    "v"(rd[0][1][1]), "v"(rd[1][0][0]), "v"(rd[1][0][1]), "v"(rd[1][1][0]), "v"(rd[1][1][1]), "v"(ew_base),      \
-    "v"(ew_s), "v"(rb_even), "v"(rb_odd), "v"(gb)
-    if constexpr (kAE5M2)
+    "v"(rd[0][1][1]), "v"(rd[1][0][0]), "v"(rd[1][0][1]), "v"(rd[1][1][0]), "v"(rd[1][1][1])
+#define GGEMM_PW_OPERANDS GGEMM_PW_TILE_OPERANDS, "v"(ew_base), "v"(ew_s), "v"(rb_even), "v"(rb_odd), "v"(gb)
+    if constexpr (kMode != kPlain) {
+      // uniform values of the epilogue, in vector registers until it: this wave's 160 columns of the bias, the
+      // activation's options, z's tensor at the tile
+      const int item = ep.bias_f32 || ep.bias == nullptr ? 4 : 2;
+      const uint8_t* bt = (const uint8_t*)ep.bias + ((int64_t)T.g * a.N + T.n0 + 160 * wn) * item;
+      const uint32_t brec = ep.bias == nullptr ? 0u : 160u * item;
+      const int vboff = 4 * item * lane;
+      const float nslope = ep.slope * -1.44269504088896f;
+      const uint16_t* zt = ep.pre + (int64_t)(T.row_base + T.m0) * ep.stride_pre + T.n0;
+      const uint32_t zrec = (uint32_t)(((int64_t)T.rows * ep.stride_pre - T.n0) * 2);
+      const uint32_t zm2 = (uint32_t)ep.stride_pre * 2u, sw_z = (uint32_t)(128 * wm * ep.stride_pre + 160 * wn) * 2u;
+#define GGEMM_PW_BIAS "v"(vboff), "v"(lo32(bt)), "v"(hi32(bt)), "v"(brec), "v"(item == 4 ? 1 : 0)
+#define GGEMM_PW_GATE "v"(nslope), "v"(ep.limit), "v"(ep.shift)
+      if constexpr (kMode == kBias)
+        asm volatile(GGEMM_WIDE_ASM_pe256x320_bias GGEMM_PW_TILE_OPERANDS,
+                     GGEMM_PW_BIAS : GGEMM_WIDE_CLOBBERS_pe256x320_bias);
+      else if constexpr (kMode == kGate)
+        asm volatile(GGEMM_WIDE_ASM_pe256x320_gate GGEMM_PW_TILE_OPERANDS, GGEMM_PW_BIAS,
+                     GGEMM_PW_GATE : GGEMM_WIDE_CLOBBERS_pe256x320_gate);
+      else
+        asm volatile(GGEMM_WIDE_ASM_pe256x320_gatekeep GGEMM_PW_TILE_OPERANDS, GGEMM_PW_BIAS, GGEMM_PW_GATE,
+                     "v"(lo32(zt)), "v"(hi32(zt)), "v"(zrec), "v"(zm2),
+                     "v"(sw_z) : GGEMM_WIDE_CLOBBERS_pe256x320_gatekeep);
+#undef GGEMM_PW_BIAS
+#undef GGEMM_PW_GATE
+    } else if constexpr (kAE5M2)
       asm volatile(GGEMM_WIDE_ASM_pk256x320_e5m2 GGEMM_PW_OPERANDS : GGEMM_WIDE_CLOBBERS_pk256x320_e5m2);
     else
       asm volatile(GGEMM_WIDE_ASM_pk256x320_e4m3 GGEMM_PW_OPERANDS : GGEMM_WIDE_CLOBBERS_pk256x320_e4m3);
 #undef GGEMM_PW_OPERANDS
+#undef GGEMM_PW_TILE_OPERANDS
 #pragma clang diagnostic pop
     c0 = (c0 + (uint32_t)nsteps) & 1u;
     if (!has_next) break;

@@ -49,6 +49,15 @@ __global__ __launch_bounds__(ggemm::kThreads) void product_512_kernel(nt::Args a
   clear_tails<kAct>(a, e);
 }
 
+// The wide tiles, one workgroup to a CU (persistent_wide.h): bias alone, or swiglu with or without z kept.
+template <int kMode>
+__global__ __launch_bounds__(ggemm::pw::kNT) __attribute__((amdgpu_waves_per_eu(1, 1)))
+void product_wide_kernel(nt::Args a, epi::Args e) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[ggemm::pw::kLdsBytes];
+  ggemm::persistent_wide_body<false, kMode>(nt::without_tail(a), (GG_LDS uint8_t*)lds, e);
+  clear_tails<kMode == ggemm::pw::kBias ? epi::kNone : epi::kSwiglu>(a, e);
+}
+
 // f(activation) with the code as a constant.
 template <typename F>
 int with_act(int act, F f) {
@@ -89,6 +98,19 @@ int validate(const nt::Args& a, const epi::Args& e, int act, int bias_dtype) {
   return GGEMM_OK;
 }
 
+// The wide kernel's epilogue for this launch, 0 where it has none: shapes as for the plain product (32-bit offsets of
+// a stage's rows and of a tile's rows of C and z), no residual, and of the activations none, without a z of its own,
+// or swiglu.
+int wide_mode(const nt::Args& a, const epi::Args& e, int act) {
+  auto rows_fit = [](int64_t stride) { return stride * 2 * ggemm::pw::kTM < nt::kOob; };
+  if (!ggemm::pw::fits(a.N, a.K) || (int64_t)a.stride_am * ggemm::pw::kTM >= nt::kOob ||
+      (int64_t)a.stride_bn * ggemm::pw::kTN >= nt::kOob || !rows_fit(a.stride_cm) || e.residual)
+    return 0;
+  if (act == GGEMM_ACT_NONE) return e.pre ? 0 : ggemm::pw::kBias;
+  if (act != GGEMM_ACT_SWIGLU) return 0;
+  return !e.pre ? ggemm::pw::kGate : rows_fit(e.stride_pre) ? ggemm::pw::kGateKeep : 0;
+}
+
 // Rows of a unit of the gradient: few enough that the units fill the chip, 64 at most (131072 x 5760: 256 rows 810 us, 64
 // 795: more rounds of workgroups even out), but for launches of more units than a grid takes.
 constexpr int64_t kMaxUnits = 1 << 22;
@@ -122,7 +144,16 @@ int ggemm_product_fp8_bias_act(const void* a, const void* b, void* out, void* pr
   rc = device_cus(&cus);
   if (rc) return rc;
   if (M_total == 0) return GGEMM_OK;
-  const int mid = mid_preferred(G, N, K, stride_out, M_total, false, cus);
+  const int wide = wide_mode(x, e, act);
+  const int mid = mid_preferred(G, N, K, stride_out, M_total, wide != 0, cus);
+  if (!mid && wide) {
+    x.num_wg = cus;
+    auto kern = wide == ggemm::pw::kBias   ? product_wide_kernel<ggemm::pw::kBias>
+                : wide == ggemm::pw::kGate ? product_wide_kernel<ggemm::pw::kGate>
+                                           : product_wide_kernel<ggemm::pw::kGateKeep>;
+    hipLaunchKernelGGL(kern, dim3(cus), dim3(ggemm::pw::kNT), 0, (hipStream_t)stream, x, e);
+    return (int)hipGetLastError();
+  }
   return with_act(act, [&](auto code) {
     constexpr int kAct = decltype(code)::value;
     if (mid) {
