@@ -91,6 +91,7 @@ PRODUCT_EXPORTS = (
     "ggemm_product_fp8_bias_act",
     "ggemm_product_act_backward",
     "ggemm_product_act_workspace",
+    "ggemm_product_tile_rows",
 )
 
 # GGEMM_VARK_ABI_VERSION of include/ggemm_vark.h that these bindings are written for. Some exports
@@ -212,6 +213,8 @@ def load():
         getattr(lib, name).restype = ctypes.c_int
     lib.ggemm_moe_plan_workspace.argtypes = [i64, i32]
     lib.ggemm_moe_plan_workspace.restype = ctypes.c_int64
+    lib.ggemm_product_tile_rows.argtypes = [i32] * 9 + [i64, i32]
+    lib.ggemm_product_tile_rows.restype = ctypes.c_int32
     lib.ggemm_product_act_workspace.argtypes = [i64, i32, i32]
     lib.ggemm_product_act_workspace.restype = ctypes.c_int64
     _lib = lib

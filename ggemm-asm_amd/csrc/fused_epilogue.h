@@ -61,11 +61,24 @@ __device__ __forceinline__ float swiglu(float g, float u, const Args& e) {
 
 __device__ __forceinline__ float from_bf16(uint32_t low) { return __uint_as_float(low << 16); }
 
+__device__ __forceinline__ v4f unpack4(const v2i& w) {
+  return v4f{from_bf16(w[0]), __uint_as_float(w[0] & 0xffff0000u), from_bf16(w[1]), __uint_as_float(w[1] & 0xffff0000u)};
+}
+
+// The activations that are not gated.
+template <int kAct>
+__device__ __forceinline__ v4f activation(v4f z) {
+  if constexpr (kAct == kSilu || kAct == kGelu) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) z[c] *= kAct == kSilu ? sigmoid(z[c]) : gelu_cdf(z[c]);
+  }
+  return z;
+}
+
 __device__ __forceinline__ v4f load_bias(const Args& e, int64_t i) {
   if (e.bias == nullptr) return v4f{0.f, 0.f, 0.f, 0.f};
   if (e.bias_f32) return *(const v4f*)((const float*)e.bias + i);
-  const v2i w = *(const v2i*)((const uint16_t*)e.bias + i);
-  return v4f{from_bf16(w[0]), __uint_as_float(w[0] & 0xffff0000u), from_bf16(w[1]), __uint_as_float(w[1] & 0xffff0000u)};
+  return unpack4(*(const v2i*)((const uint16_t*)e.bias + i));
 }
 
 typedef float v2f __attribute__((ext_vector_type(2)));
@@ -79,6 +92,10 @@ __device__ __forceinline__ int pack(float a, float b) {
 // LDS that a wave stages 32 rows of NB blocks in, rows 16 bytes apart so that 16 of them start on different banks.
 template <int NB>
 constexpr int kRegion = 32 * (32 * NB + 16);
+
+// Stores of a wave's whole block of 16 MB x 16 NB results (of z: kNone).
+template <int kAct, int MB, int NB>
+constexpr int kStores = MB / 2 * ((32 * (kAct == kSwiglu ? NB : 2 * NB) + 63) / 64);
 
 // 32 staged rows of kChunks 16-byte chunks to dst (row 0), the first `rows` of them; chunk c is stored where c < chunks.
 template <int kChunks>
@@ -153,16 +170,8 @@ __device__ __forceinline__ void store(const v4f (&acc)[MB][NB], float alpha, con
           }
           *(GG_LDS int*)(at + 16 * j + 4 * q) = pack(x, y);
         } else {
-          v4f x = z;
-          if constexpr (kAct == kSilu || kAct == kGelu) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) x[c] = z[c] * (kAct == kSilu ? sigmoid(z[c]) : gelu_cdf(z[c]));
-          }
-          if (e.residual != nullptr) {
-            const v2i w = res[i][j];
-            x += v4f{from_bf16(w[0]), __uint_as_float(w[0] & 0xffff0000u), from_bf16(w[1]),
-                     __uint_as_float(w[1] & 0xffff0000u)};
-          }
+          v4f x = activation<kAct>(z);
+          if (e.residual != nullptr) x += unpack4(res[i][j]);
           *(GG_LDS v2i*)(at + 32 * j + 8 * q) = v2i{pack(x[0], x[1]), pack(x[2], x[3])};
         }
       }

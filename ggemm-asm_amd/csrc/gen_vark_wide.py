@@ -1496,7 +1496,7 @@ class GenKE(GenK):
         e(f"s_xor_b32 {nlimit}, {limit}, 0x80000000")
 
 
-STORE_HINT = {"z": " nt", "o": " nt"}
+STORE_HINT = {"z": " nt", "o": ""}
 
 
 def render():

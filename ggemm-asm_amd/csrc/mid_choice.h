@@ -23,7 +23,8 @@ inline int64_t mid_tiles(int rows, int G, int N, int64_t M_total) {
 // tiles, 16 more than 10 %: 13 groups, 5788 rows, N = K = 2880 75 us, 51 on the wide tiles; 15, 7007, N = 2560, K
 // = 5760 112, 85. With this rule 27 and 9 are, and 7 lose a gain of 20 % or more. For up to four groups it lost
 // as often as it gained.
-inline bool rows128_faster(int N, double M, double g, double stages, double mem, bool wide, int cus) {
+// extra: us that a large tile's epilogue takes with nothing beside it.
+inline bool rows128_faster(int N, double M, double g, double stages, double mem, bool wide, int cus, double extra) {
   constexpr int kRun = ggemm::mid::kXcdRun;
   const int tn = wide ? 320 : ggemm::wide_tiles(N, false) ? 384 : 320;
   double mid = 0, big = 0;
@@ -40,6 +41,7 @@ inline bool rows128_faster(int N, double M, double g, double stages, double mem,
     big += wide        ? 2.6 + r * (1.19 * stages + 6.1) + 0.32 * mem
            : tn == 320 ? 2.0 + r * (1.12 * stages + 6.8) + 0.29 * mem
                        : 4.6 + r * (1.27 * stages + 5.0) + 0.43 * mem;
+    big += r * extra;
   }
   return mid < 1.05 * big;
 }
@@ -54,7 +56,10 @@ inline bool rows128_faster(int N, double M, double g, double stages, double mem,
 // 32: 256 rows 149 -> 95 (64), 3072 rows 148 -> 118 (128), 6144 rows 162, mid 182 (stays); N = K = 2880,
 // G = 4: 512 rows 38 -> 14, 8192 rows 83 -> 75, 16384 rows 132, mid 153 (stays); N = 2048, K = 1424, G =
 // 7: 512 rows 25 -> 9, 5003 rows 28, mid 31 (stays); N = 512, K = 1024, G = 8: 100000 rows 92 -> 77.
-inline int mid_preferred(int G, int N, int K, int scm, int64_t M_total, bool wide, int cus) {
+// Products with an epilogue give two more numbers: extra, as above, and how far below the 128-row tiles' estimate that
+// of 64 rows has to be (product_capi.hip).
+inline int mid_preferred(int G, int N, int K, int scm, int64_t M_total, bool wide, int cus, double extra = 0,
+                         double below = 0.97) {
   if (G > ggemm::mid::kMaxGroups || M_total <= 0 || mid_tiles(64, G, N, M_total) > (1 << 22)) return 0;
   if ((int64_t)scm * 2 * 64 >= (int64_t)ggemm::nt::kOob) return 0;   // a wave's rows of C: 32-bit offsets
   const double M = (double)M_total, g = G < M ? G : M;
@@ -63,17 +68,17 @@ inline int mid_preferred(int G, int N, int K, int scm, int64_t M_total, bool wid
   auto tiles = [&](double h, double w) { return std::max(g, M / h + g / 2) * std::ceil(N / w); };
   double big;
   if (wide) {
-    big = 4 + std::ceil(tiles(256, 320) / cus) * stages * 1.85;
+    big = 4 + std::ceil(tiles(256, 320) / cus) * (stages * 1.85 + extra);
   } else {
     const int tn = ggemm::wide_tiles(N, false) ? 384 : 320;
-    big = 4 + std::ceil(tiles(192, tn) / cus) * stages * (tn == 384 ? 1.75 : 1.58) + 0.2 * mem;
+    big = 4 + std::ceil(tiles(192, tn) / cus) * (stages * (tn == 384 ? 1.75 : 1.58) + extra) + 0.2 * mem;
   }
   const double f64 = tiles(64, 128) / (2 * cus), f128 = tiles(128, 128) / (2 * cus);
   const double c64 = 4 + std::max(1.0, f64) * stages * (0.41 + 0.28 * std::min(1.0, f64)) + 0.3 * mem;
   const double c128 = 4 + std::max(1.0, f128) * stages * (0.64 + 0.42 * std::min(1.0, f128)) + 0.3 * mem;
   if (std::min(c64, c128) >= 0.92 * big) return 0;   // near the line the estimate is a few per cent off
-  if (c64 < 0.97 * c128) return 64;
-  return g <= 4 || rows128_faster(N, M, g, (K + 127) / 128, mem, wide, cus) ? 128 : 0;
+  if (c64 < below * c128) return 64;
+  return g <= 4 || rows128_faster(N, M, g, (K + 127) / 128, mem, wide, cus, extra) ? 128 : 0;
 }
 
 }  // namespace host

@@ -10,6 +10,7 @@
 #include "../../include/ggemm_product.h"
 #include "act_kernel.h"
 #include "capi_common.h"
+#include "few_rows.h"
 #include "mid_choice.h"
 
 static_assert(GGEMM_PRODUCT_MAX_GROUPS == ggemm::nt::kMaxGroups && GGEMM_PRODUCT_MAX_GROUPS == ggemm::ag::kMaxGroups &&
@@ -39,6 +40,13 @@ template <int kAct, int kBM>
 __global__ __launch_bounds__(ggemm::mid::kNT, 2) void product_mid_kernel(nt::Args a, epi::Args e) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[ggemm::mid::GemmCfg<kBM>::LdsBytes];
   ggemm::mid::gemm_body<false, kBM, 1 + kAct>(nt::without_tail(a), (GG_LDS uint8_t*)lds, e);
+  clear_tails<kAct>(a, e);
+}
+
+template <int kAct, int R, int NB>
+__global__ __launch_bounds__(ggemm::few::kNT) void product_few_kernel(nt::Args a, epi::Args e) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[ggemm::few::Cfg<R, NB>::LdsBytes];
+  ggemm::few::body<kAct, R, NB>(nt::without_tail(a), (GG_LDS uint8_t*)lds, e);
   clear_tails<kAct>(a, e);
 }
 
@@ -111,6 +119,44 @@ int wide_mode(const nt::Args& a, const epi::Args& e, int act) {
   return !e.pre ? ggemm::pw::kGate : rows_fit(e.stride_pre) ? ggemm::pw::kGateKeep : 0;
 }
 
+enum class Kernel { kFew16, kFew32, kMid64, kMid128, k512, kWide };
+struct Choice {
+  Kernel kernel;
+  int wide;                // its epilogue, of the wide kernel
+  int64_t workgroups;      // of the kernels that take a tile each: whole runs over the XCDs
+};
+
+// Few rows (few_rows.h): on average at most eight to a group, so that nearly every group is one row tile, and too few
+// mid tiles to fill the chip's two per CU, where those wait out the latency of each stage in turn; with short rows of K
+// only while all workgroups fit on the chip at once. 16 columns for each as long as that is so. Measured (us, mid tiles ->
+// this; N = 5760, K = 2880 but as said): 1 row of 1 expert 12.9 -> 6.7, 2 rows of 2 13.2 -> 8.8, 4 of 4 16.8 ->
+// 14.0, 8 of 8 26.8 -> 25.7, 64 of 8 30.3 -> 29.8, 128 of 8 30.0 -> 38.5 (stays), 32 of 22 63.2 -> 67.2 (stays);
+// 128 of 16, N = K = 4096 61.8 -> 52.8; 16 of 15, N = 1536, K = 1024 8.6 -> 9.5 (stays).
+bool few_preferred(const nt::Args& a, int64_t g) {
+  const int64_t fit = 3 * 256;                         // workgroups of 32 columns, three to a CU
+  return a.G <= ggemm::mid::kMaxGroups && a.m_total <= 8 * (g + 1) && g * ((a.N + 127) / 128) <= 512 &&
+         (a.K >= 2048 || g * ((a.N + 31) / 32) <= fit / 2);
+}
+
+// The others. Against the estimates of the plain product: the large tiles' epilogue takes 3 us a tile, 12 with z
+// kept, while the mid tiles' runs beside other workgroups' products; and 64 rows have to be 10 % better. Of 70 drawn
+// launches (1 to 40 groups, 16 to 131072 rows, features 64 to 5760) with bias, swiglu, swiglu and z, gelu and residual,
+// the choice was 1.012, 1.009, 1.008 and 1.016 times the best of the three kernels in the mean, 1.028, 1.020, 1.044 and
+// 1.023 by the plain product's numbers.
+Choice choose(const nt::Args& a, const epi::Args& e, int act, int cus) {
+  const int64_t run = ggemm::kXcds * ggemm::mid::kXcdRun, g = std::min<int64_t>(a.G, a.m_total);
+  auto runs = [&](int64_t tiles) { return (tiles + run - 1) / run * run; };
+  if (few_preferred(a, g)) {
+    const bool narrow = g * ((a.N + 15) / 16) <= 3 * 256;
+    const int64_t row_tiles = a.m_total / 16 + g, bn = narrow ? 16 : 32;
+    return {narrow ? Kernel::kFew16 : Kernel::kFew32, 0, runs(row_tiles * ((a.N + bn - 1) / bn))};
+  }
+  const int wide = wide_mode(a, e, act);
+  const int mid = mid_preferred(a.G, a.N, a.K, a.stride_cm, a.m_total, wide != 0, cus, e.pre ? 12 : 3, 0.9);
+  if (mid) return {mid == 64 ? Kernel::kMid64 : Kernel::kMid128, 0, runs(mid_tiles(mid, a.G, a.N, a.m_total))};
+  return {wide ? Kernel::kWide : Kernel::k512, wide, 0};
+}
+
 // Rows of a unit of the gradient: few enough that the units fill the chip, 64 at most (131072 x 5760: 256 rows 810 us, 64
 // 795: more rounds of workgroups even out), but for launches of more units than a grid takes.
 constexpr int64_t kMaxUnits = 1 << 22;
@@ -144,30 +190,50 @@ int ggemm_product_fp8_bias_act(const void* a, const void* b, void* out, void* pr
   rc = device_cus(&cus);
   if (rc) return rc;
   if (M_total == 0) return GGEMM_OK;
-  const int wide = wide_mode(x, e, act);
-  const int mid = mid_preferred(G, N, K, stride_out, M_total, wide != 0, cus);
-  if (!mid && wide) {
-    x.num_wg = cus;
-    auto kern = wide == ggemm::pw::kBias   ? product_wide_kernel<ggemm::pw::kBias>
-                : wide == ggemm::pw::kGate ? product_wide_kernel<ggemm::pw::kGate>
-                                           : product_wide_kernel<ggemm::pw::kGateKeep>;
+  x.num_wg = cus;
+  const Choice k = choose(x, e, act, cus);
+  if (k.kernel == Kernel::kWide) {
+    auto kern = k.wide == ggemm::pw::kBias   ? product_wide_kernel<ggemm::pw::kBias>
+                : k.wide == ggemm::pw::kGate ? product_wide_kernel<ggemm::pw::kGate>
+                                             : product_wide_kernel<ggemm::pw::kGateKeep>;
     hipLaunchKernelGGL(kern, dim3(cus), dim3(ggemm::pw::kNT), 0, (hipStream_t)stream, x, e);
     return (int)hipGetLastError();
   }
   return with_act(act, [&](auto code) {
     constexpr int kAct = decltype(code)::value;
-    if (mid) {
-      const int64_t tiles = mid_tiles(mid, G, N, M_total), run = ggemm::kXcds * ggemm::mid::kXcdRun;
-      hipLaunchKernelGGL((mid == 64 ? product_mid_kernel<kAct, 64> : product_mid_kernel<kAct, 128>),
-                         dim3((uint32_t)((tiles + run - 1) / run * run)), dim3(ggemm::mid::kNT), 0, (hipStream_t)stream,
-                         x, e);
-    } else {
-      x.num_wg = cus;
-      hipLaunchKernelGGL(product_512_kernel<kAct>, dim3(cus), dim3(ggemm::kThreads), ggemm::kDynLdsBytes,
-                         (hipStream_t)stream, x, e);
+    const dim3 grid((uint32_t)k.workgroups);
+    switch (k.kernel) {
+      case Kernel::kFew16:
+        hipLaunchKernelGGL((product_few_kernel<kAct, 1, 1>), grid, dim3(ggemm::few::kNT), 0, (hipStream_t)stream, x, e);
+        break;
+      case Kernel::kFew32:
+        hipLaunchKernelGGL((product_few_kernel<kAct, 1, 2>), grid, dim3(ggemm::few::kNT), 0, (hipStream_t)stream, x, e);
+        break;
+      case Kernel::kMid64:
+        hipLaunchKernelGGL((product_mid_kernel<kAct, 64>), grid, dim3(ggemm::mid::kNT), 0, (hipStream_t)stream, x, e);
+        break;
+      case Kernel::kMid128:
+        hipLaunchKernelGGL((product_mid_kernel<kAct, 128>), grid, dim3(ggemm::mid::kNT), 0, (hipStream_t)stream, x, e);
+        break;
+      default:
+        hipLaunchKernelGGL(product_512_kernel<kAct>, dim3(cus), dim3(ggemm::kThreads), ggemm::kDynLdsBytes,
+                           (hipStream_t)stream, x, e);
     }
     return (int)hipGetLastError();
   });
+}
+
+int32_t ggemm_product_tile_rows(int32_t G, int32_t N, int32_t K, int32_t stride_am, int32_t stride_bn,
+                                int32_t stride_out, int32_t stride_pre, int32_t act, int32_t residual, int64_t M_total,
+                                int32_t num_cus) {
+  nt::Args x{};
+  x.G = G, x.N = N, x.K = K, x.stride_am = stride_am, x.stride_bn = stride_bn, x.stride_cm = stride_out;
+  x.m_total = M_total;
+  epi::Args e{};
+  uint16_t there = 0;                                  // stands for a tensor: never read
+  e.pre = stride_pre ? &there : nullptr, e.stride_pre = stride_pre, e.residual = residual ? &there : nullptr;
+  const int rows[] = {16, 16, 64, 128, ggemm::kTileM, ggemm::pw::kTM};
+  return rows[(int)choose(x, e, act, num_cus).kernel];
 }
 
 int64_t ggemm_product_act_workspace(int64_t M_total, int32_t G, int32_t N) {

@@ -29,6 +29,14 @@ def _act(activation, slope, limit, shift):
     return ACTIVATIONS[activation], float(slope), float("inf") if limit is None else float(limit), float(shift)
 
 
+def tile_rows(G: int, N: int, K: int, M: int, activation: str | None = None, *, keep_preact: bool = False,
+              residual: bool = False, num_cus: int = 256) -> int:
+    """Rows of the output tiles of the kernel that ``grouped_gemm_fp8_bias_act`` runs on contiguous tensors of these
+    sizes: 16 (few rows), 64 or 128 (mid tiles), 192 (512 threads) or 256 (wide tiles)."""
+    return _lib.load().ggemm_product_tile_rows(G, N, K, K, K, N // 2 if activation == "swiglu" else N,
+                                               N if keep_preact else 0, ACTIVATIONS[activation], int(residual), M, num_cus)
+
+
 def _on_gpu(t: torch.Tensor, what: str):
     if t.device.type != "cuda":
         raise ValueError(f"{what} runs on a gfx950 GPU only (tensors are on {t.device})")

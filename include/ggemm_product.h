@@ -52,6 +52,13 @@ int ggemm_product_fp8_bias_act(const void* a, const void* b, void* out, void* pr
                                int32_t stride_res, int32_t act, float slope, float limit, float shift,
                                int64_t M_total, int32_t zero_tail, void* stream);
 
+/* Rows of the output tiles of the kernel that such a call runs on a device of num_cus CUs: 16 (few rows), 64 or 128
+ * (mid tiles), 192 (the 512-thread kernel) or 256 (wide tiles). stride_pre 0: no pre; residual: whether there is one.
+ * Each kernel sums a row's products in an order of its own, so a row's last bit can depend on G and M_total. */
+int32_t ggemm_product_tile_rows(int32_t G, int32_t N, int32_t K, int32_t stride_am, int32_t stride_bn,
+                                int32_t stride_out, int32_t stride_pre, int32_t act, int32_t residual, int64_t M_total,
+                                int32_t num_cus);
+
 /* dpre[r, :] = dout[r, :] * act'(pre[r, :]) (bf16, from fp32) and dbias[g, :] = sum over the group's rows of it, before
  * its rounding (fp32 [G, N] contiguous, or NULL). dout: bf16 [M_total, N or N / 2]; pre, dpre: bf16 [M_total, N]; rows of
  * dpre outside the groups become zero. act NONE: dpre may be NULL (it is dout). N a multiple of 16, row strides of 8,

@@ -1,5 +1,5 @@
-"""64-bit reference of the grouped product with bias, activation and residual, and of its gradient (torch float64 on
-the CPU, test infrastructure)."""
+"""64-bit reference of the grouped product with bias, activation and residual, and of its gradient (torch float64,
+test infrastructure)."""
 from __future__ import annotations
 
 import math
@@ -49,8 +49,8 @@ def product(a, b, scale, offs, bias, activation, residual, **options):
         pad = torch.nn.functional.pad(t.abs(), (0, -K % 64))
         return pad.view(t.shape[0], pad.shape[1] // 64, 64).amax(2)
 
-    z = torch.full((M, N), math.nan, dtype=torch.float64)
-    size = torch.zeros((M, N), dtype=torch.float64)
+    z = torch.full((M, N), math.nan, dtype=torch.float64, device=a.device)
+    size = torch.zeros((M, N), dtype=torch.float64, device=a.device)
     for g, (lo, hi) in enumerate(zip(offs, offs[1:])):
         z[lo:hi] = scale * (a[lo:hi] @ b[g].t())
         size[lo:hi] = scale * (2.0 ** -8 * tops(a[lo:hi]) @ tops(b[g]).t()

@@ -100,6 +100,35 @@ def test_more_groups_than_the_small_tiles_take(pkg):
         _check(out.cpu().double(), pre.cpu().double(), z, ref, size, activation, options, torch.zeros_like(ref))
 
 
+# rows, features, group lengths, tile rows with (bias, swiglu, swiglu and z, gelu and residual): every kernel with every
+# epilogue it has, at a group's edge and past a row tile, K of a half step and of several batches
+KERNELS = [(1, 320, 2880, [0, 1, 0], (16,) * 4), (30, 5760, 2064, [17, 0, 13], (16,) * 4), (40, 1040, 8208, [9, 11, 3, 16, 1], (16,) * 4),
+           (150, 1040, 144, [80, 70], (64,) * 4), (2500, 3200, 192, [1000, 0, 1499], (128,) * 4),
+           (20000, 2560, 320, [256, 19001, 0, 700], (256, 256, 128, 192)), (16000, 1280, 1088, [15999], (256, 256, 256, 128)),
+           (20000, 2096, 2880, [5000, 4999, 0, 10001], (192,) * 4)]
+
+
+@pytest.mark.parametrize("M,N,K,lens,rows", KERNELS)
+def test_every_kernel(pkg, M, N, K, lens, rows):
+    """On the GPU's own fp64 (these are larger than the CPU's oracle takes quickly): the same formulas and bounds."""
+    from ggemm_asm_amd import product
+    a, b, sa, sb, offs, gen = _inputs(M, N, K, lens, M + N)
+    G = len(lens)
+    bias = torch.randn((G, N), generator=gen).to(torch.bfloat16).cuda()
+    cases = [(None, {}, False, False), ("swiglu", GATE, False, False), ("swiglu", GATE, True, False), ("gelu", {}, False, True)]
+    res = torch.randn((M, N), generator=gen).to(torch.bfloat16).cuda()
+    a, b, dev_offs = a.cuda(), b.cuda(), torch.tensor(offs).cuda()
+    for (activation, options, keep, residual), want in zip(cases, rows):
+        assert product.tile_rows(G, N, K, M, activation, keep_preact=keep, residual=residual) == want
+        got = pkg.grouped_gemm_fp8_bias_act(a, b, torch.tensor(sa).cuda(), torch.tensor(sb).cuda(), dev_offs, bias, activation,
+                                            res if residual else None, keep_preact=keep, zero_tail=True, **options)
+        out, pre = got if keep else (got, None)
+        z, ref, size = orx.product(a, b, sa * sb, offs, bias, activation, res if residual else None, **options)
+        _check(out.double(), None if pre is None else pre.double(), z, ref, size, activation, options,
+               res.double().abs() if residual else torch.zeros_like(ref))
+        assert not out[offs[-1]:].any() and (pre is None or not pre[offs[-1]:].any())
+
+
 @pytest.mark.parametrize("activation,options", ACTS)
 def test_clamped_and_extreme_values(pkg, activation, options):
     """z far outside the activations' bends and the clamp: nothing overflows on the way."""

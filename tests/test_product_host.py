@@ -70,6 +70,19 @@ def test_workspace_holds_every_unit(pkg):
             assert f(M, G, 64) % 64 == 0 and units >= max(1, min(G, M)) and units >= M // 256 // 4
 
 
+@pytest.mark.parametrize("args,kw,rows", [
+    ((32, 5760, 2880, 4, "swiglu"), {}, 16), ((8, 5760, 2880, 64, "gelu"), {}, 16), ((8, 5760, 2880, 128, "gelu"), {}, 64),
+    ((32, 5760, 2880, 256, "swiglu"), {}, 64), ((64, 1536, 1024, 64), {}, 64), ((7, 2048, 1424, 5003, "gelu"), dict(residual=True), 128),
+    ((32, 5760, 2880, 131072, "swiglu"), {}, 256), ((32, 5760, 2880, 131072, "swiglu"), dict(keep_preact=True), 256),
+    ((32, 5760, 2880, 131072), {}, 256), ((32, 5760, 2880, 131072), dict(keep_preact=True), 192),
+    ((32, 5760, 2880, 131072, "swiglu"), dict(residual=True), 192), ((32, 5760, 2880, 131072, "silu"), {}, 192),
+    ((32, 5744, 2880, 131072, "swiglu"), {}, 192), ((300, 352, 96, 300), {}, 192)])
+def test_kernel_choice(pkg, args, kw, rows):
+    """The kernel by sizes, activation and what else the epilogue does; more than 256 groups only on the large tiles."""
+    from ggemm_asm_amd import product
+    assert product.tile_rows(*args, **kw) == rows
+
+
 @pytest.fixture
 def anywhere(pkg, monkeypatch):
     from ggemm_asm_amd import _lib, product
