@@ -112,10 +112,10 @@ __device__ __forceinline__ void grad8(const v4i& z8, const v4i& d8, const epi::A
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float g = epi::at_most(z[2 * i], e.limit), u = epi::within(z[2 * i + 1], e.limit);
-      const float s = epi::sigmoid(e.slope * g), gs = g * s;
+      const float s = epi::sigmoid2(e.nslope * g), gs = g * s;
       const float dg = d[i] * (u + e.shift) * (s + e.slope * gs * (1.f - s));
       out[2 * i] = z[2 * i] > e.limit ? 0.f : dg;
-      out[2 * i + 1] = z[2 * i + 1] > e.limit || z[2 * i + 1] < -e.limit ? 0.f : d[i] * gs;
+      out[2 * i + 1] = fabsf(z[2 * i + 1]) > e.limit ? 0.f : d[i] * gs;
     }
   } else {
 #pragma unroll

@@ -23,13 +23,15 @@ struct Args {
   const uint16_t* residual;
   int stride_res;
   float slope, limit, shift;
+  float nslope;            // -log2(e) slope: sigmoid(slope g) = 1 / (1 + 2^(nslope g))
 };
 
-// 1 / (1 + e^-x). The hardware's exp2 and reciprocal, each within an ulp; the rounding of x log2(e) adds
-// |x| 2^-24: against the 2^-8 of the bf16 results, and 2e-7 in the fp32 sums of the bias' gradient.
-__device__ __forceinline__ float sigmoid(float x) {
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * -1.44269504088896f));
-}
+// 1 / (1 + 2^x). The hardware's exp2 and reciprocal, each within an ulp; the rounding of x = -log2(e) y adds |y| 2^-24:
+// against the 2^-8 of the bf16 results, and 2e-7 in the fp32 sums of the bias' gradient.
+constexpr float kLog2e = 1.44269504088896f;
+__device__ __forceinline__ float sigmoid2(float x) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x)); }
+__device__ __forceinline__ float sigmoid(float x) { return sigmoid2(x * -kLog2e); }
+
 // The normal distribution's cdf and e^(-x^2 / 2), by Hastings' rational approximation of the error function (Abramowitz
 // and Stegun, Handbook of Mathematical Functions, 7.1.26; absolute error 1.5e-7): erfc(y) = t (a1 + t (a2 + t (a3 +
 // t (a4 + t a5)))) e^(-y^2), t = 1 / (1 + p y), y = |x| / sqrt 2. Half of erfc is the cdf of -|x|, so small values of the
@@ -50,13 +52,15 @@ __device__ __forceinline__ float gelu_cdf(float x) {
   return normal_cdf(x, &gauss);
 }
 
-// NaN stays NaN in both (a comparison with it is false).
-__device__ __forceinline__ float at_most(float x, float m) { return x > m ? m : x; }
-__device__ __forceinline__ float within(float x, float m) { return x > m ? m : x < -m ? -m : x; }
+// NaN stays NaN in both.
+__device__ __forceinline__ float at_most(float x, float m) { return __builtin_elementwise_minimum(x, m); }
+__device__ __forceinline__ float within(float x, float m) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, m), -m);
+}
 
 __device__ __forceinline__ float swiglu(float g, float u, const Args& e) {
   g = at_most(g, e.limit);
-  return g * sigmoid(e.slope * g) * (within(u, e.limit) + e.shift);
+  return g * sigmoid2(e.nslope * g) * (within(u, e.limit) + e.shift);
 }
 
 __device__ __forceinline__ float from_bf16(uint32_t low) { return __uint_as_float(low << 16); }

@@ -13,7 +13,7 @@
 #include "route_kernel.h"
 
 static_assert(GGEMM_MOE_MAX_EXPERTS == ggemm::rt::kMaxExperts && GGEMM_MOE_MAX_TOP_K == ggemm::rt::kMaxTopK &&
-                  GGEMM_MOE_MAX_GROUPS == ggemm::ex::kMaxGroups,
+                  GGEMM_MOE_MAX_GROUPS == ggemm::ex::kMaxGroups && GGEMM_MOE_PLAN_ALONE == ggemm::ex::kPlanAlone,
               "header and kernels agree");
 
 namespace {
@@ -152,12 +152,12 @@ int64_t ggemm_moe_plan_workspace(int64_t n, int32_t G) {
   if (n < 0 || n > kMaxRows || G <= 0 || G > ex::kMaxGroups) return 0;
   int per = 0;
   const int blocks = plan_blocks(n, &per);
-  return blocks > 1 ? (int64_t)blocks * G : 1;
+  return blocks > 1 ? (int64_t)blocks * G : 0;
 }
 
 int ggemm_moe_plan(const int32_t* experts, int64_t n, int32_t G, int64_t* group_offs, int32_t* slots,
                    int32_t* workspace, void* stream) {
-  if (!group_offs || !workspace || (n > 0 && (!experts || !slots))) return GGEMM_E_NULL;
+  if (!group_offs || (n > ex::kPlanAlone && !workspace) || (n > 0 && (!experts || !slots))) return GGEMM_E_NULL;
   if (n < 0 || n > kMaxRows || G <= 0 || G > ex::kMaxGroups) return GGEMM_E_SHAPE;
   if (!aligned(experts, 4) || !aligned(slots, 4) || !aligned(workspace, 4) || !aligned(group_offs, 8))
     return GGEMM_E_ALIGN;

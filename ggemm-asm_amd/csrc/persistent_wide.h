@@ -161,12 +161,11 @@ __device__ __forceinline__ void persistent_wide_body(const nt::Args& a, GG_LDS u
       const uint8_t* bt = (const uint8_t*)ep.bias + ((int64_t)T.g * a.N + T.n0 + 160 * wn) * item;
       const uint32_t brec = ep.bias == nullptr ? 0u : 160u * item;
       const int vboff = 4 * item * lane;
-      const float nslope = ep.slope * -1.44269504088896f;
       const uint16_t* zt = ep.pre + (int64_t)(T.row_base + T.m0) * ep.stride_pre + T.n0;
       const uint32_t zrec = (uint32_t)(((int64_t)T.rows * ep.stride_pre - T.n0) * 2);
       const uint32_t zm2 = (uint32_t)ep.stride_pre * 2u, sw_z = (uint32_t)(128 * wm * ep.stride_pre + 160 * wn) * 2u;
 #define GGEMM_PW_BIAS "v"(vboff), "v"(lo32(bt)), "v"(hi32(bt)), "v"(brec), "v"(item == 4 ? 1 : 0)
-#define GGEMM_PW_GATE "v"(nslope), "v"(ep.limit), "v"(ep.shift)
+#define GGEMM_PW_GATE "v"(ep.nslope), "v"(ep.limit), "v"(ep.shift)
       if constexpr (kMode == kBias)
         asm volatile(GGEMM_WIDE_ASM_pe256x320_bias GGEMM_PW_TILE_OPERANDS,
                      GGEMM_PW_BIAS : GGEMM_WIDE_CLOBBERS_pe256x320_bias);

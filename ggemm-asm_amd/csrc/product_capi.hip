@@ -184,7 +184,7 @@ int ggemm_product_fp8_bias_act(const void* a, const void* b, void* out, void* pr
   nt::Args x{(const uint8_t*)a, (const uint8_t*)b, (uint16_t*)out, a_scale, b_scale, group_offs, G, N, K,
              stride_am, stride_bg, stride_bn, stride_out, 1, M_total, zero_tail};
   const epi::Args e{(uint16_t*)pre, stride_pre, bias, bias_dtype == GGEMM_IN_F32, (const uint16_t*)residual,
-                    stride_res, slope, limit, shift};
+                    stride_res, slope, limit, shift, slope * -epi::kLog2e};
   int rc = validate(x, e, act, bias_dtype);
   if (rc) return rc;
   rc = device_cus(&cus);
@@ -262,7 +262,7 @@ int ggemm_product_act_backward(const void* dout, const void* pre, const int64_t*
   const int64_t units = units_of(M_total, G, N);
   if (units * strips > 2 * kMaxUnits) return GGEMM_E_SHAPE;
   const ag::Args a{(const uint16_t*)dout, (const uint16_t*)pre, group_offs, G, N, stride_dout, stride_pre,
-                   epi::Args{nullptr, 0, nullptr, 0, nullptr, 0, slope, limit, shift}, M_total, unit_rows(M_total, N),
+                   epi::Args{nullptr, 0, nullptr, 0, nullptr, 0, slope, limit, shift, slope * -epi::kLog2e}, M_total, unit_rows(M_total, N),
                    (int)units, strips, (N / 8 + strips - 1) / strips, (uint16_t*)dpre, stride_dpre, dbias, workspace};
   if (M_total > 0 && (dpre || dbias)) {
     rc = with_act(act, [&](auto code) {

@@ -24,6 +24,7 @@ _SCORES = {"softmax": 0, "sigmoid": 1}
 MAX_EXPERTS = 1024      # of a router
 MAX_TOP_K = 64
 MAX_GROUPS = 2047       # of a plan
+_PLAN_ALONE = 2048      # GGEMM_MOE_PLAN_ALONE: plans up to so many choices need no workspace
 
 
 class DispatchPlan(NamedTuple):
@@ -144,9 +145,11 @@ def plan_dispatch(experts: torch.Tensor, num_experts: int) -> DispatchPlan:
     dev, n = experts.device, experts.numel()
     offs = torch.empty(num_experts + 1, dtype=torch.int64, device=dev)
     slots = torch.empty_like(experts)
-    ws = torch.empty(_lib.load().ggemm_moe_plan_workspace(n, num_experts), dtype=torch.int32, device=dev)
+    ws = None
+    if n > _PLAN_ALONE:
+        ws = torch.empty(_lib.load().ggemm_moe_plan_workspace(n, num_experts), dtype=torch.int32, device=dev)
     _lib.launch("ggemm_moe_plan", dev, num_experts, experts.data_ptr(), n, num_experts, offs.data_ptr(),
-                slots.data_ptr(), ws.data_ptr())
+                slots.data_ptr(), None if ws is None else ws.data_ptr())
     return DispatchPlan(offs, slots)
 
 

@@ -35,6 +35,7 @@ extern "C" {
 #define GGEMM_MOE_MAX_EXPERTS 1024   /* of a router */
 #define GGEMM_MOE_MAX_TOP_K 64
 #define GGEMM_MOE_MAX_GROUPS 2047    /* of a plan, as the grouped products take */
+#define GGEMM_MOE_PLAN_ALONE 2048    /* choices that one workgroup orders by itself */
 
 /* The top_k experts of each token and their weights, from router logits [T, E] (bf16 or fp32, row
  * stride `stride` >= E).
@@ -61,7 +62,7 @@ int ggemm_moe_route_backward(const float* dweights, const void* logits, int32_t 
                              const int32_t* experts, void* dlogits, void* stream);
 
 /* group_offs [G + 1] int64 and slots [n] int32 of n choices' experts (int32). workspace:
- * ggemm_moe_plan_workspace(n, G) 32-bit words. n < 2^31 - 256. */
+ * ggemm_moe_plan_workspace(n, G) 32-bit words; none (it may be NULL) up to GGEMM_MOE_PLAN_ALONE choices. n < 2^31 - 256. */
 int ggemm_moe_plan(const int32_t* experts, int64_t n, int32_t G, int64_t* group_offs, int32_t* slots,
                    int32_t* workspace, void* stream);
 int64_t ggemm_moe_plan_workspace(int64_t n, int32_t G);

@@ -59,7 +59,7 @@ def _plan(lib, **kw):
     return lib.ggemm_moe_plan(*a.values(), None)
 
 
-@pytest.mark.parametrize("kw,rc", [(dict(e=0), -1), (dict(offs=0), -1), (dict(slots=0), -1), (dict(ws=0), -1),
+@pytest.mark.parametrize("kw,rc", [(dict(e=0), -1), (dict(offs=0), -1), (dict(slots=0), -1), (dict(ws=0, n=2049), -1),
                                    (dict(n=-1), -2), (dict(n=2 ** 31), -2), (dict(G=0), -2), (dict(G=2048), -2),
                                    (dict(offs=FAKE + 4), -4), (dict(slots=FAKE + 2), -4)])
 def test_plan_validation(pkg, kw, rc):
@@ -69,8 +69,9 @@ def test_plan_validation(pkg, kw, rc):
 def test_plan_workspace(pkg):
     f = pkg.load_library().ggemm_moe_plan_workspace
     assert f(-1, 8) == 0 and f(10, 0) == 0 and f(10, 2048) == 0
-    for n in (0, 1, 2048, 2049, 131072, 131073, 2 ** 31 - 256):
-        assert 1 <= f(n, 37) <= 256 * 37
+    for n in (2049, 131072, 131073, 2 ** 31 - 256):
+        assert 37 <= f(n, 37) <= 256 * 37
+    assert f(0, 37) == f(2048, 37) == 0
 
 
 def _dispatch(lib, **kw):
