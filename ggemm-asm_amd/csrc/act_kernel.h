@@ -164,13 +164,13 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
     for (int u = 0; u < kUnroll; ++u) {
       z[u] = d[u] = v4i{0, 0, 0, 0};
       if (r + u >= r1) continue;
-      if constexpr (kAct != epi::kNone) z[u] = *(const v4i*)(a.pre + (r + u) * a.stride_pre + n);
+      if constexpr (kAct != epi::kNone) z[u] = __builtin_nontemporal_load((const v4i*)(a.pre + (r + u) * a.stride_pre + n));
       if constexpr (kAct == epi::kSwiglu) {
-        const v2i h = *(const v2i*)(a.dout + (r + u) * a.stride_dout + no);
+        const v2i h = __builtin_nontemporal_load((const v2i*)(a.dout + (r + u) * a.stride_dout + no));
         d[u][0] = h[0];
         d[u][1] = h[1];
       } else {
-        d[u] = *(const v4i*)(a.dout + (r + u) * a.stride_dout + no);
+        d[u] = __builtin_nontemporal_load((const v4i*)(a.dout + (r + u) * a.stride_dout + no));
       }
     }
 #pragma unroll

@@ -170,9 +170,18 @@ __device__ __forceinline__ void clear_rows(uint8_t* rows, int64_t stride, int64_
     for (int64_t c = lane * (int64_t)sizeof(W); c < bytes; c += 64 * sizeof(W)) *(W*)(rows + r * stride + c) = W{};
 }
 
-// A wave per token: kUnroll words of the row in each lane, stored k times; non-temporally, since the rows are k times
-// what was read and are next read by another launch (131072 fp8 rows of 2880 from 32768 tokens: 125 -> 106 us).
-template <int kBytes>
+// What is written once and next read by another launch: past the caches where rows are whole lines (131072 fp8 rows of 2880 in
+// 2944 from 32768 tokens 125 -> 106 us); else through them, which put together the lines that two stores share (30018 bf16
+// rows of 1424: 19.2 us, 21.8 past them).
+template <bool kLines, typename W>
+__device__ __forceinline__ void store_once(W w, W* p) {
+  if constexpr (kLines) __builtin_nontemporal_store(w, p);
+  else *p = w;
+}
+
+// A wave per token: kUnroll words of the row in each lane, stored k times.
+// kLines: rows start on 128-byte lines.
+template <int kBytes, bool kLines>
 __global__ __launch_bounds__(kThreads) void dispatch_kernel(CopyArgs a) {
   using W = typename Word<kBytes>::type;
   constexpr int kUnroll = 4;
@@ -193,7 +202,7 @@ __global__ __launch_bounds__(kThreads) void dispatch_kernel(CopyArgs a) {
         uint8_t* dst = a.rows + s * a.rows_stride;
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
-          if (c0 + 64 * kBytes * u < a.bytes) __builtin_nontemporal_store(v[u], (W*)(dst + c0 + 64 * kBytes * u));
+          if (c0 + 64 * kBytes * u < a.bytes) store_once<kLines>(v[u], (W*)(dst + c0 + 64 * kBytes * u));
       }
     }
   }
@@ -211,14 +220,11 @@ __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
 template <typename T, int N>
 struct Vec {
   float f[N];
-  // kOnce: the element is read by no other wave
-  template <bool kOnce = false>
-  __device__ __forceinline__ void load(const T* p) {
+  typedef typename Word<N * sizeof(T)>::type Raw;
+  __device__ __forceinline__ void set(Raw w) {
     if constexpr (N == 1) {
-      if constexpr (sizeof(T) == 2) f[0] = __uint_as_float((uint32_t)*(const uint16_t*)p << 16);
-      else f[0] = *(const float*)p;
+      f[0] = __uint_as_float(sizeof(T) == 2 ? (uint32_t)w << 16 : (uint32_t)w);
     } else {
-      const v4u w = kOnce ? __builtin_nontemporal_load((const v4u*)p) : *(const v4u*)p;
       if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -231,6 +237,7 @@ struct Vec {
       }
     }
   }
+  template <bool kLines>
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (N == 1) {
       if constexpr (sizeof(T) == 2) *(uint16_t*)p = __builtin_bit_cast(uint16_t, (__bf16)f[0]);
@@ -241,8 +248,23 @@ struct Vec {
       for (int i = 0; i < 4; ++i)
         if constexpr (sizeof(T) == 2) w[i] = bf16_pair(f[2 * i], f[2 * i + 1]);
         else w[i] = __float_as_uint(f[i]);
-      __builtin_nontemporal_store(w, (v4u*)p);
+      store_once<kLines>(w, (v4u*)p);
     }
+  }
+};
+
+// A row that may be there or not, as a buffer: loads from none give zeros, so that the loads of several rows are issued
+// without a branch between them. Non-temporal: a row is read by one wave.
+struct Row {
+  __amdgpu_buffer_rsrc_t r;
+  __device__ __forceinline__ Row(const void* p, int bytes)
+      : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000)) {}
+  // kBytes = 16, 4 or 2 at byte `at` of the row
+  template <int kBytes>
+  __device__ __forceinline__ typename Word<kBytes>::type load(int at) const {
+    if constexpr (kBytes == 16) return __builtin_bit_cast(v4u, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 2));
+    if constexpr (kBytes == 4) return __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 2);
+    if constexpr (kBytes == 2) return __builtin_amdgcn_raw_buffer_load_b16(r, at, 0, 2);
   }
 };
 
@@ -258,52 +280,54 @@ struct CombineArgs {
   int H;
   void* out;
   int64_t out_stride;
+  int parts;               // waves that share a token's columns
 };
 
-// A wave per token, N elements of the row per lane and step; the rows of four choices are loaded before
-// the first is added. Non-temporal loads and stores: each byte passes once (131072 bf16 rows of 2880 into 32768 tokens with
-// a residual: 235 us with ordinary ones, 223 with ordinary loads, 217).
-template <typename T, int N>
+// A wave per token and part of its columns, N elements of the row per lane and step; the rows of four choices are loaded
+// before the first is added. Non-temporal loads and stores: each byte passes once (131072 bf16 rows of 2880 into 32768
+// tokens with a residual: 235 us with ordinary ones, 223 with ordinary loads, 217).
+template <typename T, int N, bool kLines>
 __global__ __launch_bounds__(kThreads) void combine_kernel(CombineArgs a) {
+  constexpr int kJ = 4;
   const int lane = threadIdx.x & 63;
   const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t waves = (int64_t)gridDim.x * kWaves;
-  for (int64_t t = wave; t < a.T; t += waves) {
+  using V = Vec<T, N>;
+  constexpr int kBytes = N * sizeof(T);
+  const int bytes = a.H * (int)sizeof(T);
+  for (int64_t u = wave; u < a.T * a.parts; u += waves) {
+    const int64_t t = a.parts == 1 ? u : u / a.parts;
+    const int part = (int)(u - t * a.parts);
     const int* slots = a.slots + t * a.k;
-    for (int c = lane * N; c < a.H; c += 64 * N) {
+    const Row res(a.residual ? (const T*)a.residual + t * a.residual_stride : (const T*)a.y, a.residual ? bytes : 0);
+    for (int c = (64 * part + lane) * N; c < a.H; c += 64 * N * a.parts) {
+      const typename V::Raw first = res.load<kBytes>(c * (int)sizeof(T));
       float acc[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = 0.f;
-      for (int j0 = 0; j0 < a.k; j0 += 4) {
-        Vec<T, N> v[4];
-        float w[4];
-        bool use[4];
+      for (int j0 = 0; j0 < a.k; j0 += kJ) {
+        typename V::Raw raw[kJ];
+        float w[kJ];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < kJ; ++j) {
           const int s = j0 + j < a.k ? slots[j0 + j] : -1;
-          use[j] = s >= 0 && s < a.M;
-          if (use[j]) {
-            v[j].template load<true>((const T*)a.y + s * a.y_stride + c);
-            w[j] = a.weights ? a.weights[t * a.k + j0 + j] : 1.f;
-          }
+          const bool use = s >= 0 && s < a.M;
+          w[j] = !use ? 0.f : a.weights ? a.weights[t * a.k + j0 + j] : 1.f;
+          raw[j] = Row((const T*)a.y + (use ? s : 0) * a.y_stride, use ? bytes : 0).load<kBytes>(c * (int)sizeof(T));
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (use[j]) {
+        for (int j = 0; j < kJ; ++j) {
+          V v;
+          v.set(raw[j]);
 #pragma unroll
-            for (int i = 0; i < N; ++i) acc[i] = fmaf(w[j], v[j].f[i], acc[i]);
-          }
+          for (int i = 0; i < N; ++i) acc[i] = fmaf(w[j], v.f[i], acc[i]);
+        }
       }
-      Vec<T, N> r;
-      if (a.residual) {
-        r.template load<true>((const T*)a.residual + t * a.residual_stride + c);
+      V r;
+      r.set(first);
 #pragma unroll
-        for (int i = 0; i < N; ++i) r.f[i] += acc[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) r.f[i] = acc[i];
-      }
-      r.store((T*)a.out + t * a.out_stride + c);
+      for (int i = 0; i < N; ++i) r.f[i] += acc[i];
+      r.template store<kLines>((T*)a.out + t * a.out_stride + c);
     }
   }
 }
@@ -324,39 +348,60 @@ struct CombineBackArgs {
   float* dweights;
 };
 
-// A wave per token; the token's gradient is read again for each choice (from cache).
-template <typename T, int N>
+// A wave per token, eight choices at a time: their rows are loaded before the first is used, the token's gradient once
+// for all eight.
+template <typename T, int N, bool kLines>
 __global__ __launch_bounds__(kThreads) void combine_backward_kernel(CombineBackArgs a) {
+  constexpr int kJ = 8;
   const int lane = threadIdx.x & 63;
   const int64_t wave = (int64_t)blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t waves = (int64_t)gridDim.x * kWaves;
+  using V = Vec<T, N>;
+  constexpr int kBytes = N * sizeof(T);
+  const int bytes = a.H * (int)sizeof(T);
   for (int64_t t = wave; t < a.T; t += waves) {
-    const T* dout = (const T*)a.dout + t * a.dout_stride;
-    for (int j = 0; j < a.k; ++j) {
-      const int s = a.slots[t * a.k + j];
-      const bool use = s >= 0 && s < a.M;
-      float dot = 0.f;
-      if (use) {
-        const float w = a.weights ? a.weights[t * a.k + j] : 1.f;
-        for (int c = lane * N; c < a.H; c += 64 * N) {
-          Vec<T, N> d, y;
-          d.load(dout + c);
-          if (a.dweights) {
-            y.template load<true>((const T*)a.y + s * a.y_stride + c);
+    const Row dout((const T*)a.dout + t * a.dout_stride, bytes);
+    for (int j0 = 0; j0 < a.k; j0 += kJ) {
+      int slot[kJ];
+      float w[kJ], dot[kJ];
 #pragma unroll
-            for (int i = 0; i < N; ++i) dot = fmaf(d.f[i], y.f[i], dot);
-          }
-          if (a.dy) {
+      for (int j = 0; j < kJ; ++j) {
+        const int s = j0 + j < a.k ? a.slots[t * a.k + j0 + j] : -1;
+        slot[j] = s < a.M ? s : -1;
+        w[j] = a.weights && j0 + j < a.k ? a.weights[t * a.k + j0 + j] : 1.f;
+        dot[j] = 0.f;
+      }
+      for (int c = lane * N; c < a.H; c += 64 * N) {
+        const typename V::Raw rd = dout.load<kBytes>(c * (int)sizeof(T));
+        typename V::Raw ry[kJ];
 #pragma unroll
-            for (int i = 0; i < N; ++i) d.f[i] *= w;
-            d.store((T*)a.dy + s * a.dy_stride + c);
+        for (int j = 0; j < kJ; ++j)
+          ry[j] = (slot[j] >= 0 && a.dweights ? Row((const T*)a.y + slot[j] * a.y_stride, bytes) : Row(a.dout, 0))
+                      .load<kBytes>(c * (int)sizeof(T));
+        V d;
+        d.set(rd);
+#pragma unroll
+        for (int j = 0; j < kJ; ++j) {
+          V y;
+          y.set(ry[j]);
+#pragma unroll
+          for (int i = 0; i < N; ++i) dot[j] = fmaf(d.f[i], y.f[i], dot[j]);
+          if (a.dy && slot[j] >= 0) {
+            V g;
+#pragma unroll
+            for (int i = 0; i < N; ++i) g.f[i] = w[j] * d.f[i];
+            g.template store<kLines>((T*)a.dy + slot[j] * a.dy_stride + c);
           }
         }
       }
       if (a.dweights) {
 #pragma unroll
-        for (int d = 32; d > 0; d >>= 1) dot += __shfl_xor(dot, d, 64);
-        if (lane == 0) a.dweights[t * a.k + j] = dot;
+        for (int j = 0; j < kJ; ++j) {
+          if (j0 + j >= a.k) continue;
+#pragma unroll
+          for (int d = 32; d > 0; d >>= 1) dot[j] += __shfl_xor(dot[j], d, 64);
+          if (lane == 0) a.dweights[t * a.k + j0 + j] = slot[j] >= 0 ? dot[j] : 0.f;
+        }
       }
     }
   }

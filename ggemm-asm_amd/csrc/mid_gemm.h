@@ -93,7 +93,12 @@ __device__ __forceinline__ void gemm_body(const nt::Args& a, GG_LDS uint8_t* lds
     for (int j = 0; j < C::PerWave; ++j) {
       const bool lhs = j < C::LhsJ;
       const int voff = lhs ? va + 32 * j * a.stride_am : vb + 32 * (j - C::LhsJ) * a.stride_bn;
-      dma16(lhs ? ra : rb, base + 4096 * j, dead ? (int)kOob : voff);
+      // a product's weights that no other row tile reads pass the caches by: 256 rows of 32 experts 5760 x 2880 93.0 ->
+      // 84.3 us, 6.3 TB/s of weights
+      if (kEpi != 0 && !lhs && n_tm == 1)
+        dma16<true>(rb, base + 4096 * j, dead ? (int)kOob : voff);
+      else
+        dma16(lhs ? ra : rb, base + 4096 * j, dead ? (int)kOob : voff);
     }
   };
 

@@ -23,6 +23,7 @@ using ggemm::host::device_cus;
 namespace rt = ggemm::rt;
 namespace ex = ggemm::ex;
 
+constexpr int kMaxWidth = 1 << 28;                       // elements of a row: 32-bit byte offsets
 constexpr int64_t kMaxRows = (int64_t(1) << 31) - 256;   // rows and choices: 32-bit numbers
 
 int check_logits(const void* logits, int dtype, int64_t T, int E, int64_t stride, int k, int score) {
@@ -190,11 +191,12 @@ int ggemm_moe_dispatch(const void* x, int64_t row_bytes, int64_t x_stride, int64
   if (M == 0) return GGEMM_OK;
   const ex::CopyArgs a{(const uint8_t*)x, row_bytes, x_stride, T, top_k, slots, group_offs, G, (uint8_t*)rows,
                        rows_stride, M};
-  auto kern = ex::dispatch_kernel<1>;
+  const bool lines = (bits(rows) | (uint64_t)rows_stride) % 128 == 0;
+  auto kern = ex::dispatch_kernel<1, false>;
   switch (common_bytes(bits(x) | bits(rows) | (uint64_t)(row_bytes | x_stride | rows_stride))) {
-    case 16: kern = ex::dispatch_kernel<16>; break;
-    case 4: kern = ex::dispatch_kernel<4>; break;
-    case 2: kern = ex::dispatch_kernel<2>; break;
+    case 16: kern = lines ? ex::dispatch_kernel<16, true> : ex::dispatch_kernel<16, false>; break;
+    case 4: kern = ex::dispatch_kernel<4, false>; break;
+    case 2: kern = ex::dispatch_kernel<2, false>; break;
   }
   hipLaunchKernelGGL(kern, dim3(row_grid(std::max(T, M / 8), cus)), dim3(ex::kThreads), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
@@ -207,7 +209,7 @@ int ggemm_moe_combine(const void* y, int32_t dtype, int64_t y_stride, int64_t M,
   if (rc) return rc;
   if (!y || !out) return GGEMM_E_NULL;
   if (dtype != GGEMM_IN_BF16 && dtype != GGEMM_IN_F32) return GGEMM_E_FORMAT;
-  if (H <= 0) return GGEMM_E_SHAPE;
+  if (H <= 0 || H > kMaxWidth) return GGEMM_E_SHAPE;
   if (y_stride < H || out_stride < H || (residual && residual_stride < H)) return GGEMM_E_STRIDE;
   const int item = dtype == GGEMM_IN_BF16 ? 2 : 4;
   if (!aligned(y, item) || !aligned(out, item) || !aligned(residual, item) || !aligned(weights, 4))
@@ -216,13 +218,22 @@ int ggemm_moe_combine(const void* y, int32_t dtype, int64_t y_stride, int64_t M,
   rc = device_cus(&cus);
   if (rc) return rc;
   if (T == 0) return GGEMM_OK;
-  const ex::CombineArgs a{y, y_stride, M, slots, T, top_k, weights, residual, residual_stride, H, out, out_stride};
+  ex::CombineArgs a{y, y_stride, M, slots, T, top_k, weights, residual, residual_stride, H, out, out_stride, 1};
+  const bool lines = (bits(out) | (uint64_t)(item * out_stride)) % 128 == 0;
   const uint64_t all = bits(y) | bits(out) | bits(residual) |
                        (uint64_t)item * (uint64_t)(y_stride | out_stride | (residual ? residual_stride : 0) | H);
   const bool wide = common_bytes(all) == 16;
-  auto kern = dtype == GGEMM_IN_BF16 ? (wide ? ex::combine_kernel<uint16_t, 8> : ex::combine_kernel<uint16_t, 1>)
-                                     : (wide ? ex::combine_kernel<float, 4> : ex::combine_kernel<float, 1>);
-  hipLaunchKernelGGL(kern, dim3(row_grid(T, cus)), dim3(ex::kThreads), 0, (hipStream_t)stream, a);
+  auto kern = dtype == GGEMM_IN_BF16 ? (!wide   ? ex::combine_kernel<uint16_t, 1, false>
+              : lines ? ex::combine_kernel<uint16_t, 8, true>
+                      : ex::combine_kernel<uint16_t, 8, false>)
+                                     : (!wide   ? ex::combine_kernel<float, 1, false>
+              : lines ? ex::combine_kernel<float, 4, true>
+                      : ex::combine_kernel<float, 4, false>);
+  // a token's columns go to as many waves as they have steps while that fills no more than a wave per SIMD: one token of
+  // 2880 takes one round trip to memory then, not six
+  const int steps = (H + 64 * (wide ? 16 / item : 1) - 1) / (64 * (wide ? 16 / item : 1));
+  a.parts = (int)std::min<int64_t>(steps, std::max<int64_t>(1, (int64_t)cus * 4 / T));
+  hipLaunchKernelGGL(kern, dim3(row_grid(T * a.parts, cus)), dim3(ex::kThreads), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }
 
@@ -234,7 +245,7 @@ int ggemm_moe_combine_backward(const void* dout, int32_t dtype, int64_t dout_str
   if (rc) return rc;
   if (!dout || !group_offs || (dweights && !y)) return GGEMM_E_NULL;
   if (dtype != GGEMM_IN_BF16 && dtype != GGEMM_IN_F32) return GGEMM_E_FORMAT;
-  if (H <= 0 || G <= 0 || G > ex::kMaxGroups) return GGEMM_E_SHAPE;
+  if (H <= 0 || H > kMaxWidth || G <= 0 || G > ex::kMaxGroups) return GGEMM_E_SHAPE;
   if (dout_stride < H || (dweights && y_stride < H) || (dy && dy_stride < H)) return GGEMM_E_STRIDE;
   const int item = dtype == GGEMM_IN_BF16 ? 2 : 4;
   if (!aligned(dout, item) || !aligned(y, item) || !aligned(dy, item) || !aligned(weights, 4) ||
@@ -246,12 +257,17 @@ int ggemm_moe_combine_backward(const void* dout, int32_t dtype, int64_t dout_str
   if ((!dy && !dweights) || (T == 0 && M == 0)) return GGEMM_OK;
   const ex::CombineBackArgs a{dout, dout_stride, y,          y_stride, M, slots, T,         top_k,
                               weights, group_offs, G, H, dy, dy_stride, dweights};
+  const bool lines = (bits(dy) | (uint64_t)(item * dy_stride)) % 128 == 0;
   const uint64_t all = bits(dout) | (dweights ? bits(y) : 0) | bits(dy) |
                        (uint64_t)item * (uint64_t)(dout_stride | (dweights ? y_stride : 0) | (dy ? dy_stride : 0) | H);
   const bool wide = common_bytes(all) == 16;
   auto kern = dtype == GGEMM_IN_BF16
-                  ? (wide ? ex::combine_backward_kernel<uint16_t, 8> : ex::combine_backward_kernel<uint16_t, 1>)
-                  : (wide ? ex::combine_backward_kernel<float, 4> : ex::combine_backward_kernel<float, 1>);
+                  ? (!wide   ? ex::combine_backward_kernel<uint16_t, 1, false>
+              : lines ? ex::combine_backward_kernel<uint16_t, 8, true>
+                      : ex::combine_backward_kernel<uint16_t, 8, false>)
+                  : (!wide   ? ex::combine_backward_kernel<float, 1, false>
+              : lines ? ex::combine_backward_kernel<float, 4, true>
+                      : ex::combine_backward_kernel<float, 4, false>);
   hipLaunchKernelGGL(kern, dim3(row_grid(std::max(T, M / 8), cus)), dim3(ex::kThreads), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }

@@ -189,16 +189,24 @@ __device__ __forceinline__ v4i make_rsrc(const void* base, int num_records) {
 // code in these kernels uses m0 (a CPU test disassembles the built code object to keep it so).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+// kOnce: non-temporal, for what no other workgroup reads.
+template <bool kOnce = false>
 __device__ __forceinline__ void dma16(v4i rsrc, uint32_t lds_addr, int voff) {
   // the LDS address and the resource are wave-uniform by construction; readfirstlane pins them to
   // SGPRs (m0 and the resource operand must be scalar)
   const uint32_t m0v = __builtin_amdgcn_readfirstlane(lds_addr);
   const v4i r = v4i{__builtin_amdgcn_readfirstlane(rsrc[0]), __builtin_amdgcn_readfirstlane(rsrc[1]),
                     __builtin_amdgcn_readfirstlane(rsrc[2]), __builtin_amdgcn_readfirstlane(rsrc[3])};
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :
-               : "s"(m0v), "v"(voff), "s"(r)
-               : "memory", "m0");
+  if constexpr (kOnce)
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+                 :
+                 : "s"(m0v), "v"(voff), "s"(r)
+                 : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :
+                 : "s"(m0v), "v"(voff), "s"(r)
+                 : "memory", "m0");
 }
 #pragma clang diagnostic pop
 

@@ -75,7 +75,7 @@ int ggemm_moe_dispatch(const void* x, int64_t row_bytes, int64_t x_stride, int64
 
 /* out[t] = residual[t] + sum over j of weights[t, j] * y[slots[t, j]], j in order, in fp32, rounded once.
  * Choices with a slot outside [0, M) have no term. weights fp32 [T, top_k] or NULL (ones); residual NULL for
- * none; y [M, H], residual and out [T, H] of `dtype`. */
+ * none; y [M, H], residual and out [T, H] of `dtype`, H up to 2^28. */
 int ggemm_moe_combine(const void* y, int32_t dtype, int64_t y_stride, int64_t M, const int32_t* slots, int64_t T,
                       int32_t top_k, const float* weights, const void* residual, int64_t residual_stride, int32_t H,
                       void* out, int64_t out_stride, void* stream);
