@@ -368,16 +368,10 @@ __device__ __forceinline__ void persistent_body(const Args& a, GG_LDS uint8_t* l
     const bool stores_after_stage0 = prefetched && full_prev;
     prefetched = false;
     for (int s = 0; s < nsteps; ++s) {
-      if (s == 0 && stores_after_stage0) {
-        if constexpr (kEpi == 0) {
-          wait_vmcnt<C::EpiStores>();
-        } else {
-          constexpr int kOut = epi::kStores<kEpi - 1, kMB, NB>, kPre = epi::kStores<epi::kNone, kMB, NB>;
-          if (e.pre != nullptr) wait_vmcnt<kOut + kPre>(); else wait_vmcnt<kOut>();
-        }
-      } else {
+      if (s == 0 && stores_after_stage0)
+        wait_vmcnt<C::EpiStores>();
+      else
         wait_vmcnt<0>();
-      }
       lds_barrier();
       // The next stage's A rows go out at the barrier, its B rows after the first m-block's MFMAs:
       // the request stream spread over the stage measured 1.9-3.1 % faster at the four sites than
@@ -436,7 +430,6 @@ __device__ __forceinline__ void persistent_body(const Args& a, GG_LDS uint8_t* l
       if (wcol < a.N)
         epi::store<kEpi - 1, kMB, NB>(acc, alpha, e, a.c, a.stride_cm, T.g, a.N, (int64_t)T.row_base + T.m0 + wrow,
                                        T.rows - wrow, wcol, lds + (cur ^ 1) * C2::kSlot + wave * epi::kRegion<NB>, el);
-      full_prev = T.rows == kTileM && T.n0 + kTN <= a.N;
       t = t_next;
       T = N;
       continue;

@@ -112,7 +112,9 @@ def grouped_gemm_fp8_bias_act(a: torch.Tensor, b: torch.Tensor, a_scale: torch.T
     out = torch.empty((M, width), dtype=torch.bfloat16, device=dev)
     pre = torch.empty((M, N), dtype=torch.bfloat16, device=dev) if keep_preact else None
     if M:
-        sam, (sbg, sbn, _) = a.stride(0) if M > 1 else max(a.stride(0), K), b.stride()
+        # the strides of dimensions of size one are arbitrary and not used
+        sam, sbn = a.stride(0) if M > 1 else K, b.stride(1)
+        sbg = b.stride(0) if G > 1 else N * sbn
         sres = 0 if residual is None else _stride(residual)
         _lib.launch("ggemm_product_fp8_bias_act", dev, G | N | K | sam | sbg | sbn | sres, a.data_ptr(), b.data_ptr(),
                     out.data_ptr(), None if pre is None else pre.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(),
@@ -126,11 +128,12 @@ def bias_act_backward(dout: torch.Tensor, preact: torch.Tensor | None, group_off
                       activation: str | None = None, *, slope: float = 1.0, limit: float | None = None,
                       shift: float = 0.0, bias_grad: bool = True):
     """``(dpreact, dbias)`` of ``act(preact)`` and its bias: dpreact bf16 [M, N] = dout * act'(preact), dbias fp32 [G, N]
-    the sum of it over each group's rows before its rounding (None without ``bias_grad``).
+    the sum of it over each group's rows before its rounding (None without ``bias_grad``). Rows outside the groups are
+    in no sum and get zero gradient.
 
     dout: bf16 [M, N] ([M, N / 2] for "swiglu"); preact: what ``grouped_gemm_fp8_bias_act`` kept; without an activation
-    it may be None, and dpreact is dout itself. Rows outside the groups get zero gradient and are in no sum. Sums are
-    made in a fixed order: the same inputs give the same bits."""
+    it may be None, and dpreact is dout itself, all its rows. Sums are made in a fixed order: the same inputs give the
+    same bits."""
     code, slope, limit, shift = _act(activation, slope, limit, shift)
     if dout.dim() != 2 or dout.dtype != torch.bfloat16:
         raise TypeError("dout must be a bf16 [M, N] tensor")

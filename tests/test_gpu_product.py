@@ -166,6 +166,20 @@ def test_empty_and_offsets_past_the_rows(pkg):
         pkg.grouped_gemm_fp8_bias_act(a.cuda(), b.cuda(), one, one, torch.tensor([0, 50, 40]).cuda(), validate=True)
 
 
+def test_strides_of_single_rows_and_groups(pkg):
+    """Where there is one row or one group its stride is whatever the view has."""
+    a, b, sa, sb, offs, _ = _inputs(3, 64, 96, [3], 12)
+    one = torch.tensor(1.0).cuda()
+    wide = torch.zeros((3, 104), dtype=torch.uint8, device="cuda")
+    wide[:, :96] = a.view(torch.uint8).cuda()
+    row = wide.view(a.dtype)[:1, :96]
+    group = b.cuda().as_strided((1, 64, 96), (8, 96, 1))
+    assert row.stride(0) % 16 and group.stride(0) == 8
+    got = pkg.grouped_gemm_fp8_bias_act(row, group, one, one, torch.tensor([0, 1]).cuda())
+    want = pkg.grouped_gemm_fp8_bias_act(a[:1].cuda(), b.cuda(), one, one, torch.tensor([0, 1]).cuda())
+    assert torch.equal(got, want)
+
+
 BACK = [(1, 16, [1]), (7, 48, [0, 3, 0, 2]), (100, 2064, [33, 1, 60]), (1000, 320, [0, 999]), (2500, 5760, [400, 0, 1, 2000, 50]),
         (40000, 64, [13000, 27000]), (600, 32, [2] * 300)]
 
