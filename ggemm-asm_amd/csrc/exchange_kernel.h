@@ -15,8 +15,11 @@ namespace ex {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxGroups = 2047;
-constexpr int kPlanBlocks = 64;             // workgroups of a plan, at most
-constexpr int kPlanEntries = 1024;            // choices that a workgroup takes, at least
+// Workgroups of a plan: each 1024 choices or more, at most 256 and fewer the more experts there are, since each reads all
+// workgroups' counts of each. Measured (us, at most 64 -> 128 -> 256): 131072 choices of 32 experts 8.9, 8.1, 8.7; 2^20 of 64
+// 40.8, 24.8, 18.5; 131072 of 256 14.3, 17.5, 26.6.
+constexpr int kPlanEntries = 1024;
+inline int plan_blocks_most(int G) { return 16384 / G > 256 ? 256 : 16384 / G < 64 ? 64 : 16384 / G; }
 constexpr int kPlanAlone = 2048;             // choices that one workgroup orders by itself
 typedef unsigned int v4u __attribute__((ext_vector_type(4)));
 
@@ -32,9 +35,16 @@ struct PlanArgs {
   int* hist;               // [workgroups][G]: choices of each expert (plan_count_kernel)
 };
 
-__device__ __forceinline__ int group_of(const PlanArgs& a, int64_t i) {
-  const int e = a.experts[i];
-  return e >= 0 && e < a.G ? e : -1;
+// The experts of kAhead choices from i on, `step` apart, all loads in flight; at or past end, and of no group, negative.
+constexpr int kAhead = 8;
+__device__ __forceinline__ void groups_of(const PlanArgs& a, int64_t i, int64_t end, int step, int (&g)[kAhead]) {
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) {
+    const int64_t at = i + (int64_t)u * step;
+    g[u] = at < end ? a.experts[at] : -1;
+  }
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) g[u] = g[u] < a.G ? g[u] : -1;
 }
 
 __global__ __launch_bounds__(kThreads) void plan_count_kernel(PlanArgs a) {
@@ -42,9 +52,12 @@ __global__ __launch_bounds__(kThreads) void plan_count_kernel(PlanArgs a) {
   for (int g = threadIdx.x; g < a.G; g += kThreads) s_cnt[g] = 0;
   __syncthreads();
   const int64_t lo = (int64_t)blockIdx.x * a.per, end = min(lo + a.per, a.n);
-  for (int64_t i = lo + threadIdx.x; i < end; i += kThreads) {
-    const int g = group_of(a, i);
-    if (g >= 0) atomicAdd(&s_cnt[g], 1);
+  for (int64_t i = lo + threadIdx.x; i < end; i += kAhead * kThreads) {
+    int g[kAhead];
+    groups_of(a, i, end, kThreads, g);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (g[u] >= 0) atomicAdd(&s_cnt[g[u]], 1);
   }
   __syncthreads();
   for (int g = threadIdx.x; g < a.G; g += kThreads) a.hist[(int64_t)blockIdx.x * a.G + g] = s_cnt[g];
@@ -67,9 +80,17 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
   const int64_t lo = (int64_t)blockIdx.x * a.per, end = min(lo + a.per, a.n);
   const int each = a.per / kWaves;           // a multiple of 64
   const int64_t wlo = lo + wave * each, wend = min(wlo + each, end);
-  for (int64_t i = wlo + lane; i < wend; i += 64) {
-    const int g = group_of(a, i);
-    if (g >= 0) atomicAdd(&s_wave[wave * G + g], 1);
+  int first[kAhead];                         // the wave's choices, or the first of them
+  groups_of(a, wlo + lane, wend, 64, first);
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u)
+    if (first[u] >= 0) atomicAdd(&s_wave[wave * G + first[u]], 1);
+  for (int64_t i = wlo + lane + 64 * kAhead; i < wend; i += 64 * kAhead) {
+    int g[kAhead];
+    groups_of(a, i, wend, 64, g);
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (g[u] >= 0) atomicAdd(&s_wave[wave * G + g[u]], 1);
   }
   const int blocks = gridDim.x;
   if (blocks > 1) {
@@ -123,21 +144,32 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
   __syncthreads();
   const int bits = 32 - __builtin_clz(G);    // of expert numbers below G
   int* next = s_wave + wave * G;
-  for (int64_t i = wlo; i < wend; i += 64) {
-    const bool in = i + lane < wend;
-    const int g = in ? group_of(a, i + lane) : -1;
-    uint64_t same = __ballot(g >= 0);
-    for (int b = 0; b < bits; ++b) {
-      const bool bit = (g >> b) & 1;
-      const uint64_t with = __ballot(bit);
-      same &= bit ? with : ~with;
+  for (int64_t i0 = wlo; i0 < wend; i0 += 64 * kAhead) {
+    int gs[kAhead];
+    if (i0 == wlo) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) gs[u] = first[u];
+    } else {
+      groups_of(a, i0 + lane, wend, 64, gs);
     }
-    int row = -1;
-    if (g >= 0) row = next[g] + __popcll(same & ((1ull << lane) - 1));
-    if (in) a.slots[i + lane] = row;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    if (g >= 0 && __builtin_ctzll(same) == lane) next[g] = row + __popcll(same);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t i = i0 + 64 * u;
+      if (i >= wend) break;
+      const int g = gs[u];
+      uint64_t same = __ballot(g >= 0);
+      for (int b = 0; b < bits; ++b) {
+        const bool bit = (g >> b) & 1;
+        const uint64_t with = __ballot(bit);
+        same &= bit ? with : ~with;
+      }
+      int row = -1;
+      if (g >= 0) row = next[g] + __popcll(same & ((1ull << lane) - 1));
+      if (i + lane < wend) a.slots[i + lane] = row;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (g >= 0 && __builtin_ctzll(same) == lane) next[g] = row + __popcll(same);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
   }
 }
 

@@ -75,12 +75,13 @@ int check_slots(const int32_t* slots, int64_t T, int k, int64_t M) {
   return aligned(slots, 4) ? GGEMM_OK : GGEMM_E_ALIGN;
 }
 
-int plan_blocks(int64_t n, int* per) {
+int plan_blocks(int64_t n, int G, int* per) {
   if (n <= ex::kPlanAlone) {
     *per = (int)std::max<int64_t>(ex::kThreads, (n + ex::kThreads - 1) / ex::kThreads * ex::kThreads);
     return 1;
   }
-  int64_t p = std::max<int64_t>(ex::kPlanEntries, (n + ex::kPlanBlocks - 1) / ex::kPlanBlocks);
+  const int most = ex::plan_blocks_most(G);
+  int64_t p = std::max<int64_t>(ex::kPlanEntries, (n + most - 1) / most);
   p = (p + ex::kThreads - 1) / ex::kThreads * ex::kThreads;
   *per = (int)p;
   return (int)((n + p - 1) / p);
@@ -152,7 +153,7 @@ int ggemm_moe_route_backward(const float* dweights, const void* logits, int32_t 
 int64_t ggemm_moe_plan_workspace(int64_t n, int32_t G) {
   if (n < 0 || n > kMaxRows || G <= 0 || G > ex::kMaxGroups) return 0;
   int per = 0;
-  const int blocks = plan_blocks(n, &per);
+  const int blocks = plan_blocks(n, G, &per);
   return blocks > 1 ? (int64_t)blocks * G : 0;
 }
 
@@ -166,7 +167,7 @@ int ggemm_moe_plan(const int32_t* experts, int64_t n, int32_t G, int64_t* group_
   const int rc = device_cus(&cus);
   if (rc) return rc;
   ex::PlanArgs a{experts, n, G, 0, group_offs, slots, workspace};
-  const int blocks = plan_blocks(n, &a.per);
+  const int blocks = plan_blocks(n, G, &a.per);
   if (blocks > 1) {
     hipLaunchKernelGGL(ex::plan_count_kernel, dim3(blocks), dim3(ex::kThreads), 4 * G, (hipStream_t)stream, a);
     const int e = (int)hipGetLastError();
