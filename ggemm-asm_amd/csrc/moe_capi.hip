@@ -224,12 +224,12 @@ int ggemm_moe_combine(const void* y, int32_t dtype, int64_t y_stride, int64_t M,
   const uint64_t all = bits(y) | bits(out) | bits(residual) |
                        (uint64_t)item * (uint64_t)(y_stride | out_stride | (residual ? residual_stride : 0) | H);
   const bool wide = common_bytes(all) == 16;
-  auto kern = dtype == GGEMM_IN_BF16 ? (!wide   ? ex::combine_kernel<uint16_t, 1, false>
-              : lines ? ex::combine_kernel<uint16_t, 8, true>
-                      : ex::combine_kernel<uint16_t, 8, false>)
-                                     : (!wide   ? ex::combine_kernel<float, 1, false>
-              : lines ? ex::combine_kernel<float, 4, true>
-                      : ex::combine_kernel<float, 4, false>);
+  auto pick = [&](auto narrow, auto whole, auto shared) { return !wide ? narrow : lines ? whole : shared; };
+  auto kern = dtype == GGEMM_IN_BF16
+                  ? pick(ex::combine_kernel<uint16_t, 1, false>, ex::combine_kernel<uint16_t, 8, true>,
+                         ex::combine_kernel<uint16_t, 8, false>)
+                  : pick(ex::combine_kernel<float, 1, false>, ex::combine_kernel<float, 4, true>,
+                         ex::combine_kernel<float, 4, false>);
   // a token's columns go to as many waves as they have steps while that fills no more than a wave per SIMD: one token of
   // 2880 takes one round trip to memory then, not six
   const int steps = (H + 64 * (wide ? 16 / item : 1) - 1) / (64 * (wide ? 16 / item : 1));
@@ -262,13 +262,12 @@ int ggemm_moe_combine_backward(const void* dout, int32_t dtype, int64_t dout_str
   const uint64_t all = bits(dout) | (dweights ? bits(y) : 0) | bits(dy) |
                        (uint64_t)item * (uint64_t)(dout_stride | (dweights ? y_stride : 0) | (dy ? dy_stride : 0) | H);
   const bool wide = common_bytes(all) == 16;
+  auto pick = [&](auto narrow, auto whole, auto shared) { return !wide ? narrow : lines ? whole : shared; };
   auto kern = dtype == GGEMM_IN_BF16
-                  ? (!wide   ? ex::combine_backward_kernel<uint16_t, 1, false>
-              : lines ? ex::combine_backward_kernel<uint16_t, 8, true>
-                      : ex::combine_backward_kernel<uint16_t, 8, false>)
-                  : (!wide   ? ex::combine_backward_kernel<float, 1, false>
-              : lines ? ex::combine_backward_kernel<float, 4, true>
-                      : ex::combine_backward_kernel<float, 4, false>);
+                  ? pick(ex::combine_backward_kernel<uint16_t, 1, false>, ex::combine_backward_kernel<uint16_t, 8, true>,
+                         ex::combine_backward_kernel<uint16_t, 8, false>)
+                  : pick(ex::combine_backward_kernel<float, 1, false>, ex::combine_backward_kernel<float, 4, true>,
+                         ex::combine_backward_kernel<float, 4, false>);
   hipLaunchKernelGGL(kern, dim3(row_grid(std::max(T, M / 8), cus)), dim3(ex::kThreads), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }

@@ -5,7 +5,10 @@
 //   w_j = scale * p_j  or  scale * p_j / sum_i p_i over the taken experts.
 //
 // Reads T E logits and writes T k pairs: bound by latency below some thousand tokens, by instruction
-// issue above (32 experts are 64 bytes of logits for ~150 wave instructions).
+// issue above (32 experts, 4 taken: 298 vector instructions a wave for
+// eight tokens, 0.73 of the SIMDs' cycles while the CUs run). One token of 32 experts takes
+// 3.2 us, 131072 tokens with bf16 logits and 4 taken 12.6 (1.0 TB/s of logits and pairs); 16384 of 256 with fp32
+// logits, a bias, 8 groups and 8 taken 21.4, the gradient 10.8.
 //
 // L lanes hold a token's experts, V consecutive ones each, in registers; 64 / L tokens per wave. A round
 // of the top-k takes the largest key over the lanes (a DPP max of one 32-bit word per step: keys are the
