@@ -229,3 +229,64 @@ def test_gradient_of_no_rows_and_odd_offsets(pkg):
     zero = torch.zeros_like(one)
     dpre, _ = pkg.bias_act_backward(one, zero, offs, "silu")
     assert dpre[:, 0].tolist() == [0.0, 0.5, 0.5, 0.5, 0.5, 0.5]
+
+
+# z, the result and the residual past 2^32 bytes; the last group's rows against the oracle
+@pytest.mark.parametrize("K,activation,options,keep,residual,rows",
+                         [(128, None, {}, False, False, 256), (128, "swiglu", GATE, True, False, 128),
+                          (1088, "swiglu", GATE, True, False, 256), (128, "gelu", {}, False, True, 192)])
+def test_rows_past_32_bits(pkg, K, activation, options, keep, residual, rows):
+    from ggemm_asm_amd import product
+    M, N, last = 900000, 2560, 300
+    a, b, sa, sb, _, gen = _inputs(last, N, K, [0, last], 3)
+    full = torch.zeros((M, K), dtype=torch.uint8, device="cuda")
+    full[-last:] = a.view(torch.uint8).cuda()
+    bias = torch.randn((2, N), generator=gen)
+    tail = torch.randn((last, N), generator=gen).to(torch.bfloat16)
+    res = None
+    if residual:
+        res = torch.zeros((M, N), dtype=torch.bfloat16, device="cuda")
+        res[-last:] = tail.cuda()
+    assert product.tile_rows(2, N, K, M, activation, keep_preact=keep, residual=residual) == rows
+    got = pkg.grouped_gemm_fp8_bias_act(full.view(a.dtype), b.cuda(), torch.tensor(sa).cuda(), torch.tensor(sb).cuda(),
+                                        torch.tensor([0, M - last, M]).cuda(), bias.cuda(), activation, res, keep_preact=keep, **options)
+    out, pre = got if keep else (got, None)
+    z, ref, size = orx.product(a, b, sa * sb, [0, 0, last], bias, activation, tail if residual else None, **options)
+    _check(out[-last:].cpu().double(), None if pre is None else pre[-last:].cpu().double(), z, ref, size, activation, options,
+           tail.double().abs() if residual else torch.zeros_like(ref))
+
+
+# weights of 256 groups, 2^32 bytes and more
+@pytest.mark.parametrize("M,N,K,rows", [(2, 4096, 4224, 16), (600, 4096, 4224, 64), (20000, 2560, 6720, 256)])
+def test_weights_past_32_bits(pkg, M, N, K, rows):
+    from ggemm_asm_amd import product
+    G = 256
+    a, b, sa, sb, _, gen = _inputs(M, N, K, [1], 4)
+    weights = torch.zeros((G, N, K), dtype=torch.uint8, device="cuda")
+    weights[-1] = b[0].view(torch.uint8).cuda()
+    bias = torch.randn((1, N), generator=gen)
+    biases = torch.zeros((G, N), device="cuda")
+    biases[-1] = bias[0].cuda()
+    offs = torch.zeros(G + 1, dtype=torch.int64)
+    offs[-1] = M
+    assert product.tile_rows(G, N, K, M, "swiglu") == rows
+    out = pkg.grouped_gemm_fp8_bias_act(a.cuda(), weights.view(b.dtype), torch.tensor(sa).cuda(), torch.tensor(sb).cuda(), offs.cuda(),
+                                        biases, "swiglu", **GATE)
+    part = slice(max(0, M - 300), M)
+    z, ref, size = orx.product(a[part], b, sa * sb, [0, part.stop - part.start], bias, "swiglu", None, **GATE)
+    _check(out[part].cpu().double(), None, z, ref, size, "swiglu", GATE, torch.zeros_like(ref))
+
+
+def test_gradient_past_32_bits(pkg):
+    M, N, last = 900000, 2560, 300
+    gen = torch.Generator().manual_seed(5)
+    tail, dtail = torch.randn((last, N), generator=gen).to(torch.bfloat16), torch.randn((last, N), generator=gen).to(torch.bfloat16)
+    pre, dout = torch.zeros((M, N), dtype=torch.bfloat16, device="cuda"), torch.zeros((M, N), dtype=torch.bfloat16, device="cuda")
+    pre[-last:], dout[-last:] = tail.cuda(), dtail.cuda()
+    dpre, dbias = pkg.bias_act_backward(dout, pre, torch.tensor([0, M - last, M]).cuda(), "gelu")
+    # the same rows by themselves: equal in dpre; the sums' units are cut alike from the group's first row, but may be of fewer rows
+    few, fewb = pkg.bias_act_backward(dtail.cuda(), tail.cuda(), torch.tensor([0, 0, last]).cuda(), "gelu")
+    assert torch.equal(dpre[-last:], few) and not dpre[:-last].any() and not dbias[0].any()
+    want = few.double().sum(0)
+    err = few.double().abs().sum(0) * (BF / 2 + (last + 16) * U)      # few is rounded, the sums are not
+    assert ((dbias[1].double() - want).abs() <= err).all() and ((fewb[1].double() - want).abs() <= err).all()
