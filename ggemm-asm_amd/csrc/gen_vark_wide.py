@@ -1444,10 +1444,11 @@ class GenKE(GenK):
                 e(f"v_add_f32 v{z + r}, {shift}, v{z + r}")
             for k in (0, 1):
                 e(f"v_rcp_f32 v{ex + k}, v{ex + k}")
-            for r in (0, 2):
-                e(f"v_mul_f32 v{z + r}, v{z + r}, v{z + r + 1}")
+            # the sigmoid first: a gate far below zero times it is zero, times the up half could be infinite
             for r in (0, 2):
                 e(f"v_mul_f32 v{z + r}, v{z + r}, v{ex + r // 2}")
+            for r in (0, 2):
+                e(f"v_mul_f32 v{z + r}, v{z + r}, v{z + r + 1}")
             e(f"v_cvt_pk_bf16_f32 v{pk + 2}, v{z}, v{z + 2}")
             e(f"ds_write_b32 {L['ow']}, v{pk + 2} offset:{OREGION + 32 * j + 8 * g}")
 

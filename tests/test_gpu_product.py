@@ -290,3 +290,37 @@ def test_gradient_past_32_bits(pkg):
     want = few.double().sum(0)
     err = few.double().abs().sum(0) * (BF / 2 + (last + 16) * U)      # few is rounded, the sums are not
     assert ((dbias[1].double() - want).abs() <= err).all() and ((fewb[1].double() - want).abs() <= err).all()
+
+
+@pytest.mark.parametrize("M,N,K,lens,rows", [(30, 5760, 2064, [17, 0, 13], 16), (150, 1040, 144, [80, 70], 64),
+                                             (2500, 3200, 192, [1000, 0, 1499], 128), (20000, 2096, 2880, [5000, 4999, 0, 10001], 192),
+                                             (16000, 1280, 1088, [15999], 256)])
+@pytest.mark.parametrize("options", [{}, GATE])
+@pytest.mark.parametrize("keep", [False, True])
+def test_special_values_on_every_kernel(pkg, M, N, K, lens, rows, options, keep):
+    """Gates switched off by a bias near the lowest finite value give zeros, whatever the up half; NaN stays in its
+    columns; infinities do what the formula says. Other columns are finite."""
+    from ggemm_asm_amd import product
+    a, b, sa, sb, offs, _ = _inputs(M, N, K, lens, M)
+    G = len(lens)
+    assert product.tile_rows(G, N, K, M, "swiglu", keep_preact=keep) == rows
+    bias = torch.zeros((G, N))
+    off = [0, 14, 322, N - 2]                             # gate columns, of several waves and tiles
+    for c in off[:2]:
+        bias[:, c] = -3.2e38
+    for c in off[2:]:
+        bias[:, c] = -5e37
+    bias[:, 41] = math.nan                               # an up half
+    bias[:, 100] = math.nan                              # a gate
+    bias[:, 200] = -math.inf                             # -inf times a sigmoid of 0
+    got = pkg.grouped_gemm_fp8_bias_act(a.cuda(), b.cuda(), torch.tensor(sa).cuda(), torch.tensor(sb).cuda(),
+                                        torch.tensor(offs).cuda(), bias.cuda(), "swiglu", keep_preact=keep, **options)
+    out = (got[0] if keep else got)[:offs[-1]].float()
+    nan = torch.zeros(N // 2, dtype=torch.bool, device="cuda")
+    nan[[20, 50, 100]] = True
+    assert torch.equal(torch.isnan(out).all(0), nan) and torch.equal(torch.isnan(out).any(0), nan)
+    assert not out[:, [c // 2 for c in off]].any()
+    assert torch.isfinite(out[:, ~nan]).all()
+    if keep:
+        assert torch.equal(torch.isnan(got[1][:offs[-1]]).all(0).nonzero().flatten().cpu(), torch.tensor([41, 100]))
+        assert (got[1][:offs[-1], off] < -4e37).all()

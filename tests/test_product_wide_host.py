@@ -370,3 +370,41 @@ def test_generated_include_lists_the_configurations():
     text = open(W.GEN_PATH.replace("gen_vark_wide.py", "vark_wide_asm.inc")).read()
     for c in GEN.KECONFIGS:
         assert f"#define GGEMM_WIDE_NOPERANDS_{c.name} {len(c.operands)}" in text
+
+
+@pytest.mark.parametrize("name", [c.name for c in GEN.KECONFIGS if c.gate])
+def test_a_gate_far_below_zero_gives_zero(name):
+    """Gates near the lowest finite value, whose product with the up half overflows, times a sigmoid of exactly zero:
+    the result is the formula's zero, not NaN. One tile without a bias, z = alpha times its values."""
+    cfg = CFGS[name]
+    width, sc, sz, K = 160, 168, 328, 64
+    tile = np.random.default_rng(1).normal(size=(256, 320)).astype(np.float32) * 6
+    tile[::3, 0::4] = -3.3e38
+    tile[1::3, 2::4] = -1e37
+    tile[2::3, 0::8] = -400.0
+    mems = [Memory(OUT, np.full(2 * 256 * sc, 0xAB, np.uint8)), Memory(PRE, np.full(2 * 256 * sz, 0xAB, np.uint8)),
+            Memory(BIAS, np.zeros(16, np.uint8))]
+    lane = np.arange(64, dtype=np.uint32)
+    for wave in range(4):
+        wm, wn = wave & 1, wave >> 1
+        w = Wave(cfg, wave, mems)
+        w.tile = tile
+        ops = dict(c0=0, nis=0, vmt=0, q0=0, q1=0, q2=0, np=0)
+        for k, p in dict(bLT=A, bRT=B, bLN=A, bRN=B, cT=OUT, zT=PRE, b=BIAS).items():
+            ops[f"{k}_lo"], ops[f"{k}_hi"] = p & M32, p >> 32
+        ops.update(lds_base=0, w1k=1024 * wave, klenT=K, recAT=255 * 2880, recBT=319 * 2880, klenN=0, recAN=255 * 2880,
+                   recBN=319 * 2880, crecT=256 * sc * 2, cm2=2 * sc, alpha=int(_bits(ALPHA)),
+                   sw_epi=(128 * wm * sc + 80 * wn) * 2, vboff=lane * np.uint32(16), brec=0, bf32=1,
+                   nslope=int(_bits(-SLOPE * 1.44269504)), limit=int(_bits(LIMIT)), shift=int(_bits(SHIFT)),
+                   zrecT=256 * sz * 2, zm2=2 * sz, sw_z=(128 * wm * sz + 160 * wn) * 2)
+        ops.update({f"voffL{j}": lane for j in range(cfg.nl)})
+        ops.update({f"voffR{j}": lane for j in range(cfg.nr)})
+        for side, base in (("am", 0), ("bn", cfg.rhs_off)):
+            ops.update({side + x: np.full(64, base, np.uint32) for x in ("lo0", "lo1", "hi0", "hi1")})
+        w.run(ops)
+    z = ALPHA * tile.astype(np.float64)
+    with np.errstate(over="ignore"):
+        want = _silu_gate(z[:, 0::2], z[:, 1::2])
+    got = _bf16_value(mems[0].data.reshape(256, 2 * sc)[:, :2 * width].reshape(-1)).reshape(want.shape)
+    assert not np.isnan(got).any()
+    assert (np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + 1e-5).all()
