@@ -68,6 +68,7 @@ QUANT_EXPORTS = (
     "ggemm_quant_amax",
     "ggemm_quant_fp8_tensorwise",
     "ggemm_quant_fp8_tensorwise_ws",
+    "ggemm_quant_fp8_tensorwise_rows",
     "ggemm_quant_fp8_tensorwise_delayed",
     "ggemm_quant_fp8_tensorwise_delayed_dev",
     "ggemm_quant_fp8_tensorwise_transpose",
@@ -97,7 +98,7 @@ PRODUCT_EXPORTS = (
 # GGEMM_VARK_ABI_VERSION of include/ggemm_vark.h that these bindings are written for. Some exports
 # changed signature between versions (ggemm_vark_wgrad_fp8_out and ggemm_vark_wgrad_mxfp8 took
 # M_total from version 3 on), so a library of another version is refused at load.
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 ERRORS = {
     0: "GGEMM_OK", -1: "GGEMM_E_NULL", -2: "GGEMM_E_SHAPE", -3: "GGEMM_E_STRIDE",
@@ -181,6 +182,8 @@ def load():
     lib.ggemm_quant_fp8_tensorwise.restype = ctypes.c_int
     lib.ggemm_quant_fp8_tensorwise_ws.argtypes = [vp, i32, i64, i32, i64, i32, vp, i64, vp, vp, vp, vp]
     lib.ggemm_quant_fp8_tensorwise_ws.restype = ctypes.c_int
+    lib.ggemm_quant_fp8_tensorwise_rows.argtypes = [vp, i32, i64, i32, i64, vp, i32, i32, vp, i64, vp, vp, vp, vp]
+    lib.ggemm_quant_fp8_tensorwise_rows.restype = ctypes.c_int
     lib.ggemm_quant_fp8_tensorwise_delayed.argtypes = [vp, i32, i64, i32, i64, i32, vp, i64, vp, i32, i32, vp, vp]
     lib.ggemm_quant_fp8_tensorwise_delayed.restype = ctypes.c_int
     lib.ggemm_quant_fp8_tensorwise_delayed_dev.argtypes = [vp, i32, i64, i32, i64, i32, vp, i64, vp, i32, vp, vp,

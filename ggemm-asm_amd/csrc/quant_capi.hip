@@ -91,6 +91,27 @@ int launch_amax(const void* x, int in_dtype, int64_t rows, int cols, int64_t str
   return workspace ? grid : 1;
 }
 
+// The rows of x that count: those with a slot (ggemm_quant_fp8_tensorwise_rows); all of them without slots.
+struct Rows {
+  const int32_t* slots;
+  int k;
+};
+
+// The partial maxima over those rows, their number returned.
+int launch_amax_rows(const void* x, int in_dtype, int64_t rows, int cols, int64_t stride, const Rows& r,
+                     uint32_t* workspace, int cus, hipStream_t s) {
+  if (rows == 0) return 0;
+  constexpr int64_t kWaves = qt::kThreads / 64;
+  const int64_t most = (int64_t)cus * kAmaxPerCu < qt::kMaxPartials ? (int64_t)cus * kAmaxPerCu : qt::kMaxPartials;
+  const int64_t want = (rows + kWaves - 1) / kWaves;
+  const int grid = (int)(want < most ? want : most);
+  const bool f32 = in_dtype == GGEMM_IN_F32, keep = amax_keeps(rows * cols * (f32 ? 4 : 2), f32, Next::kStreaming);
+  auto k = f32 ? (keep ? qt::amax_rows_kernel<true, true> : qt::amax_rows_kernel<true, false>)
+               : (keep ? qt::amax_rows_kernel<false, true> : qt::amax_rows_kernel<false, false>);
+  hipLaunchKernelGGL(k, dim3(grid), dim3(qt::kThreads), 0, s, x, rows, cols, stride, r.slots, r.k, workspace);
+  return grid;
+}
+
 // Arguments of the transposing quantizer (all but the amax / history pointers).
 int check_transpose(const void* x, int in_dtype, int batch, int rows, int cols, int out_format, const void* out,
                     int64_t out_stride, const void* out_t, int64_t out_t_stride, const float* scale_out) {
@@ -142,7 +163,7 @@ int ggemm_quant_amax(const void* x, int32_t in_dtype, int64_t rows, int32_t cols
 
 static int tensorwise(const void* x, int32_t in_dtype, int64_t rows, int32_t cols, int64_t stride, int32_t out_format,
                       void* out, int64_t out_stride, float* scale_out, float* amax_out, uint32_t* workspace,
-                      void* stream) {
+                      const Rows& counted, void* stream) {
   int rc = check_2d(x, in_dtype, rows, cols, stride);
   if (rc) return rc;
   if (!out || !scale_out || !amax_out) return GGEMM_E_NULL;
@@ -154,7 +175,9 @@ static int tensorwise(const void* x, int32_t in_dtype, int64_t rows, int32_t col
   rc = device_cus(&cus);
   if (rc) return rc;
   hipStream_t s = (hipStream_t)stream;
-  const int n = launch_amax(x, in_dtype, rows, cols, stride, amax_out, workspace, Next::kStreaming, cus, s);
+  const int n = counted.slots
+                    ? launch_amax_rows(x, in_dtype, rows, cols, stride, counted, workspace, cus, s)
+                    : launch_amax(x, in_dtype, rows, cols, stride, amax_out, workspace, Next::kStreaming, cus, s);
   const int grid = grid_for(rows * (cols / 8), cus, kQuantPerCu);
   const uint32_t* partials = workspace ? workspace : reinterpret_cast<const uint32_t*>(amax_out);
   uint8_t* o = static_cast<uint8_t*>(out);
@@ -169,7 +192,8 @@ static int tensorwise(const void* x, int32_t in_dtype, int64_t rows, int32_t col
 int ggemm_quant_fp8_tensorwise(const void* x, int32_t in_dtype, int64_t rows, int32_t cols, int64_t stride,
                                int32_t out_format, void* out, int64_t out_stride, float* scale_out,
                                float* amax_out, void* stream) {
-  return tensorwise(x, in_dtype, rows, cols, stride, out_format, out, out_stride, scale_out, amax_out, nullptr, stream);
+  return tensorwise(x, in_dtype, rows, cols, stride, out_format, out, out_stride, scale_out, amax_out, nullptr,
+                    {nullptr, 0}, stream);
 }
 
 int ggemm_quant_fp8_tensorwise_ws(const void* x, int32_t in_dtype, int64_t rows, int32_t cols, int64_t stride,
@@ -177,7 +201,18 @@ int ggemm_quant_fp8_tensorwise_ws(const void* x, int32_t in_dtype, int64_t rows,
                                   float* amax_out, uint32_t* workspace, void* stream) {
   if (!workspace) return GGEMM_E_NULL;
   return tensorwise(x, in_dtype, rows, cols, stride, out_format, out, out_stride, scale_out, amax_out, workspace,
-                    stream);
+                    {nullptr, 0}, stream);
+}
+
+int ggemm_quant_fp8_tensorwise_rows(const void* x, int32_t in_dtype, int64_t rows, int32_t cols, int64_t stride,
+                                    const int32_t* slots, int32_t top_k, int32_t out_format, void* out,
+                                    int64_t out_stride, float* scale_out, float* amax_out, uint32_t* workspace,
+                                    void* stream) {
+  if (!slots || !workspace) return GGEMM_E_NULL;
+  if (top_k <= 0 || rows > INT32_MAX || rows * top_k > INT32_MAX) return GGEMM_E_SHAPE;
+  if (!aligned(slots, 4)) return GGEMM_E_ALIGN;
+  return tensorwise(x, in_dtype, rows, cols, stride, out_format, out, out_stride, scale_out, amax_out, workspace,
+                    {slots, top_k}, stream);
 }
 
 // The delayed quantizers' history argument: a host slot in [0, H), or (slot_dev != nullptr) a device

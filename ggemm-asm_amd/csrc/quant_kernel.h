@@ -232,6 +232,39 @@ __global__ void __launch_bounds__(kThreads) amax_kernel(const void* x, int64_t r
   }
 }
 
+// The same over the rows that go somewhere: those with one of their k slots (a row's choices in expert order,
+// negative for none) in [0, rows * k). A wave takes a row, its slots asked for beside the row itself, which is in
+// bounds either way: a row that goes nowhere, whatever it holds, is left out once both are there.
+template <bool kF32, bool kKeep>
+__global__ void __launch_bounds__(kThreads) amax_rows_kernel(const void* x, int64_t rows, int cols, int64_t stride,
+                                                             const int32_t* slots, int k, uint32_t* partials) {
+  constexpr int kAhead = kF32 ? 3 : 6;               // 16-byte loads of a lane in flight: a row of 2880 bf16 whole
+  const int lane = threadIdx.x & 63, cpr = cols / 8;
+  const int64_t waves = (int64_t)gridDim.x * (kThreads / 64);
+  uint32_t m = 0;
+  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6); r < rows; r += waves) {
+    const int first = lane < k ? slots[r * k + lane] : -1;
+    uint32_t row_max = 0;
+    for (int c0 = lane; c0 < cpr; c0 += 64 * kAhead) {
+      float v[kAhead][8];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (c0 + 64 * u < cpr) load8<kF32, kKeep>(x, r, stride, c0 + 64 * u, v[u]);
+        else for (int e = 0; e < 8; ++e) v[u][e] = 0.0f;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) row_max = max(row_max, __float_as_uint(v[u][e]) & 0x7fffffffu);
+    }
+    bool goes = first >= 0 && first < rows * k;
+    for (int j = lane + 64; j < k; j += 64) goes |= slots[r * k + j] >= 0 && slots[r * k + j] < rows * k;
+    if (__ballot(goes) != 0) m = max(m, row_max);
+  }
+  m = block_max(m);
+  if (threadIdx.x == 0) partials[blockIdx.x] = m;
+}
+
 // ---------------------------------------------------------------------------------- tensorwise
 
 template <bool kE5M2>

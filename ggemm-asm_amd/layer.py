@@ -37,8 +37,9 @@ def moe_layer_fp8(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, w_d
     the two products.
 
     With gradients: rows are dispatched in bf16 and the products are the autograd layer's. Without: x is quantized once
-    and its fp8 rows dispatched, an eighth of the bytes at top_k = 4, and nothing is kept for a backward pass (delayed
-    scaling is a training recipe and is not used there)."""
+    and its fp8 rows dispatched, half the bytes of bf16 ones, and nothing is kept for a backward pass (delayed scaling
+    is a training recipe and is not used there). Either way x's scale is that of the tokens that go to an expert:
+    what a masked token (all logits -inf) holds reaches no other token."""
     if x.dim() != 2 or x.dtype != torch.bfloat16:
         raise TypeError("x must be a bf16 [T, H] tensor")
     if logits.dim() != 2 or logits.shape[0] != x.shape[0] or logits.shape[1] != w_up.shape[0]:
@@ -56,7 +57,7 @@ def moe_layer_fp8(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, w_d
                                bias=bias_up, activation=activation, **gate)
         y = grouped_linear_fp8(h, w_down, plan.group_offs, mains[1], caches[1], scales[1], bias=bias_down)
         return combine_tokens(y, plan, weights, residual)
-    q, sx, _ = quantize_fp8_tensorwise(x, "e4m3")
+    q, sx, _ = quantize_fp8_tensorwise(x, "e4m3", slots=plan.slots)
     rows = dispatch_tokens(q, plan, row_align=_LINE)
     qu, su = _weight(w_up, caches[0])
     h = grouped_gemm_fp8_bias_act(rows, qu, sx, su, plan.group_offs, bias_up, activation, zero_tail=True, **gate)

@@ -87,25 +87,38 @@ def _padded_empty(shape, row_align, dt, device):
     return torch.empty(tuple(shape[:-1]) + (padded,), dtype=dt, device=device)[..., :last]
 
 
-def quantize_fp8_tensorwise(x: torch.Tensor, fmt: str = "e4m3", row_align: int | None = None):
+def quantize_fp8_tensorwise(x: torch.Tensor, fmt: str = "e4m3", row_align: int | None = None, *,
+                            slots: torch.Tensor | None = None):
     """Per-tensor FP8 quantization. Returns ``(q, scale, amax)``: q has x's shape and dtype
     float8_e4m3fn / float8_e5m2, ``scale = amax / fmax`` (1 when amax == 0) and ``amax`` are
     single-element fp32 device tensors; ``q * scale`` dequantizes. The GEMM entry points take
     ``scale`` as their per-tensor scale. ``row_align=128`` returns q as a view whose rows start on
     128-byte lines (a padded buffer; the padding is not written): the persistent GEMM reads such
-    operands with one cache line per row segment instead of 1.5 (K = 2880: 6-9% faster)."""
+    operands with one cache line per row segment instead of 1.5 (K = 2880: 6-9% faster).
+
+    ``slots``: int32 [rows, k], those of a ``DispatchPlan`` of x's rows: ``amax`` and ``scale`` are of the rows with a
+    slot in [0, rows * k) alone, so that tokens which go nowhere (padding) reach no other token, whatever they hold."""
     _check(x, fmt)
     x2 = _as_2d(x)
     code, dt = _OUT[fmt]
     dev, (rows, cols) = x.device, x2.shape
+    if slots is not None:
+        if slots.dtype != torch.int32 or slots.dim() != 2 or slots.shape[0] != rows or slots.device != dev:
+            raise ValueError(f"slots must be int32 [{rows}, k] on x's device")
+        slots = slots.contiguous()
     # q's rows, contiguous or padded, are evenly strided over one buffer
     q = _padded_empty(x.shape, row_align, dt, dev)
     scale = torch.empty((), dtype=torch.float32, device=dev)
     am = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(WORKSPACE, dtype=torch.int32, device=dev)
     qp = q if rows > 0 else torch.empty((1, cols), dtype=dt, device=dev)
-    _lib.launch("ggemm_quant_fp8_tensorwise_ws", dev, cols, _ptr(x2), _IN[x.dtype], rows, cols, _row_stride(x2), code,
-                qp.data_ptr(), q.stride(-2) if rows > 1 else cols, scale.data_ptr(), am.data_ptr(), ws.data_ptr())
+    out = (code, qp.data_ptr(), q.stride(-2) if rows > 1 else cols, scale.data_ptr(), am.data_ptr(), ws.data_ptr())
+    if slots is not None and rows:
+        k = slots.shape[1]
+        _lib.launch("ggemm_quant_fp8_tensorwise_rows", dev, cols | k, x2.data_ptr(), _IN[x.dtype], rows, cols,
+                    _row_stride(x2), slots.data_ptr(), k, *out)
+    else:
+        _lib.launch("ggemm_quant_fp8_tensorwise_ws", dev, cols, _ptr(x2), _IN[x.dtype], rows, cols, _row_stride(x2), *out)
     return q, scale, am
 
 

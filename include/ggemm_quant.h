@@ -62,6 +62,15 @@ int ggemm_quant_fp8_tensorwise_ws(const void* x, int32_t in_dtype, int64_t rows,
                                   int32_t out_format, void* out, int64_t out_stride, float* scale_out,
                                   float* amax_out, uint32_t* workspace, void* stream);
 
+/* ggemm_quant_fp8_tensorwise_ws for tokens of which some go nowhere (ABI version 12): slots is the int32
+ * [rows, top_k] of a dispatch plan (ggemm_moe.h), and amax_out is the max |x| over the rows with a slot in
+ * [0, rows * top_k) alone, 0 where there is none. All rows are quantized by its scale: what the others hold,
+ * NaN and infinities included, changes no row's bytes but their own. rows * top_k < 2^31; slots 4-byte aligned. */
+int ggemm_quant_fp8_tensorwise_rows(const void* x, int32_t in_dtype, int64_t rows, int32_t cols, int64_t stride,
+                                    const int32_t* slots, int32_t top_k, int32_t out_format, void* out,
+                                    int64_t out_stride, float* scale_out, float* amax_out, uint32_t* workspace,
+                                    void* stream);
+
 /* Per-tensor quantization with delayed scaling: the scale comes from earlier amax values, and this
  * tensor's amax is recorded in the same pass (no separate amax pass over x). amax_history is a
  * device fp32 array of history_len entries; scale_out = m / fmax with m the largest entry other

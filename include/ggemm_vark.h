@@ -17,7 +17,7 @@
 extern "C" {
 #endif
 
-#define GGEMM_VARK_ABI_VERSION 11
+#define GGEMM_VARK_ABI_VERSION 12
 
 enum {
   GGEMM_OK = 0,

@@ -405,3 +405,30 @@ def test_guarded_quotient_with_given_scale():
                     assert b_got == b_ref, (fmt, x, s, got, exact)
                 n += 1
     assert n > 4000
+
+
+def _rows(lib, **kw):
+    a = dict(x=FAKE, dt=0, rows=100, cols=64, stride=64, slots=FAKE, k=4, fmt=0, out=FAKE, ostride=64, scale=FAKE, amax=FAKE,
+             ws=FAKE)
+    a.update(kw)
+    return lib.ggemm_quant_fp8_tensorwise_rows(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(x=0), -1), (dict(out=0), -1), (dict(scale=0), -1), (dict(amax=0), -1), (dict(slots=0), -1), (dict(ws=0), -1),
+    (dict(dt=2), -8), (dict(fmt=3), -8), (dict(cols=60), -2), (dict(rows=-1), -2), (dict(k=0), -2), (dict(k=-1), -2),
+    (dict(rows=2 ** 29), -2), (dict(rows=2 ** 62), -2), (dict(stride=56), -3), (dict(ostride=60), -3), (dict(x=FAKE + 8), -4),
+    (dict(out=FAKE + 4), -4), (dict(slots=FAKE + 2), -4), (dict(ws=FAKE + 2), -4),
+])
+def test_tensorwise_rows_validation(pkg, kw, rc):
+    assert _rows(pkg.load_library(), **kw) == rc
+
+
+@pytest.mark.parametrize("slots", [torch.zeros((8, 2), dtype=torch.int64), torch.zeros(8, dtype=torch.int32),
+                                   torch.zeros((7, 2), dtype=torch.int32), torch.zeros((8, 2), dtype=torch.int32, device="meta")])
+def test_slots_refusals(pkg, monkeypatch, slots):
+    from ggemm_asm_amd import _lib, quant
+    monkeypatch.setattr(quant, "_check", lambda *a: None)
+    monkeypatch.setattr(_lib, "launch", lambda *a: pytest.fail("launched"))
+    with pytest.raises(ValueError, match="slots"):
+        pkg.quantize_fp8_tensorwise(torch.zeros(8, 16), slots=slots)
