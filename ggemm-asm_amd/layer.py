@@ -9,7 +9,7 @@ import torch
 
 from .autograd import FP8DelayedScaling, FP8WeightCache, grouped_linear_fp8
 from .moe import combine_tokens, dispatch_tokens, plan_dispatch, route_experts
-from .product import grouped_gemm_fp8_bias_act
+from .product import _rows16, grouped_gemm_fp8_bias_act
 from .quant import quantize_fp8_tensorwise
 
 _LINE = 128
@@ -57,7 +57,7 @@ def moe_layer_fp8(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, w_d
                                bias=bias_up, activation=activation, **gate)
         y = grouped_linear_fp8(h, w_down, plan.group_offs, mains[1], caches[1], scales[1], bias=bias_down)
         return combine_tokens(y, plan, weights, residual)
-    q, sx, _ = quantize_fp8_tensorwise(x, "e4m3", slots=plan.slots)
+    q, sx, _ = quantize_fp8_tensorwise(_rows16(x), "e4m3", slots=plan.slots)
     rows = dispatch_tokens(q, plan, row_align=_LINE)
     qu, su = _weight(w_up, caches[0])
     h = grouped_gemm_fp8_bias_act(rows, qu, sx, su, plan.group_offs, bias_up, activation, zero_tail=True, **gate)

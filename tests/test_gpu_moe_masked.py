@@ -1,4 +1,5 @@
-"""The MoE layer on batches whose routing drops tokens (padding: all logits -inf), whatever those tokens hold."""
+"""The MoE layer on batches whose routing drops tokens (padding: all logits -inf), whatever those tokens hold, and on
+views of x."""
 import pytest
 import torch
 
@@ -63,3 +64,30 @@ def test_rows_counted_by_their_slots(pkg):
     assert am.item() == 0 and scale.item() == 1
     q, scale, am = pkg.quantize_fp8_tensorwise(torch.zeros((0, 16), device="cuda"), slots=none[:0])
     assert tuple(q.shape) == (0, 16) and am.item() == 0 and scale.item() == 1
+
+
+@pytest.mark.parametrize("view", ["columns", "odd rows", "transposed", "every second", "expanded"])
+def test_views_of_x(pkg, view):
+    """Rows that start off 16 bytes, rows that lie apart by odd strides, columns that are not contiguous, one row for
+    all tokens: both paths take what a copy of x gives."""
+    x, logits, w, layer = _layer(pkg, 40, 8, 128, 96, 3)
+    wide = torch.zeros((80, 141), dtype=torch.bfloat16, device="cuda")
+    if view == "columns":
+        wide[:40, 5:133] = x
+        v = wide[:40, 5:133]
+    elif view == "odd rows":
+        wide[:40, :128] = x
+        v = wide[:40, :128]
+    elif view == "transposed":
+        v = x.t().contiguous().t()
+    elif view == "every second":
+        wide[::2, :128] = x
+        v = wide[::2, :128]
+    else:
+        x = x[:1].expand(40, 128).contiguous()
+        v = x[:1].expand(40, 128)
+    assert torch.equal(v, x)
+    with torch.no_grad():
+        want = layer(x, logits, 3)
+        assert torch.equal(layer(v, logits, 3), want)
+    assert torch.equal(layer(v.detach().requires_grad_(), logits, 3), want)
