@@ -78,7 +78,8 @@ __device__ __forceinline__ void group_table(const Args& a, Table& t) {
   int units[kPer], sum = 0;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
-    units[k] = (o[k + 1] - o[k] + a.rows - 1) / a.rows;
+    // unsigned: 2^31 - 256 rows and a unit's 512 are more than 31 bits hold
+    units[k] = (int)(((uint32_t)(o[k + 1] - o[k]) + (uint32_t)a.rows - 1u) / (uint32_t)a.rows);
     sum += units[k];
   }
   int acc = sum;

@@ -324,3 +324,13 @@ def test_special_values_on_every_kernel(pkg, M, N, K, lens, rows, options, keep)
     if keep:
         assert torch.equal(torch.isnan(got[1][:offs[-1]]).all(0).nonzero().flatten().cpu(), torch.tensor([41, 100]))
         assert (got[1][:offs[-1], off] < -4e37).all()
+
+
+def test_bias_gradient_of_the_most_rows(pkg):
+    """2^31 - 256 rows in one group (and a few before it): their number plus a unit's rows is past 31 bits."""
+    M = 2 ** 31 - 256
+    dout = torch.ones((M, 16), dtype=torch.bfloat16, device="cuda")
+    _, dbias = pkg.bias_act_backward(dout, None, torch.tensor([0, M]).cuda())
+    assert (dbias == float(M)).all()                      # every partial sum is a multiple of 256 below 2^24 of them
+    _, dbias = pkg.bias_act_backward(dout, None, torch.tensor([0, 256, M]).cuda())
+    assert (dbias[0] == 256).all() and (dbias[1] == float(M - 256)).all()
