@@ -127,7 +127,7 @@ __device__ __forceinline__ void grad8(const v4i& z8, const v4i& d8, const epi::A
         out[i] = d[i] * (s + z[i] * s * (1.f - s));
       } else if constexpr (kAct == epi::kGelu) {
         float gauss;
-        const float cdf = epi::normal_cdf(z[i], &gauss);
+        const float cdf = epi::normal_cdf_fp32(z[i], &gauss);
         out[i] = d[i] * (cdf + z[i] * gauss * 0.398942280401433f);
       } else {
         out[i] = d[i];
