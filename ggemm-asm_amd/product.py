@@ -60,6 +60,61 @@ def _stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _product(a, b, a_scale, b_scale, group_offs, bias, residual, code, slope, limit, shift, keep, zero_tail):
+    """(out, preact or None) of checked arguments."""
+    (M, K), (G, N, _), dev = a.shape, b.shape, a.device
+    width = N // 2 if code == ACTIVATIONS["swiglu"] else N
+    if bias is not None:
+        bias = bias.detach().contiguous()
+        if bias.data_ptr() % 16:
+            bias = bias.clone()
+    if residual is not None:
+        residual = _rows16(residual)
+    out = torch.empty((M, width), dtype=torch.bfloat16, device=dev)
+    pre = torch.empty((M, N), dtype=torch.bfloat16, device=dev) if keep else None
+    if M:
+        # the strides of dimensions of size one are arbitrary and not used
+        sam, sbn = a.stride(0) if M > 1 else K, b.stride(1)
+        sbg = b.stride(0) if G > 1 else N * sbn
+        sres = 0 if residual is None else _stride(residual)
+        _lib.launch("ggemm_product_fp8_bias_act", dev, G | N | K | sam | sbg | sbn | sres, a.data_ptr(), b.data_ptr(),
+                    out.data_ptr(), None if pre is None else pre.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(),
+                    None if bias is None else bias.data_ptr(), 0 if bias is None else _IN[bias.dtype],
+                    None if residual is None else residual.data_ptr(), group_offs.data_ptr(), G, N, K, sam, sbg, sbn,
+                    width, N, sres, code, slope, limit, shift, M, int(bool(zero_tail)))
+    return out, pre
+
+
+class _BiasAct(torch.autograd.Function):
+    """The product as a function of its bias and residual: the fp8 operands have no gradients."""
+
+    @staticmethod
+    def forward(ctx, bias, residual, operands, epilogue, activation, options, keep_preact, zero_tail):
+        for_bias = activation is not None and ctx.needs_input_grad[0]     # its gradient reads z
+        out, pre = _product(*operands, bias, residual, *epilogue, keep_preact or for_bias, zero_tail)
+        ctx.save_for_backward(operands[-1], pre if for_bias else None)
+        ctx.activation, ctx.options = activation, options
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.set_materialize_grads(False)
+        if not keep_preact:
+            return out
+        ctx.mark_non_differentiable(pre)
+        return out, pre
+
+    @staticmethod
+    def backward(ctx, dout, *_):
+        group_offs, pre = ctx.saved_tensors
+        dbias = dres = None
+        if dout is not None and ctx.needs_input_grad[0]:
+            _, dbias = bias_act_backward(dout, pre, group_offs, ctx.activation, **ctx.options)
+            dbias = dbias.to(ctx.bias_dtype)
+        if dout is not None and ctx.needs_input_grad[1]:
+            # rows of no group are not written: they are no function of the residual
+            row = torch.arange(dout.shape[0], device=dout.device)
+            dres = torch.where(((row >= group_offs[0]) & (row < group_offs[-1]))[:, None], dout, 0)
+        return dbias, dres, None, None, None, None, None, None
+
+
 def grouped_gemm_fp8_bias_act(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor,
                               group_offs: torch.Tensor, bias: torch.Tensor | None = None,
                               activation: str | None = None, residual: torch.Tensor | None = None, *,
@@ -75,7 +130,10 @@ def grouped_gemm_fp8_bias_act(a: torch.Tensor, b: torch.Tensor, a_scale: torch.T
     +-limit, which halves the width. residual: bf16, as wide as the result. With ``keep_preact`` the result is
     ``(out, preact)``, preact the bf16 [M, N] value before the activation, for ``bias_act_backward``. Rows outside
     ``[0, offs[G])`` are left unwritten, or zero from offs[G] on with ``zero_tail``. ``validate=True`` checks group_offs
-    on the host first (a sync)."""
+    on the host first (a sync).
+
+    Differentiable by bias and residual (``grouped_linear_fp8`` is by the activations and weights too); the value before
+    the activation is then kept for the bias' gradient, and a ``preact`` that is returned carries no gradient itself."""
     if a.dim() != 2 or b.dim() != 3:
         raise ValueError("a must be 2-D [M, K] and b 3-D [G, N, K]")
     if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
@@ -100,27 +158,16 @@ def grouped_gemm_fp8_bias_act(a: torch.Tensor, b: torch.Tensor, a_scale: torch.T
     if bias is not None:
         if bias.dtype not in _IN or tuple(bias.shape) != (G, N) or bias.device != dev:
             raise ValueError(f"bias must be bf16 or fp32 [{G}, {N}] on a's device")
-        bias = bias.detach().contiguous()
-        if bias.data_ptr() % 16:
-            bias = bias.clone()
     if residual is not None:
         if residual.dtype != torch.bfloat16 or tuple(residual.shape) != (M, width) or residual.device != dev:
             raise ValueError(f"residual must be bf16 [{M}, {width}] on a's device")
-        residual = _rows16(residual)
     if validate:
         _validate_offsets(group_offs, M, mx=False)
-    out = torch.empty((M, width), dtype=torch.bfloat16, device=dev)
-    pre = torch.empty((M, N), dtype=torch.bfloat16, device=dev) if keep_preact else None
-    if M:
-        # the strides of dimensions of size one are arbitrary and not used
-        sam, sbn = a.stride(0) if M > 1 else K, b.stride(1)
-        sbg = b.stride(0) if G > 1 else N * sbn
-        sres = 0 if residual is None else _stride(residual)
-        _lib.launch("ggemm_product_fp8_bias_act", dev, G | N | K | sam | sbg | sbn | sres, a.data_ptr(), b.data_ptr(),
-                    out.data_ptr(), None if pre is None else pre.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(),
-                    None if bias is None else bias.data_ptr(), 0 if bias is None else _IN[bias.dtype],
-                    None if residual is None else residual.data_ptr(), group_offs.data_ptr(), G, N, K, sam, sbg, sbn,
-                    width, N, sres, code, slope, limit, shift, M, int(bool(zero_tail)))
+    operands, epilogue = (a, b, a_scale, b_scale, group_offs), (code, slope, limit, shift)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (bias, residual)):
+        options = {"slope": slope, "limit": limit, "shift": shift} if activation == "swiglu" else {}
+        return _BiasAct.apply(bias, residual, operands, epilogue, activation, options, keep_preact, zero_tail)
+    out, pre = _product(*operands, bias, residual, *epilogue, keep_preact, zero_tail)
     return (out, pre) if keep_preact else out
 
 
@@ -133,7 +180,7 @@ def bias_act_backward(dout: torch.Tensor, preact: torch.Tensor | None, group_off
 
     dout: bf16 [M, N] ([M, N / 2] for "swiglu"); preact: what ``grouped_gemm_fp8_bias_act`` kept; without an activation
     it may be None, and dpreact is dout itself, all its rows. Sums are made in a fixed order: the same inputs give the
-    same bits."""
+    same bits. The results carry no graph."""
     code, slope, limit, shift = _act(activation, slope, limit, shift)
     if dout.dim() != 2 or dout.dtype != torch.bfloat16:
         raise TypeError("dout must be a bf16 [M, N] tensor")

@@ -334,3 +334,32 @@ def test_bias_gradient_of_the_most_rows(pkg):
     assert (dbias == float(M)).all()                      # every partial sum is a multiple of 256 below 2^24 of them
     _, dbias = pkg.bias_act_backward(dout, None, torch.tensor([0, 256, M]).cuda())
     assert (dbias[0] == 256).all() and (dbias[1] == float(M - 256)).all()
+
+
+@pytest.mark.parametrize("activation,options", ACTS)
+@pytest.mark.parametrize("bias_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("keep", [False, True])
+def test_gradients_of_bias_and_residual(pkg, activation, options, bias_dtype, keep):
+    """The result as without gradients, bit for bit; the bias' gradient that of the kept z, the residual's the result's own
+    in the groups' rows and zero outside them. Tolerances as in test_gradient, and one rounding to the bias' type."""
+    lens = [0, 33, 1, 0, 36]
+    M, N, K = 77, 48, 144
+    a, b, sa, sb, offs, gen = _inputs(M, N, K, lens, 21)
+    width = N // 2 if activation == "swiglu" else N
+    args = (a.cuda(), b.cuda(), torch.tensor(sa).cuda(), torch.tensor(sb).cuda(), torch.tensor(offs).cuda())
+    bias = torch.randn((len(lens), N), generator=gen).to(bias_dtype).cuda()
+    res = torch.randn((M, width), generator=gen).to(torch.bfloat16).cuda()
+    dout = torch.randn((M, width), generator=gen).to(torch.bfloat16).cuda()
+    plain, pre = pkg.grouped_gemm_fp8_bias_act(*args, bias, activation, res, keep_preact=True, zero_tail=True, **options)
+    bias.requires_grad_()
+    res.requires_grad_()
+    got = pkg.grouped_gemm_fp8_bias_act(*args, bias, activation, res, keep_preact=keep, zero_tail=True, **options)
+    out = got[0] if keep else got
+    assert torch.equal(out, plain) and (not keep or torch.equal(got[1], pre))
+    out.backward(dout)
+    _, want, size = orx.backward(dout.cpu(), pre.cpu(), offs, activation, **options)
+    half = BF if bias_dtype == torch.bfloat16 else 0.0
+    reach = (float(pre[:offs[-1]].abs().max()) + 2) ** 2 * float(dout.abs().max()) * max(lens)
+    assert bias.grad.dtype == bias_dtype
+    assert ((bias.grad.cpu().double() - want).abs() <= 32 * U * reach + 17 * 2.0 ** -24 * size + 1.01 * half * want.abs()).all()
+    assert torch.equal(res.grad[:offs[-1]], dout[:offs[-1]]) and not res.grad[offs[-1]:].any()

@@ -1,0 +1,76 @@
+"""CPU checks of what autograd sees of the ops: which tensors get gradients, what is kept for them, and that
+derivatives the ops do not have are refused. Launches are replaced by nothing: values are arbitrary here."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+E4, BF = torch.float8_e4m3fn, torch.bfloat16
+
+
+@pytest.fixture
+def unlaunched(pkg, monkeypatch):
+    from ggemm_asm_amd import _lib, moe, product
+    calls = []
+    monkeypatch.setattr(_lib, "launch", lambda name, dev, sizes, *args: calls.append((name, args)))
+    for m in (moe, product):
+        monkeypatch.setattr(m, "_on_gpu", lambda *a: None)
+    return calls
+
+
+def _plan(pkg, T=4, k=2, G=3):
+    return pkg.DispatchPlan(torch.zeros(G + 1, dtype=torch.int64), torch.zeros((T, k), dtype=torch.int32))
+
+
+# name: (inputs that may require a gradient, the call on them)
+def _ops(pkg):
+    plan = _plan(pkg)
+    y, w, res = torch.randn(8, 16), torch.randn(4, 2), torch.randn(4, 16)
+    return {
+        "route": ([torch.randn(4, 6)], lambda x: pkg.route_experts(x, 2)[0]),
+        "dispatch": ([torch.randn(4, 16)], lambda x: pkg.dispatch_tokens(x, plan)),
+        "combine": ([y, w, res], lambda a, b, c: pkg.combine_tokens(a, plan, b, c)),
+        "product": ([torch.randn(3, 64), torch.randn((8, 32)).to(BF)], lambda b, r: _product(pkg, b, r, "swiglu")),
+    }
+
+
+def _product(pkg, bias, residual, activation, **kw):
+    a, b = torch.zeros((8, 32), dtype=E4), torch.zeros((3, 64, 32), dtype=E4)
+    return pkg.grouped_gemm_fp8_bias_act(a, b, torch.ones(()), torch.ones(()), torch.tensor([0, 2, 2, 6]), bias, activation,
+                                         residual, **kw)
+
+
+# --------------------------------------------------------------------------- bias and residual of the product
+
+@pytest.mark.parametrize("activation", [None, "silu", "swiglu"])
+@pytest.mark.parametrize("which", ["bias", "residual", "both"])
+@pytest.mark.parametrize("keep", [False, True])
+def test_product_keeps_the_graph_of_bias_and_residual(pkg, unlaunched, activation, which, keep):
+    bias = torch.randn((3, 64), dtype=BF).requires_grad_(which != "residual")
+    residual = torch.randn((8, 32 if activation == "swiglu" else 64)).to(BF).requires_grad_(which != "bias")
+    got = _product(pkg, bias, residual, activation, keep_preact=keep)
+    out = got[0] if keep else got
+    assert out.requires_grad and (not keep or not got[1].requires_grad)
+    assert [n for n, _ in unlaunched] == ["ggemm_product_fp8_bias_act"]
+    with torch.no_grad():
+        out.copy_(torch.zeros_like(out))
+    dout = torch.randn(out.shape).to(BF)
+    out.backward(dout)
+    if which != "residual":
+        assert bias.grad.dtype == BF and tuple(bias.grad.shape) == (3, 64)
+    else:
+        assert bias.grad is None
+    if which != "bias":
+        want = dout.clone()
+        want[6:] = 0                                  # rows of no group: the result does not depend on the residual there
+        assert torch.equal(residual.grad, want)
+    else:
+        assert residual.grad is None
+    assert [n for n, _ in unlaunched[1:]] == ([] if which == "residual" else ["ggemm_product_act_backward"])
+
+
+def test_product_without_gradients_keeps_nothing(pkg, unlaunched):
+    bias = torch.randn((3, 64)).requires_grad_()
+    with torch.no_grad():
+        assert not _product(pkg, bias, None, "silu").requires_grad
+    assert not _product(pkg, bias.detach(), None, "silu").requires_grad
+    assert all(args[3] is None for _, args in unlaunched)          # no z is written
