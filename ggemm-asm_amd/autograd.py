@@ -39,6 +39,7 @@ from __future__ import annotations
 import weakref
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .persistent import grouped_gemm_fp8_tensorwise
 from .product import bias_act_backward, grouped_gemm_fp8_bias_act
@@ -235,6 +236,7 @@ class GroupedLinearFP8(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         dx, dw = _backward_products(ctx, dy, *ctx.saved_tensors)
         return dx, dw, None, None, None, None
@@ -256,6 +258,7 @@ class GroupedLinearActFP8(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         *saved, pre = ctx.saved_tensors
         activation, options = ctx.act

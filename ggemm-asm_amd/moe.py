@@ -16,6 +16,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -76,6 +77,7 @@ class _Route(torch.autograd.Function):
         return weights, experts
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dweights, _):
         if dweights is None:
             return (None,) * 9
@@ -198,6 +200,7 @@ class _Dispatch(torch.autograd.Function):
         return _dispatch(x, offs, slots, row_align)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, drows):
         slots, = ctx.saved_tensors
         return _combine(_rows(drows), slots, None, None), None, None, None
@@ -210,6 +213,7 @@ class _Combine(torch.autograd.Function):
         return _combine(y, slots, weights, residual)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         y, weights, offs, slots = ctx.saved_tensors
         need_y, need_w, need_r = ctx.needs_input_grad[:3]

@@ -9,6 +9,7 @@ bench.py:238-247). Every launch goes through libggemm_vark.so on torch's current
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .vark import _validate_offsets
@@ -102,6 +103,7 @@ class _BiasAct(torch.autograd.Function):
         return out, pre
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, *_):
         group_offs, pre = ctx.saved_tensors
         dbias = dres = None

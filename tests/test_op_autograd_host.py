@@ -74,3 +74,24 @@ def test_product_without_gradients_keeps_nothing(pkg, unlaunched):
         assert not _product(pkg, bias, None, "silu").requires_grad
     assert not _product(pkg, bias.detach(), None, "silu").requires_grad
     assert all(args[3] is None for _, args in unlaunched)          # no z is written
+
+
+# --------------------------------------------------------------------------- derivatives that there are not
+
+@pytest.mark.parametrize("op", ["route", "dispatch", "combine", "product"])
+def test_second_derivatives_are_refused(pkg, unlaunched, op):
+    inputs, f = _ops(pkg)[op]
+    inputs = [t.requires_grad_() for t in inputs]
+    out = f(*inputs)
+    d = torch.randn_like(out).requires_grad_()
+    grads = torch.autograd.grad(out, inputs, d, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        sum(g.float().sum() for g in grads).backward()
+
+
+def test_every_backward_is_once_differentiable(pkg):
+    from ggemm_asm_amd import autograd, moe, product
+    for m in (autograd, moe, product):
+        for f in vars(m).values():
+            if isinstance(f, type) and issubclass(f, torch.autograd.Function) and f is not torch.autograd.Function:
+                assert hasattr(f.backward, "__wrapped__"), f
