@@ -39,8 +39,8 @@ from __future__ import annotations
 import weakref
 
 import torch
-from torch.autograd.function import once_differentiable
 
+from ._tensors import once_differentiable
 from .persistent import grouped_gemm_fp8_tensorwise
 from .product import bias_act_backward, grouped_gemm_fp8_bias_act
 from .quant import (quantize_fp8_tensorwise, quantize_fp8_tensorwise_delayed, quantize_fp8_tensorwise_transpose,

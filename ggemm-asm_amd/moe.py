@@ -16,9 +16,9 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
+from ._tensors import once_differentiable
 
 _IN = {torch.bfloat16: 0, torch.float32: 1}
 _SCORES = {"softmax": 0, "sigmoid": 1}
