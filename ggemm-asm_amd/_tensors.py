@@ -4,6 +4,7 @@ from __future__ import annotations
 import functools
 
 import torch
+import torch.autograd.forward_ad as fwAD
 from torch.autograd.function import once_differentiable as _once_differentiable
 
 
@@ -17,3 +18,14 @@ def once_differentiable(backward):
         return refusing(ctx, *args) if torch.is_grad_enabled() else backward(ctx, *args)
 
     return wrapper
+
+
+def tracked(*tensors: torch.Tensor | None) -> bool:
+    """Whether autograd has to see a call on these tensors (None for none): one requires a gradient, or has a
+    forward-mode tangent, which the ops have no rule for and their autograd functions refuse."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    # the level is asked first: outside of dual levels, nearly always, no tensor has to be
+    return fwAD._current_level >= 0 and any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors)

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import torch
 
+from ._tensors import tracked
 from .autograd import FP8DelayedScaling, FP8WeightCache, grouped_linear_fp8
 from .moe import combine_tokens, dispatch_tokens, plan_dispatch, route_experts
 from .product import _rows16, grouped_gemm_fp8_bias_act
@@ -51,7 +52,7 @@ def moe_layer_fp8(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, w_d
     gate = {"slope": slope, "limit": limit, "shift": shift}
     caches = weight_caches or (None, None)
     params = (x, logits, w_up, w_down, bias_up, bias_down, residual)
-    if torch.is_grad_enabled() and (main_grads is not None or any(t is not None and t.requires_grad for t in params)):
+    if (torch.is_grad_enabled() and main_grads is not None) or tracked(*params):
         mains, scales = main_grads or (None, None), scalings or (None, None)
         h = grouped_linear_fp8(dispatch_tokens(x, plan), w_up, plan.group_offs, mains[0], caches[0], scales[0],
                                bias=bias_up, activation=activation, **gate)

@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from ._tensors import once_differentiable
+from ._tensors import once_differentiable, tracked
 
 _IN = {torch.bfloat16: 0, torch.float32: 1}
 _SCORES = {"softmax": 0, "sigmoid": 1}
@@ -127,7 +127,7 @@ def route_experts(logits: torch.Tensor, top_k: int, *, score: str = "softmax", b
             raise ValueError(f"bias must be fp32 [{E}] on the logits' device")
         bias = bias.detach().contiguous()
     args = (top_k, _SCORES[score], bias, num_groups, top_groups, group_best, int(bool(renormalize)), float(scale))
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if tracked(logits):
         return _Route.apply(_rows(logits), *args)
     return _route(_rows(logits), *args)
 
@@ -247,7 +247,7 @@ def dispatch_tokens(x: torch.Tensor, plan: DispatchPlan, row_align: int | None =
         raise ValueError(f"x holds {x.shape[0]} tokens, the plan {slots.shape[0]}")
     if row_align is not None and (row_align < 1 or row_align % x.element_size()):
         raise ValueError("row_align must be a multiple of the element size")
-    if torch.is_grad_enabled() and x.requires_grad:
+    if tracked(x):
         if x.dtype not in _IN:
             raise TypeError(f"gradients flow to bf16 or fp32 tokens only, got {x.dtype}")
         return _Dispatch.apply(_rows(x), offs, slots, row_align)
@@ -273,6 +273,6 @@ def combine_tokens(y: torch.Tensor, plan: DispatchPlan, weights: torch.Tensor | 
         if residual.dtype != y.dtype or tuple(residual.shape) != (T, y.shape[1]) or residual.device != y.device:
             raise ValueError(f"residual must be {y.dtype} [{T}, {y.shape[1]}] on y's device")
         residual = _rows(residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (y, weights, residual)):
+    if tracked(y, weights, residual):
         return _Combine.apply(_rows(y), weights, residual, offs, slots)
     return _combine(_rows(y), slots, weights, residual)

@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._tensors import once_differentiable
+from ._tensors import once_differentiable, tracked
 from .vark import _validate_offsets
 
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "swiglu": 3}
@@ -166,8 +166,7 @@ def grouped_gemm_fp8_bias_act(a: torch.Tensor, b: torch.Tensor, a_scale: torch.T
     if validate:
         _validate_offsets(group_offs, M, mx=False)
     operands, epilogue = (a, b, a_scale, b_scale, group_offs), (code, slope, limit, shift)
-    if torch.is_grad_enabled() and (bias is not None and bias.requires_grad or
-                                    residual is not None and residual.requires_grad):
+    if tracked(bias, residual):
         options = {"slope": slope, "limit": limit, "shift": shift} if activation == "swiglu" else {}
         return _BiasAct.apply(bias, residual, operands, epilogue, activation, options, keep_preact, zero_tail)
     out, pre = _product(*operands, bias, residual, *epilogue, keep_preact, zero_tail)

@@ -95,3 +95,16 @@ def test_every_backward_is_once_differentiable(pkg):
         for f in vars(m).values():
             if isinstance(f, type) and issubclass(f, torch.autograd.Function) and f is not torch.autograd.Function:
                 assert hasattr(f.backward, "__wrapped__"), f
+
+
+@pytest.mark.parametrize("op", ["route", "dispatch", "combine", "product"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(pkg, unlaunched, op, grad):
+    """Forward-mode derivatives of each input, with reverse mode on or off: an error, not a result without them."""
+    inputs, f = _ops(pkg)[op]
+    for i in range(len(inputs)):
+        with fwAD.dual_level(), torch.set_grad_enabled(grad):
+            args = [fwAD.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(inputs)]
+            with pytest.raises(RuntimeError, match="jvp"):
+                f(*args)
+            assert not f(*inputs).requires_grad
