@@ -209,7 +209,9 @@ class _Dispatch(torch.autograd.Function):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, residual, offs, slots):
-        ctx.save_for_backward(y, weights, offs, slots)
+        need_y, need_w, _ = ctx.needs_input_grad[:3]      # y is read for the weights' gradient alone, the weights for y's
+        ctx.save_for_backward(y if need_w else None, weights if need_y else None, offs, slots)
+        ctx.y_shape = y.shape
         return _combine(y, slots, weights, residual)
 
     @staticmethod
@@ -217,15 +219,15 @@ class _Combine(torch.autograd.Function):
     def backward(ctx, dout):
         y, weights, offs, slots = ctx.saved_tensors
         need_y, need_w, need_r = ctx.needs_input_grad[:3]
-        (M, H), (T, k) = y.shape, slots.shape
+        (M, H), (T, k), dev = ctx.y_shape, slots.shape, slots.device
         dres = dout if need_r else None
         dout = _rows(dout)
-        dy = torch.empty((M, H), dtype=y.dtype, device=y.device) if need_y else None
-        dw = torch.empty((T, k), dtype=torch.float32, device=y.device) if need_w else None
+        dy = torch.empty((M, H), dtype=dout.dtype, device=dev) if need_y else None
+        dw = torch.empty((T, k), dtype=torch.float32, device=dev) if need_w else None
         if T and H and M:
             G = offs.numel() - 1
-            _lib.launch("ggemm_moe_combine_backward", y.device, H | k | G, dout.data_ptr(), _IN[y.dtype], _stride(dout),
-                        y.data_ptr(), _stride(y), M, slots.data_ptr(), T, k,
+            _lib.launch("ggemm_moe_combine_backward", dev, H | k | G, dout.data_ptr(), _IN[dout.dtype], _stride(dout),
+                        None if y is None else y.data_ptr(), H if y is None else _stride(y), M, slots.data_ptr(), T, k,
                         None if weights is None else weights.data_ptr(), offs.data_ptr(), G, H,
                         None if dy is None else dy.data_ptr(), H, None if dw is None else dw.data_ptr())
         else:

@@ -341,3 +341,20 @@ def test_long_tensors_use_64_bit_offsets(pkg):
     assert (rows[T - 2] == 3).all() and (rows[T // 2 - 1] == 5).all() and (rows[T - 1] == 0).all()
     back = pkg.combine_tokens(rows, plan)
     assert torch.equal(back[-1], x[-1]) and torch.equal(back[T // 2], x[T // 2]) and not back[:T // 2].any()
+
+
+@pytest.mark.parametrize("T,k,G,H,dropped", SIZES)
+@pytest.mark.parametrize("which", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1)])
+def test_combine_gradients_one_by_one(pkg, T, k, G, H, dropped, which):
+    """Each gradient by itself is what it is among the others, bit for bit."""
+    plan, gen = _some_plan(pkg, T, k, G, dropped)
+    parts = [torch.randn((T * k, H), generator=gen), torch.randn((T, k), generator=gen), torch.randn((T, H), generator=gen)]
+    dout = torch.randn((T, H), generator=gen).cuda()
+
+    def grads(on):
+        leaves = [t.cuda().requires_grad_(bool(g)) for t, g in zip(parts, on)]
+        pkg.combine_tokens(leaves[0], plan, leaves[1], leaves[2]).backward(dout)
+        return [t.grad for t in leaves]
+
+    for some, full, g in zip(grads(which), grads((1, 1, 1)), which):
+        assert (some is not None) == bool(g) and (not g or torch.equal(some, full))

@@ -108,3 +108,26 @@ def test_tangents_are_refused(pkg, unlaunched, op, grad):
             with pytest.raises(RuntimeError, match="jvp"):
                 f(*args)
             assert not f(*inputs).requires_grad
+
+
+# --------------------------------------------------------------------------- what is kept
+
+def test_combine_keeps_only_what_its_gradients_read(pkg, unlaunched):
+    """y for the weights' gradient, the weights for y's."""
+    plan = _plan(pkg)
+    for grads, kept in (((1, 0, 0), "w"), ((0, 1, 0), "y"), ((1, 1, 0), "yw"), ((0, 0, 1), ""), ((1, 0, 1), "w")):
+        t = {n: v.requires_grad_(bool(g)) for (n, v), g in
+             zip(dict(y=torch.randn(8, 16), w=torch.randn(4, 2), r=torch.randn(4, 16)).items(), grads)}
+        out = pkg.combine_tokens(t["y"], plan, t["w"], t["r"])
+        held = {s.data_ptr() for s in out.grad_fn.saved_tensors if s is not None}
+        assert {n for n in "yw" if t[n].data_ptr() in held} == set(kept), grads
+        out.backward(torch.randn_like(out))
+        for (n, v), g in zip(t.items(), grads):
+            assert (v.grad is not None) == bool(g) and (not g or v.grad.shape == v.shape)
+
+
+def test_combine_gradient_of_y_alone_reads_no_y(pkg, unlaunched):
+    y = torch.randn(8, 16).requires_grad_()
+    pkg.combine_tokens(y, _plan(pkg), torch.randn(4, 2)).sum().backward()
+    name, args = unlaunched[-1]
+    assert name == "ggemm_moe_combine_backward" and args[3] is None and args[-1] is None
