@@ -132,10 +132,10 @@ struct Choice {
 // this; N = 5760, K = 2880 but as said): 1 row of 1 expert 12.9 -> 6.7, 2 rows of 2 13.2 -> 8.8, 4 of 4 16.8 ->
 // 14.0, 8 of 8 26.8 -> 25.7, 64 of 8 30.3 -> 29.8, 128 of 8 30.0 -> 38.5 (stays), 32 of 22 63.2 -> 67.2 (stays);
 // 128 of 16, N = K = 4096 61.8 -> 52.8; 16 of 15, N = 1536, K = 1024 8.6 -> 9.5 (stays).
-bool few_preferred(const nt::Args& a, int64_t g) {
-  const int64_t fit = 3 * 256;                         // workgroups of 32 columns, three to a CU
-  return a.G <= ggemm::mid::kMaxGroups && a.m_total <= 8 * (g + 1) && g * ((a.N + 127) / 128) <= 512 &&
-         (a.K >= 2048 || g * ((a.N + 31) / 32) <= fit / 2);
+constexpr int64_t kFewPerCu = 3;                         // workgroups of either width that a CU holds
+bool few_preferred(const nt::Args& a, int64_t g, int64_t cus) {
+  return a.G <= ggemm::mid::kMaxGroups && a.m_total <= 8 * (g + 1) && g * ((a.N + 127) / 128) <= 2 * cus &&
+         (a.K >= 2048 || g * ((a.N + 31) / 32) <= kFewPerCu * cus / 2);
 }
 
 // The others. Against the estimates of the plain product: the large tiles' epilogue takes 3 us a tile, 12 with z
@@ -146,8 +146,8 @@ bool few_preferred(const nt::Args& a, int64_t g) {
 Choice choose(const nt::Args& a, const epi::Args& e, int act, int cus) {
   const int64_t run = ggemm::kXcds * ggemm::mid::kXcdRun, g = std::min<int64_t>(a.G, a.m_total);
   auto runs = [&](int64_t tiles) { return (tiles + run - 1) / run * run; };
-  if (few_preferred(a, g)) {
-    const bool narrow = g * ((a.N + 15) / 16) <= 3 * 256;
+  if (few_preferred(a, g, cus)) {
+    const bool narrow = g * ((a.N + 15) / 16) <= kFewPerCu * cus;
     const int64_t row_tiles = a.m_total / 16 + g, bn = narrow ? 16 : 32;
     return {narrow ? Kernel::kFew16 : Kernel::kFew32, 0, runs(row_tiles * ((a.N + bn - 1) / bn))};
   }

@@ -150,3 +150,17 @@ def test_oracle_gradient_against_differences(activation, options):
         dn[:, c] -= h
         diff = ((orx.act(up, activation, **options) - orx.act(dn, activation, **options)) * d).sum(1) / (2 * h)
         torch.testing.assert_close(dpre[:, c], diff, atol=1e-8, rtol=0)
+
+
+def test_few_rows_by_the_devices_cus(pkg):
+    """The few-rows kernel is for launches whose mid tiles leave CUs without their two: on a quarter or an eighth of the
+    CUs (a partitioned card) that is a quarter or an eighth of the tiles."""
+    from ggemm_asm_amd import product
+    for cus in (256, 128, 64, 32):
+        for G in (1, 2, 4, 8, 16, 32):
+            for N in (640, 1536, 2880, 5760):
+                mid = G * -(-N // 128)
+                rows = product.tile_rows(G, N, 4096, G, "silu", num_cus=cus)
+                assert (rows == 16) == (mid <= 2 * cus), (cus, G, N, rows)
+    # short rows of K: while the workgroups of 32 columns, three to a CU, leave half of the places free
+    assert product.tile_rows(2, 1536, 1024, 2, num_cus=256) == 16 and product.tile_rows(2, 1536, 1024, 2, num_cus=32) == 64
