@@ -3,7 +3,7 @@
 //   z[r, :] = s_a s_b A[r, :] @ B[g]^T + bias[g, :];  out = act(z) + residual     (fused_epilogue.h)
 //
 // Such a launch is bound by reading the weights once, so nothing but loads in flight counts: a workgroup
-// takes 16 R rows of one group and 16 NB columns, and its four waves share the K axis, wave w the 128-byte
+// takes 16 rows of one group and 16 NB columns, and its four waves share the K axis, wave w the 128-byte
 // steps w, w + 4, ..: a row's consecutive lines are asked for at once, by different waves, and a wave of
 // K = 2880 has its whole part, 12 KiB per 16 columns, in flight before its first MFMA. No LDS stages and no barrier before
 // the end, where the waves' sums are added in their order through LDS. 4 rows of 4 experts, 5760 x 2880 (66 MB of
@@ -25,15 +25,15 @@ namespace few {
 constexpr int kNT = 256, kWaves = 4;
 constexpr int kBatch = 6;            // steps a wave has in flight: all of its share of up to 24
 
-template <int R, int NB>
+template <int NB>
 struct Cfg {
-  static constexpr int BM = 16 * R, BN = 16 * NB;
-  static constexpr int LdsBytes = kWaves * R * NB * 1024;
+  static constexpr int BM = 16, BN = 16 * NB;
+  static constexpr int LdsBytes = kWaves * NB * 1024;
 };
 
-template <int kAct, int R, int NB>
+template <int kAct, int NB>
 __device__ __forceinline__ void body(const nt::Args& a, GG_LDS uint8_t* lds, const epi::Args& e) {
-  using C = Cfg<R, NB>;
+  using C = Cfg<NB>;
   constexpr bool kGated = kAct == epi::kSwiglu;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -76,11 +76,9 @@ __device__ __forceinline__ void body(const nt::Args& a, GG_LDS uint8_t* lds, con
   const auto rb = __builtin_amdgcn_make_buffer_rsrc(
       const_cast<uint8_t*>(a.b) + (int64_t)g * a.stride_bg + (int64_t)n0 * a.stride_bn, 0,
       (cols - 1) * a.stride_bn + a.K, kRsrcWord3);
-  v4f acc[R][NB];
+  v4f acc[NB];
 #pragma unroll
-  for (int i = 0; i < R; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < NB; ++j) acc[j] = v4f{0.f, 0.f, 0.f, 0.f};
   const int nsteps = (a.K + 127) / 128;
   auto load = [&](__amdgpu_buffer_rsrc_t r, int row, int stride, int k) {
     v8i x;
@@ -95,39 +93,34 @@ __device__ __forceinline__ void body(const nt::Args& a, GG_LDS uint8_t* lds, con
     return x;
   };
   for (int s0 = wave; s0 < nsteps; s0 += kWaves * kBatch) {
-    v8i w[kBatch][NB], x[kBatch][R];
+    v8i w[kBatch][NB], x[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const int k = 128 * (s0 + kWaves * u);                 // at or past K: zeros
 #pragma unroll
       for (int j = 0; j < NB; ++j) w[u][j] = load(rb, 16 * j + s, a.stride_bn, k);
-#pragma unroll
-      for (int i = 0; i < R; ++i) x[u][i] = load(ra, 16 * i + s, a.stride_am, k);
+      x[u] = load(ra, s, a.stride_am, k);
     }
     __builtin_amdgcn_sched_barrier(0);                       // every load before the first use
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
 #pragma unroll
-      for (int i = 0; i < R; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[u][j], x[u][i], acc[i][j], 0, 0, 0, 0, 0, 0);
+      for (int j = 0; j < NB; ++j)
+        acc[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[u][j], x[u], acc[j], 0, 0, 0, 0, 0, 0);
   }
 
   // ---- the waves' sums, block b of the tile finished by wave b % 4
   GG_LDS v4f* s_acc = (GG_LDS v4f*)lds;                      // [wave][block][lane]
 #pragma unroll
-  for (int i = 0; i < R; ++i)
-#pragma unroll
-    for (int j = 0; j < NB; ++j) s_acc[(wave * R * NB + i * NB + j) * 64 + lane] = acc[i][j];
+  for (int j = 0; j < NB; ++j) s_acc[(wave * NB + j) * 64 + lane] = acc[j];
   __syncthreads();
   const float alpha = *a.a_scale * *a.b_scale;
-  for (int b = wave; b < R * NB; b += kWaves) {
-    const int r = 16 * (b / NB) + s, n = n0 + 16 * (b % NB) + 4 * q;
+  for (int b = wave; b < NB; b += kWaves) {
+    const int r = s, n = n0 + 16 * b + 4 * q;
     if (r >= rows || n >= a.N) continue;
     v4f z = s_acc[b * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) z += s_acc[(w * R * NB + b) * 64 + lane];
+    for (int w = 1; w < kWaves; ++w) z += s_acc[(w * NB + b) * 64 + lane];
     z = z * alpha + epi::load_bias(e, (int64_t)g * a.N + n);
     const int64_t row = (int64_t)row_base + m0 + r;
     if (e.pre != nullptr) *(v2i*)(e.pre + row * e.stride_pre + n) = v2i{epi::pack(z[0], z[1]), epi::pack(z[2], z[3])};

@@ -43,10 +43,10 @@ __global__ __launch_bounds__(ggemm::mid::kNT, 2) void product_mid_kernel(nt::Arg
   clear_tails<kAct>(a, e);
 }
 
-template <int kAct, int R, int NB>
+template <int kAct, int NB>
 __global__ __launch_bounds__(ggemm::few::kNT) void product_few_kernel(nt::Args a, epi::Args e) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[ggemm::few::Cfg<R, NB>::LdsBytes];
-  ggemm::few::body<kAct, R, NB>(nt::without_tail(a), (GG_LDS uint8_t*)lds, e);
+  __shared__ __attribute__((aligned(16))) uint8_t lds[ggemm::few::Cfg<NB>::LdsBytes];
+  ggemm::few::body<kAct, NB>(nt::without_tail(a), (GG_LDS uint8_t*)lds, e);
   clear_tails<kAct>(a, e);
 }
 
@@ -204,10 +204,10 @@ int ggemm_product_fp8_bias_act(const void* a, const void* b, void* out, void* pr
     const dim3 grid((uint32_t)k.workgroups);
     switch (k.kernel) {
       case Kernel::kFew16:
-        hipLaunchKernelGGL((product_few_kernel<kAct, 1, 1>), grid, dim3(ggemm::few::kNT), 0, (hipStream_t)stream, x, e);
+        hipLaunchKernelGGL((product_few_kernel<kAct, 1>), grid, dim3(ggemm::few::kNT), 0, (hipStream_t)stream, x, e);
         break;
       case Kernel::kFew32:
-        hipLaunchKernelGGL((product_few_kernel<kAct, 1, 2>), grid, dim3(ggemm::few::kNT), 0, (hipStream_t)stream, x, e);
+        hipLaunchKernelGGL((product_few_kernel<kAct, 2>), grid, dim3(ggemm::few::kNT), 0, (hipStream_t)stream, x, e);
         break;
       case Kernel::kMid64:
         hipLaunchKernelGGL((product_mid_kernel<kAct, 64>), grid, dim3(ggemm::mid::kNT), 0, (hipStream_t)stream, x, e);
