@@ -8,6 +8,16 @@ import torch.autograd.forward_ad as fwAD
 from torch.autograd.function import once_differentiable as _once_differentiable
 
 
+def on_gpu(t: torch.Tensor, what: str) -> None:
+    if t.device.type != "cuda":
+        raise ValueError(f"{what} runs on a gfx950 GPU only (tensors are on {t.device})")
+
+
+def row_stride(t: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor; where there is one row its own is arbitrary and not used."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
 def once_differentiable(backward):
     """torch's once_differentiable, entered only under create_graph=True: everywhere else a backward pass runs without
     grad mode anyway, where torch's wrapper would cost 4 us (of the 86 of a routing step and its gradient)."""

@@ -18,7 +18,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from ._tensors import once_differentiable, tracked
+from ._tensors import on_gpu as _on_gpu, once_differentiable, row_stride as _stride, tracked
 
 _IN = {torch.bfloat16: 0, torch.float32: 1}
 _SCORES = {"softmax": 0, "sigmoid": 1}
@@ -35,20 +35,11 @@ class DispatchPlan(NamedTuple):
     slots: torch.Tensor
 
 
-def _on_gpu(t: torch.Tensor, what: str):
-    if t.device.type != "cuda":
-        raise ValueError(f"{what} runs on a gfx950 GPU only (tensors are on {t.device})")
-
-
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """A 2-D tensor whose rows are contiguous and do not overlap (a copy where they are not)."""
     if t.stride(1) != 1 and t.shape[1] > 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
         return t.contiguous()
     return t
-
-
-def _stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 # --------------------------------------------------------------------------- routing

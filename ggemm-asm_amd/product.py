@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._tensors import once_differentiable, tracked
+from ._tensors import on_gpu as _on_gpu, once_differentiable, row_stride as _stride, tracked
 from .vark import _validate_offsets
 
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "swiglu": 3}
@@ -38,11 +38,6 @@ def tile_rows(G: int, N: int, K: int, M: int, activation: str | None = None, *, 
                                                N if keep_preact else 0, ACTIVATIONS[activation], int(residual), M, num_cus)
 
 
-def _on_gpu(t: torch.Tensor, what: str):
-    if t.device.type != "cuda":
-        raise ValueError(f"{what} runs on a gfx950 GPU only (tensors are on {t.device})")
-
-
 def _check_offs(group_offs, dev):
     if group_offs.dtype != torch.int64 or group_offs.dim() != 1 or not 2 <= group_offs.numel() <= MAX_GROUPS + 1:
         raise ValueError(f"group_offs must be int64 [G+1] with G <= {MAX_GROUPS}")
@@ -55,10 +50,6 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     if t.stride(1) != 1 or t.data_ptr() % 16 or t.shape[0] > 1 and (t.stride(0) % 8 or t.stride(0) < t.shape[1]):
         return t.clone(memory_format=torch.contiguous_format)
     return t
-
-
-def _stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _product(sizes, operands, bias, residual, epilogue, keep, zero_tail):

@@ -14,6 +14,7 @@ import operator
 import torch
 
 from . import _lib
+from ._tensors import row_stride as _row_stride
 
 GGEMM_IN_BF16 = 0
 GGEMM_IN_F32 = 1
@@ -37,12 +38,6 @@ def _as_2d(x: torch.Tensor) -> torch.Tensor:
         # distinct elements, so hand them a copy that holds them
         x = x.contiguous()
     return x
-
-
-def _row_stride(x2: torch.Tensor) -> int:
-    """Row stride to hand the library for a 2-D view from ``_as_2d``: its own, except for a view of
-    at most one row, whose stride(0) torch leaves arbitrary and the kernels never use."""
-    return x2.stride(0) if x2.shape[0] > 1 else x2.shape[1]
 
 
 def _ptr(x2: torch.Tensor) -> int:
