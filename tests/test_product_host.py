@@ -164,3 +164,38 @@ def test_few_rows_by_the_devices_cus(pkg):
                 assert (rows == 16) == (mid <= 2 * cus), (cus, G, N, rows)
     # short rows of K: while the workgroups of 32 columns, three to a CU, leave half of the places free
     assert product.tile_rows(2, 1536, 1024, 2, num_cus=256) == 16 and product.tile_rows(2, 1536, 1024, 2, num_cus=32) == 64
+
+
+def _unit_rows(M, N):
+    """Rows of a unit as the launcher cuts them: 64, down to 16 while the units are fewer than 2048, more where they
+    would be more than 2^22."""
+    strips = -(-N // 8 // 256)
+    rows = 64
+    while rows > 16 and M // rows * strips < 2048:
+        rows //= 2
+    while M // rows * strips > 1 << 22:
+        rows *= 2
+    return rows
+
+
+@pytest.mark.parametrize("N", [16, 64, 2064, 5760])
+def test_workspace_of_the_worst_groups(pkg, N):
+    """A group of n rows leaves ceil(n / rows) rows of partial sums. The most units that M rows of G groups can have, each
+    group one row past a multiple of a unit, are within the workspace."""
+    f = pkg.load_library().ggemm_product_act_workspace
+    for M in (1, 2, 15, 16, 17, 1000, 4099, 32768, 131072, 131073, 10 ** 7, 2 ** 31 - 256):
+        rows = _unit_rows(M, N)
+        for G in (1, 2, 5, 32, 60, 2047):
+            lens, left = [], M
+            for _ in range(min(G, M)):                        # one row each: a unit each
+                lens.append(1)
+                left -= 1
+            lens[0] += left // rows * rows                    # whole units
+            left -= left // rows * rows
+            if left:
+                lens[-1] += left
+            assert sum(lens) == M
+            units, g = sum(-(-n // rows) for n in lens), min(G, M)
+            assert units == g + (M - g) // rows               # the most: ceil(n / rows) is one more than (n - 1) // rows
+            have = f(M, G, N)
+            assert have % N == 0 and units * N <= have <= (M // rows + g) * N
