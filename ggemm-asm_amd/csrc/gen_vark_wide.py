@@ -1250,7 +1250,7 @@ class GenK(Gen):
 
 # ---------------------------------------------------------------- products with an epilogue
 #
-# The K-major forward tile with bias and activation (product_wide.h): z = alpha acc + bias, then
+# The K-major forward tile with bias and activation (persistent_wide.h, launched by product_capi.hip): z = alpha acc + bias, then
 #   bias      z rounded to bf16 is C;
 #   gate      swiglu of neighbouring columns (z0, z1), (z2, z3) .., half as wide as the tile: v = min(z0, limit)
 #             sigmoid(slope v) (clamp(z1, limit) + shift);
@@ -1502,8 +1502,8 @@ STORE_HINT = {"z": " nt", "o": ""}
 
 def render():
     out = ["// Generated by gen_vark_wide.py; do not edit. Per-tile bodies of the wide-tile FP8 grouped",
-           "// wgrad kernels (vark_wide.h) and of the wide persistent fwd / dgrad kernel (persistent_wide.h, with an",
-           "// epilogue product_wide.h):",
+           "// wgrad kernels (vark_wide.h) and of the wide persistent fwd / dgrad kernel (persistent_wide.h), plain",
+           "// and with an epilogue:",
            "// gfx950 assembly, one inline asm statement per tile shape."]
     total = 0
     for c in CONFIGS + SWAPPED_CONFIGS + KCONFIGS + KECONFIGS:
