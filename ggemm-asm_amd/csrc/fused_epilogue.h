@@ -33,21 +33,20 @@ __device__ __forceinline__ float sigmoid2(float x) { return __builtin_amdgcn_rcp
 __device__ __forceinline__ float sigmoid(float x) { return sigmoid2(x * -kLog2e); }
 
 // The normal distribution's cdf and e^(-x^2 / 2). With y = |x| / sqrt 2, erfc(y) e^(y^2) is smooth and falls like 1 / y: it
-// is fitted as t P(t), t = 1 / (1 + 0.42 y), P of degree 9 with the least largest relative error over y = 0 .. 10.5, 2.7e-9
-// (the coefficients hold the half of cdf(-|x|) = erfc(y) / 2). In fp32 the cdf of x < 0 is off by at most 3 units of 2^-23 of
-// its own value and, by the exponent's rounding, x^2 / 2 more (7.5e-6 at -12.5); of x > 0 by 2.6e-7. Four more fused
-// multiply-adds than an approximation bounded by 1.5e-7 of one, which is all error at x = -6.
+// is fitted as t P(t), t = 1 / (1 + 0.44 y), P of degree 7 with the least largest relative error over y = 0 .. 10.5, 1.8e-7
+// (the coefficients hold the half of cdf(-|x|) = erfc(y) / 2). In fp32 the cdf of x < 0 is off by at most 5 units of 2^-23 of
+// its own value and, by the exponent's rounding, x^2 / 2 more (7.4e-6 at -12.5); of x > 0 by 3.2e-7. An instruction more
+// than an approximation that is bounded by 1.5e-7 of one, which is all error far below zero. Degree 9 (2.7e-9) took two
+// more: 131072 x 5760 x 2880 with gelu and a residual 2.352 ms, 2.330 so, 2.331 with the former.
 __device__ __forceinline__ float normal_cdf(float x, float* gauss) {
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.296984851f, fabsf(x), 1.f));
-  float p = fmaf(t, -0.0203895364f, 0.114417687f);
-  p = fmaf(t, p, -0.241212383f);
-  p = fmaf(t, p, 0.21588105f);
-  p = fmaf(t, p, -0.0965218768f);
-  p = fmaf(t, p, 0.105768539f);
-  p = fmaf(t, p, 0.0753823146f);
-  p = fmaf(t, p, 0.109873407f);
-  p = fmaf(t, p, 0.118314557f);
-  p = fmaf(t, p, 0.118486248f);
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.311126977f, fabsf(x), 1.f));
+  float p = fmaf(t, 0.0356666967f, -0.139214039f);
+  p = fmaf(t, p, 0.148778901f);
+  p = fmaf(t, p, -0.0105133327f);
+  p = fmaf(t, p, 0.108143263f);
+  p = fmaf(t, p, 0.108580425f);
+  p = fmaf(t, p, 0.124448597f);
+  p = fmaf(t, p, 0.124109574f);
   *gauss = __builtin_amdgcn_exp2f(x * x * -0.721347520444482f);
   const float below = t * p * *gauss;
   return x > 0.f ? 1.f - below : below;
@@ -58,7 +57,7 @@ __device__ __forceinline__ float gelu_cdf(float x) {
 }
 
 // The same for sums that are kept in fp32: up to |x| = 1.25 the cdf as 1/2 + x Q(x^2), whose error is that of its last
-// rounding (Q of degree 5 with the least largest error of x Q, 2.1e-9): 5e-8, 7e-8 past it.
+// rounding (Q of degree 5 with the least largest error of x Q, 2.1e-9): 4e-8, 8e-8 past it.
 __device__ __forceinline__ float normal_cdf_fp32(float x, float* gauss) {
   const float far = normal_cdf(x, gauss), h = x * x;
   float q = fmaf(h, -6.64485742e-06f, 0.000110327448f);
