@@ -52,10 +52,9 @@ def _rows16(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _product(sizes, operands, bias, residual, epilogue, keep, zero_tail):
+def _product(bias, residual, keep, a, b, a_scale, b_scale, group_offs, M, N, K, G, width, dev, code, slope, limit, shift,
+             zero_tail):
     """(out, preact or None) of checked arguments."""
-    M, N, K, G, width, dev = sizes
-    a, b, a_scale, b_scale, group_offs = operands
     if bias is not None:
         bias = bias.detach().contiguous()
         if bias.data_ptr() % 16:
@@ -73,7 +72,7 @@ def _product(sizes, operands, bias, residual, epilogue, keep, zero_tail):
                     out.data_ptr(), None if pre is None else pre.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(),
                     None if bias is None else bias.data_ptr(), 0 if bias is None else _IN[bias.dtype],
                     None if residual is None else residual.data_ptr(), group_offs.data_ptr(), G, N, K, sam, sbg, sbn,
-                    width, N, sres, *epilogue, M, int(bool(zero_tail)))
+                    width, N, sres, code, slope, limit, shift, M, int(bool(zero_tail)))
     return out, pre
 
 
@@ -81,10 +80,10 @@ class _BiasAct(torch.autograd.Function):
     """The product as a function of its bias and residual: the fp8 operands have no gradients."""
 
     @staticmethod
-    def forward(ctx, bias, residual, sizes, operands, epilogue, activation, options, keep_preact, zero_tail):
+    def forward(ctx, bias, residual, keep_preact, group_offs, activation, options, args):
         for_bias = activation is not None and ctx.needs_input_grad[0]     # its gradient reads z
-        out, pre = _product(sizes, operands, bias, residual, epilogue, keep_preact or for_bias, zero_tail)
-        ctx.save_for_backward(operands[-1], pre if for_bias else None)
+        out, pre = _product(bias, residual, keep_preact or for_bias, *args)
+        ctx.save_for_backward(group_offs, pre if for_bias else None)
         ctx.activation, ctx.options = activation, options
         ctx.bias_dtype = None if bias is None else bias.dtype
         ctx.set_materialize_grads(False)
@@ -105,7 +104,7 @@ class _BiasAct(torch.autograd.Function):
             # rows of no group are not written: they are no function of the residual
             row = torch.arange(dout.shape[0], device=dout.device)
             dres = torch.where(((row >= group_offs[0]) & (row < group_offs[-1]))[:, None], dout, 0)
-        return (dbias, dres) + (None,) * 7
+        return dbias, dres, None, None, None, None, None
 
 
 def grouped_gemm_fp8_bias_act(a: torch.Tensor, b: torch.Tensor, a_scale: torch.Tensor, b_scale: torch.Tensor,
@@ -156,11 +155,12 @@ def grouped_gemm_fp8_bias_act(a: torch.Tensor, b: torch.Tensor, a_scale: torch.T
             raise ValueError(f"residual must be bf16 [{M}, {width}] on a's device")
     if validate:
         _validate_offsets(group_offs, M, mx=False)
-    sizes, operands, epilogue = (M, N, K, G, width, dev), (a, b, a_scale, b_scale, group_offs), (code, slope, limit, shift)
     if tracked(bias, residual):
         options = {"slope": slope, "limit": limit, "shift": shift} if activation == "swiglu" else {}
-        return _BiasAct.apply(bias, residual, sizes, operands, epilogue, activation, options, keep_preact, zero_tail)
-    out, pre = _product(sizes, operands, bias, residual, epilogue, keep_preact, zero_tail)
+        return _BiasAct.apply(bias, residual, keep_preact, group_offs, activation, options,
+                              (a, b, a_scale, b_scale, group_offs, M, N, K, G, width, dev, code, slope, limit, shift, zero_tail))
+    out, pre = _product(bias, residual, keep_preact, a, b, a_scale, b_scale, group_offs, M, N, K, G, width, dev, code, slope,
+                        limit, shift, zero_tail)
     return (out, pre) if keep_preact else out
 
 

@@ -107,13 +107,15 @@ def quantize_fp8_tensorwise(x: torch.Tensor, fmt: str = "e4m3", row_align: int |
     am = torch.empty((), dtype=torch.float32, device=dev)
     ws = torch.empty(WORKSPACE, dtype=torch.int32, device=dev)
     qp = q if rows > 0 else torch.empty((1, cols), dtype=dt, device=dev)
-    out = (code, qp.data_ptr(), q.stride(-2) if rows > 1 else cols, scale.data_ptr(), am.data_ptr(), ws.data_ptr())
+    q_stride = q.stride(-2) if rows > 1 else cols
     if slots is not None and rows:
         k = slots.shape[1]
         _lib.launch("ggemm_quant_fp8_tensorwise_rows", dev, cols | k, x2.data_ptr(), _IN[x.dtype], rows, cols,
-                    _row_stride(x2), slots.data_ptr(), k, *out)
+                    _row_stride(x2), slots.data_ptr(), k, code, qp.data_ptr(), q_stride, scale.data_ptr(), am.data_ptr(),
+                    ws.data_ptr())
     else:
-        _lib.launch("ggemm_quant_fp8_tensorwise_ws", dev, cols, _ptr(x2), _IN[x.dtype], rows, cols, _row_stride(x2), *out)
+        _lib.launch("ggemm_quant_fp8_tensorwise_ws", dev, cols, _ptr(x2), _IN[x.dtype], rows, cols, _row_stride(x2), code,
+                    qp.data_ptr(), q_stride, scale.data_ptr(), am.data_ptr(), ws.data_ptr())
     return q, scale, am
 
 
