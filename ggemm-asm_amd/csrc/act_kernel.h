@@ -115,7 +115,7 @@ __device__ __forceinline__ void grad8(const v4i& z8, const v4i& d8, const epi::A
     for (int i = 0; i < 4; ++i) {
       const float g = epi::at_most(z[2 * i], e.limit), u = epi::within(z[2 * i + 1], e.limit);
       const float s = epi::sigmoid2(e.nslope * g), gs = g * s;
-      const float dg = d[i] * (u + e.shift) * (s + e.slope * gs * (1.f - s));
+      const float dg = d[i] * ((u + e.shift) * (s + e.slope * gs * (1.f - s)));   // a closed gate closes before d
       out[2 * i] = z[2 * i] > e.limit ? 0.f : dg;
       out[2 * i + 1] = fabsf(z[2 * i + 1]) > e.limit ? 0.f : d[i] * gs;
     }

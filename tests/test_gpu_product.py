@@ -363,3 +363,20 @@ def test_gradients_of_bias_and_residual(pkg, activation, options, bias_dtype, ke
     assert bias.grad.dtype == bias_dtype
     assert ((bias.grad.cpu().double() - want).abs() <= 32 * U * reach + 17 * 2.0 ** -24 * size + 1.01 * half * want.abs()).all()
     assert torch.equal(res.grad[:offs[-1]], dout[:offs[-1]]) and not res.grad[offs[-1]:].any()
+
+
+def test_gradient_of_gates_far_below_zero(pkg):
+    """Where the gate is closed its gradient is zero, and where it nearly is their product is what counts, however large the
+    up half times dout would be by themselves."""
+    pre = torch.zeros((3, 16), dtype=torch.bfloat16)
+    pre[0, 0::2], pre[0, 1::2] = -3e38, 1e10
+    pre[1, 0::2], pre[1, 1::2] = -64.0, 1e20
+    pre[2, 0::2], pre[2, 1::2] = -3e38, -1e37
+    dout = torch.full((3, 8), 1e30, dtype=torch.bfloat16)
+    offs = [0, 1, 2, 3]
+    dpre, dbias = pkg.bias_act_backward(dout.cuda(), pre.cuda(), torch.tensor(offs).cuda(), "swiglu", shift=1.0)
+    ref, rbias, _ = orx.backward(dout, pre, offs, "swiglu", shift=1.0)
+    assert torch.isfinite(ref).all() and torch.isfinite(dpre).all() and torch.isfinite(dbias).all()
+    # sigmoid(-64): the exponent's rounding, 64 log2 e 2^-24 ln 2 = 3.8e-6, and the difference 1 - 64 of two terms
+    for got, want, half in ((dpre, ref, BF), (dbias, rbias, 0.0)):
+        assert ((got.cpu().double() - want).abs() <= (1e-5 + half) * want.abs()).all()
