@@ -10,6 +10,7 @@ include/ggemm_persistent.h. Modules:
 * ``persistent`` -- fwd/dgrad grouped GEMM torch op over the C ABI (same)
 * ``product``    -- the fwd grouped GEMM with bias, activation and residual, and their gradient, over the C ABI
 * ``quant``      -- FP8 quantization producer (per-tensor and MX with group padding) over the C ABI
+* ``mx``         -- microscaled rows (4 and 8 bits) and the grouped product of 4-bit weights, over the C ABI
 * ``moe``        -- routing tokens to experts, their rows into expert order and back, over the C ABI
 * ``autograd``   -- the FP8 grouped linear layer (forward, dgrad, wgrad) as a torch autograd op
 * ``layer``      -- a whole MoE layer from router logits to the combined tokens
@@ -23,6 +24,7 @@ from .autograd import (FP8DelayedScaling, FP8WeightCache, GroupedLinearActFP8, G
                        grouped_linear_fp8)
 from .layer import moe_layer_fp8  # noqa: F401
 from .moe import DispatchPlan, combine_tokens, dispatch_tokens, plan_dispatch, route_experts  # noqa: F401
+from .mx import MXTensor, dequantize_mx, grouped_gemm_mx_bias_act, quantize_mx  # noqa: F401
 from .persistent import grouped_gemm_fp8_tensorwise  # noqa: F401
 from .product import bias_act_backward, grouped_gemm_fp8_bias_act  # noqa: F401
 from .quant import (amax, padded_rows, quantize_fp8_tensorwise, quantize_fp8_tensorwise_delayed,  # noqa: F401

@@ -1,5 +1,5 @@
 """ctypes binding of libggemm_vark.so (declarations in include/ggemm_vark.h, include/ggemm_persistent.h,
-include/ggemm_quant.h, include/ggemm_moe.h and include/ggemm_product.h)."""
+include/ggemm_quant.h, include/ggemm_moe.h, include/ggemm_product.h and include/ggemm_mx.h)."""
 from __future__ import annotations
 
 import ctypes
@@ -95,10 +95,17 @@ PRODUCT_EXPORTS = (
     "ggemm_product_tile_rows",
 )
 
+MX_EXPORTS = (
+    "ggemm_mx_quantize",
+    "ggemm_mx_dequantize",
+    "ggemm_mx_product",
+    "ggemm_mx_tile_rows",
+)
+
 # GGEMM_VARK_ABI_VERSION of include/ggemm_vark.h that these bindings are written for. Some exports
 # changed signature between versions (ggemm_vark_wgrad_fp8_out and ggemm_vark_wgrad_mxfp8 took
 # M_total from version 3 on), so a library of another version is refused at load.
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 ERRORS = {
     0: "GGEMM_OK", -1: "GGEMM_E_NULL", -2: "GGEMM_E_SHAPE", -3: "GGEMM_E_STRIDE",
@@ -212,7 +219,11 @@ def load():
                                                vp]
     lib.ggemm_product_fp8_bias_act.argtypes = [vp] * 7 + [i32, vp, vp] + [i32] * 10 + [f32, f32, f32, i64, i32, vp]
     lib.ggemm_product_act_backward.argtypes = [vp, vp, vp] + [i32] * 5 + [f32, f32, f32, i64, vp, i32, vp, vp, vp]
-    for name in MOE_EXPORTS + PRODUCT_EXPORTS:
+    lib.ggemm_mx_quantize.argtypes = [vp, i32, i64, i32, i64, i32, vp, i64, vp, i64, vp]
+    lib.ggemm_mx_dequantize.argtypes = [vp, i32, i64, i32, i64, vp, i64, i64, vp, i32, i64, vp]
+    lib.ggemm_mx_product.argtypes = [vp, i32, vp, vp, vp, vp, vp, i32, vp, vp, i32, i32, i32] + [i64] * 6 + \
+        [i32, i32, i32, f32, f32, f32, i64, i32, i32, vp]
+    for name in MOE_EXPORTS + PRODUCT_EXPORTS + MX_EXPORTS:
         getattr(lib, name).restype = ctypes.c_int
     lib.ggemm_moe_plan_workspace.argtypes = [i64, i32]
     lib.ggemm_moe_plan_workspace.restype = ctypes.c_int64
@@ -220,6 +231,8 @@ def load():
     lib.ggemm_product_tile_rows.restype = ctypes.c_int32
     lib.ggemm_product_act_workspace.argtypes = [i64, i32, i32]
     lib.ggemm_product_act_workspace.restype = ctypes.c_int64
+    lib.ggemm_mx_tile_rows.argtypes = [i32] * 5 + [i64, i32]
+    lib.ggemm_mx_tile_rows.restype = ctypes.c_int32
     _lib = lib
     return lib
 

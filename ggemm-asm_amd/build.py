@@ -3,8 +3,9 @@
 * ``lib/libggemm_vark.so`` -- the extern "C" launcher library: the variable-K wgrad kernels
   (tensorwise, K=32-MFMA, MXFP8; include/ggemm_vark.h), the persistent fwd/dgrad grouped GEMM
   (include/ggemm_persistent.h), the same product with bias, activation and residual
-  (include/ggemm_product.h), the FP8 quantization producer (include/ggemm_quant.h), and expert
-  routing with the rows' way to the experts and back (include/ggemm_moe.h).
+  (include/ggemm_product.h), the FP8 quantization producer (include/ggemm_quant.h), expert
+  routing with the rows' way to the experts and back (include/ggemm_moe.h), and microscaled rows with
+  the product of 4-bit weights (include/ggemm_mx.h).
 * ``lib/variable_k_wgrad.co`` -- the drop-in code object exporting only
   ``_grouped_variable_k_gemm_kernel`` with the reference kernarg layout.
 * ``lib/persistent_e4m3.co`` / ``lib/persistent_e5m2.co`` -- drop-in code objects exporting only
@@ -26,7 +27,7 @@ PERSISTENT_CO_PATHS = {"e4m3": os.path.join(LIB_DIR, "persistent_e4m3.co"),
                        "e5m2": os.path.join(LIB_DIR, "persistent_e5m2.co")}
 ARCH = "gfx950"
 LIB_SOURCES = [os.path.join(CSRC, f) for f in ("vark_capi.hip", "persistent_capi.hip", "quant_capi.hip",
-                                               "moe_capi.hip", "product_capi.hip")]
+                                               "moe_capi.hip", "product_capi.hip", "mx_capi.hip")]
 
 # Packed-FP32 VALU ops are disabled for all device code (they are left to no hand-written use).
 DEVICE_FLAGS = ["-O3", "-std=c++17", f"--offload-arch={ARCH}",

@@ -1,0 +1,230 @@
+// extern "C" launchers of microscaled rows (include/ggemm_mx.h), part of libggemm_vark.so. Arguments are validated on
+// the host; nothing is launched on a validation error.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/ggemm_mx.h"
+#include "capi_common.h"
+#include "mx_gemm.h"
+#include "mx_quant.h"
+
+namespace {
+
+using ggemm::host::aligned;
+using ggemm::host::device_cus;
+namespace epi = ggemm::epi;
+namespace mx = ggemm::mx;
+namespace mxq = ggemm::mxq;
+namespace nt = ggemm::nt;
+
+static_assert(GGEMM_ACT_SILU == epi::kSilu && GGEMM_ACT_GELU == epi::kGelu && GGEMM_ACT_SWIGLU == epi::kSwiglu &&
+                  GGEMM_PRODUCT_MAX_GROUPS == mx::kMaxGroups,
+              "header and kernels agree");
+
+// ------------------------------------------------------------------------------ quantization
+
+constexpr int64_t kUnit = mxq::kThreads * mxq::kUnroll;    // units of a workgroup
+constexpr int64_t kMaxUnits = (int64_t(1) << 31) - kUnit;  // of a launch: 31-bit indices
+
+int check_rows(const mxq::Args& a, int dtype, int fmt, const void* x, const void* q) {
+  if (!x || !q || !a.scales) return GGEMM_E_NULL;
+  if ((dtype != GGEMM_IN_BF16 && dtype != GGEMM_IN_F32) || (fmt != GGEMM_MX_E4M3 && fmt != GGEMM_MX_E2M1))
+    return GGEMM_E_FORMAT;
+  if (a.rows < 0 || a.cols <= 0 || a.cols % 16) return GGEMM_E_SHAPE;
+  const int64_t bytes = fmt == GGEMM_MX_E4M3 ? a.cols : a.cols / 2, unit = fmt == GGEMM_MX_E4M3 ? 8 : 4;
+  if (a.stride < a.cols || a.stride % (dtype == GGEMM_IN_BF16 ? 8 : 4) || a.q_stride < bytes || a.q_stride % unit)
+    return GGEMM_E_STRIDE;
+  if (!aligned(x, 16) || !aligned(q, (uintptr_t)unit)) return GGEMM_E_ALIGN;
+  return GGEMM_OK;
+}
+
+// kernel(dtype, format)(a) over all rows, as many at a time as 31 bits index.
+template <typename F>
+int over_rows(mxq::Args a, int dtype, F launch) {
+  int cus = 0;
+  const int rc = device_cus(&cus);
+  if (rc) return rc;
+  const int64_t per = 4 * ((a.cols + 31) / 32), most = std::max<int64_t>(1, kMaxUnits / per), rows = a.rows;
+  if (per > kMaxUnits) return GGEMM_E_SHAPE;
+  a.per = mxq::Divisor::of((uint32_t)per);
+  for (int64_t r = 0; r < rows; r += most) {
+    a.rows = std::min(most, rows - r);
+    launch(a, dim3((uint32_t)((a.rows * per + kUnit - 1) / kUnit)));
+    const int err = (int)hipGetLastError();
+    if (err) return err;
+    a.x = (const uint8_t*)a.x + a.rows * a.stride * (dtype == GGEMM_IN_BF16 ? 2 : 4);
+    a.q += a.rows * a.q_stride;
+    a.scales += a.rows * a.scale_row;
+  }
+  return GGEMM_OK;
+}
+
+// ------------------------------------------------------------------------------ the product
+
+template <bool kA8>
+using Tile256 = mx::Cfg<kA8, 256, 256, 2, 2, kA8 ? 3 : 2>;
+template <bool kA8>
+using Tile128 = mx::Cfg<kA8, 128, 128, 2, 2, kA8 ? 3 : 2>;
+template <bool kA8>
+using Tile64 = mx::Cfg<kA8, 64, 128, 1, 4, kA8 ? 3 : 2>;
+
+__device__ __forceinline__ void clear_tail(int kAct, const mx::Args& a) {
+  if (a.zero_tail)
+    nt::clear_tail_rows(a.out, a.stride_out, kAct == epi::kSwiglu ? a.N / 2 : a.N, a.group_offs, a.G, a.m_total);
+}
+
+// kPerCu: workgroups on a CU at once
+template <int kAct, bool kA8, typename C, int kPerCu>
+__global__ __launch_bounds__(mx::kNT) __attribute__((amdgpu_waves_per_eu(kPerCu, kPerCu)))
+void mx_product_kernel(mx::Args a, epi::Args e) {
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[C::LdsBytes];
+  mx::gemm_body<kAct, kA8, C>(a, (GG_LDS uint8_t*)lds, e);
+  clear_tail(kAct, a);
+}
+
+template <int kAct, bool kA8, int NB>
+__global__ __launch_bounds__(mx::kNT) void mx_few_kernel(mx::Args a, epi::Args e) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[mx::few::kWaves * NB * 1024];
+  mx::few::body<kAct, kA8, NB>(a, (GG_LDS uint8_t*)lds, e);
+  clear_tail(kAct, a);
+}
+
+template <typename F>
+int with_act(int act, F f) {
+  using std::integral_constant;
+  switch (act) {
+    case GGEMM_ACT_SILU: return f(integral_constant<int, epi::kSilu>{});
+    case GGEMM_ACT_GELU: return f(integral_constant<int, epi::kGelu>{});
+    case GGEMM_ACT_SWIGLU: return f(integral_constant<int, epi::kSwiglu>{});
+    default: return f(integral_constant<int, epi::kNone>{});
+  }
+}
+
+int64_t tiles_of(int64_t M, int64_t g, int N, int bm, int bn) { return (M / bm + g) * ((N + bn - 1) / bn); }
+
+int choose(int fmt, int G, int N, int K, int act, int64_t M, int cus) {
+  const int64_t g = std::min<int64_t>(G, M);
+  if (M <= 8 * g) return 16;
+  if (tiles_of(M, g, N, 256, 256) >= cus) return 256;
+  return tiles_of(M, g, N, 128, 128) >= cus ? 128 : 64;
+}
+
+// Whole runs of tiles over the XCDs (mid_common.h).
+uint32_t grid_of(int64_t tiles) {
+  const int64_t run = ggemm::kXcds * ggemm::mid::kXcdRun;
+  return (uint32_t)((tiles + run - 1) / run * run);
+}
+
+template <int kAct, bool kA8>
+int launch(const mx::Args& a, const epi::Args& e, int tile, int cus, hipStream_t stream) {
+  const int64_t g = std::min<int64_t>(a.G, a.m_total);
+  auto run = [&](auto kernel, int bm, int bn) {
+    hipLaunchKernelGGL(kernel, dim3(grid_of(tiles_of(a.m_total, g, a.N, bm, bn))), dim3(mx::kNT), 0, stream, a, e);
+  };
+  if (tile == 16) {
+    if (tiles_of(a.m_total, g, a.N, 16, 16) <= 3 * cus) run(mx_few_kernel<kAct, kA8, 1>, 16, 16);
+    else run(mx_few_kernel<kAct, kA8, 2>, 16, 32);
+  } else if (tile == 64) {
+    run(mx_product_kernel<kAct, kA8, Tile64<kA8>, 2>, 64, 128);
+  } else if (tile == 128) {
+    run(mx_product_kernel<kAct, kA8, Tile128<kA8>, 2>, 128, 128);
+  } else {
+    run(mx_product_kernel<kAct, kA8, Tile256<kA8>, 1>, 256, 256);
+  }
+  return (int)hipGetLastError();
+}
+
+int validate(const mx::Args& a, const epi::Args& e, int fmt, int act, int bias_dtype, const int64_t (&strides)[6]) {
+  if (!a.a || !a.a_scales || !a.b || !a.b_scales || !a.out || !a.group_offs) return GGEMM_E_NULL;
+  if (fmt != GGEMM_MX_E4M3 && fmt != GGEMM_MX_E2M1) return GGEMM_E_FORMAT;
+  if (e.bias && bias_dtype != GGEMM_IN_BF16 && bias_dtype != GGEMM_IN_F32) return GGEMM_E_FORMAT;
+  if (act < GGEMM_ACT_NONE || act > GGEMM_ACT_SWIGLU) return GGEMM_E_FORMAT;
+  if (act == GGEMM_ACT_SWIGLU && !(e.limit > 0.f)) return GGEMM_E_SHAPE;
+  if (a.G <= 0 || a.G > mx::kMaxGroups || a.N <= 0 || a.K <= 0 || a.N % 16 || a.K % 32) return GGEMM_E_SHAPE;
+  if (a.m_total < 0 || a.m_total > nt::kMaxRow) return GGEMM_E_SHAPE;
+  if ((a.m_total / 16 + a.G) * (int64_t)((a.N + 15) / 16) > nt::kMaxTiles * 2) return GGEMM_E_SHAPE;
+  const int64_t chunk = (int64_t)(a.K + 511) / 512 * 16, bytes_a = fmt == GGEMM_MX_E4M3 ? a.K : a.K / 2;
+  const int64_t sa = strides[0], sas = strides[1], sbg = strides[2], sbn = strides[3], sbsg = strides[4], sbsn = strides[5];
+  if (sa < bytes_a || sas < chunk || sbn < a.K / 2 || sbsn < chunk) return GGEMM_E_STRIDE;
+  if (a.G > 1 && (sbg < (a.N - 1) * sbn + a.K / 2 || sbsg < a.N * sbsn)) return GGEMM_E_STRIDE;
+  for (int64_t s : strides)
+    if (s % 16) return GGEMM_E_STRIDE;
+  // 32-bit buffer offsets of a tile's 256 rows
+  for (int64_t s : {sa, sas, sbn, sbsn})
+    if (s * 256 >= (int64_t)nt::kOob) return GGEMM_E_SHAPE;
+  const int width = act == GGEMM_ACT_SWIGLU ? a.N / 2 : a.N;
+  if (a.stride_out < width || a.stride_out % 8) return GGEMM_E_STRIDE;
+  if (e.residual && (e.stride_res < width || e.stride_res % 8)) return GGEMM_E_STRIDE;
+  for (const void* p : {(const void*)a.a, (const void*)a.a_scales, (const void*)a.b, (const void*)a.b_scales,
+                        (const void*)a.out, (const void*)e.bias, (const void*)e.residual})
+    if (!aligned(p, 16)) return GGEMM_E_ALIGN;
+  return GGEMM_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ggemm_mx_quantize(const void* x, int32_t dtype, int64_t rows, int32_t cols, int64_t stride, int32_t fmt, void* q,
+                      int64_t q_stride, uint8_t* scales, int64_t scale_stride, void* stream) {
+  const mxq::Args a{x, rows, stride, cols, {}, (uint8_t*)q, q_stride, scales, scale_stride, 1};
+  const int rc = check_rows(a, dtype, fmt, x, q);
+  if (rc) return rc;
+  if (scale_stride < (cols + 31) / 32) return GGEMM_E_STRIDE;
+  const bool f32 = dtype == GGEMM_IN_F32, e4m3 = fmt == GGEMM_MX_E4M3;
+  return over_rows(a, dtype, [&](const mxq::Args& part, dim3 grid) {
+    auto kernel = f32 ? (e4m3 ? mxq::quantize_kernel<true, true> : mxq::quantize_kernel<true, false>)
+                      : (e4m3 ? mxq::quantize_kernel<false, true> : mxq::quantize_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(mxq::kThreads), 0, (hipStream_t)stream, part);
+  });
+}
+
+int ggemm_mx_dequantize(const void* q, int32_t fmt, int64_t rows, int32_t cols, int64_t q_stride, const uint8_t* scales,
+                        int64_t scale_row, int64_t scale_block, void* out, int32_t dtype, int64_t out_stride,
+                        void* stream) {
+  const mxq::Args a{out, rows, out_stride, cols, {}, (uint8_t*)q, q_stride, (uint8_t*)scales, scale_row, scale_block};
+  const int rc = check_rows(a, dtype, fmt, out, q);
+  if (rc) return rc;
+  if (scale_row < 0 || scale_block < 0) return GGEMM_E_STRIDE;
+  const bool f32 = dtype == GGEMM_IN_F32, e4m3 = fmt == GGEMM_MX_E4M3;
+  return over_rows(a, dtype, [&](const mxq::Args& part, dim3 grid) {
+    auto kernel = f32 ? (e4m3 ? mxq::dequantize_kernel<true, true> : mxq::dequantize_kernel<true, false>)
+                      : (e4m3 ? mxq::dequantize_kernel<false, true> : mxq::dequantize_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, grid, dim3(mxq::kThreads), 0, (hipStream_t)stream, part);
+  });
+}
+
+int32_t ggemm_mx_tile_rows(int32_t a_fmt, int32_t G, int32_t N, int32_t K, int32_t act, int64_t M_total, int32_t num_cus) {
+  return choose(a_fmt, G, N, K, act, M_total, num_cus);
+}
+
+int ggemm_mx_product(const void* a, int32_t a_fmt, const uint8_t* a_scales, const void* b, const uint8_t* b_scales,
+                     void* out, const void* bias, int32_t bias_dtype, const void* residual, const int64_t* group_offs,
+                     int32_t G, int32_t N, int32_t K, int64_t stride_a, int64_t stride_as, int64_t stride_bg,
+                     int64_t stride_bn, int64_t stride_bsg, int64_t stride_bsn, int32_t stride_out, int32_t stride_res,
+                     int32_t act, float slope, float limit, float shift, int64_t M_total, int32_t zero_tail,
+                     int32_t tile, void* stream) {
+  const mx::Args x{(const uint8_t*)a, a_scales, (const uint8_t*)b, b_scales, (uint16_t*)out, group_offs, G, N, K,
+                   (int)stride_a, (int)stride_as, (int)stride_bn, (int)stride_bsn, stride_out, stride_bg, stride_bsg,
+                   M_total, zero_tail};
+  const epi::Args e{nullptr, 0, bias, bias_dtype == GGEMM_IN_F32, (const uint16_t*)residual, stride_res, slope, limit,
+                    shift, slope * -epi::kLog2e};
+  int rc = validate(x, e, a_fmt, act, bias_dtype, {stride_a, stride_as, stride_bg, stride_bn, stride_bsg, stride_bsn});
+  if (rc) return rc;
+  if (tile != 0 && tile != 16 && tile != 64 && tile != 128 && tile != 256) return GGEMM_E_SHAPE;
+  int cus = 0;
+  rc = device_cus(&cus);
+  if (rc) return rc;
+  if (M_total == 0) return GGEMM_OK;
+  if (tile == 0) tile = choose(a_fmt, G, N, K, act, M_total, cus);
+  return with_act(act, [&](auto code) {
+    constexpr int kAct = decltype(code)::value;
+    return a_fmt == GGEMM_MX_E4M3 ? launch<kAct, true>(x, e, tile, cus, (hipStream_t)stream)
+                                  : launch<kAct, false>(x, e, tile, cus, (hipStream_t)stream);
+  });
+}
+
+}  // extern "C"

@@ -17,7 +17,7 @@
 extern "C" {
 #endif
 
-#define GGEMM_VARK_ABI_VERSION 12
+#define GGEMM_VARK_ABI_VERSION 13
 
 enum {
   GGEMM_OK = 0,
