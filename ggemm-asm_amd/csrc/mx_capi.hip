@@ -65,28 +65,27 @@ int over_rows(mxq::Args a, int dtype, F launch) {
 // ------------------------------------------------------------------------------ the product
 
 template <bool kA8>
-using Tile256 = mx::Cfg<kA8, 256, 256, 2, 2, kA8 ? 3 : 2>;
+using Tile256 = mx::Cfg<kA8, 256, 256, 2, 4, true>;
 template <bool kA8>
-using Tile128 = mx::Cfg<kA8, 128, 128, 2, 2, kA8 ? 3 : 2>;
+using Tile128 = mx::Cfg<kA8, 128, 128, 2, 2, false>;
 template <bool kA8>
-using Tile64 = mx::Cfg<kA8, 64, 128, 1, 4, kA8 ? 3 : 2>;
+using Tile64 = mx::Cfg<kA8, 64, 128, 1, 4, false>;
 
 __device__ __forceinline__ void clear_tail(int kAct, const mx::Args& a) {
   if (a.zero_tail)
     nt::clear_tail_rows(a.out, a.stride_out, kAct == epi::kSwiglu ? a.N / 2 : a.N, a.group_offs, a.G, a.m_total);
 }
 
-// kPerCu: workgroups on a CU at once
-template <int kAct, bool kA8, typename C, int kPerCu>
-__global__ __launch_bounds__(mx::kNT) __attribute__((amdgpu_waves_per_eu(kPerCu, kPerCu)))
-void mx_product_kernel(mx::Args a, epi::Args e) {
+template <int kAct, bool kA8, typename C>
+__global__ __launch_bounds__(C::NT) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mx_product_kernel(mx::Args a, epi::Args e, int grid, int blocks) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[C::LdsBytes];
-  mx::gemm_body<kAct, kA8, C>(a, (GG_LDS uint8_t*)lds, e);
+  mx::gemm_body<kAct, kA8, C>(a, (GG_LDS uint8_t*)lds, e, grid, blocks);
   clear_tail(kAct, a);
 }
 
 template <int kAct, bool kA8, int NB>
-__global__ __launch_bounds__(mx::kNT) void mx_few_kernel(mx::Args a, epi::Args e) {
+__global__ __launch_bounds__(mx::few::kNT) void mx_few_kernel(mx::Args a, epi::Args e) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[mx::few::kWaves * NB * 1024];
   mx::few::body<kAct, kA8, NB>(a, (GG_LDS uint8_t*)lds, e);
   clear_tail(kAct, a);
@@ -121,18 +120,24 @@ uint32_t grid_of(int64_t tiles) {
 template <int kAct, bool kA8>
 int launch(const mx::Args& a, const epi::Args& e, int tile, int cus, hipStream_t stream) {
   const int64_t g = std::min<int64_t>(a.G, a.m_total);
-  auto run = [&](auto kernel, int bm, int bn) {
-    hipLaunchKernelGGL(kernel, dim3(grid_of(tiles_of(a.m_total, g, a.N, bm, bn))), dim3(mx::kNT), 0, stream, a, e);
+  auto tiles = [&](int bm, int bn) { return grid_of(tiles_of(a.m_total, g, a.N, bm, bn)); };
+  auto run = [&](auto cfg) {
+    using C = decltype(cfg);
+    const uint32_t blocks = tiles(C::BM, C::BN);
+    const uint32_t grid = C::kWalk && a.K > C::KS ? std::min<uint32_t>(blocks, cus) : blocks;
+    hipLaunchKernelGGL((mx_product_kernel<kAct, kA8, C>), dim3(grid), dim3(C::NT), 0, stream, a, e, (int)grid, (int)blocks);
   };
   if (tile == 16) {
-    if (tiles_of(a.m_total, g, a.N, 16, 16) <= 3 * cus) run(mx_few_kernel<kAct, kA8, 1>, 16, 16);
-    else run(mx_few_kernel<kAct, kA8, 2>, 16, 32);
+    if (tiles_of(a.m_total, g, a.N, 16, 16) <= 3 * cus)
+      hipLaunchKernelGGL((mx_few_kernel<kAct, kA8, 1>), dim3(tiles(16, 16)), dim3(mx::few::kNT), 0, stream, a, e);
+    else
+      hipLaunchKernelGGL((mx_few_kernel<kAct, kA8, 2>), dim3(tiles(16, 32)), dim3(mx::few::kNT), 0, stream, a, e);
   } else if (tile == 64) {
-    run(mx_product_kernel<kAct, kA8, Tile64<kA8>, 2>, 64, 128);
+    run(Tile64<kA8>{});
   } else if (tile == 128) {
-    run(mx_product_kernel<kAct, kA8, Tile128<kA8>, 2>, 128, 128);
+    run(Tile128<kA8>{});
   } else {
-    run(mx_product_kernel<kAct, kA8, Tile256<kA8>, 1>, 256, 256);
+    run(Tile256<kA8>{});
   }
   return (int)hipGetLastError();
 }

@@ -6,17 +6,20 @@
 // block's products and multiplies by both powers. Two e2m1 sides run at twice the rate of fp8; with e4m3 on one side at
 // fp8's.
 //
-// One tile of BM rows of one group x BN columns for each workgroup of four waves. A stage is 128 bytes of every A row
-// (256 values of e2m1, 128 of e4m3) and as many values of every B row, loaded by LDS-DMA into one of S slots. The
-// scales are 1/16 of the bytes, but rows far apart: 16 bytes of a row, 512 values, come at once and serve two or four
-// stages, since one more request for each row and stage would double the requests of the load path.
+// A tile is BM rows of one group x BN columns. A stage is 128 bytes of every A row (256 values of e2m1, 128 of e4m3) and as
+// many values of every B row, loaded by LDS-DMA into one of two slots. The scales are 1/16 of the bytes, but rows far
+// apart: 16 bytes of a row, 512 values, come at once and serve two or four stages, since one more request for each row
+// and stage would double the requests of the load path.
 //
 // Which K bytes a lane feeds is free as long as both sides and the scales agree: lane half h takes blocks 4 h .. 4 h +
 // 3 of a stage's eight (e2m1) or 2 h, 2 h + 1 of its four (e4m3), one to a step, so that its scales of a whole stage
 // are one word, whose byte the instruction picks, and its operands neighbouring chunks of 16 bytes.
 //
-// The operands of step t + 1 are read while step t multiplies; the barrier that frees a stage's slot stands before its
-// last step, whose operands are in registers by then, so that the next stage's first reads run beside its products.
+// The operands of step t + 1 are read while step t multiplies; the barrier that frees a stage's slot stands in its
+// last step, whose operands are in registers by then, so that the next stage's loads and first reads run beside its products.
+//
+// 256 x 256: eight waves of 128 x 64, two on a SIMD, one workgroup on a CU that walks over its tiles and loads the next
+// tile's first stages while it finishes one. 128 x 128 and 64 x 128: four waves, two workgroups on a CU, a tile each.
 #pragma once
 
 #include "fused_epilogue.h"
@@ -26,7 +29,6 @@
 namespace ggemm {
 namespace mx {
 
-constexpr int kNT = 256;
 constexpr int kMaxGroups = 2047;
 using nt::kOob;
 
@@ -50,62 +52,81 @@ __device__ __forceinline__ int64_t tile_rows_end(const Args& a) {
   return clamp_off(a.group_offs[a.G], a.m_total);
 }
 
-// Tile t of a launch whose groups hold ceil(rows / BM) n_tn tiles each. Offsets count as the largest one so far, in
-// [0, m_total]. Lane l sums up ceil(G / 64) consecutive groups; a scan finds the lane, a walk over its groups the tile.
+// The groups of a launch as tiles: lane l holds ceil(G / 64) consecutive ones. Offsets count as the largest one so far, in
+// [0, m_total].
+struct Groups {
+  const int64_t* offs;
+  int64_t m;
+  int G, per;
+  int before, first, len;           // the rows' end before the lane's groups; its first group: first row, rows
+  int sum, incl;                    // tiles of the lane's groups, and of those up to it
+  __device__ __forceinline__ int row(int g) const { return (int)clamp_off(offs[g], m); }
+};
+template <int BM>
+__device__ __forceinline__ Groups load_groups(const int64_t* offs, int G, int64_t m, int n_tn, int lane) {
+  Groups r{offs, m, G, (G + 63) >> 6};
+  const int g0 = min(lane * r.per, G), g1 = min(g0 + r.per, G);
+  int top = 0;
+  for (int g = g0; g < g1; ++g) top = max(top, r.row(g));
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int v = __shfl_up(top, d, 64);
+    if (lane >= d) top = max(top, v);
+  }
+  r.before = __shfl_up(top, 1, 64);
+  if (lane == 0) r.before = 0;
+  int run = r.before;
+  r.sum = r.first = r.len = 0;
+  for (int g = g0; g < g1; ++g) {
+    run = max(run, r.row(g));
+    const int len = max(run, r.row(g + 1)) - run;
+    if (g == g0) r.first = run, r.len = len;
+    r.sum += (len + BM - 1) / BM * n_tn;
+  }
+  r.incl = mid::wave_scan(r.sum, lane);
+  return r;
+}
+
 struct Tile {
   int g, start, len, in_g;          // group, its first row and rows, the tile's index in it; g < 0: none
 };
 template <int BM>
-__device__ __forceinline__ Tile find_tile(const int64_t* offs, int G, int64_t m, int n_tn, int t, int lane) {
-  const int per = (G + 63) >> 6, g0 = min(lane * per, G), g1 = min(g0 + per, G);
-  auto row = [&](int g) { return (int)clamp_off(offs[g], m); };
-  int top = 0;
-  for (int g = g0; g < g1; ++g) top = max(top, row(g));
-  int before = top;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int v = __shfl_up(before, d, 64);
-    if (lane >= d) before = max(before, v);
-  }
-  before = __shfl_up(before, 1, 64);
-  if (lane == 0) before = 0;
-  int sum = 0, run = before;
-  for (int g = g0; g < g1; ++g) {
-    run = max(run, row(g));
-    sum += (max(run, row(g + 1)) - run + BM - 1) / BM * n_tn;
-  }
-  const int incl = mid::wave_scan(sum, lane);
-  const uint64_t past = __ballot(incl > t);
+__device__ __forceinline__ Tile find_tile(const Groups& r, int n_tn, int t) {
+  const uint64_t past = __ballot(r.incl > t);
   if (past == 0) return {-1, 0, 0, 0};
   const int gl = __builtin_ctzll(past);
-  int in_g = t - __builtin_amdgcn_readlane(incl - sum, gl), start = __builtin_amdgcn_readlane(before, gl);
-  for (int g = gl * per;; ++g) {                              // ends in the lane's groups: in_g is below their sum
-    start = max(start, row(g));
-    const int len = max(start, row(g + 1)) - start, n = (len + BM - 1) / BM * n_tn;
-    if (in_g < n || g + 1 >= G) return {g, start, len, in_g};
+  int in_g = t - __builtin_amdgcn_readlane(r.incl - r.sum, gl);
+  int start = __builtin_amdgcn_readlane(r.first, gl), len = __builtin_amdgcn_readlane(r.len, gl);
+  for (int g = gl * r.per;;) {                                // ends in the lane's groups: in_g is below their sum
+    const int n = (len + BM - 1) / BM * n_tn;
+    if (in_g < n || ++g >= r.G) return {g, start, len, in_g};
     in_g -= n;
+    start += len;
+    start = max(start, __builtin_amdgcn_readfirstlane(r.row(g)));
+    len = max(start, __builtin_amdgcn_readfirstlane(r.row(g + 1))) - start;
   }
 }
 
-template <bool kA8, int kBM, int kBN, int kWM, int kWN, int kStages>
+// kWalk: one workgroup on a CU, which walks over its tiles; else two, with a tile each.
+template <bool kA8, int kBM, int kBN, int kWM, int kWN, bool kWalk_>
 struct Cfg {
-  static constexpr int BM = kBM, BN = kBN, WM = kWM, WN = kWN, S = kStages;
+  static constexpr int BM = kBM, BN = kBN, WM = kWM, WN = kWN, W = WM * WN, NT = 64 * W;   // waves and threads
+  static constexpr bool kWalk = kWalk_;
   static constexpr int KS = kA8 ? 128 : 256;                    // values of K in a stage
-  static constexpr int RowA = 128, RowB = kA8 ? 64 : 128;       // bytes of a row in it
+  static constexpr int RowA = kA8 ? KS : KS / 2, RowB = KS / 2; // bytes of a row in it
+  static constexpr int Blocks = KS / 32;                        // and blocks
   static constexpr int T = KS / 64;                             // steps of a stage
   static constexpr int Super = 512 / KS;                        // stages that a row's 16 scale bytes serve
   static constexpr int ABytes = BM * RowA, BBytes = BN * RowB, Slot = ABytes + BBytes;
-  static constexpr int PA = ABytes / 4096, PB = BBytes / 4096;  // LDS-DMA instructions for each wave and stage
+  static constexpr int PA = ABytes / 1024 / W, PB = BBytes / 1024 / W;   // LDS-DMA instructions for each wave and stage
   static constexpr int SA = (BM + 63) / 64, SB = (BN + 63) / 64;   // of scales for the workgroup, 64 rows each
-  static constexpr int ScaleOff = S * Slot, ScaleBytes = 1024 * (SA + SB);
+  static constexpr int ScaleOff = 2 * Slot, ScaleBytes = 1024 * (SA + SB);
   static constexpr int LdsBytes = ScaleOff + 2 * ScaleBytes;
   static constexpr int MB = BM / WM / 32, NB = BN / WN / 32;    // 32-wide blocks of a wave
-  static constexpr int Region = 32 * (64 * NB + 16);            // a wave's staged rows of results
   static constexpr int BandN = 8;                               // column tiles of a band, row tiles walked inside
-  static_assert(WM * WN == 4 && MB >= 1 && NB >= 1 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "waves");
-  static_assert(ABytes % 4096 == 0 && BBytes % 4096 == 0, "uniform LDS-DMA split");
-  static_assert(S >= 2 && S <= Super + 1, "a scale buffer is free when its next chunk is asked for");
-  static_assert(4 * Region <= LdsBytes && LdsBytes <= 160 * 1024, "LDS");
+  static_assert(W % 2 == 0 && MB >= 1 && NB >= 1 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "waves");
+  static_assert(ABytes % (1024 * W) == 0 && BBytes % (1024 * W) == 0, "uniform LDS-DMA split");
+  static_assert(LdsBytes <= (kWalk ? 160 : 80) * 1024, "LDS");
 };
 
 template <int kSel, bool kA8>
@@ -127,209 +148,289 @@ __device__ __forceinline__ void keep_here(v16f (&acc)[MB][NB]) {
 #pragma unroll
   for (int i = 0; i < MB; ++i)
 #pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      if constexpr (MB * NB >= 16) asm volatile("" : "+a"(acc[i][j]));
-      else asm volatile("" : "+v"(acc[i][j]));
-    }
+    for (int j = 0; j < NB; ++j) asm volatile("" : "+v"(acc[i][j]));
+}
+
+// x and y of lanes l and l + 32 to (x of both) and (y of both): lane half 0 holds x's, half 1 y's. Its own inverse.
+__device__ __forceinline__ void by_half(int& x, int& y) {
+  const auto r = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)y, false, false);
+  x = (int)r[0];
+  y = (int)r[1];
 }
 
 // A wave's MB x NB blocks of 32 x 32: lane 32 h + s holds row s, columns 8 g + 4 h .. + 3 of a block in accumulators
-// 4 g .. 4 g + 3. Rows row0 .. of the launch (the first `rows` of them exist), columns n0 .. of group g's product; reg:
-// the wave's Region of LDS, through which the rows leave as 16-byte chunks.
+// 4 g .. 4 g + 3. Rows row0 .. of the launch (the first `rows` of them exist), columns n0 .. of group g's product. The halves
+// of a row's columns change places between lanes s and s + 32, so that a lane stores (and reads of a residual) 16
+// bytes at a time, a row's 32 or 64 bytes of a block in one go, without LDS.
 template <int kAct, int MB, int NB>
 __device__ __forceinline__ void store(const v16f (&acc)[MB][NB], const epi::Args& e, uint16_t* out, int stride_out, int g,
-                                      int N, int64_t row0, int rows, int n0, GG_LDS uint8_t* reg, int lane) {
+                                      int N, int64_t row0, int rows, int n0, int lane) {
   constexpr bool kGated = kAct == epi::kSwiglu;
-  constexpr int kChunks = kGated ? 2 * NB : 4 * NB;
+  constexpr int kParts = kGated ? 1 : 2;                       // 16-byte chunks of a lane and block
   const int h = lane >> 5, s = lane & 31;
-  const int cols = min(32 * NB, N - n0);                       // a multiple of 16; none where not positive
-  if (cols <= 0) return;
-  v4f bias[NB][4];
 #pragma unroll
-  for (int j = 0; j < NB; ++j)
+  for (int j = 0; j < NB; ++j) {
+    const int nj = n0 + 32 * j, cols = min(32, N - nj);        // a multiple of 16
+    if (cols <= 0) return;                                     // uniform in the wave, as all but the rows
+    v4f bias[4];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int n = 32 * j + 8 * c + 4 * h;
-      bias[j][c] = n < cols ? epi::load_bias(e, (int64_t)g * N + n0 + n) : v4f{0.f, 0.f, 0.f, 0.f};
-    }
-  const int o0 = kGated ? n0 / 2 : n0;
-  GG_LDS uint8_t* at = reg + s * (16 * kChunks + 16);
+    for (int c = 0; c < 4; ++c)
+      bias[c] = 8 * c < cols ? epi::load_bias(e, (int64_t)g * N + nj + 8 * c + 4 * h) : v4f{0.f, 0.f, 0.f, 0.f};
+    // chunk p of the lane: columns 16 h (gated: of z 16 h .. + 15; else 16 h + 8 p .. + 7) of the block
+    const int o0 = (kGated ? nj / 2 : nj) + (kGated ? 8 : 16) * h;
+    const bool live_cols = 16 * h < cols;
 #pragma unroll
-  for (int i = 0; i < MB; ++i) {
-    const int prows = rows - 32 * i;
-    if (prows <= 0) return;                                    // uniform in the wave
-    const int64_t prow = row0 + 32 * i;
-    const uint16_t* res = e.residual == nullptr ? nullptr : e.residual + (prow + s) * e.stride_res + o0;
+    for (int i = 0; i < MB; ++i) {
+      if (rows <= 32 * i) break;
+      const int64_t row = row0 + 32 * i + s;
+      const bool live = live_cols && 32 * i + s < rows;
+      int w[kParts][4];
+      if (e.residual != nullptr) {
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
+        for (int p = 0; p < kParts; ++p) {
+          const v4i r = live ? *(const v4i*)(e.residual + row * e.stride_res + o0 + 8 * p) : v4i{0, 0, 0, 0};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int n = 32 * j + 8 * c + 4 * h;
-        const bool live = res != nullptr && s < prows && n < cols;
-        v4f z = bias[j][c];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) z[k] += acc[i][j][4 * c + k];
-        if constexpr (kGated) {
-          float x = epi::swiglu(z[0], z[1], e), y = epi::swiglu(z[2], z[3], e);
-          if (live) {
-            const uint32_t w = *(const uint32_t*)(res + n / 2);
-            x += epi::from_bf16(w);
-            y += __uint_as_float(w & 0xffff0000u);
-          }
-          *(GG_LDS int*)(at + n) = epi::pack(x, y);
-        } else {
-          v4f x = epi::activation<kAct>(z);
-          if (live) x += epi::unpack4(*(const v2i*)(res + n));
-          *(GG_LDS v2i*)(at + 2 * n) = v2i{epi::pack(x[0], x[1]), epi::pack(x[2], x[3])};
+          for (int k = 0; k < 4; ++k) w[p][k] = r[k];
+          // gated: words (0, 1) of a lane are column groups 2 h and, its other half, ..; else groups 2 h + p
+          by_half(w[p][0], w[p][kGated ? 1 : 2]);
+          by_half(w[p][kGated ? 2 : 1], w[p][3]);
         }
       }
-    epi::store_rows<kChunks>(reg, out + prow * stride_out + o0, stride_out, prows, kGated ? cols / 16 : cols / 8, lane);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        v4f z = bias[c];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) z[k] += acc[i][j][4 * c + k];
+        // group c: the two lanes' halves end up in lane half c / 2
+        if constexpr (kGated) {
+          int& at = w[0][2 * (c & 1) + (c >> 1)];
+          float x = epi::swiglu(z[0], z[1], e), y = epi::swiglu(z[2], z[3], e);
+          if (e.residual != nullptr) {
+            x += epi::from_bf16((uint32_t)at);
+            y += __uint_as_float((uint32_t)at & 0xffff0000u);
+          }
+          at = epi::pack(x, y);
+        } else {
+          int &lo = w[c & 1][2 * (c >> 1)], &hi = w[c & 1][2 * (c >> 1) + 1];
+          v4f x = epi::activation<kAct>(z);
+          if (e.residual != nullptr) x += epi::unpack4(v2i{lo, hi});
+          lo = epi::pack(x[0], x[1]);
+          hi = epi::pack(x[2], x[3]);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) {
+        by_half(w[p][0], w[p][kGated ? 1 : 2]);
+        by_half(w[p][kGated ? 2 : 1], w[p][3]);
+        if (live) *(v4i*)(out + row * stride_out + o0 + 8 * p) = v4i{w[p][0], w[p][1], w[p][2], w[p][3]};
+      }
+    }
   }
 }
 
+// grid: workgroups of the launch; blocks: what it would have with one for each tile. A grid of fewer needs tiles of two
+// stages at least: loads are asked for two stages ahead, which may not reach past the next tile.
 template <int kAct, bool kA8, typename C>
-__device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, const epi::Args& e) {
+__device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, const epi::Args& e, int grid, int blocks) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n_tn = (a.N + C::BN - 1) / C::BN;
-  const Tile w = find_tile<C::BM>(a.group_offs, a.G, tile_rows_end(a), n_tn, mid::tile_of_block(blockIdx.x), lane);
-  if (w.g < 0) return;                                         // more workgroups than tiles
-  const int g = __builtin_amdgcn_readfirstlane(w.g), start = __builtin_amdgcn_readfirstlane(w.start);
-  const int len = __builtin_amdgcn_readfirstlane(w.len), in_g = __builtin_amdgcn_readfirstlane(w.in_g);
-  const int n_tm = (len + C::BM - 1) / C::BM;
-  const int band = in_g / (n_tm * C::BandN), r = in_g - band * n_tm * C::BandN;
-  const int bw = min(C::BandN, n_tn - band * C::BandN), tm = r / bw;
-  const int m0 = tm * C::BM, n0 = (band * C::BandN + r - tm * bw) * C::BN;
-  const int rows = min(C::BM, len - m0), cols = min(C::BN, a.N - n0);
-  const int64_t row0 = (int64_t)start + m0;
+  const Groups groups = load_groups<C::BM>(a.group_offs, a.G, tile_rows_end(a), n_tn, lane);
+  struct At {
+    int g, rows, n0;                // rows 0: no tile
+    int64_t row0;
+  };
+  auto tile_at = [&](int block) {
+    Tile w{-1, 0, 0, 0};
+    if (block < blocks) w = find_tile<C::BM>(groups, n_tn, mid::tile_of_block(block));
+    if (w.g < 0) return At{0, 0, 0, 0};
+    const int n_tm = (w.len + C::BM - 1) / C::BM;
+    const int band = w.in_g / (n_tm * C::BandN), r = w.in_g - band * n_tm * C::BandN;
+    const int bw = min(C::BandN, n_tn - band * C::BandN), tm = r / bw;
+    return At{w.g, min(C::BM, w.len - tm * C::BM), (band * C::BandN + r - tm * bw) * C::BN, (int64_t)w.start + tm * C::BM};
+  };
+  int block = blockIdx.x;
+  At tile = tile_at(block);
+  if (tile.rows == 0) return;                                  // more workgroups than tiles
+  block += grid;
+  At next = C::kWalk ? tile_at(block) : At{0, 0, 0, 0};
 
-  const uint8_t* pa = a.a + row0 * a.stride_a;
-  const uint8_t* pb = a.b + (int64_t)g * a.stride_bg + (int64_t)n0 * a.stride_bn;
-  const v4i ras = make_rsrc(a.a_scales + row0 * a.stride_as, rows * a.stride_as);
-  const v4i rbs = make_rsrc(a.b_scales + (int64_t)g * a.stride_bsg + (int64_t)n0 * a.stride_bsn, cols * a.stride_bsn);
-  const int rec_a = rows * a.stride_a, rec_b = cols * a.stride_bn;
-  const int bytes_a = kA8 ? a.K : a.K / 2, bytes_b = a.K / 2;
-
-  // ---- loads: rows of 128 bytes as in persistent_kernel.h; of 64 bytes chunk c of row r at c ^ ((r >> 2) & 3)
-  const int lca = (lane & 7) ^ (lane >> 3) ^ (wave & 1);
-  const int va = (8 * wave + (lane >> 3)) * a.stride_a + 16 * lca;
-  const int lcb = kA8 ? (lane & 3) ^ (lane >> 4) : lca;
-  const int vb = kA8 ? (16 * wave + (lane >> 2)) * a.stride_bn + 16 * lcb : (8 * wave + (lane >> 3)) * a.stride_bn + 16 * lcb;
-  constexpr int kRowsB = kA8 ? 64 : 32;                        // B rows of the four waves' instructions
+  // ---- loads, two stages ahead of the products, across the end of a tile. Rows of 128 bytes as in persistent_kernel.h;
+  // of 64 bytes chunk c of row r at c ^ ((r >> 2) & 3)
+  const int bytes_a = kA8 ? a.K : a.K / 2, bytes_b = a.K / 2, all_blocks = a.K / 32;
+  const int nst = (a.K + C::KS - 1) / C::KS;
+  const int lc128 = (lane & 7) ^ (lane >> 3) ^ (wave & 1), lc64 = (lane & 3) ^ (lane >> 4);
+  auto lane_row = [&](int row) { return row == 128 ? 8 * wave + (lane >> 3) : 16 * wave + (lane >> 2); };
+  const int lca = C::RowA == 128 ? lc128 : lc64, lcb = C::RowB == 128 ? lc128 : lc64;
+  const int va = lane_row(C::RowA) * a.stride_a + 16 * lca, vb = lane_row(C::RowB) * a.stride_bn + 16 * lcb;
+  const int step_a = 1024 * C::W / C::RowA * a.stride_a, step_b = 1024 * C::W / C::RowB * a.stride_bn;   // the waves' rows
+  constexpr int kPer = C::PA + C::PB;
   const uint32_t base = lds_u32(lds);
-  auto issue = [&](int st, int slot) {
-    if (st % C::Super == 0) {
-      const int u = st / C::Super;
-      const uint32_t at = base + C::ScaleOff + (u & 1) * C::ScaleBytes;
+  int ahead = 0, ahead_chunk = 0;                              // the stage in its tile, the chunk of scales
+  const uint8_t *pa, *pb;                                      // at the stage
+  int left_a, left_b;                                          // bytes of the tile's rows from there on
+  v4i ra, rb, ras, rbs;
+  bool dead_a, dead_b;
+  auto load_from = [&](const At& t) {
+    const int cols = min(C::BN, a.N - t.n0), live = t.rows > 0;   // no tile: everything is out of range and reads as zero
+    pa = a.a + t.row0 * a.stride_a;
+    pb = a.b + (int64_t)t.g * a.stride_bg + (int64_t)t.n0 * a.stride_bn;
+    left_a = t.rows * a.stride_a;
+    left_b = live * cols * a.stride_bn;
+    ras = make_rsrc(a.a_scales + t.row0 * a.stride_as, t.rows * a.stride_as);
+    rbs = make_rsrc(a.b_scales + (int64_t)t.g * a.stride_bsg + (int64_t)t.n0 * a.stride_bsn, live * cols * a.stride_bsn);
+  };
+  // what instructions of a stage share: its resources, and whether this lane's chunk lies past K (and reads as zero)
+  auto begin_stage = [&] {
+    if (ahead == nst) {                                        // asked for once `next` follows the tile of the products
+      ahead = 0;
+      load_from(next);
+    }
+    ra = make_rsrc(pa, max(left_a, 0));                        // of no tile nothing is left: never a negative count
+    rb = make_rsrc(pb, max(left_b, 0));
+    dead_a = 16 * lca >= bytes_a - ahead * C::RowA;
+    dead_b = 16 * lcb >= bytes_b - ahead * C::RowB;
+    if (ahead % C::Super == 0) {                               // the rows' 16 scale bytes from here on
+      const uint32_t at = base + C::ScaleOff + (ahead_chunk++ & 1) * C::ScaleBytes;
+      const int u = 16 * (ahead / C::Super);
 #pragma unroll
-      for (int k = 0; k < (C::SA + C::SB + 3) / 4; ++k) {
-        const int i = wave + 4 * k;                            // uniform
+      for (int k = 0; k < (C::SA + C::SB + C::W - 1) / C::W; ++k) {
+        const int i = wave + C::W * k;                            // uniform
         if (i < C::SA)
-          dma16(ras, at + 1024 * i, (64 * i + lane) * a.stride_as + 16 * u);
+          dma16(ras, at + 1024 * i, (64 * i + lane) * a.stride_as + u);
         else if (i < C::SA + C::SB)
-          dma16(rbs, at + 1024 * i, (64 * (i - C::SA) + lane) * a.stride_bsn + 16 * u);
+          dma16(rbs, at + 1024 * i, (64 * (i - C::SA) + lane) * a.stride_bsn + u);
       }
     }
-    const int ka = st * C::RowA, kb = st * C::RowB;
-    const v4i ra = make_rsrc(pa + ka, rec_a - ka), rb = make_rsrc(pb + kb, rec_b - kb);
-    const bool dead_a = 16 * lca >= bytes_a - ka, dead_b = 16 * lcb >= bytes_b - kb;   // chunks past K read as zero
+  };
+  auto issue_one = [&](int slot, int j) {                      // of this wave's PA + PB
     const uint32_t at = base + slot * C::Slot + 1024 * wave;
-#pragma unroll
-    for (int j = 0; j < C::PA; ++j) dma16(ra, at + 4096 * j, dead_a ? (int)kOob : va + 32 * j * a.stride_a);
-#pragma unroll
-    for (int j = 0; j < C::PB; ++j)
-      dma16(rb, at + C::ABytes + 4096 * j, dead_b ? (int)kOob : vb + kRowsB * j * a.stride_bn);
+    if (j < C::PA) dma16(ra, at + 1024 * C::W * j, dead_a ? (int)kOob : va + j * step_a);
+    else dma16(rb, at + C::ABytes + 1024 * C::W * (j - C::PA), dead_b ? (int)kOob : vb + (j - C::PA) * step_b);
+  };
+  auto end_stage = [&] {
+    pa += C::RowA, left_a -= C::RowA;
+    pb += C::RowB, left_b -= C::RowB;
+    ++ahead;
   };
 
   // ---- operand reads
   const int wm = wave % C::WM, wn = wave / C::WM;
   const int h = lane >> 5, s = lane & 31;
   const int ra0 = (32 * C::MB * wm + s) * C::RowA, rb0 = C::ABytes + (32 * C::NB * wn + s) * C::RowB;
-  const int sws = nt::swz(s), swb = kA8 ? (s >> 2) & 3 : sws;
-  const int sa0 = C::ScaleOff + 16 * (32 * C::MB * wm + s) + (kA8 ? 2 : 4) * h;
-  const int sb0 = C::ScaleOff + 1024 * C::SA + 16 * (32 * C::NB * wn + s) + (kA8 ? 2 : 4) * h;
-  const int blocks = a.K / 32;
+  const int swa = C::RowA == 128 ? nt::swz(s) : (s >> 2) & 3, swb = C::RowB == 128 ? nt::swz(s) : (s >> 2) & 3;
+  const int sa0 = C::ScaleOff + 16 * (32 * C::MB * wm + s) + C::Blocks / 2 * h;
+  const int sb0 = C::ScaleOff + 1024 * C::SA + 16 * (32 * C::NB * wn + s) + C::Blocks / 2 * h;
   v4i xl[2][C::MB], xh[2][C::MB], wt[2][C::NB];
   int sx[C::MB], sw[C::NB], nsx[C::MB], nsw[C::NB];
-  auto read = [&](auto set, int slot, int t) {
-    constexpr int k = decltype(set)::value;
+  // operand r of step t, in the order of their first use: the first column block, the row blocks, the other columns
+  auto read_one = [&](auto set, int slot, int t, auto which) {
+    constexpr int k = decltype(set)::value, r = decltype(which)::value;
     const GG_LDS uint8_t* p = lds + slot * C::Slot;
-    const int ca = kA8 ? 2 * t + h : 4 * h + t, cb = kA8 ? 2 * h + t : 4 * h + t;
-#pragma unroll
-    for (int j = 0; j < C::NB; ++j) wt[k][j] = *(const GG_LDS v4i*)(p + rb0 + 32 * C::RowB * j + 16 * (cb ^ swb));
-#pragma unroll
-    for (int i = 0; i < C::MB; ++i) {
-      xl[k][i] = *(const GG_LDS v4i*)(p + ra0 + 32 * C::RowA * i + 16 * (ca ^ sws));
-      if constexpr (kA8) xh[k][i] = *(const GG_LDS v4i*)(p + ra0 + 32 * C::RowA * i + 16 * ((ca + 4) ^ sws));
+    if constexpr (r >= 1 && r <= C::MB) {
+      constexpr int i = r - 1;
+      const int c = kA8 ? 2 * t + h : C::Blocks / 2 * h + t;
+      xl[k][i] = *(const GG_LDS v4i*)(p + ra0 + 32 * C::RowA * i + 16 * (c ^ swa));
+      if constexpr (kA8) xh[k][i] = *(const GG_LDS v4i*)(p + ra0 + 32 * C::RowA * i + 16 * ((c + 4) ^ swa));
+    } else {
+      constexpr int j = r == 0 ? 0 : r - C::MB;
+      const int c = C::Blocks / 2 * h + t;
+      wt[k][j] = *(const GG_LDS v4i*)(p + rb0 + 32 * C::RowB * j + 16 * (c ^ swb));
     }
   };
-  // a lane's scales of a stage, those of blocks past K as zero: what follows them in a row is not looked at
-  auto read_scales = [&](int st) {
-    const GG_LDS uint8_t* p = lds + (st / C::Super & 1) * C::ScaleBytes + (kA8 ? 4 * (st & 3) : 8 * (st & 1));
-    const int left = blocks - (kA8 ? 4 * st + 2 * h : 8 * st + 4 * h);
-    const uint32_t mask = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
-#pragma unroll
-    for (int j = 0; j < C::NB; ++j) {
-      const GG_LDS uint8_t* q = p + sb0 + 512 * j;
-      nsw[j] = (int)((kA8 ? (uint32_t)*(const GG_LDS uint16_t*)q : *(const GG_LDS uint32_t*)q) & mask);
-    }
-#pragma unroll
-    for (int i = 0; i < C::MB; ++i) {
-      const GG_LDS uint8_t* q = p + sa0 + 512 * i;
-      nsx[i] = (int)((kA8 ? (uint32_t)*(const GG_LDS uint16_t*)q : *(const GG_LDS uint32_t*)q) & mask);
-    }
+  // a lane's scales of stage st of its tile, in the buffer of chunk c
+  auto read_scale = [&](int c, int st, auto which) {
+    constexpr int r = decltype(which)::value;
+    const GG_LDS uint8_t* p = lds + (c & 1) * C::ScaleBytes + C::Blocks * (st % C::Super);
+    auto word = [&](const GG_LDS uint8_t* q) {
+      return C::Blocks == 4 ? (int)*(const GG_LDS uint16_t*)q : *(const GG_LDS int*)q;
+    };
+    if constexpr (r < C::NB) nsw[r] = word(p + sb0 + 512 * r);
+    else nsx[r - C::NB] = word(p + sa0 + 512 * (r - C::NB));
   };
   v16f acc[C::MB][C::NB];
+  auto clear = [&] {
 #pragma unroll
-  for (int i = 0; i < C::MB; ++i)
-#pragma unroll
-    for (int j = 0; j < C::NB; ++j)
-#pragma unroll
-      for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.f;
-
-  const int nst = (a.K + C::KS - 1) / C::KS;
-  constexpr int kPer = C::PA + C::PB;
-#pragma unroll
-  for (int st = 0; st < C::S; ++st)
-    if (st < nst) issue(st, st);
-  if (nst >= C::S) wait_vmcnt<(C::S - 1) * kPer>(); else wait_vmcnt<0>();
-  lds_barrier();
-  read(std::integral_constant<int, 0>{}, 0, 0);
-  read_scales(0);
-  int cur = 0;
-  for (int st = 0; st < nst; ++st) {
-#pragma unroll
-    for (int j = 0; j < C::NB; ++j) sw[j] = nsw[j];
-#pragma unroll
-    for (int i = 0; i < C::MB; ++i) sx[i] = nsx[i];
-    const int nxt = cur + 1 == C::S ? 0 : cur + 1;
-    static_for<C::T>([&](auto step) {
-      constexpr int t = decltype(step)::value;
-      if constexpr (t + 1 < C::T) {
-        read(std::integral_constant<int, (t + 1) & 1>{}, cur, t + 1);
-      } else if (st + 1 < nst) {
-        // stage st + 1 has landed for this wave (those after it may be in flight), then for all; every wave holds
-        // its last operands of stage st, whose slot is free
-        if (st + C::S <= nst) wait_vmcnt<(C::S - 2) * kPer>(); else wait_vmcnt<0>();
-        lds_barrier();
-        if (st + C::S < nst) issue(st + C::S, cur);
-        read(std::integral_constant<int, 0>{}, nxt, 0);
-        read_scales(st + 1);
-      }
-      __builtin_amdgcn_sched_barrier(0);                       // the reads go out before the products
+    for (int i = 0; i < C::MB; ++i)
 #pragma unroll
       for (int j = 0; j < C::NB; ++j)
 #pragma unroll
-        for (int i = 0; i < C::MB; ++i)
-          acc[i][j] = mma<t, kA8>(wt[t & 1][j], xl[t & 1][i], xh[t & 1][i], acc[i][j], sw[j], sx[i]);
-      keep_here(acc);
-    });
-    cur = nxt;
-  }
+        for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.f;
+  };
 
-  lds_barrier();                                               // every wave is past its reads: the slots are free
-  store<kAct, C::MB, C::NB>(acc, e, a.out, a.stride_out, g, a.N, row0 + 32 * C::MB * wm, rows - 32 * C::MB * wm,
-                            n0 + 32 * C::NB * wn, lds + wave * C::Region, lane);
+  load_from(tile);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    begin_stage();
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) issue_one(k, j);
+    end_stage();
+  }
+  wait_vmcnt<kPer>();
+  lds_barrier();
+  constexpr int kMma = C::MB * C::NB, kReads = C::MB + C::NB;
+  static_for<kReads>([&](auto r) {
+    read_scale(0, 0, r);
+    read_one(std::integral_constant<int, 0>{}, 0, 0, r);
+  });
+  clear();
+  // Instructions go out in their order, and one that waits for its turn at LDS or the load path holds up the products
+  // behind it: reads and loads are dealt out between the products, as many to each.
+  int cur = 0, st = 0, chunk = 0;
+  for (;;) {
+    // scales of blocks past K count as zero: what follows them in a row is not looked at
+    const int left = all_blocks - C::Blocks * st - C::Blocks / 2 * h;
+    const int mask = left >= 4 ? ~0 : left <= 0 ? 0 : (int)((1u << (8 * left)) - 1u);
+#pragma unroll
+    for (int j = 0; j < C::NB; ++j) sw[j] = nsw[j] & mask;
+#pragma unroll
+    for (int i = 0; i < C::MB; ++i) sx[i] = nsx[i] & mask;
+    st = st + 1 == nst ? 0 : st + 1;
+    chunk += st % C::Super == 0;                               // of the stage that comes, of this tile or the next
+    static_for<C::T>([&](auto step) {
+      constexpr int t = decltype(step)::value;
+      constexpr bool kLast = t + 1 == C::T;
+      static_for<kMma>([&](auto at) {
+        constexpr int n = decltype(at)::value, j = n / C::MB, i = n % C::MB;
+        acc[i][j] = mma<t, kA8>(wt[t & 1][j], xl[t & 1][i], xh[t & 1][i], acc[i][j], sw[j], sx[i]);
+        if constexpr (kLast && n == 0) {
+          // the stage that comes has landed for this wave, then for all; every wave holds its last operands of this one,
+          // whose slot is free
+          keep_here(acc);
+          wait_vmcnt<0>();
+          lds_barrier();
+          begin_stage();
+        }
+        constexpr auto share = [](int all, int k) { return all * k / kMma; };
+        static_for<share(kReads, n + 1) - share(kReads, n)>([&](auto d) {
+          constexpr std::integral_constant<int, share(kReads, n) + decltype(d)::value> r;
+          if constexpr (kLast) {
+            read_scale(chunk, st, r);
+            read_one(std::integral_constant<int, 0>{}, cur ^ 1, 0, r);
+          } else {
+            read_one(std::integral_constant<int, (t + 1) & 1>{}, cur, t + 1, r);
+          }
+        });
+        if constexpr (kLast) {
+#pragma unroll
+          for (int d = share(kPer, n); d < share(kPer, n + 1); ++d) issue_one(cur, d);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    });
+    keep_here(acc);
+    end_stage();
+    cur ^= 1;
+    if (st != 0) continue;
+    store<kAct, C::MB, C::NB>(acc, e, a.out, a.stride_out, tile.g, a.N, tile.row0 + 32 * C::MB * wm,
+                              tile.rows - 32 * C::MB * wm, tile.n0 + 32 * C::NB * wn, lane);
+    if (next.rows == 0) break;
+    tile = next;
+    block += grid;
+    next = tile_at(block);
+    clear();
+  }
+  wait_vmcnt<0>();                                             // loads of no tile write zeros to LDS
 }
 
 // Few rows (decoding): bound by reading the weights once, so nothing but loads in flight counts. A workgroup takes 16
@@ -338,7 +439,7 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
 // v_mfma_scale_f32_16x16x128, weights as rows: lane 16 q + s feeds row s of either side, blocks 2 q and 2 q + 1 of
 // the pair's eight, one to a step, its scales two neighbouring bytes.
 namespace few {
-constexpr int kWaves = 4, kBatch = 3;    // pairs a wave has in flight: all of its share of up to 12
+constexpr int kWaves = 4, kNT = 256, kBatch = 3;    // pairs a wave has in flight: all of its share of up to 12
 
 template <int kSel, bool kA8>
 __device__ __forceinline__ v4f mma(const v4i& w, const v4i& lo, const v4i& hi, v4f c, int sw, int sx) {
@@ -359,14 +460,14 @@ __device__ __forceinline__ void body(const Args& a, GG_LDS uint8_t* lds, const e
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n_tn = (a.N + BN - 1) / BN;
-  const Tile at = find_tile<16>(a.group_offs, a.G, tile_rows_end(a), n_tn, mid::tile_of_block(blockIdx.x), lane);
-  if (at.g < 0) return;
-  const int g = __builtin_amdgcn_readfirstlane(at.g), start = __builtin_amdgcn_readfirstlane(at.start);
-  const int len = __builtin_amdgcn_readfirstlane(at.len), in_g = __builtin_amdgcn_readfirstlane(at.in_g);
-  const int n_tm = (len + 15) / 16;                            // row tiles fastest: those of one group share its columns
-  const int tn = in_g / n_tm, m0 = (in_g - tn * n_tm) * 16, n0 = tn * BN;
-  const int rows = min(16, len - m0), cols = min(BN, a.N - n0);
-  const int64_t row0 = (int64_t)start + m0;
+  const Tile at = find_tile<16>(load_groups<16>(a.group_offs, a.G, tile_rows_end(a), n_tn, lane), n_tn,
+                                mid::tile_of_block(blockIdx.x));
+  if (at.g < 0) return;                                        // more workgroups than tiles
+  const int g = at.g;
+  const int n_tm = (at.len + 15) / 16;                         // row tiles fastest: those of one group share its columns
+  const int tn = at.in_g / n_tm, m0 = (at.in_g - tn * n_tm) * 16, n0 = tn * BN;
+  const int rows = min(16, at.len - m0), cols = min(BN, a.N - n0);
+  const int64_t row0 = (int64_t)at.start + m0;
 
   const int q = lane >> 4, s = lane & 15;
   auto rsrc = [](const uint8_t* p, int bytes) {
