@@ -231,7 +231,7 @@ def load():
     lib.ggemm_product_tile_rows.restype = ctypes.c_int32
     lib.ggemm_product_act_workspace.argtypes = [i64, i32, i32]
     lib.ggemm_product_act_workspace.restype = ctypes.c_int64
-    lib.ggemm_mx_tile_rows.argtypes = [i32] * 5 + [i64, i32]
+    lib.ggemm_mx_tile_rows.argtypes = [i32] * 4 + [i64, i32]
     lib.ggemm_mx_tile_rows.restype = ctypes.c_int32
     _lib = lib
     return lib

@@ -65,11 +65,13 @@ int over_rows(mxq::Args a, int dtype, F launch) {
 // ------------------------------------------------------------------------------ the product
 
 template <bool kA8>
-using Tile256 = mx::Cfg<kA8, 256, 256, 2, 4, true>;
+using Tile256 = mx::Cfg<kA8, 256, 256, 2, 4, kA8 ? 128 : 256, 2, true>;
 template <bool kA8>
-using Tile128 = mx::Cfg<kA8, 128, 128, 2, 2, false>;
+using Tile128 = mx::Cfg<kA8, 128, 128, 2, 2, kA8 ? 128 : 256, kA8 ? 3 : 2, false>;
 template <bool kA8>
-using Tile64 = mx::Cfg<kA8, 64, 128, 1, 4, false>;
+using Tile64 = mx::Cfg<kA8, 64, 128, 1, 4, 256, kA8 ? 2 : 3, false>;
+template <bool kA8>
+using Tile32 = mx::Cfg<kA8, 32, 128, 1, 4, 256, 3, false>;
 
 __device__ __forceinline__ void clear_tail(int kAct, const mx::Args& a) {
   if (a.zero_tail)
@@ -104,11 +106,32 @@ int with_act(int act, F f) {
 
 int64_t tiles_of(int64_t M, int64_t g, int N, int bm, int bn) { return (M / bm + g) * ((N + bn - 1) / bn); }
 
-int choose(int fmt, int G, int N, int K, int act, int64_t M, int cus) {
+// Rows of the output tiles of the fastest kernel. Few rows go to few::body while its tiles of 16 columns are what fills the chip: up
+// to 16 rows to a group in the mean and 160 tiles of 32 x 128. Measured (us, 32-row tiles -> it; weights not in a
+// cache): N = 5760, K = 2880, e4m3: 1 row of 1 expert 10.2 -> 6.3, 16 of 2 10.7 -> 9.5, 4 of 4 13.0 -> 13.4 (stays),
+// 64 of 32 55.8 -> 70.0 (stays); 2 of 2, N = K = 2880 9.7 -> 5.9; 2 of 1, N = K = 4096 11.6 -> 6.1.
+// The others by an estimate in us, c + rounds (e + s K / 1000), where a round is as many tiles as the chip holds at once.
+// The numbers are a fit to 32 (e4m3) and 26 launches (e2m1) of 32 to 32768 rows, 1 to 32 groups, N 512 to 5760, K 512 to
+// 4096: single times are off by up to 0.5 to 1.35, the choice by 3.5 % and 1.2 % in the mean, 22 % and 17 % at most.
+struct Fit {
+  int rows, cols, per_cu;
+  double c, e, s;
+};
+constexpr Fit kFits[2][4] = {{{32, 128, 2, 0.6, 3.8, 3.05}, {64, 128, 2, -1.7, 4.7, 4.36},
+                              {128, 128, 2, -6.3, 10.5, 5.55}, {256, 256, 1, -0.1, 8.0, 11.6}},
+                             {{32, 128, 2, 0.1, 4.4, 2.22}, {64, 128, 2, -3.9, 8.6, 2.04},
+                              {128, 128, 2, -8.7, 14.4, 3.03}, {256, 256, 1, -5.0, 14.0, 6.51}}};
+int choose(int fmt, int G, int N, int K, int64_t M, int cus) {
   const int64_t g = std::min<int64_t>(G, M);
-  if (M <= 8 * g) return 16;
-  if (tiles_of(M, g, N, 256, 256) >= cus) return 256;
-  return tiles_of(M, g, N, 128, 128) >= cus ? 128 : 64;
+  if (M <= 16 * g && g * ((N + 127) / 128) <= 5 * cus / 8) return 16;
+  int best = 0;
+  double least = 0;
+  for (const Fit& f : kFits[fmt == GGEMM_MX_E2M1]) {
+    const double tiles = std::max<double>(g, (double)M / f.rows + g / 2.0) * ((N + f.cols - 1) / f.cols);
+    const double t = f.c + std::max(1.0, tiles / (f.per_cu * cus)) * (f.e + f.s * K / 1000);
+    if (best == 0 || t < least) best = f.rows, least = t;
+  }
+  return best;
 }
 
 // Whole runs of tiles over the XCDs (mid_common.h).
@@ -132,6 +155,8 @@ int launch(const mx::Args& a, const epi::Args& e, int tile, int cus, hipStream_t
       hipLaunchKernelGGL((mx_few_kernel<kAct, kA8, 1>), dim3(tiles(16, 16)), dim3(mx::few::kNT), 0, stream, a, e);
     else
       hipLaunchKernelGGL((mx_few_kernel<kAct, kA8, 2>), dim3(tiles(16, 32)), dim3(mx::few::kNT), 0, stream, a, e);
+  } else if (tile == 32) {
+    run(Tile32<kA8>{});
   } else if (tile == 64) {
     run(Tile64<kA8>{});
   } else if (tile == 128) {
@@ -202,8 +227,8 @@ int ggemm_mx_dequantize(const void* q, int32_t fmt, int64_t rows, int32_t cols, 
   });
 }
 
-int32_t ggemm_mx_tile_rows(int32_t a_fmt, int32_t G, int32_t N, int32_t K, int32_t act, int64_t M_total, int32_t num_cus) {
-  return choose(a_fmt, G, N, K, act, M_total, num_cus);
+int32_t ggemm_mx_tile_rows(int32_t a_fmt, int32_t G, int32_t N, int32_t K, int64_t M_total, int32_t num_cus) {
+  return choose(a_fmt, G, N, K, M_total, num_cus);
 }
 
 int ggemm_mx_product(const void* a, int32_t a_fmt, const uint8_t* a_scales, const void* b, const uint8_t* b_scales,
@@ -219,12 +244,12 @@ int ggemm_mx_product(const void* a, int32_t a_fmt, const uint8_t* a_scales, cons
                     shift, slope * -epi::kLog2e};
   int rc = validate(x, e, a_fmt, act, bias_dtype, {stride_a, stride_as, stride_bg, stride_bn, stride_bsg, stride_bsn});
   if (rc) return rc;
-  if (tile != 0 && tile != 16 && tile != 64 && tile != 128 && tile != 256) return GGEMM_E_SHAPE;
+  if (tile != 0 && tile != 16 && tile != 32 && tile != 64 && tile != 128 && tile != 256) return GGEMM_E_SHAPE;
   int cus = 0;
   rc = device_cus(&cus);
   if (rc) return rc;
   if (M_total == 0) return GGEMM_OK;
-  if (tile == 0) tile = choose(a_fmt, G, N, K, act, M_total, cus);
+  if (tile == 0) tile = choose(a_fmt, G, N, K, M_total, cus);
   return with_act(act, [&](auto code) {
     constexpr int kAct = decltype(code)::value;
     return a_fmt == GGEMM_MX_E4M3 ? launch<kAct, true>(x, e, tile, cus, (hipStream_t)stream)

@@ -7,7 +7,7 @@
 // fp8's.
 //
 // A tile is BM rows of one group x BN columns. A stage is 128 bytes of every A row (256 values of e2m1, 128 of e4m3) and as
-// many values of every B row, loaded by LDS-DMA into one of two slots. The scales are 1/16 of the bytes, but rows far
+// many values of every B row, loaded by LDS-DMA into one of S slots. The scales are 1/16 of the bytes, but rows far
 // apart: 16 bytes of a row, 512 values, come at once and serve two or four stages, since one more request for each row
 // and stage would double the requests of the load path.
 //
@@ -18,8 +18,6 @@
 // The operands of step t + 1 are read while step t multiplies; the barrier that frees a stage's slot stands in its
 // last step, whose operands are in registers by then, so that the next stage's loads and first reads run beside its products.
 //
-// 256 x 256: eight waves of 128 x 64, two on a SIMD, one workgroup on a CU that walks over its tiles and loads the next
-// tile's first stages while it finishes one. 128 x 128 and 64 x 128: four waves, two workgroups on a CU, a tile each.
 #pragma once
 
 #include "fused_epilogue.h"
@@ -52,38 +50,57 @@ __device__ __forceinline__ int64_t tile_rows_end(const Args& a) {
   return clamp_off(a.group_offs[a.G], a.m_total);
 }
 
+// Inclusive maximum or sum over a wave's lanes of values that are not negative, by DPP: lanes 1, 2, 4 and 8 to the left in a
+// row of 16, then the last lane of a row to the next ones. (Shuffles go through LDS: twelve in turn are a microsecond.)
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int dpp(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xF, false);
+}
+template <typename F>
+__device__ __forceinline__ int scan(int v, F f) {
+  v = f(v, dpp<0x111, 0xF>(v));
+  v = f(v, dpp<0x112, 0xF>(v));
+  v = f(v, dpp<0x114, 0xF>(v));
+  v = f(v, dpp<0x118, 0xF>(v));
+  v = f(v, dpp<0x142, 0xA>(v));
+  return f(v, dpp<0x143, 0xC>(v));
+}
+struct Max {
+  __device__ int operator()(int a, int b) const { return max(a, b); }
+};
+struct Sum {
+  __device__ int operator()(int a, int b) const { return a + b; }
+};
+
 // The groups of a launch as tiles: lane l holds ceil(G / 64) consecutive ones. Offsets count as the largest one so far, in
 // [0, m_total].
 struct Groups {
   const int64_t* offs;
   int64_t m;
   int G, per;
-  int before, first, len;           // the rows' end before the lane's groups; its first group: first row, rows
+  int first, len;                   // the lane's first group: first row, rows
   int sum, incl;                    // tiles of the lane's groups, and of those up to it
   __device__ __forceinline__ int row(int g) const { return (int)clamp_off(offs[g], m); }
 };
 template <int BM>
 __device__ __forceinline__ Groups load_groups(const int64_t* offs, int G, int64_t m, int n_tn, int lane) {
-  Groups r{offs, m, G, (G + 63) >> 6};
+  Groups r{offs, m, G, (G + 63) >> 6, 0, 0, 0, 0};
   const int g0 = min(lane * r.per, G), g1 = min(g0 + r.per, G);
-  int top = 0;
-  for (int g = g0; g < g1; ++g) top = max(top, r.row(g));
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int v = __shfl_up(top, d, 64);
-    if (lane >= d) top = max(top, v);
-  }
-  r.before = __shfl_up(top, 1, 64);
-  if (lane == 0) r.before = 0;
-  int run = r.before;
-  r.sum = r.first = r.len = 0;
-  for (int g = g0; g < g1; ++g) {
-    run = max(run, r.row(g));
-    const int len = max(run, r.row(g + 1)) - run;
-    if (g == g0) r.first = run, r.len = len;
-    r.sum += (len + BM - 1) / BM * n_tn;
-  }
-  r.incl = mid::wave_scan(r.sum, lane);
+  const int begin = r.row(g0);                                // lanes past the last group: offs[G], of no group
+  int end = r.row(min(g0 + 1, G)), top = max(begin, 0);
+  if (r.per > 1)
+    for (int g = g0 + 1; g < g1; ++g) top = max(top, r.row(g));
+  top = scan(top, Max{});
+  const int before = dpp<0x138, 0xF>(top);                    // of the lane to the left; 0 for the first
+  r.first = max(before, begin);
+  r.len = g0 < g1 ? max(r.first, end) - r.first : 0;
+  r.sum = (r.len + BM - 1) / BM * n_tn;
+  if (r.per > 1)
+    for (int g = g0 + 1, run = r.first + r.len; g < g1; ++g) {
+      run = max(run, r.row(g));
+      r.sum += (max(run, r.row(g + 1)) - run + BM - 1) / BM * n_tn;
+    }
+  r.incl = scan(r.sum, Sum{});
   return r;
 }
 
@@ -108,11 +125,11 @@ __device__ __forceinline__ Tile find_tile(const Groups& r, int n_tn, int t) {
 }
 
 // kWalk: one workgroup on a CU, which walks over its tiles; else two, with a tile each.
-template <bool kA8, int kBM, int kBN, int kWM, int kWN, bool kWalk_>
+template <bool kA8, int kBM, int kBN, int kWM, int kWN, int kKS, int kStages, bool kWalk_>
 struct Cfg {
   static constexpr int BM = kBM, BN = kBN, WM = kWM, WN = kWN, W = WM * WN, NT = 64 * W;   // waves and threads
   static constexpr bool kWalk = kWalk_;
-  static constexpr int KS = kA8 ? 128 : 256;                    // values of K in a stage
+  static constexpr int KS = kKS, S = kStages;                   // values of K in a stage, and slots
   static constexpr int RowA = kA8 ? KS : KS / 2, RowB = KS / 2; // bytes of a row in it
   static constexpr int Blocks = KS / 32;                        // and blocks
   static constexpr int T = KS / 64;                             // steps of a stage
@@ -120,14 +137,21 @@ struct Cfg {
   static constexpr int ABytes = BM * RowA, BBytes = BN * RowB, Slot = ABytes + BBytes;
   static constexpr int PA = ABytes / 1024 / W, PB = BBytes / 1024 / W;   // LDS-DMA instructions for each wave and stage
   static constexpr int SA = (BM + 63) / 64, SB = (BN + 63) / 64;   // of scales for the workgroup, 64 rows each
-  static constexpr int ScaleOff = 2 * Slot, ScaleBytes = 1024 * (SA + SB);
+  static constexpr int ScaleOff = S * Slot, ScaleBytes = 1024 * (SA + SB);
   static constexpr int LdsBytes = ScaleOff + 2 * ScaleBytes;
   static constexpr int MB = BM / WM / 32, NB = BN / WN / 32;    // 32-wide blocks of a wave
   static constexpr int BandN = 8;                               // column tiles of a band, row tiles walked inside
   static_assert(W % 2 == 0 && MB >= 1 && NB >= 1 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "waves");
   static_assert(ABytes % (1024 * W) == 0 && BBytes % (1024 * W) == 0, "uniform LDS-DMA split");
+  static_assert(S >= 2 && (kWalk ? S == 2 : S <= Super + 1), "a buffer of scales is read out when its next chunk is asked for");
   static_assert(LdsBytes <= (kWalk ? 160 : 80) * 1024, "LDS");
 };
+
+// Chunk c of row r, `row` bytes a stage, lies at c ^ swizzle: 16 rows' equal chunks on 16 different groups of banks. Rows that
+// are a multiple of 16 apart have the same one, and so have the rows of a wave's load instructions.
+__device__ __forceinline__ constexpr int swizzle(int row, int r) {
+  return row == 256 ? r & 15 : row == 128 ? (r & 7) ^ ((r >> 3) & 1) : (r >> 2) & 3;
+}
 
 template <int kSel, bool kA8>
 __device__ __forceinline__ v16f mma(const v4i& w, const v4i& lo, const v4i& hi, v16f c, int sw, int sx) {
@@ -255,13 +279,13 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
   block += grid;
   At next = C::kWalk ? tile_at(block) : At{0, 0, 0, 0};
 
-  // ---- loads, two stages ahead of the products, across the end of a tile. Rows of 128 bytes as in persistent_kernel.h;
-  // of 64 bytes chunk c of row r at c ^ ((r >> 2) & 3)
+  // ---- loads, S stages ahead of the products, across the end of a tile
   const int bytes_a = kA8 ? a.K : a.K / 2, bytes_b = a.K / 2, all_blocks = a.K / 32;
   const int nst = (a.K + C::KS - 1) / C::KS;
-  const int lc128 = (lane & 7) ^ (lane >> 3) ^ (wave & 1), lc64 = (lane & 3) ^ (lane >> 4);
-  auto lane_row = [&](int row) { return row == 128 ? 8 * wave + (lane >> 3) : 16 * wave + (lane >> 2); };
-  const int lca = C::RowA == 128 ? lc128 : lc64, lcb = C::RowB == 128 ? lc128 : lc64;
+  // the row of a wave's first instruction that this lane loads, and its chunk of it
+  auto lane_row = [&](int row) { return row == 256 ? 4 * wave + (lane >> 4) : row == 128 ? 8 * wave + (lane >> 3) : 16 * wave + (lane >> 2); };
+  auto lane_chunk = [&](int row) { return (lane & (row / 16 - 1)) ^ swizzle(row, lane_row(row)); };
+  const int lca = lane_chunk(C::RowA), lcb = lane_chunk(C::RowB);
   const int va = lane_row(C::RowA) * a.stride_a + 16 * lca, vb = lane_row(C::RowB) * a.stride_bn + 16 * lcb;
   const int step_a = 1024 * C::W / C::RowA * a.stride_a, step_b = 1024 * C::W / C::RowB * a.stride_bn;   // the waves' rows
   constexpr int kPer = C::PA + C::PB;
@@ -290,7 +314,8 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
     rb = make_rsrc(pb, max(left_b, 0));
     dead_a = 16 * lca >= bytes_a - ahead * C::RowA;
     dead_b = 16 * lcb >= bytes_b - ahead * C::RowB;
-    if (ahead % C::Super == 0) {                               // the rows' 16 scale bytes from here on
+    if (ahead % C::Super == 0 && left_b > 0) {                 // the rows' 16 scale bytes from here on; none of no tile, whose
+                                                               // place a scale of this one may still have
       const uint32_t at = base + C::ScaleOff + (ahead_chunk++ & 1) * C::ScaleBytes;
       const int u = 16 * (ahead / C::Super);
 #pragma unroll
@@ -318,7 +343,7 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
   const int wm = wave % C::WM, wn = wave / C::WM;
   const int h = lane >> 5, s = lane & 31;
   const int ra0 = (32 * C::MB * wm + s) * C::RowA, rb0 = C::ABytes + (32 * C::NB * wn + s) * C::RowB;
-  const int swa = C::RowA == 128 ? nt::swz(s) : (s >> 2) & 3, swb = C::RowB == 128 ? nt::swz(s) : (s >> 2) & 3;
+  const int swa = swizzle(C::RowA, s), swb = swizzle(C::RowB, s);
   const int sa0 = C::ScaleOff + 16 * (32 * C::MB * wm + s) + C::Blocks / 2 * h;
   const int sb0 = C::ScaleOff + 1024 * C::SA + 16 * (32 * C::NB * wn + s) + C::Blocks / 2 * h;
   v4i xl[2][C::MB], xh[2][C::MB], wt[2][C::NB];
@@ -329,9 +354,9 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
     const GG_LDS uint8_t* p = lds + slot * C::Slot;
     if constexpr (r >= 1 && r <= C::MB) {
       constexpr int i = r - 1;
-      const int c = kA8 ? 2 * t + h : C::Blocks / 2 * h + t;
+      const int c = kA8 ? 2 * t + h : C::Blocks / 2 * h + t;   // e4m3: halves of two blocks, Blocks / 2 blocks apart
       xl[k][i] = *(const GG_LDS v4i*)(p + ra0 + 32 * C::RowA * i + 16 * (c ^ swa));
-      if constexpr (kA8) xh[k][i] = *(const GG_LDS v4i*)(p + ra0 + 32 * C::RowA * i + 16 * ((c + 4) ^ swa));
+      if constexpr (kA8) xh[k][i] = *(const GG_LDS v4i*)(p + ra0 + 32 * C::RowA * i + 16 * ((c + C::Blocks) ^ swa));
     } else {
       constexpr int j = r == 0 ? 0 : r - C::MB;
       const int c = C::Blocks / 2 * h + t;
@@ -360,13 +385,13 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
 
   load_from(tile);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = 0; k < C::S; ++k) {
     begin_stage();
 #pragma unroll
     for (int j = 0; j < kPer; ++j) issue_one(k, j);
     end_stage();
   }
-  wait_vmcnt<kPer>();
+  wait_vmcnt<(C::S - 1) * kPer>();
   lds_barrier();
   constexpr int kMma = C::MB * C::NB, kReads = C::MB + C::NB;
   static_for<kReads>([&](auto r) {
@@ -376,7 +401,7 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
   clear();
   // Instructions go out in their order, and one that waits for its turn at LDS or the load path holds up the products
   // behind it: reads and loads are dealt out between the products, as many to each.
-  int cur = 0, st = 0, chunk = 0;
+  int cur = 0, nxt = 1, st = 0, chunk = 0;
   for (;;) {
     // scales of blocks past K count as zero: what follows them in a row is not looked at
     const int left = all_blocks - C::Blocks * st - C::Blocks / 2 * h;
@@ -394,10 +419,10 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
         constexpr int n = decltype(at)::value, j = n / C::MB, i = n % C::MB;
         acc[i][j] = mma<t, kA8>(wt[t & 1][j], xl[t & 1][i], xh[t & 1][i], acc[i][j], sw[j], sx[i]);
         if constexpr (kLast && n == 0) {
-          // the stage that comes has landed for this wave, then for all; every wave holds its last operands of this one,
-          // whose slot is free
+          // the stage that comes has landed for this wave (those after it may be in flight), then for all; every wave holds
+          // its last operands of this one, whose slot is free
           keep_here(acc);
-          wait_vmcnt<0>();
+          wait_vmcnt<(C::S - 2) * kPer>();
           lds_barrier();
           begin_stage();
         }
@@ -406,7 +431,7 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
           constexpr std::integral_constant<int, share(kReads, n) + decltype(d)::value> r;
           if constexpr (kLast) {
             read_scale(chunk, st, r);
-            read_one(std::integral_constant<int, 0>{}, cur ^ 1, 0, r);
+            read_one(std::integral_constant<int, 0>{}, nxt, 0, r);
           } else {
             read_one(std::integral_constant<int, (t + 1) & 1>{}, cur, t + 1, r);
           }
@@ -420,7 +445,8 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
     });
     keep_here(acc);
     end_stage();
-    cur ^= 1;
+    cur = nxt;
+    nxt = nxt + 1 == C::S ? 0 : nxt + 1;
     if (st != 0) continue;
     store<kAct, C::MB, C::NB>(acc, e, a.out, a.stride_out, tile.g, a.N, tile.row0 + 32 * C::MB * wm,
                               tile.rows - 32 * C::MB * wm, tile.n0 + 32 * C::NB * wn, lane);

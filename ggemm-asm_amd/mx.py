@@ -23,7 +23,7 @@ from .vark import _validate_offsets
 
 BLOCK = 32                       # values that share a scale
 _FORMATS = {"e4m3": 0, "e2m1": 1}
-TILES = (0, 16, 64, 128, 256)    # of ggemm_mx_product
+TILES = (0, 16, 32, 64, 128, 256)    # of ggemm_mx_product
 
 
 class MXTensor(NamedTuple):
@@ -49,10 +49,10 @@ def _columns(t: MXTensor, what: str) -> tuple[int, int]:
     return code, cols
 
 
-def tile_rows(a_format: str, G: int, N: int, K: int, M: int, activation: str | None = None, *, num_cus: int = 256) -> int:
-    """Rows of the output tiles of the kernel that ``grouped_gemm_mx_bias_act`` runs on these sizes: 16 (few rows), 64,
+def tile_rows(a_format: str, G: int, N: int, K: int, M: int, num_cus: int = 256) -> int:
+    """Rows of the output tiles of the kernel that ``grouped_gemm_mx_bias_act`` runs on these sizes: 16, 32, 64,
     128 or 256."""
-    return _lib.load().ggemm_mx_tile_rows(_FORMATS[a_format], G, N, K, _act(activation, 1.0, None, 0.0)[0], M, num_cus)
+    return _lib.load().ggemm_mx_tile_rows(_FORMATS[a_format], G, N, K, M, num_cus)
 
 
 # --------------------------------------------------------------------------- rows to blocks and back
@@ -133,21 +133,23 @@ def _padded(t: torch.Tensor, row: int) -> torch.Tensor:
     return out
 
 
-def _product_rows(t: torch.Tensor, row: int):
-    """(tensor, row stride, group stride) of an operand's bytes or scales, of whose rows ``row`` bytes are read: a copy
-    where the rows are not contiguous, do not start on multiples of 16 bytes, overlap or end before that."""
-    def strides(t):
-        rs = t.stride(-2) if t.shape[-2] > 1 else -(-row // 16) * 16
-        gs = 0 if t.dim() == 2 else t.stride(0) if t.shape[0] > 1 else t.shape[1] * rs
-        return rs, gs
-
-    rs, gs = strides(t)
-    last = (t.shape[-2] - 1) * rs
-    if (t.stride(-1) != 1 and t.shape[-1] > 1 or t.data_ptr() % 16 or rs % 16 or gs % 16 or rs < row
-            or t.dim() == 3 and t.shape[0] > 1 and gs < last + row
-            or t.storage_offset() + (gs * (t.shape[0] - 1) if t.dim() == 3 else 0) + last + row > t.untyped_storage().nbytes()):
+def _product_rows(t: torch.Tensor, row: int, past: bool):
+    """(tensor, row stride, group stride) of an operand's bytes or scales, of whose rows ``row`` bytes are read, more than
+    they hold where ``past``: a copy where the rows are not contiguous, do not start on multiples of 16 bytes, overlap or end
+    before that."""
+    shape, strides = t.shape, t.stride()
+    rows, rs = shape[-2], strides[-2]
+    if rows == 1:
+        rs = -(-row // 16) * 16
+    last = (rows - 1) * rs + row                       # bytes of a group
+    groups, gs = (shape[0], strides[0]) if len(shape) == 3 else (1, 0)
+    if groups == 1:
+        gs = -(-last // 16) * 16
+    if (strides[-1] != 1 and shape[-1] > 1 or (t.data_ptr() | rs | gs) & 15 or rs < row or gs < last
+            or past and t.storage_offset() + (groups - 1) * gs + last > t.untyped_storage().nbytes()):
         t = _padded(t, row)
-        rs, gs = strides(t)
+        rs = t.stride(-2)
+        gs = rows * rs
     return t, rs, gs
 
 
@@ -164,7 +166,7 @@ def grouped_gemm_mx_bias_act(a: MXTensor, b: MXTensor, group_offs: torch.Tensor,
 
     Operands as ``quantize_mx`` lays them out are read where they are. Others are copied at each call, unless rows of q
     and of scales start on multiples of 16 bytes and rows of scales can be read up to a multiple of 16: weights from
-    elsewhere are laid out so once. ``tile``: rows of the output tiles (16, 64, 128 or 256), 0 for the library's choice.
+    elsewhere are laid out so once. ``tile``: rows of the output tiles (16, 32, 64, 128 or 256), 0 for the library's choice.
     An operator of inference: it has no gradients and refuses a bias or residual that asks for one."""
     code, K = _columns(a, "a")
     b_code, Kb = _columns(b, "b")
@@ -209,10 +211,11 @@ def grouped_gemm_mx_bias_act(a: MXTensor, b: MXTensor, group_offs: torch.Tensor,
     if residual is not None:
         residual = _rows16(residual)
     chunk = -(-K // 512) * 16
-    aq, sa, _ = _product_rows(aq, K // 2 if code else K)
-    a_scales, sas, _ = _product_rows(a.scales, chunk)
-    bq, sbn, sbg = _product_rows(bq, K // 2)
-    b_scales, sbsn, sbsg = _product_rows(b.scales, chunk)
+    past = chunk > K // BLOCK
+    aq, sa, _ = _product_rows(aq, K // 2 if code else K, False)
+    a_scales, sas, _ = _product_rows(a.scales, chunk, past)
+    bq, sbn, sbg = _product_rows(bq, K // 2, False)
+    b_scales, sbsn, sbsg = _product_rows(b.scales, chunk, past)
     sres = 0 if residual is None else _stride(residual)
     _lib.launch("ggemm_mx_product", dev, G | N | K | sa | sas | sbn | sbsn | sres, aq.data_ptr(), code, a_scales.data_ptr(),
                 bq.data_ptr(), b_scales.data_ptr(), out.data_ptr(), None if bias is None else bias.data_ptr(),

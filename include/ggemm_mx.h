@@ -47,7 +47,7 @@ int ggemm_mx_dequantize(const void* q, int32_t fmt, int64_t rows, int32_t cols, 
  * Rows of A, B and of both scales start on multiples of 16 bytes, and a row of scales is ceil(K / 512) * 16 bytes that
  * may be read (those past K / 32 are not used). Offsets count as the largest one so far, within [0, M_total]: groups
  * never overlap. Rows of no group are not written, or rows from offs[G] on become zero with zero_tail != 0.
- * tile: rows of the output tiles, 16, 64, 128 or 256, or 0 for the library's choice. Each kernel sums a row's products in
+ * tile: rows of the output tiles, 16, 32, 64, 128 or 256, or 0 for the library's choice. Each kernel sums a row's products in
  * an order of its own, so a row's last bit can depend on G and M_total. */
 int ggemm_mx_product(const void* a, int32_t a_fmt, const uint8_t* a_scales, const void* b, const uint8_t* b_scales,
                      void* out, const void* bias, int32_t bias_dtype, const void* residual, const int64_t* group_offs,
@@ -57,7 +57,7 @@ int ggemm_mx_product(const void* a, int32_t a_fmt, const uint8_t* a_scales, cons
                      int32_t tile, void* stream);
 
 /* The tile that such a call takes by itself on a device of num_cus CUs. */
-int32_t ggemm_mx_tile_rows(int32_t a_fmt, int32_t G, int32_t N, int32_t K, int32_t act, int64_t M_total, int32_t num_cus);
+int32_t ggemm_mx_tile_rows(int32_t a_fmt, int32_t G, int32_t N, int32_t K, int64_t M_total, int32_t num_cus);
 
 #ifdef __cplusplus
 }

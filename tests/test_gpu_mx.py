@@ -172,7 +172,7 @@ SHAPES = [(1, 16, 32, [0, 1, 0]), (4, 320, 2880, [1, 0, 1, 1, 0, 1]), (70, 48, 1
 
 @pytest.mark.parametrize("M,N,K,lens", SHAPES)
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("tile", [0, 16, 64, 128, 256])
+@pytest.mark.parametrize("tile", [0, 16, 32, 64, 128, 256])
 def test_product(pkg, M, N, K, lens, fmt, tile):
     a, b, offs, gen = _case(M, N, K, lens, fmt, M + N)
     pad = 16 if tile else 0
@@ -199,7 +199,7 @@ LARGE = [(5000, 2048, 1440, [1200, 0, 1, 3700, 99]), (20000, 2880, 2880, [256, 1
 
 @pytest.mark.parametrize("M,N,K,lens", LARGE)
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("tile", [0, 64, 128, 256])
+@pytest.mark.parametrize("tile", [0, 32, 64, 128, 256])
 def test_large_product(pkg, M, N, K, lens, fmt, tile):
     a, b, offs, gen = _case(M, N, K, lens, fmt, M + N)
     da, db = (pkg.MXTensor(_laid_out(q, 0), _laid_out(s, 0)) for q, s in (a, b))
@@ -213,7 +213,7 @@ def test_large_product(pkg, M, N, K, lens, fmt, tile):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("tile", [16, 64, 128, 256])
+@pytest.mark.parametrize("tile", [16, 32, 64, 128, 256])
 def test_many_groups_and_odd_offsets(pkg, fmt, tile):
     """More groups than lanes, and the most there may be; offsets that start late, fall, leave the tensor or are negative."""
     lens = [1, 0, 2, 5] * 75
@@ -242,7 +242,7 @@ def test_many_groups_and_odd_offsets(pkg, fmt, tile):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("tile", [16, 64, 128, 256])
+@pytest.mark.parametrize("tile", [16, 32, 64, 128, 256])
 def test_nan_blocks_reach_their_rows_alone(pkg, fmt, tile):
     a, b, offs, _ = _case(90, 64, 352, [50, 40], fmt, 6)
     a[1][7, 3] = 255

@@ -70,7 +70,7 @@ def _product(lib, **kw):
     (dict(sbn=16), -3), (dict(sbn=40), -3), (dict(sbsn=8), -3), (dict(sbg=2032), -3), (dict(sbsg=1008), -3), (dict(sbg=2056), -3),
     (dict(sa=2 ** 24), -2), (dict(sbsn=2 ** 24, sbsg=2 ** 30), -2), (dict(so=56), -3), (dict(so=68), -3), (dict(sr=56), -3),
     (dict(act=3, so=24), -3), (dict(a=FAKE + 8), -4), (dict(asc=FAKE + 8), -4), (dict(b=FAKE + 8), -4), (dict(bsc=FAKE + 4), -4),
-    (dict(out=FAKE + 8), -4), (dict(bias=FAKE + 8), -4), (dict(res=FAKE + 8), -4), (dict(tile=32), -2), (dict(tile=-1), -2),
+    (dict(out=FAKE + 8), -4), (dict(bias=FAKE + 8), -4), (dict(res=FAKE + 8), -4), (dict(tile=48), -2), (dict(tile=-1), -2),
 ])
 def test_product_validation(pkg, kw, rc):
     assert _product(pkg.load_library(), **kw) == rc
@@ -78,10 +78,10 @@ def test_product_validation(pkg, kw, rc):
 
 def test_choice_of_a_kernel(pkg):
     from ggemm_asm_amd import mx
-    assert mx.tile_rows("e4m3", 32, 5760, 2880, 4, "swiglu") == 16
     for fmt in ("e4m3", "e2m1"):
-        assert mx.tile_rows(fmt, 32, 5760, 2880, 131072, "swiglu") == 256
-    assert mx.tile_rows("e4m3", 1, 16, 32, 1) in mx.TILES
+        assert [mx.tile_rows(fmt, 32, 5760, 2880, m) for m in (1, 256, 2048, 131072)] == [16, 32, 128, 256]
+        assert all(mx.tile_rows(fmt, G, N, K, M) in mx.TILES[1:] for G in (1, 64, 2047) for N in (16, 5760) for K in (32, 8192)
+                   for M in (1, 100, 10 ** 6))
 
 
 # --------------------------------------------------------------------------- the torch ops
