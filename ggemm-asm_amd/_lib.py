@@ -100,6 +100,9 @@ MX_EXPORTS = (
     "ggemm_mx_dequantize",
     "ggemm_mx_product",
     "ggemm_mx_tile_rows",
+    "ggemm_mx_keep_product",
+    "ggemm_mx_keep_tile_rows",
+    "ggemm_mx_act_backward",
 )
 
 # GGEMM_VARK_ABI_VERSION of include/ggemm_vark.h that these bindings are written for. Some exports
@@ -223,6 +226,9 @@ def load():
     lib.ggemm_mx_dequantize.argtypes = [vp, i32, i64, i32, i64, vp, i64, i64, vp, i32, i64, vp]
     lib.ggemm_mx_product.argtypes = [vp, i32, vp, vp, vp, vp, vp, i32, vp, vp, i32, i32, i32] + [i64] * 6 + \
         [i32, i32, i32, f32, f32, f32, i64, i32, i32, vp]
+    lib.ggemm_mx_keep_product.argtypes = [vp] * 8 + [i32, vp, vp] + [i32] * 8 + [i64, i32, i32, f32, f32, f32, i64, i32, vp]
+    lib.ggemm_mx_act_backward.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, i64, i64, i32, f32, f32, f32, i64, vp, i32, vp,
+                                          vp, vp]
     for name in MOE_EXPORTS + PRODUCT_EXPORTS + MX_EXPORTS:
         getattr(lib, name).restype = ctypes.c_int
     lib.ggemm_moe_plan_workspace.argtypes = [i64, i32]
@@ -233,6 +239,8 @@ def load():
     lib.ggemm_product_act_workspace.restype = ctypes.c_int64
     lib.ggemm_mx_tile_rows.argtypes = [i32] * 4 + [i64, i32]
     lib.ggemm_mx_tile_rows.restype = ctypes.c_int32
+    lib.ggemm_mx_keep_tile_rows.argtypes = [i32] * 9 + [i64, i32]
+    lib.ggemm_mx_keep_tile_rows.restype = ctypes.c_int32
     _lib = lib
     return lib
 

@@ -2,10 +2,38 @@
 from __future__ import annotations
 
 import functools
+from typing import NamedTuple
 
 import torch
 import torch.autograd.forward_ad as fwAD
 from torch.autograd.function import once_differentiable as _once_differentiable
+
+
+class MXTensor(NamedTuple):
+    """Rows in blocks of 32 that share a power of two: ``q`` float8_e4m3fn [.., K], or uint8 [.., K / 2] with two e2m1
+    values in a byte, the even column in its low half; ``scales`` uint8 [.., ceil(K / 32)], a block's power of two as its
+    exponent + 127 (255: NaN)."""
+    q: torch.Tensor
+    scales: torch.Tensor
+
+
+MX_BLOCK = 32                    # values that share a scale
+
+
+def mx_columns(t: MXTensor, what: str) -> tuple[int, int]:
+    """(format code, columns) of a microscaled tensor whose parts fit each other."""
+    q, scales = t
+    if q.dtype == torch.float8_e4m3fn:
+        code, cols = 0, q.shape[-1]
+    elif q.dtype == torch.uint8:
+        code, cols = 1, 2 * q.shape[-1]
+    else:
+        raise TypeError(f"{what} must hold float8_e4m3fn values or uint8 pairs of e2m1, got {q.dtype}")
+    if scales.dtype != torch.uint8 or tuple(scales.shape) != tuple(q.shape[:-1]) + (-(-cols // MX_BLOCK),):
+        raise ValueError(f"{what}'s scales must be uint8 {list(q.shape[:-1]) + [-(-cols // MX_BLOCK)]}")
+    if scales.device != q.device:
+        raise ValueError(f"{what}'s values and scales must be on the same device")
+    return code, cols
 
 
 def on_gpu(t: torch.Tensor, what: str) -> None:

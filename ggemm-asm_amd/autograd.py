@@ -32,6 +32,8 @@ the autograd wiring left to the framework (Primus-Turbo, not vendored).
 * ``bias=``, ``activation=``: the expert's bias (bf16 / fp32 [G, N]) and activation in the forward product's
   epilogue (``grouped_gemm_fp8_bias_act``); the value before the activation is kept in bf16, and backward begins with
   ``bias_act_backward``, whose result is what is quantized as dy.
+* ``checkpoint="mxfp8"``: that value is kept in 8 bits and a scale for 32 columns, half the memory of the layer's
+  largest saved tensor, and the activation's gradient taken at the kept values.
 There is no CPU path: the tensors must live on a gfx950 GPU.
 """
 from __future__ import annotations
@@ -40,9 +42,9 @@ import weakref
 
 import torch
 
-from ._tensors import once_differentiable
+from ._tensors import MXTensor, once_differentiable
 from .persistent import grouped_gemm_fp8_tensorwise
-from .product import bias_act_backward, grouped_gemm_fp8_bias_act
+from .product import MX8, _kept, bias_act_backward, grouped_gemm_fp8_bias_act
 from .quant import (quantize_fp8_tensorwise, quantize_fp8_tensorwise_delayed, quantize_fp8_tensorwise_transpose,
                     quantize_fp8_tensorwise_transpose_delayed)
 from .vark import grouped_gemm_fp8_tensorwise_variable_k, weight_grad_fp8
@@ -246,13 +248,13 @@ class GroupedLinearActFP8(torch.autograd.Function):
     """The same with bias and activation in the forward product's epilogue."""
 
     @staticmethod
-    def forward(ctx, x, w, bias, group_offs, main_grad, weight_cache, scaling, activation, options):
+    def forward(ctx, x, w, bias, group_offs, main_grad, weight_cache, scaling, activation, options, checkpoint=None):
         qx, qw, qwt, sx, sw = _forward_operands(ctx, x, w, group_offs, main_grad, weight_cache, scaling)
-        keep = activation is not None and any(ctx.needs_input_grad)
+        keep = activation is not None and any(ctx.needs_input_grad) and (checkpoint or True)
         got = grouped_gemm_fp8_bias_act(qx, qw, sx, sw, group_offs, bias, activation, keep_preact=keep, zero_tail=True,
                                         **options)
         out, pre = got if keep else (got, None)
-        ctx.save_for_backward(qx, sx, qwt, sw, group_offs, pre)
+        ctx.save_for_backward(qx, sx, qwt, sw, group_offs, *(pre if isinstance(pre, MXTensor) else (pre,)))
         ctx.act = activation, options
         ctx.bias_dtype = None if bias is None else bias.dtype
         return out
@@ -260,11 +262,11 @@ class GroupedLinearActFP8(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        *saved, pre = ctx.saved_tensors
+        saved, pre = ctx.saved_tensors[:5], _kept(ctx.saved_tensors[5:])
         activation, options = ctx.act
         dy, db = bias_act_backward(dout, pre, saved[-1], activation, bias_grad=ctx.needs_input_grad[2], **options)
         dx, dw = _backward_products(ctx, dy, *saved)
-        return dx, dw, None if db is None else db.to(ctx.bias_dtype), None, None, None, None, None, None
+        return (dx, dw, None if db is None else db.to(ctx.bias_dtype)) + (None,) * 7
 
 
 def grouped_linear_fp8(x: torch.Tensor, w: torch.Tensor, group_offs: torch.Tensor,
@@ -272,7 +274,7 @@ def grouped_linear_fp8(x: torch.Tensor, w: torch.Tensor, group_offs: torch.Tenso
                        weight_cache: FP8WeightCache | None = None,
                        scaling: FP8DelayedScaling | None = None, *, bias: torch.Tensor | None = None,
                        activation: str | None = None, slope: float = 1.0, limit: float | None = None,
-                       shift: float = 0.0) -> torch.Tensor:
+                       shift: float = 0.0, checkpoint: str | None = None) -> torch.Tensor:
     """FP8 grouped linear layer: ``out[r] = act(x[r] @ w[g]^T + bias[g])`` for the rows of group g, bf16 out.
 
     x: bf16 / fp32 [M, K] (rows grouped by expert); w: bf16 / fp32 [G, N, K]; group_offs: int64
@@ -281,11 +283,13 @@ def grouped_linear_fp8(x: torch.Tensor, w: torch.Tensor, group_offs: torch.Tenso
     ``weight_cache`` the weight's fp8 copy is reused while the weight is unchanged. With ``scaling``
     (one FP8DelayedScaling per layer) x, w and dy take delayed scaling (module docstring). bias: bf16 / fp32 [G, N],
     with a gradient of its type; ``activation`` and its options as for ``grouped_gemm_fp8_bias_act`` ("swiglu" halves
-    the width)."""
+    the width). ``checkpoint="mxfp8"`` keeps what the activation's gradient reads in 8 bits instead of 16."""
+    if checkpoint not in (None, MX8):
+        raise ValueError(f"checkpoint must be None or {MX8!r}, got {checkpoint!r}")
     if main_grad is not None:
         if main_grad.dtype != torch.float32 or tuple(main_grad.shape) != (w.shape[0], w.shape[2], w.shape[1]):
             raise ValueError(f"main_grad must be fp32 [G, K, N] = {[w.shape[0], w.shape[2], w.shape[1]]}")
     if bias is None and activation is None:
         return GroupedLinearFP8.apply(x, w, group_offs, main_grad, weight_cache, scaling)
     options = {"slope": slope, "limit": limit, "shift": shift}
-    return GroupedLinearActFP8.apply(x, w, bias, group_offs, main_grad, weight_cache, scaling, activation, options)
+    return GroupedLinearActFP8.apply(x, w, bias, group_offs, main_grad, weight_cache, scaling, activation, options, checkpoint)

@@ -27,7 +27,7 @@ PERSISTENT_CO_PATHS = {"e4m3": os.path.join(LIB_DIR, "persistent_e4m3.co"),
                        "e5m2": os.path.join(LIB_DIR, "persistent_e5m2.co")}
 ARCH = "gfx950"
 LIB_SOURCES = [os.path.join(CSRC, f) for f in ("vark_capi.hip", "persistent_capi.hip", "quant_capi.hip",
-                                               "moe_capi.hip", "product_capi.hip", "mx_capi.hip")]
+                                               "moe_capi.hip", "product_capi.hip", "keep_capi.hip", "mx_capi.hip")]
 
 # Packed-FP32 VALU ops are disabled for all device code (they are left to no hand-written use).
 DEVICE_FLAGS = ["-O3", "-std=c++17", f"--offload-arch={ARCH}",

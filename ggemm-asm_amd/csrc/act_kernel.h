@@ -36,6 +36,9 @@ struct Args {
   int stride_dpre;
   float* dbias;
   float* partial;          // [units][N]
+  const uint8_t* q8 = nullptr;   // z in 8 bits instead of pre: e4m3 values (rows stride_pre bytes apart) and the scale of
+  const uint8_t* scales = nullptr;   // row r and block of 32 columns b at [r scale_row + b scale_block]
+  int64_t scale_row = 0, scale_block = 0;
 };
 
 // Group g has rows start[g] .. start[g + 1] - 1 and units pre[g] .. pre[g + 1] - 1. Offsets are clamped to
@@ -101,12 +104,10 @@ __device__ __forceinline__ void group_table(const Args& a, Table& t) {
 }
 
 template <int kAct>
-__device__ __forceinline__ void grad8(const v4i& z8, const v4i& d8, const epi::Args& e, float (&out)[8]) {
-  float z[8], d[8];
+__device__ __forceinline__ void grad8(const float (&z)[8], const v4i& d8, const epi::Args& e, float (&out)[8]) {
+  float d[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    z[2 * i] = epi::from_bf16(z8[i]);
-    z[2 * i + 1] = __uint_as_float(z8[i] & 0xffff0000u);
     d[2 * i] = epi::from_bf16(d8[i]);
     d[2 * i + 1] = __uint_as_float(d8[i] & 0xffff0000u);
   }
@@ -136,8 +137,8 @@ __device__ __forceinline__ void grad8(const v4i& z8, const v4i& d8, const epi::A
   }
 }
 
-// grid: units x strips
-template <int kAct>
+// grid: units x strips; kMx: z from its 8-bit checkpoint
+template <int kAct, bool kMx>
 __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
   __shared__ Table t;
   group_table(a, t);
@@ -162,11 +163,18 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
   for (int i = 0; i < 8; ++i) sum[i] = 0.f;
   for (int64_t r = r0; r < r1; r += kUnroll) {
     v4i z[kUnroll], d[kUnroll];
+    uint32_t scale[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       z[u] = d[u] = v4i{0, 0, 0, 0};
+      scale[u] = 0;
       if (r + u >= r1) continue;
-      if constexpr (kAct != epi::kNone) z[u] = __builtin_nontemporal_load((const v4i*)(a.pre + (r + u) * a.stride_pre + n));
+      if constexpr (kMx) {
+        const v2i h = __builtin_nontemporal_load((const v2i*)(a.q8 + (r + u) * a.stride_pre + n));
+        z[u][0] = h[0];
+        z[u][1] = h[1];
+        scale[u] = a.scales[(r + u) * a.scale_row + (int64_t)(n / 32) * a.scale_block];
+      } else if constexpr (kAct != epi::kNone) z[u] = __builtin_nontemporal_load((const v4i*)(a.pre + (r + u) * a.stride_pre + n));
       if constexpr (kAct == epi::kSwiglu) {
         const v2i h = __builtin_nontemporal_load((const v2i*)(a.dout + (r + u) * a.stride_dout + no));
         d[u][0] = h[0];
@@ -178,8 +186,17 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       if (r + u >= r1) continue;
-      float x[8];
-      grad8<kAct>(z[u], d[u], a.act, x);
+      float x[8], v[8];
+      if constexpr (kMx) {
+        mxq::restore_f32<true>(mxq::v2u{(unsigned)z[u][0], (unsigned)z[u][1]}, __uint_as_float(scale[u] << 23), v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] = epi::from_bf16(z[u][i]);
+          v[2 * i + 1] = __uint_as_float(z[u][i] & 0xffff0000u);
+        }
+      }
+      grad8<kAct>(v, d[u], a.act, x);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] += x[i];
       if (a.dpre != nullptr) {
@@ -197,7 +214,7 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
 
 // dbias[g, n] over the group's units; grid (columns / 64, G): a wave takes 64 columns and every kWaves-th unit, eight
 // of them in flight, and the waves' sums are added in their order.
-__global__ __launch_bounds__(kThreads) void bias_sum_kernel(Args a) {
+static __global__ __launch_bounds__(kThreads) void bias_sum_kernel(Args a) {
   __shared__ Table t;
   __shared__ float s_sum[kThreads];
   group_table(a, t);

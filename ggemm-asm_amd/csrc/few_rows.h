@@ -34,7 +34,7 @@ struct Cfg {
 template <int kAct, int NB>
 __device__ __forceinline__ void body(const nt::Args& a, GG_LDS uint8_t* lds, const epi::Args& e) {
   using C = Cfg<NB>;
-  constexpr bool kGated = kAct == epi::kSwiglu;
+  constexpr bool kGated = epi::act_of(kAct) == epi::kSwiglu;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n_tn = (a.N + C::BN - 1) / C::BN;
@@ -115,15 +115,15 @@ __device__ __forceinline__ void body(const nt::Args& a, GG_LDS uint8_t* lds, con
   for (int j = 0; j < NB; ++j) s_acc[(wave * NB + j) * 64 + lane] = acc[j];
   __syncthreads();
   const float alpha = *a.a_scale * *a.b_scale;
-  for (int b = wave; b < NB; b += kWaves) {
-    const int r = s, n = n0 + 16 * b + 4 * q;
-    if (r >= rows || n >= a.N) continue;
+  const int64_t row = (int64_t)row_base + m0 + s;
+  auto value = [&](int b) {
     v4f z = s_acc[b * 64 + lane];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) z += s_acc[(w * NB + b) * 64 + lane];
-    z = z * alpha + epi::load_bias(e, (int64_t)g * a.N + n);
-    const int64_t row = (int64_t)row_base + m0 + r;
-    if (e.pre != nullptr) *(v2i*)(e.pre + row * e.stride_pre + n) = v2i{epi::pack(z[0], z[1]), epi::pack(z[2], z[3])};
+    return z;
+  };
+  auto finish = [&](int b, const v4f& z) {
+    const int n = n0 + 16 * b + 4 * q;
     if constexpr (kGated) {
       float x = epi::swiglu(z[0], z[1], e), y = epi::swiglu(z[2], z[3], e);
       if (e.residual != nullptr) {
@@ -133,9 +133,36 @@ __device__ __forceinline__ void body(const nt::Args& a, GG_LDS uint8_t* lds, con
       }
       *(int*)(a.c + row * a.stride_cm + n / 2) = epi::pack(x, y);
     } else {
-      v4f x = epi::activation<kAct>(z);
+      v4f x = epi::activation<epi::act_of(kAct)>(z);
       if (e.residual != nullptr) x += epi::unpack4(*(const v2i*)(e.residual + row * e.stride_res + n));
       *(v2i*)(a.c + row * a.stride_cm + n) = v2i{epi::pack(x[0], x[1]), epi::pack(x[2], x[3])};
+    }
+  };
+  if constexpr ((kAct & epi::kKeepMx) != 0) {
+    static_assert(NB == 2, "a block of 32 columns");
+    if (wave != 0) return;                                   // one wave holds a block's scale
+    const bool whole = n0 + 16 < a.N;                        // else the block's second half is past N
+    v4f z[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+      z[b] = b == 0 || whole ? value(b) * alpha + epi::load_bias(e, (int64_t)g * a.N + n0 + 16 * b + 4 * q) : v4f{0.f, 0.f, 0.f, 0.f};
+    int w[2];
+    const uint32_t byte = epi::quantize32(z[0], z[1], w);
+    if (s >= rows) return;
+    if (q == 0) e.scales[(int64_t)(n0 / 32) * e.scale_block + row] = (uint8_t)byte;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if (b == 1 && !whole) break;
+      *(int*)(e.q8 + row * e.stride_q + n0 + 16 * b + 4 * q) = w[b];
+      finish(b, z[b]);
+    }
+  } else {
+    for (int b = wave; b < NB; b += kWaves) {
+      const int n = n0 + 16 * b + 4 * q;
+      if (s >= rows || n >= a.N) continue;
+      const v4f z = value(b) * alpha + epi::load_bias(e, (int64_t)g * a.N + n);
+      if (e.pre != nullptr) *(v2i*)(e.pre + row * e.stride_pre + n) = v2i{epi::pack(z[0], z[1]), epi::pack(z[2], z[3])};
+      finish(b, z);
     }
   }
 }

@@ -8,12 +8,15 @@
 // wide as the product.
 #pragma once
 
+#include "mx_quant.h"
 #include "vark_kernel.h"
 
 namespace ggemm {
 namespace epi {
 
 constexpr int kNone = 0, kSilu = 1, kGelu = 2, kSwiglu = 3;
+constexpr int kKeepMx = 4;   // added to an activation: z is kept in 8 bits (Args' q8 and scales) instead of bf16
+constexpr int act_of(int code) { return code & 3; }
 
 struct Args {
   uint16_t* pre;           // z in bf16, or null
@@ -24,6 +27,10 @@ struct Args {
   int stride_res;
   float slope, limit, shift;
   float nslope;            // -log2(e) slope: sigmoid(slope g) = 1 / (1 + 2^(nslope g))
+  uint8_t* q8 = nullptr;   // kKeepMx: z as e4m3 in blocks of 32 columns (mx_quant.h),
+  int stride_q = 0;
+  uint8_t* scales = nullptr;   // and the scale of row r and block b at [b scale_block + r]: rows are neighbours, as
+  int64_t scale_block = 0;     // the lanes that hold a block's scales are
 };
 
 // 1 / (1 + 2^x). The hardware's exp2 and reciprocal, each within an ulp; the rounding of x = -log2(e) y adds |y| 2^-24:
@@ -109,6 +116,29 @@ __device__ __forceinline__ int pack(float a, float b) {
   return __builtin_bit_cast(int, __builtin_convertvector(v2f{a, b}, v2b));
 }
 
+// z of a row's 16 columns x 2 in four lanes 16 apart, eight each, as MX: the scale byte of the 32 columns and the lane's
+// values of either half, four bytes each.
+__device__ __forceinline__ uint32_t quantize32(const v4f& a, const v4f& b, int (&q)[2]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) m = max(m, max(__float_as_uint(a[k]) & 0x7fffffffu, __float_as_uint(b[k]) & 0x7fffffffu));
+  auto r = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  m = max(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  m = max(r[0], r[1]);
+  const uint32_t byte = mxq::scale_byte<true>(m);
+  const float scale = __uint_as_float(byte << 23);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const v4f& z = h ? b : a;
+    mxq::v2s w{};
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, z[0], z[1], scale, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, z[2], z[3], scale, true);
+    q[h] = byte == 255u ? 0 : __builtin_bit_cast(int, w);
+  }
+  return byte;
+}
+
 // LDS that a wave stages 32 rows of NB blocks in, rows 16 bytes apart so that 16 of them start on different banks.
 template <int NB>
 constexpr int kRegion = 32 * (32 * NB + 16);
@@ -132,7 +162,8 @@ __device__ __forceinline__ void store(const v4f (&acc)[MB][NB], float alpha, con
                                       int stride_out, int g, int N, int64_t row0, int rows, int n0,
                                       GG_LDS uint8_t* reg, int lane) {
   static_assert(MB % 2 == 0, "two blocks of rows per pass");
-  constexpr bool kGated = kAct == kSwiglu, kRoom = MB * NB <= 16;   // registers for a pass's residual beside acc
+  static_assert(!(kAct & kKeepMx) || NB % 2 == 0, "blocks of 32 columns");
+  constexpr bool kGated = act_of(kAct) == kSwiglu, kRoom = MB * NB <= 16;   // registers for a pass's residual beside acc
   const int q = lane >> 4, s = lane & 15;
   const int blocks = min(NB, (N - n0 + 15) / 16);      // N is a multiple of 16; none past it
   v4f bias[NB];
@@ -163,7 +194,23 @@ __device__ __forceinline__ void store(const v4f (&acc)[MB][NB], float alpha, con
     };
     load_residual(0);
     if constexpr (kRoom) load_residual(1);
-    if (e.pre != nullptr) {
+    if constexpr ((kAct & kKeepMx) != 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; j += 2) {
+          // columns past N are zeros of the block that the last 16 are in
+          const v4f z0 = acc[2 * p + i][j] * alpha + bias[j];
+          const v4f z1 = j + 1 < blocks ? acc[2 * p + i][j + 1] * alpha + bias[j + 1] : v4f{0.f, 0.f, 0.f, 0.f};
+          int w[2];
+          const uint32_t byte = quantize32(z0, z1, w);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) *(GG_LDS int*)(reg + (16 * i + s) * (16 * NB + 16) + 16 * (j + h) + 4 * q) = w[h];
+          if (q == 0 && j < blocks && 16 * i + s < prows)
+            e.scales[(int64_t)((n0 + 16 * j) / 32) * e.scale_block + prow + 16 * i + s] = (uint8_t)byte;
+        }
+      store_rows<NB>(reg, (uint16_t*)(e.q8 + prow * e.stride_q + n0), e.stride_q / 2, prows, blocks, lane);
+    } else if (e.pre != nullptr) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -191,7 +238,7 @@ __device__ __forceinline__ void store(const v4f (&acc)[MB][NB], float alpha, con
           }
           *(GG_LDS int*)(at + 16 * j + 4 * q) = pack(x, y);
         } else {
-          v4f x = activation<kAct>(z);
+          v4f x = activation<act_of(kAct)>(z);
           if (e.residual != nullptr) x += unpack4(res[i][j]);
           *(GG_LDS v2i*)(at + 32 * j + 8 * q) = v2i{pack(x[0], x[1]), pack(x[2], x[3])};
         }

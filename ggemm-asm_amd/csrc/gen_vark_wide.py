@@ -1254,7 +1254,9 @@ class GenK(Gen):
 #   bias      z rounded to bf16 is C;
 #   gate      swiglu of neighbouring columns (z0, z1), (z2, z3) .., half as wide as the tile: v = min(z0, limit)
 #             sigmoid(slope v) (clamp(z1, limit) + shift);
-#   gatekeep  both, z into a second tensor.
+#   gatekeep  both, z into a second tensor;
+#   gatekeep8 the same with z as e4m3 in blocks of 32 columns, whose scale byte (mx_quant.h) goes into a third. A lane
+#             and its neighbour 32 lanes on hold a row's 32 columns of a block: sixteen maxima in a lane, one exchange.
 # A lane's accumulators 4 g .. 4 g + 3 of a block are four neighbouring columns of one row (32 j + 8 g + 4 h + r, h = l /
 # 32), so a pair never leaves its lane. The tile's bias comes as one load per wave at the tile's start, 160 columns of
 # fp32 or bf16 in lanes 0-39, and is handed to all lanes through LDS in the epilogue. A wave stages 32 rows x 160
@@ -1271,16 +1273,21 @@ class KEConfig(KConfig):
     def __init__(self, mode):
         super().__init__(256, 320, False)
         self.mode, self.name = mode, f"pe256x320_{mode}"
-        self.keep_z, self.gate = mode != "gate", mode != "bias"
-        self.e_stores = self.bm * (10 * self.keep_z + 5 * self.gate)
+        self.keep8 = mode == "gatekeep8"
+        self.keep_z, self.gate = mode in ("bias", "gatekeep"), mode != "bias"
+        self.e_stores = self.bm * (10 * self.keep_z + 5 * self.gate + 10 * self.keep8)
         self.vbias = self.epi_x - 4                     # four registers, loaded at the tile's start
         self.vgpr_clobber = list(range(self.vbias, 256))
         ops = [o for o in self.operands if o[0] not in ("ew_base", "ew_s", "rb_even", "rb_odd", "gb")]
         ops += [(n, "v") for n in ("vboff", "b_lo", "b_hi", "brec", "bf32")]
         if self.gate:
             ops += [(n, "v") for n in ("nslope", "limit", "shift")]
-        if mode == "gatekeep":
+        if mode in ("gatekeep", "gatekeep8"):
             ops += [(n, "v") for n in ("zT_lo", "zT_hi", "zrecT", "zm2", "sw_z")]
+        if self.keep8:
+            ops += [(n, "v") for n in ("xT_lo", "xT_hi", "xrows", "xstep", "xoff")]
+            self.sgpr_clobber = SGPR_CLOBBER_MX
+            self.more_clobber = ["vcc"]
         self.operands = ops
         self.op = {name: f"%{i}" for i, (name, _) in enumerate(ops)}
         assert BIAS_OFF + 4096 <= self.slot and OREGION + 32 * OPITCH == 16384
@@ -1288,6 +1295,7 @@ class KEConfig(KConfig):
 
 
 KECONFIGS = (KEConfig("bias"), KEConfig("gate"), KEConfig("gatekeep"))
+KEEP8_CONFIGS = (KEConfig("gatekeep8"),)
 
 
 class GenKE(GenK):
@@ -1337,11 +1345,13 @@ class GenKE(GenK):
         s, OP, e, c = SGPR_K, self.OP, self.emit, self.cfg
         v0 = c.vop0                                    # the 72 operand registers are free here
         bset, data = (v0, v0 + 16), v0 + 16            # bias of a block, two sets; read-back data (over the second)
-        z, ex, pk = v0 + 32, v0 + 36, v0 + 38          # z of four columns, exponentials, packed results
+        # z of four columns (of a block's sixteen with their maximum and scale), exponentials, packed results
+        z, ex, pk = (v0 + 32, v0 + 48, v0 + 50) if c.keep8 else (v0 + 32, v0 + 36, v0 + 38)
+        top, other, byte, one, nan = v0 + 53, v0 + 54, v0 + 55, v0 + 70, v0 + 71
         lane = {n: v0 + 56 + k for k, n in enumerate(("zw", "ow", "ba", "zr0", "zr1", "or0", "or1", "zg0", "zg1", "og0",
                                                       "og1"))}
         ln, t0, t1 = (v0 + 67 + k for k in range(3))
-        assert data + 40 <= v0 + 56 and v0 + 70 <= c.vacc0
+        assert data + 40 <= v0 + 56 and v0 + 72 <= c.vacc0
         L = {n: f"v{r}" for n, r in lane.items()}
         limit, nlimit, nslope, shift = s["K"], s["LIM"], s["NEED"], s["LIMTOP"]   # free after the last stage
         zres, zm2, swz = s["RL"], s["RR0"], s["RR1"]
@@ -1350,7 +1360,13 @@ class GenKE(GenK):
         e("s_nop 7")
         e("s_barrier")                                 # every wave is past its reads of the last stage's slot
         self.gate_values(limit, nlimit, nslope, shift)
-        if c.mode == "gatekeep":
+        if c.keep8:                                    # the scales' resource, RS, follows the blocks
+            for d, n in (("RS2", "xrows"), ("NSSR", "xstep")):
+                e(f"v_readfirstlane_b32 {s[d]}, {OP[n]}")
+            e(f"s_mov_b32 {s['RS3']}, 0x{WORD3:x}")
+            e(f"v_mov_b32 v{one}, 0x7f")
+            e(f"v_mov_b32 v{nan}, 0xff")
+        if c.mode in ("gatekeep", "gatekeep8"):
             for d, n in (("RL0", "zT_lo"), ("RL1", "zT_hi"), ("RL2", "zrecT"), ("RR0", "zm2"), ("RR1", "sw_z")):
                 e(f"v_readfirstlane_b32 {s[d]}, {OP[n]}")
             e(f"s_mov_b32 {s['RL3']}, 0x{WORD3:x}")
@@ -1393,7 +1409,9 @@ class GenKE(GenK):
         e(f"v_mul_u32_u24 {L['ow']}, {OPITCH}, v{t0}")
         e(f"v_lshl_add_u32 {L['ow']}, v{t1}, 2, {L['ow']}")
         e(f"v_add_u32 {L['ow']}, {s['EPI']}, {L['ow']}")
+        # 8-bit rows of z have the bytes of the result's
         for on, pitch, stride, wide in ((c.keep_z, ZPITCH, zm2, (("z", 0, 4, 0), ("z", 1, 2, 256))),
+                                        (c.keep8, OPITCH, zm2, (("z", 0, 3, 0), ("z", 1, 1, 128))),
                                         (c.gate, OPITCH, OP["cm2"], (("o", 0, 3, 0), ("o", 1, 1, 128)))):
             for n, k, shift_, first in wide if on else ():
                 # row l >> shift, chunk l % 2^shift, from byte `first` of the row
@@ -1412,8 +1430,8 @@ class GenKE(GenK):
             for g in range(4):
                 e(f"ds_read_b128 v[{dst + 4 * g}:{dst + 4 * g + 3}], {L['ba']} offset:{128 * j + 32 * g}")
 
-        def columns(i, j, g, bias):
-            """Four columns of block (i, j): z, the pairs' results, both staged."""
+        def z_of(i, j, g, bias, z):
+            """z of four columns of block (i, j)."""
             kind, base = c.acc(i, j)
             for r in range(4):
                 src = f"v{base + 4 * g + r}"
@@ -1421,6 +1439,54 @@ class GenKE(GenK):
                     e(f"v_accvgpr_read_b32 v{z + r}, a{base + 4 * g + r}")
                     src = f"v{z + r}"
                 e(f"v_fma_f32 v{z + r}, {src}, {OP['alpha']}, v{bias + 4 * g + r}")
+
+        def kept8(i, j):
+            """The block's sixteen z of this lane and its neighbour's as e4m3 with one scale, staged; the scale byte stored.
+            Rows are neighbours in the scales' tensor: a block's resource begins at the tile's first row and ends with
+            its last."""
+            if j == 0:
+                e(f"v_readfirstlane_b32 {s['RS0']}, {OP['xT_lo']}")
+                e(f"v_readfirstlane_b32 {s['RS1']}, {OP['xT_hi']}")
+            e(f"v_maximum3_f32 v{top}, |v{z}|, |v{z + 1}|, |v{z + 2}|")
+            for r in range(3, 15, 2):
+                e(f"v_maximum3_f32 v{top}, v{top}, |v{z + r}|, |v{z + r + 1}|")
+            e(f"v_maximum3_f32 v{top}, v{top}, |v{z + 15}|, |v{z + 15}|")
+            e(f"v_mov_b32 v{other}, v{top}")
+            e("s_nop 4")
+            e(f"v_permlane32_swap_b32 v{top}, v{other}")
+            e("s_nop 1")
+            e(f"v_maximum3_f32 v{top}, v{top}, v{other}, v{other}")
+            e(f"v_and_b32 v{top}, 0x7fffffff, v{top}")
+            # byte: the exponent field less 8, one more from a mantissa of 1.8125 on; 127 for zeros, 255 for inf and NaN
+            e(f"v_add_u32 v{byte}, 0x180000, v{top}")
+            e(f"v_lshrrev_b32 v{byte}, 23, v{byte}")
+            e(f"v_add_u32 v{byte}, -8, v{byte}")
+            e(f"v_max_i32 v{byte}, 0, v{byte}")
+            e(f"v_cmp_ne_u32 vcc, 0, v{top}")
+            e("s_nop 1")
+            e(f"v_cndmask_b32 v{byte}, v{one}, v{byte}, vcc")
+            e(f"v_cmp_gt_u32 vcc, 0x7f800000, v{top}")
+            e("s_nop 1")
+            e(f"v_cndmask_b32 v{byte}, v{nan}, v{byte}, vcc")
+            e(f"v_lshlrev_b32 v{other}, 23, v{byte}")
+            e(f"s_and_b32 {s['RS1']}, {s['RS1']}, 0xffff")
+            e(f"v_add_u32 v{top}, {32 * i}, {OP['xoff']}")
+            e("s_nop 1")
+            e(f"buffer_store_byte v{byte}, v{top}, {s['RS']}, 0 offen")
+            e(f"s_add_u32 {s['RS0']}, {s['RS0']}, {s['NSSR']}")
+            e(f"s_addc_u32 {s['RS1']}, {s['RS1']}, 0")
+            for g in range(4):
+                e(f"v_cvt_scalef32_pk_fp8_f32 v{pk + g % 2}, v{z + 4 * g}, v{z + 4 * g + 1}, v{other}")
+                e(f"v_cvt_scalef32_pk_fp8_f32 v{pk + g % 2}, v{z + 4 * g + 2}, v{z + 4 * g + 3}, v{other} op_sel:[0,0,0,1]")
+                e("s_nop 1")
+                e(f"v_cndmask_b32 v{pk + g % 2}, 0, v{pk + g % 2}, vcc")
+                e(f"ds_write_b32 {L['ow']}, v{pk + g % 2} offset:{32 * j + 8 * g}")
+
+        def columns(i, j, g, bias):
+            """Four columns of block (i, j): z, the pairs' results, both staged."""
+            if not c.keep8:
+                z_of(i, j, g, bias, z0)
+            z = z0 + (4 * g if c.keep8 else 0)
             if c.keep_z:
                 e(f"v_cvt_pk_bf16_f32 v{pk}, v{z}, v{z + 1}")
                 e(f"v_cvt_pk_bf16_f32 v{pk + 1}, v{z + 2}, v{z + 3}")
@@ -1454,8 +1520,9 @@ class GenKE(GenK):
 
         def read_back(n, i, first, res, stride, wave, region):
             """Staged rows 32 i .. + 31 to memory: (instructions, rows of one, bytes of a staged row)."""
-            parts = ((0, 8, 4), (1, 2, 16)) if n == "z" else ((0, 4, 8), (1, 1, 32))
-            pitch = ZPITCH if n == "z" else OPITCH
+            wide = n == "z" and c.keep_z
+            parts = ((0, 8, 4), (1, 2, 16)) if wide else ((0, 4, 8), (1, 1, 32))
+            pitch = ZPITCH if wide else OPITCH
             d, steps = first, []
             for k, count, rows in parts:
                 for q in range(count):
@@ -1469,18 +1536,23 @@ class GenKE(GenK):
                 e(f"v_add_u32 {c.vt2}, {s['T']}, {L[f'{n}g{k}']}")
                 e(f"buffer_store_dwordx4 v[{d}:{d + 3}], {c.vt2}, {res}, 0 offen" + STORE_HINT[n])
 
-        writes = 4 * (c.keep_z + c.gate)               # of a block, younger than the next block's bias
+        z0 = z
+        writes = 4 * (c.keep_z + c.keep8 + c.gate)     # of a block, younger than the next block's bias
         bias_reads(0, bset[0])
         for i in range(c.bm):
             for j in range(c.bn):
                 e(f"s_waitcnt lgkmcnt({writes if j else 0})")
                 if j + 1 < c.bn:
                     bias_reads(j + 1, bset[(j + 1) % 2])
+                if c.keep8:
+                    for g in range(4):
+                        z_of(i, j, g, bset[j % 2], z0 + 4 * g)
+                    kept8(i, j)
                 for g in range(4):
                     columns(i, j, g, bset[j % 2])
             if i + 1 < c.bm:
                 bias_reads(0, bset[0])
-            if c.keep_z:
+            if c.keep_z or c.keep8:
                 read_back("z", i, data, zres, zm2, swz, 0)
             if c.gate:
                 read_back("o", i, data, s["RC"], OP["cm2"], OP["sw_epi"], OREGION)
@@ -1506,13 +1578,14 @@ def render():
            "// and with an epilogue:",
            "// gfx950 assembly, one inline asm statement per tile shape."]
     total = 0
-    for c in CONFIGS + SWAPPED_CONFIGS + KCONFIGS + KECONFIGS:
+    for c in CONFIGS + SWAPPED_CONFIGS + KCONFIGS + KECONFIGS + KEEP8_CONFIGS:
         g = GenKE(c) if isinstance(c, KEConfig) else GenK(c) if isinstance(c, KConfig) else Gen(c)
         g.tile()
         total += len(g.lines)
         text = "\\n\\t".join(g.lines)
         clob = ([f'"a{r}"' for r in range(256)] + [f'"v{r}"' for r in c.vgpr_clobber]
-                + [f'"s{r}"' for r in c.sgpr_clobber] + ['"m0"', '"scc"', '"memory"'])
+                + [f'"s{r}"' for r in c.sgpr_clobber] + ['"m0"', '"scc"', '"memory"']
+                + [f'"{r}"' for r in getattr(c, "more_clobber", ())])
         order = ", ".join(f"{i}:{n}" for i, (n, _) in enumerate(c.operands))
         t = c.name
         out += [

@@ -504,9 +504,11 @@ __device__ __forceinline__ void persistent_entry(const Args& a, GG_LDS uint8_t* 
     poison_out(a);
     return;
   }
-  if (wide_tiles(a.N, false))
+  // z kept in 8 bits: a wave's 96 columns are whole blocks of 32, the 80 of a 320-wide tile are not
+  constexpr bool kBlocks = kEpi != 0 && ((kEpi - 1) & epi::kKeepMx) != 0;
+  if (kBlocks || wide_tiles(a.N, false))
     persistent_body<kAE5M2, 384, kEpi>(a, st, e);
-  else
+  else if constexpr (!kBlocks)
     persistent_body<kAE5M2, 320, kEpi>(a, st, e);
 }
 

@@ -47,13 +47,13 @@ static_assert(kLdsBytes <= 160 * 1024, "gfx950 LDS");
 static_assert(GGEMM_WIDE_NOPERANDS_pk256x320_e4m3 == 60 && GGEMM_WIDE_NOPERANDS_pk256x320_e5m2 == 60,
               "operand list of vark_wide_asm.inc");
 static_assert(GGEMM_WIDE_NOPERANDS_pe256x320_bias == 60 && GGEMM_WIDE_NOPERANDS_pe256x320_gate == 63 &&
-                  GGEMM_WIDE_NOPERANDS_pe256x320_gatekeep == 68,
+                  GGEMM_WIDE_NOPERANDS_pe256x320_gatekeep == 68 && GGEMM_WIDE_NOPERANDS_pe256x320_gatekeep8 == 73,
               "operand lists of vark_wide_asm.inc");
 static_assert(8 * kNT <= kSlot, "the group scan's scratch fits slot 1");
 
 // What a tile's assembly ends with: C as it is, or the epilogues of products with bias and activation
-// (gen_vark_wide.py): z = alpha acc + bias is C; swiglu of z's pairs of columns is C; the same, with z kept.
-constexpr int kPlain = 0, kBias = 1, kGate = 2, kGateKeep = 3;
+// (gen_vark_wide.py): z = alpha acc + bias is C; swiglu of z's pairs of columns is C; the same, with z kept, in 8 bits.
+constexpr int kPlain = 0, kBias = 1, kGate = 2, kGateKeep = 3, kGateKeep8 = 4;
 
 // Shapes the wide kernel takes (the host also checks strides and bases as for every launch).
 __host__ __device__ constexpr bool fits(int N, int K) { return N % kTN == 0 && K % 64 == 0 && K > 0; }
@@ -64,7 +64,7 @@ template <bool kAE5M2, int kMode = pw::kPlain>
 __device__ __forceinline__ void persistent_wide_body(const nt::Args& a, GG_LDS uint8_t* lds, const epi::Args& ep = {}) {
   using namespace pw;
   static_assert(kMode == kPlain || !kAE5M2, "epilogues of the forward's format");
-  constexpr bool kGated = kMode == kGate || kMode == kGateKeep;
+  constexpr bool kGated = kMode == kGate || kMode == kGateKeep || kMode == kGateKeep8;
   GG_LDS int* s_pre = (GG_LDS int*)(lds + kPreOff);
   GG_LDS int* s_offs = (GG_LDS int*)(lds + kOffsOff);
   GG_LDS int64_t* s_scan = (GG_LDS int64_t*)(lds + kSlot);   // slot 1: no stage is issued before the scan ends
@@ -172,7 +172,17 @@ __device__ __forceinline__ void persistent_wide_body(const nt::Args& a, GG_LDS u
       else if constexpr (kMode == kGate)
         asm volatile(GGEMM_WIDE_ASM_pe256x320_gate GGEMM_PW_TILE_OPERANDS, GGEMM_PW_BIAS,
                      GGEMM_PW_GATE : GGEMM_WIDE_CLOBBERS_pe256x320_gate);
-      else
+      else if constexpr (kMode == kGateKeep8) {
+        // q's rows and, from the tile's first row on, the scales of this wave's five blocks of columns
+        const uint8_t* qt = ep.q8 + (int64_t)(T.row_base + T.m0) * ep.stride_q + T.n0;
+        const uint32_t qrec = (uint32_t)((int64_t)T.rows * ep.stride_q - T.n0), sw_q = (uint32_t)(128 * wm * ep.stride_q + 160 * wn);
+        const uint8_t* xt = ep.scales + (int64_t)(T.n0 / 32 + 5 * wn) * ep.scale_block + T.row_base + T.m0;
+        const uint32_t xoff = lane < 32 ? (uint32_t)(128 * wm + lane) : nt::kOob;   // both halves hold a row's scale
+        asm volatile(GGEMM_WIDE_ASM_pe256x320_gatekeep8 GGEMM_PW_TILE_OPERANDS, GGEMM_PW_BIAS, GGEMM_PW_GATE,
+                     "v"(lo32(qt)), "v"(hi32(qt)), "v"(qrec), "v"((uint32_t)ep.stride_q), "v"(sw_q), "v"(lo32(xt)),
+                     "v"(hi32(xt)), "v"((uint32_t)T.rows), "v"((uint32_t)ep.scale_block),
+                     "v"(xoff) : GGEMM_WIDE_CLOBBERS_pe256x320_gatekeep8);
+      } else
         asm volatile(GGEMM_WIDE_ASM_pe256x320_gatekeep GGEMM_PW_TILE_OPERANDS, GGEMM_PW_BIAS, GGEMM_PW_GATE,
                      "v"(lo32(zt)), "v"(hi32(zt)), "v"(zrec), "v"(zm2),
                      "v"(sw_z) : GGEMM_WIDE_CLOBBERS_pe256x320_gatekeep);

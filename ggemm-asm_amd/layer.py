@@ -29,13 +29,14 @@ def moe_layer_fp8(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, w_d
                   activation: str | None = "swiglu", slope: float = 1.0, limit: float | None = None,
                   shift: float = 0.0, residual: torch.Tensor | None = None, routing: dict | None = None,
                   main_grads: tuple | None = None, weight_caches: tuple[FP8WeightCache, FP8WeightCache] | None = None,
-                  scalings: tuple[FP8DelayedScaling, FP8DelayedScaling] | None = None) -> torch.Tensor:
+                  scalings: tuple[FP8DelayedScaling, FP8DelayedScaling] | None = None,
+                  checkpoint: str | None = None) -> torch.Tensor:
     """``residual + sum_j weight_j * expert_j(x)`` of every token, [T, H] bf16.
 
     x: bf16 [T, H]; logits: the router's, [T, E]; w_up: [E, N, H] and w_down: [E, H, I], bf16 / fp32, I = N / 2 for
     "swiglu" and N otherwise; biases [E, N] and [E, H]. ``routing``: options of ``route_experts``; ``slope``, ``limit``,
     ``shift``: of the activation; ``main_grads``, ``weight_caches``, ``scalings``: those of ``grouped_linear_fp8``, for
-    the two products.
+    the two products; ``checkpoint``: its, for the first one (nothing is kept without gradients).
 
     With gradients: rows are dispatched in bf16 and the products are the autograd layer's. Without: x is quantized once
     and its fp8 rows dispatched, half the bytes of bf16 ones, and nothing is kept for a backward pass (delayed scaling
@@ -55,7 +56,7 @@ def moe_layer_fp8(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, w_d
     if (torch.is_grad_enabled() and main_grads is not None) or tracked(*params):
         mains, scales = main_grads or (None, None), scalings or (None, None)
         h = grouped_linear_fp8(dispatch_tokens(x, plan), w_up, plan.group_offs, mains[0], caches[0], scales[0],
-                               bias=bias_up, activation=activation, **gate)
+                               bias=bias_up, activation=activation, checkpoint=checkpoint, **gate)
         y = grouped_linear_fp8(h, w_down, plan.group_offs, mains[1], caches[1], scales[1], bias=bias_down)
         return combine_tokens(y, plan, weights, residual)
     q, sx, _ = quantize_fp8_tensorwise(_rows16(x), "e4m3", slots=plan.slots)

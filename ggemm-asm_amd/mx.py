@@ -5,48 +5,25 @@ of two, the values are e2m1 (4 bits) or e4m3 (8 bits).
 * ``grouped_gemm_mx_bias_act``         -- the grouped product of e2m1 weights with e2m1 or e4m3 activations, with bias,
   activation and residual in its epilogue
 
+The training layer keeps the value before its activation so (``keep_preact="mxfp8"`` of ``grouped_gemm_fp8_bias_act``,
+``checkpoint="mxfp8"`` of ``grouped_linear_fp8``).
+
 ``quantize_mxfp8_grouped`` makes its blocks along the token axis, for the weight gradient; these lie along the features,
 the axis that the forward product sums over. The reference's products take per-tensor scales (reference
 bench.py:238-247). Every launch goes through libggemm_vark.so on torch's current stream; there is no CPU path.
 """
 from __future__ import annotations
 
-from typing import NamedTuple
-
 import torch
 
 from . import _lib
-from ._tensors import on_gpu as _on_gpu, row_stride as _stride, tracked
+from ._tensors import MX_BLOCK as BLOCK, MXTensor, mx_columns as _columns, on_gpu as _on_gpu, row_stride as _stride, tracked
 from .product import _act, _check_offs, _rows16
 from .quant import _IN, _padded_empty
 from .vark import _validate_offsets
 
-BLOCK = 32                       # values that share a scale
 _FORMATS = {"e4m3": 0, "e2m1": 1}
 TILES = (0, 16, 32, 64, 128, 256)    # of ggemm_mx_product
-
-
-class MXTensor(NamedTuple):
-    """Rows in blocks of 32: ``q`` float8_e4m3fn [.., K], or uint8 [.., K / 2] with two e2m1 values in a byte, the even
-    column in its low half; ``scales`` uint8 [.., ceil(K / 32)], a block's power of two as its exponent + 127 (255: NaN)."""
-    q: torch.Tensor
-    scales: torch.Tensor
-
-
-def _columns(t: MXTensor, what: str) -> tuple[int, int]:
-    """(format code, columns) of a microscaled tensor whose parts fit."""
-    q, scales = t
-    if q.dtype == torch.float8_e4m3fn:
-        code, cols = 0, q.shape[-1]
-    elif q.dtype == torch.uint8:
-        code, cols = 1, 2 * q.shape[-1]
-    else:
-        raise TypeError(f"{what} must hold float8_e4m3fn values or uint8 pairs of e2m1, got {q.dtype}")
-    if scales.dtype != torch.uint8 or tuple(scales.shape) != tuple(q.shape[:-1]) + (-(-cols // BLOCK),):
-        raise ValueError(f"{what}'s scales must be uint8 {list(q.shape[:-1]) + [-(-cols // BLOCK)]}")
-    if scales.device != q.device:
-        raise ValueError(f"{what}'s values and scales must be on the same device")
-    return code, cols
 
 
 def tile_rows(a_format: str, G: int, N: int, K: int, M: int, num_cus: int = 256) -> int:

@@ -59,6 +59,30 @@ int ggemm_mx_product(const void* a, int32_t a_fmt, const uint8_t* a_scales, cons
 /* The tile that such a call takes by itself on a device of num_cus CUs. */
 int32_t ggemm_mx_tile_rows(int32_t a_fmt, int32_t G, int32_t N, int32_t K, int64_t M_total, int32_t num_cus);
 
+/* ggemm_product_fp8_bias_act (ggemm_product.h) with z kept in 8 bits for the backward pass instead of bf16: quantized from
+ * fp32 as by ggemm_mx_quantize. Without an activation (GGEMM_E_FORMAT) z is the result and nothing is kept.
+ *   q: e4m3 [M_total, N], rows stride_q bytes apart, a multiple of 16, 16-byte aligned;
+ *   scales: of row r and block b at scales[b * scale_block + r], scale_block >= M_total.
+ * Rows outside [0, offs[G]) are not written, or rows from offs[G] on become zero (scale 127) with zero_tail != 0. */
+int ggemm_mx_keep_product(const void* a, const void* b, void* out, void* q, uint8_t* scales, const float* a_scale,
+                          const float* b_scale, const void* bias, int32_t bias_dtype, const void* residual,
+                          const int64_t* group_offs, int32_t G, int32_t N, int32_t K, int32_t stride_am, int32_t stride_bg,
+                          int32_t stride_bn, int32_t stride_out, int32_t stride_q, int64_t scale_block, int32_t stride_res,
+                          int32_t act, float slope, float limit, float shift, int64_t M_total, int32_t zero_tail,
+                          void* stream);
+
+/* Rows of the output tiles of the kernel that such a call runs, as ggemm_product_tile_rows. */
+int32_t ggemm_mx_keep_tile_rows(int32_t G, int32_t N, int32_t K, int32_t stride_am, int32_t stride_bn, int32_t stride_out,
+                                int32_t stride_q, int32_t act, int32_t residual, int64_t M_total, int32_t num_cus);
+
+/* ggemm_product_act_backward (ggemm_product.h) from such a z: q and scales as above, or of any strides (scale of row r and
+ * block b at scales[r * scale_row + b * scale_block]); stride_q a multiple of 8, q 8-byte aligned. The gradient is
+ * that of the values that were kept; a block with scale 255 gives NaN. Workspace: ggemm_product_act_workspace. */
+int ggemm_mx_act_backward(const void* dout, const void* q, const uint8_t* scales, const int64_t* group_offs, int32_t G,
+                          int32_t N, int32_t stride_dout, int32_t stride_q, int64_t scale_row, int64_t scale_block,
+                          int32_t act, float slope, float limit, float shift, int64_t M_total, void* dpre,
+                          int32_t stride_dpre, float* dbias, float* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

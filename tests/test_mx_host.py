@@ -76,6 +76,40 @@ def test_product_validation(pkg, kw, rc):
     assert _product(pkg.load_library(), **kw) == rc
 
 
+def _keep(lib, **kw):
+    a = dict(a=FAKE, b=FAKE, out=FAKE, q=FAKE, s=FAKE, sa=FAKE, sb=FAKE, bias=FAKE, bdt=0, res=FAKE, offs=FAKE, G=4, N=64, K=32,
+             sam=32, sbg=2048, sbn=32, so=64, sq=64, blk=100, sr=64, act=1, slope=1.0, limit=7.0, shift=0.0, M=100, tail=0)
+    a.update(kw)
+    return lib.ggemm_mx_keep_product(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(a=0), -1), (dict(q=0), -1), (dict(s=0), -1), (dict(out=0), -1), (dict(offs=0), -1), (dict(act=0), -8), (dict(act=4), -8),
+    (dict(act=3, limit=0.0), -2), (dict(G=0), -2), (dict(N=40), -2), (dict(K=24), -2), (dict(M=-1), -2), (dict(sam=16), -3),
+    (dict(so=56), -3), (dict(sq=48), -3), (dict(sq=72), -3), (dict(blk=99), -3), (dict(blk=2 ** 31), -2),
+    (dict(sq=2 ** 24), -2), (dict(q=FAKE + 8), -4), (dict(out=FAKE + 8), -4), (dict(res=FAKE + 8), -4),
+])
+def test_keep_validation(pkg, kw, rc):
+    assert _keep(pkg.load_library(), **kw) == rc
+
+
+def _back(lib, **kw):
+    a = dict(dout=FAKE, q=FAKE, s=FAKE, offs=FAKE, G=4, N=64, sd=64, sq=64, sr=2, sb=1, act=1, slope=1.0, limit=7.0, shift=0.0,
+             M=100, dpre=FAKE, sdp=64, db=FAKE, ws=FAKE)
+    a.update(kw)
+    return lib.ggemm_mx_act_backward(*a.values(), None)
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(dout=0), -1), (dict(q=0), -1), (dict(s=0), -1), (dict(dpre=0), -1), (dict(offs=0), -1), (dict(ws=0), -1),
+    (dict(act=0), -8), (dict(act=9), -8), (dict(act=3, limit=0.0), -2), (dict(G=0), -2), (dict(N=24), -2), (dict(M=-1), -2),
+    (dict(sd=56), -3), (dict(sq=56), -3), (dict(sq=68), -3), (dict(sdp=60), -3), (dict(sr=-1), -3), (dict(sb=-1), -3),
+    (dict(dout=FAKE + 8), -4), (dict(q=FAKE + 4), -4), (dict(dpre=FAKE + 4), -4), (dict(db=FAKE + 8), -4), (dict(ws=FAKE + 8), -4),
+])
+def test_kept_gradient_validation(pkg, kw, rc):
+    assert _back(pkg.load_library(), **kw) == rc
+
+
 def test_choice_of_a_kernel(pkg):
     from ggemm_asm_amd import mx
     for fmt in ("e4m3", "e2m1"):
