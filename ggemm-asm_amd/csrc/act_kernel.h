@@ -7,6 +7,11 @@
 // columns down the unit's rows, and leaves the unit's sums in a row of the workspace, which a second kernel
 // adds up per group in unit order: no atomics, so the sums do not depend on what ran first. 131072 x 5760 with
 // swiglu: 761 us, 5.0 TB/s, and 16 for the second kernel.
+//
+// With z in 8 bits (kMx) a quarter less is read and written in all: 629 us, 4.8 TB/s, where the bf16 form takes 761. A
+// row's eight values are 8 bytes, half of what the bf16 form loads, so eight rows are in flight and not four (700 us
+// against 686 with the scales read alike), and scales are read two rows to a lane (row_scales). 16 columns to a thread,
+// one load each of z and dout, store in halves of lines: 870 us, 1228 past the caches.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -20,7 +25,6 @@ namespace ag {
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxGroups = 2047;
 constexpr int kPer = (kMaxGroups + 1) / kThreads;      // group offsets a thread holds
-constexpr int kUnroll = 4;                             // rows a thread has in flight
 
 struct Args {
   const uint16_t* dout;
@@ -137,6 +141,26 @@ __device__ __forceinline__ void grad8(const float (&z)[8], const v4i& d8, const 
   }
 }
 
+// The scales of eight rows and a block of columns, in the four lanes that hold its columns: lane k has those of rows 2 k
+// and 2 k + 1, low byte first. A byte a row and lane takes 16 us
+// more of 645 (131072 x 5760, swiglu; silu on 2880 columns: 47 of 415): by blocks, as the
+// product leaves them, a wave's bytes of a row lie in 16 lines.
+__device__ __forceinline__ uint32_t row_scales(const Args& a, int64_t r, int64_t r1, int n) {
+  const uint8_t* s = a.scales + (int64_t)(n / 32) * a.scale_block;
+  const int64_t k = r + 2 * (threadIdx.x & 3);
+  uint32_t v = 0;
+  if (k < r1) v = s[k * a.scale_row];
+  if (k + 1 < r1) v |= (uint32_t)s[(k + 1) * a.scale_row] << 16;
+  return v;
+}
+
+// Row u's of them, as 2^X.
+template <int u>
+__device__ __forceinline__ float row_scale(uint32_t v) {
+  const uint32_t b = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, u / 2 * 0x55, 0xf, 0xf, true);
+  return __uint_as_float(u & 1 ? b >> 16 << 23 : (b & 0xff) << 23);
+}
+
 // grid: units x strips; kMx: z from its 8-bit checkpoint
 template <int kAct, bool kMx>
 __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
@@ -144,8 +168,10 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
   group_table(a, t);
   const int unit = (int)blockIdx.x / a.strips, strip = (int)blockIdx.x % a.strips;
   const int n = 8 * (strip * a.lanes + (int)threadIdx.x), no = kAct == epi::kSwiglu ? n / 2 : n;
-  if ((int)threadIdx.x >= a.lanes || n >= a.N) return;
-  if (a.dpre != nullptr) {                            // rows of no group
+  // four lanes hold a block's columns and read its scales for each other: they go together, the last two of a half block idle
+  if ((int)threadIdx.x >= a.lanes || (kMx ? n & ~31 : n) >= a.N) return;
+  const bool live = !kMx || n < a.N;
+  if (live && a.dpre != nullptr) {                    // rows of no group
     for (int64_t r = unit; r < t.start[0]; r += a.units) *(v4i*)(a.dpre + r * a.stride_dpre + n) = v4i{0, 0, 0, 0};
     for (int64_t r = t.start[a.G] + (int64_t)unit; r < a.m_total; r += a.units)
       *(v4i*)(a.dpre + r * a.stride_dpre + n) = v4i{0, 0, 0, 0};
@@ -161,19 +187,19 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
   float sum[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+  constexpr int kUnroll = kMx ? 8 : 4;                // rows a thread has in flight
   for (int64_t r = r0; r < r1; r += kUnroll) {
     v4i z[kUnroll], d[kUnroll];
-    uint32_t scale[kUnroll];
+    uint32_t scales = 0;
+    if constexpr (kMx) scales = row_scales(a, r, r1, n);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       z[u] = d[u] = v4i{0, 0, 0, 0};
-      scale[u] = 0;
-      if (r + u >= r1) continue;
+      if (!live || r + u >= r1) continue;
       if constexpr (kMx) {
         const v2i h = __builtin_nontemporal_load((const v2i*)(a.q8 + (r + u) * a.stride_pre + n));
         z[u][0] = h[0];
         z[u][1] = h[1];
-        scale[u] = a.scales[(r + u) * a.scale_row + (int64_t)(n / 32) * a.scale_block];
       } else if constexpr (kAct != epi::kNone) z[u] = __builtin_nontemporal_load((const v4i*)(a.pre + (r + u) * a.stride_pre + n));
       if constexpr (kAct == epi::kSwiglu) {
         const v2i h = __builtin_nontemporal_load((const v2i*)(a.dout + (r + u) * a.stride_dout + no));
@@ -183,12 +209,18 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
         d[u] = __builtin_nontemporal_load((const v4i*)(a.dout + (r + u) * a.stride_dout + no));
       }
     }
+    float power[kUnroll];
+    if constexpr (kMx) {
+      power[0] = row_scale<0>(scales), power[1] = row_scale<1>(scales), power[2] = row_scale<2>(scales);
+      power[3] = row_scale<3>(scales), power[4] = row_scale<4>(scales), power[5] = row_scale<5>(scales);
+      power[6] = row_scale<6>(scales), power[7] = row_scale<7>(scales);
+    }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (r + u >= r1) continue;
+      if (!live || r + u >= r1) continue;
       float x[8], v[8];
       if constexpr (kMx) {
-        mxq::restore_f32<true>(mxq::v2u{(unsigned)z[u][0], (unsigned)z[u][1]}, __uint_as_float(scale[u] << 23), v);
+        mxq::restore_f32<true>(mxq::v2u{(unsigned)z[u][0], (unsigned)z[u][1]}, power[u], v);
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -205,7 +237,7 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
       }
     }
   }
-  if (a.dbias != nullptr) {
+  if (live && a.dbias != nullptr) {
     float* p = a.partial + (int64_t)unit * a.N + n;
     *(v4f*)p = v4f{sum[0], sum[1], sum[2], sum[3]};
     *(v4f*)(p + 4) = v4f{sum[4], sum[5], sum[6], sum[7]};

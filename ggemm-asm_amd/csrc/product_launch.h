@@ -227,7 +227,7 @@ int launch_act_backward(ag::Args a, int act, hipStream_t stream) {
   a.rows = unit_rows(a.m_total, a.N);
   a.units = (int)units;
   a.strips = strips;
-  a.lanes = (a.N / 8 + strips - 1) / strips;
+  a.lanes = ((a.N / 8 + strips - 1) / strips + 3) / 4 * 4;      // whole blocks of 32 columns
   if (a.m_total > 0 && (a.dpre || a.dbias)) {
     const int rc = with_act(act, [&](auto code) {
       constexpr int kAct = decltype(code)::value;
