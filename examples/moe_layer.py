@@ -3,7 +3,8 @@
     python examples/moe_layer.py [--tokens 8192] [--experts 32] [--top-k 4] [--hidden 2880] [--inner 2880] [--steps 5]
 
 The router is a plain torch product; everything behind it is the package's: routing, dispatch, the experts' FP8
-products with bias and gated activation, and the combination, forward and backward. Weights and tokens are random.
+products with bias and gated activation, and the combination, forward and backward; then decoding on FP8 and on 4-bit
+weights. Weights and tokens are random.
 """
 import argparse
 import os
@@ -32,6 +33,19 @@ class MoE(torch.nn.Module):
         return ggemm.moe_layer_fp8(x, logits, self.w_up, self.w_down, self.top_k, bias_up=self.b_up,
                                    bias_down=self.b_down, slope=1.702, limit=7.0, shift=1.0, residual=x,
                                    weight_caches=self.caches)
+
+
+class Served:
+    """The trained layer on weights in 4 bits, for inference."""
+
+    def __init__(self, layer):
+        self.layer = layer
+        self.w_up, self.w_down = (ggemm.quantize_mx(w.detach(), row_align=128) for w in (layer.w_up, layer.w_down))
+
+    def __call__(self, x):
+        m = self.layer
+        return ggemm.moe_layer_mx(x, x @ m.router.t(), self.w_up, self.w_down, m.top_k, bias_up=m.b_up, bias_down=m.b_down,
+                                  slope=1.702, limit=7.0, shift=1.0, residual=x)
 
 
 def timed(f, n):
@@ -74,6 +88,9 @@ def main():
         one = x[:1]
         _, ms = timed(lambda: layer(one), 50)
         print(f"decoding: 1 token, {ms * 1e3:.0f} us")
+        served = Served(layer)
+        _, ms = timed(lambda: served(one), 50)
+        print(f"decoding: 1 token, weights in 4 bits, {ms * 1e3:.0f} us")
     return losses
 
 

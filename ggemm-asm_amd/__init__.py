@@ -22,10 +22,10 @@ from . import build, inputs  # noqa: F401
 from ._lib import GGemmError, bf16_kernel, launch_geometry, library_path, load as load_library  # noqa: F401
 from .autograd import (FP8DelayedScaling, FP8WeightCache, GroupedLinearActFP8, GroupedLinearFP8,  # noqa: F401
                        grouped_linear_fp8)
-from .layer import moe_layer_fp8  # noqa: F401
+from .layer import moe_layer_fp8, moe_layer_mx  # noqa: F401
 from .moe import DispatchPlan, combine_tokens, dispatch_tokens, plan_dispatch, route_experts  # noqa: F401
 from ._tensors import MXTensor  # noqa: F401
-from .mx import dequantize_mx, grouped_gemm_mx_bias_act, quantize_mx  # noqa: F401
+from .mx import dequantize_mx, dispatch_mx, grouped_gemm_mx_bias_act, quantize_mx  # noqa: F401
 from .persistent import grouped_gemm_fp8_tensorwise  # noqa: F401
 from .product import bias_act_backward, grouped_gemm_fp8_bias_act  # noqa: F401
 from .quant import (amax, padded_rows, quantize_fp8_tensorwise, quantize_fp8_tensorwise_delayed,  # noqa: F401

@@ -65,7 +65,7 @@ int over_rows(mxq::Args a, int dtype, F launch) {
 // ------------------------------------------------------------------------------ the product
 
 template <bool kA8>
-using Tile256 = mx::Cfg<kA8, 256, 256, 2, 4, kA8 ? 128 : 256, 2, true>;
+using Tile256 = mx::Cfg<kA8, 256, 256, 4, 2, kA8 ? 128 : 256, 2, true>;
 template <bool kA8>
 using Tile128 = mx::Cfg<kA8, 128, 128, 2, 2, kA8 ? 128 : 256, kA8 ? 3 : 2, false>;
 template <bool kA8>
@@ -185,6 +185,7 @@ int validate(const mx::Args& a, const epi::Args& e, int fmt, int act, int bias_d
   // 32-bit buffer offsets of a tile's 256 rows
   for (int64_t s : {sa, sas, sbn, sbsn})
     if (s * 256 >= (int64_t)nt::kOob) return GGEMM_E_SHAPE;
+  if ((int64_t)a.stride_out * 2 * 256 >= (int64_t)nt::kOob) return GGEMM_E_SHAPE;
   const int width = act == GGEMM_ACT_SWIGLU ? a.N / 2 : a.N;
   if (a.stride_out < width || a.stride_out % 8) return GGEMM_E_STRIDE;
   if (e.residual && (e.stride_res < width || e.stride_res % 8)) return GGEMM_E_STRIDE;

@@ -138,7 +138,11 @@ struct Cfg {
   static constexpr int PA = ABytes / 1024 / W, PB = BBytes / 1024 / W;   // LDS-DMA instructions for each wave and stage
   static constexpr int SA = (BM + 63) / 64, SB = (BN + 63) / 64;   // of scales for the workgroup, 64 rows each
   static constexpr int ScaleOff = S * Slot, ScaleBytes = 1024 * (SA + SB);
-  static constexpr int LdsBytes = ScaleOff + 2 * ScaleBytes;
+  static constexpr int LineOff = ScaleOff + 2 * ScaleBytes;     // where results are put together, Line bytes of 32 rows of each wave
+  static constexpr int Line = !kWalk ? 0 : LineOff + 4096 * W <= 160 * 1024 ? 128 : 64;
+  static constexpr int BiasOff = Line == 128 ? LineOff + 4096 * W : LineOff;   // a wave's columns of the bias; in its lines' place
+  static constexpr int BiasBytes = Line == 128 ? 1024 : 32 * Line;
+  static constexpr int LdsBytes = LineOff + 32 * Line * W + (Line == 128 ? 1024 * W : 0);
   static constexpr int MB = BM / WM / 32, NB = BN / WN / 32;    // 32-wide blocks of a wave
   static constexpr int BandN = 8;                               // column tiles of a band, row tiles walked inside
   static_assert(W % 2 == 0 && MB >= 1 && NB >= 1 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "waves");
@@ -184,70 +188,152 @@ __device__ __forceinline__ void by_half(int& x, int& y) {
 
 // A wave's MB x NB blocks of 32 x 32: lane 32 h + s holds row s, columns 8 g + 4 h .. + 3 of a block in accumulators
 // 4 g .. 4 g + 3. Rows row0 .. of the launch (the first `rows` of them exist), columns n0 .. of group g's product. The halves
-// of a row's columns change places between lanes s and s + 32, so that a lane stores (and reads of a residual) 16
-// bytes at a time, a row's 32 or 64 bytes of a block in one go, without LDS.
-template <int kAct, int MB, int NB>
+// of a row's columns change places between lanes s and s + 32, so that a lane holds (and reads of a residual) 16 bytes at a
+// time. kLine = 0: it stores them as they are. Else they go through 32 kLine bytes of the wave's LDS (`lines`) and are stored
+// kLine bytes of a row to neighbouring lanes, which for 131072 x 5760 x 2880 takes 9 % less (e4m3, whole lines) and 4 %
+// (e2m1, halves, as LDS has no more room), and the bias lies in LDS too (`bias_at`, raw, this wave's columns): a load's
+// wait would drain the stores before it and the next tile's loads.
+template <int kAct, int MB, int NB, int kLine>
 __device__ __forceinline__ void store(const v16f (&acc)[MB][NB], const epi::Args& e, uint16_t* out, int stride_out, int g,
-                                      int N, int64_t row0, int rows, int n0, int lane) {
+                                      int N, int64_t row0, int rows, int n0, int lane, GG_LDS uint8_t* lines,
+                                      GG_LDS uint8_t* bias_at) {
   constexpr bool kGated = kAct == epi::kSwiglu;
   constexpr int kParts = kGated ? 1 : 2;                       // 16-byte chunks of a lane and block
+  // or what follows from them is kept from tile to tile
+  if constexpr (kLine != 0) asm volatile("" : "+s"(stride_out));
+  if constexpr (kLine == 128) asm volatile("" : "+v"(lane));
   const int h = lane >> 5, s = lane & 31;
+  const int width = kGated ? N / 2 : N;
+  // block (i, j): chunk p of the lane has columns 16 h (gated: of z 16 h .. + 15; else 16 h + 8 p .. + 7)
+  auto block = [&](int i, int j, const v4f (&bias)[4], int (&w)[kParts][4]) {
+    const int nj = n0 + 32 * j, o0 = (kGated ? nj / 2 : nj) + (kGated ? 8 : 16) * h;
+    if (e.residual != nullptr) {
+      const int64_t row = row0 + 32 * i + s;
+      const bool live = 16 * h < min(32, N - nj) && 32 * i + s < rows;
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const int nj = n0 + 32 * j, cols = min(32, N - nj);        // a multiple of 16
-    if (cols <= 0) return;                                     // uniform in the wave, as all but the rows
-    v4f bias[4];
+      for (int p = 0; p < kParts; ++p) {
+        const v4i r = live ? *(const v4i*)(e.residual + row * e.stride_res + o0 + 8 * p) : v4i{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[p][k] = r[k];
+        // gated: words (0, 1) of a lane are column groups 2 h and, its other half, ..; else groups 2 h + p
+        by_half(w[p][0], w[p][kGated ? 1 : 2]);
+        by_half(w[p][kGated ? 2 : 1], w[p][3]);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      v4f z = bias[c];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[k] += acc[i][j][4 * c + k];
+      // group c: the two lanes' halves end up in lane half c / 2
+      if constexpr (kGated) {
+        int& at = w[0][2 * (c & 1) + (c >> 1)];
+        float x = epi::swiglu(z[0], z[1], e), y = epi::swiglu(z[2], z[3], e);
+        if (e.residual != nullptr) {
+          x += epi::from_bf16((uint32_t)at);
+          y += __uint_as_float((uint32_t)at & 0xffff0000u);
+        }
+        at = epi::pack(x, y);
+      } else {
+        int &lo = w[c & 1][2 * (c >> 1)], &hi = w[c & 1][2 * (c >> 1) + 1];
+        v4f x = epi::activation<kAct>(z);
+        if (e.residual != nullptr) x += epi::unpack4(v2i{lo, hi});
+        lo = epi::pack(x[0], x[1]);
+        hi = epi::pack(x[2], x[3]);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kParts; ++p) {
+      by_half(w[p][0], w[p][kGated ? 1 : 2]);
+      by_half(w[p][kGated ? 2 : 1], w[p][3]);
+    }
+  };
+  auto load_bias = [&](int j, v4f (&bias)[4]) {
+    const int nj = n0 + 32 * j, cols = N - nj;                 // a multiple of 16
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       bias[c] = 8 * c < cols ? epi::load_bias(e, (int64_t)g * N + nj + 8 * c + 4 * h) : v4f{0.f, 0.f, 0.f, 0.f};
-    // chunk p of the lane: columns 16 h (gated: of z 16 h .. + 15; else 16 h + 8 p .. + 7) of the block
-    const int o0 = (kGated ? nj / 2 : nj) + (kGated ? 8 : 16) * h;
-    const bool live_cols = 16 * h < cols;
+  };
+  if constexpr (kLine != 0) {
+    constexpr int kRow = kLine / (32 * kParts), kChunks = kLine / 16;   // blocks and chunks of a piece
+    constexpr bool kOwn = kLine == 128;                        // the bias has a place of its own
+    static_assert(NB == 4 && NB % kRow == 0, "two columns of bias to a lane, whole pieces");
+    float own[2] = {0.f, 0.f};                                 // bias of columns `lane` and 64 + `lane`
+    if (!kOwn && e.bias != nullptr)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        own[k] = e.bias_f32 ? *(const GG_LDS float*)(bias_at + 4 * (64 * k + lane))
+                            : __uint_as_float((uint32_t)*(const GG_LDS uint16_t*)(bias_at + 2 * (64 * k + lane)) << 16);
+    auto read_bias = [&](int j, bool f32, v4f (&bias)[4]) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int at = 32 * j + 8 * c + 4 * h;
+        bias[c] = e.bias == nullptr ? v4f{0.f, 0.f, 0.f, 0.f}
+                  : f32             ? *(const GG_LDS v4f*)(bias_at + 4 * at)
+                                    : epi::unpack4(v2i(*(const GG_LDS v2i*)(bias_at + 2 * at)));
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < NB; j += kRow) {
+      const int nj = n0 + 32 * j, c = lane & (kChunks - 1), oj = kGated ? nj / 2 : nj;
+      if (nj >= N) return;                                     // uniform in the wave, as all but the rows
+      v4f bias[kRow][4];
+      if constexpr (!kOwn) {
+        if (e.bias != nullptr) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) *(GG_LDS float*)(bias_at + 4 * (64 * k + lane)) = own[k];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+#pragma unroll
+        for (int k = 0; k < kRow; ++k) read_bias(j + k, true, bias[k]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+      // rows that do not exist are out of the buffer's range, and so are columns by their offset
+      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(out + row0 * stride_out + oj, 0, 2 * max(rows, 0) * stride_out, kRsrcWord3);
+      const int to = 8 * c < width - oj ? 2 * (lane / kChunks * stride_out + 8 * c) : (int)kOob;
+#pragma unroll
+      for (int i = 0; i < MB; ++i) {
+        if (rows <= 32 * i) break;
+#pragma unroll
+        for (int k = 0; k < kRow; ++k) {
+          int w[kParts][4];
+          if constexpr (kOwn) read_bias(j + k, e.bias_f32, bias[k]);
+          block(i, j + k, bias[k], w);
+#pragma unroll
+          for (int p = 0; p < kParts; ++p)
+            *(GG_LDS v4i*)(lines + kLine * s + 16 * ((2 * kParts * k + kParts * h + p) ^ (s & (kChunks - 1)))) =
+                v4i{w[p][0], w[p][1], w[p][2], w[p][3]};
+          __builtin_amdgcn_sched_barrier(0);                   // one block's values (and bias) in registers at a time
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int q = 0; q < kChunks / 2; ++q) {
+          const int r = 64 / kChunks * q + lane / kChunks;
+          const v4i v = *(const GG_LDS v4i*)(lines + kLine * r + 16 * (c ^ (r & (kChunks - 1))));
+          // whole lines past the caches: (e4m3) 32768 x 2880 x 2880 294 -> 261 us; halves through them
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(mid::v4u32, v), rsrc,
+                                                 to + 2 * (32 * i + 64 / kChunks * q) * stride_out, 0, kLine == 128 ? 2 : 0);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int nj = n0 + 32 * j, o0 = (kGated ? nj / 2 : nj) + (kGated ? 8 : 16) * h;
+    if (nj >= N) return;
+    v4f bias[4];
+    load_bias(j, bias);
 #pragma unroll
     for (int i = 0; i < MB; ++i) {
       if (rows <= 32 * i) break;
-      const int64_t row = row0 + 32 * i + s;
-      const bool live = live_cols && 32 * i + s < rows;
       int w[kParts][4];
-      if (e.residual != nullptr) {
+      block(i, j, bias, w);
+      if (16 * h < min(32, N - nj) && 32 * i + s < rows)
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) {
-          const v4i r = live ? *(const v4i*)(e.residual + row * e.stride_res + o0 + 8 * p) : v4i{0, 0, 0, 0};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[p][k] = r[k];
-          // gated: words (0, 1) of a lane are column groups 2 h and, its other half, ..; else groups 2 h + p
-          by_half(w[p][0], w[p][kGated ? 1 : 2]);
-          by_half(w[p][kGated ? 2 : 1], w[p][3]);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        v4f z = bias[c];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) z[k] += acc[i][j][4 * c + k];
-        // group c: the two lanes' halves end up in lane half c / 2
-        if constexpr (kGated) {
-          int& at = w[0][2 * (c & 1) + (c >> 1)];
-          float x = epi::swiglu(z[0], z[1], e), y = epi::swiglu(z[2], z[3], e);
-          if (e.residual != nullptr) {
-            x += epi::from_bf16((uint32_t)at);
-            y += __uint_as_float((uint32_t)at & 0xffff0000u);
-          }
-          at = epi::pack(x, y);
-        } else {
-          int &lo = w[c & 1][2 * (c >> 1)], &hi = w[c & 1][2 * (c >> 1) + 1];
-          v4f x = epi::activation<kAct>(z);
-          if (e.residual != nullptr) x += epi::unpack4(v2i{lo, hi});
-          lo = epi::pack(x[0], x[1]);
-          hi = epi::pack(x[2], x[3]);
-        }
-      }
-#pragma unroll
-      for (int p = 0; p < kParts; ++p) {
-        by_half(w[p][0], w[p][kGated ? 1 : 2]);
-        by_half(w[p][kGated ? 2 : 1], w[p][3]);
-        if (live) *(v4i*)(out + row * stride_out + o0 + 8 * p) = v4i{w[p][0], w[p][1], w[p][2], w[p][3]};
-      }
+        for (int p = 0; p < kParts; ++p)
+          *(v4i*)(out + (row0 + 32 * i + s) * stride_out + o0 + 8 * p) = v4i{w[p][0], w[p][1], w[p][2], w[p][3]};
     }
   }
 }
@@ -383,6 +469,18 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
         for (int k = 0; k < 16; ++k) acc[i][j][k] = 0.f;
   };
 
+  GG_LDS uint8_t* const lines = lds + C::LineOff + 32 * C::Line * wave;
+  GG_LDS uint8_t* const bias_at = lds + C::BiasOff + C::BiasBytes * wave;
+  auto fetch_bias = [&](const At& t) {                         // lands with the first stage that is waited for after it
+    if constexpr (C::Line != 0) {
+      if (e.bias == nullptr) return;
+      const int n = t.n0 + 32 * C::NB * wn, size = e.bias_f32 ? 4 : 2;
+      dma16(make_rsrc((const uint8_t*)e.bias + ((int64_t)t.g * a.N + n) * size, max(0, min(32 * C::NB, a.N - n)) * size),
+            lds_u32(bias_at), 16 * lane);
+    }
+  };
+
+  fetch_bias(tile);
   load_from(tile);
 #pragma unroll
   for (int k = 0; k < C::S; ++k) {
@@ -448,10 +546,12 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
     cur = nxt;
     nxt = nxt + 1 == C::S ? 0 : nxt + 1;
     if (st != 0) continue;
-    store<kAct, C::MB, C::NB>(acc, e, a.out, a.stride_out, tile.g, a.N, tile.row0 + 32 * C::MB * wm,
-                              tile.rows - 32 * C::MB * wm, tile.n0 + 32 * C::NB * wn, lane);
+    store<kAct, C::MB, C::NB, C::Line>(acc, e, a.out, a.stride_out, tile.g, a.N, tile.row0 + 32 * C::MB * wm,
+                              tile.rows - 32 * C::MB * wm, tile.n0 + 32 * C::NB * wn, lane,
+                                       lines, bias_at);
     if (next.rows == 0) break;
     tile = next;
+    fetch_bias(tile);
     block += grid;
     next = tile_at(block);
     clear();

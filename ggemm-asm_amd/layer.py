@@ -1,15 +1,16 @@
 """A whole MoE layer: routing, dispatch, the experts' two FP8 products and the combination.
 
-``moe_layer_fp8`` is how the package's operators are meant to follow one another; a model with another order of steps
-calls them one by one. The reference's harness runs the products alone, on random rows (reference bench.py:196-268).
+``moe_layer_fp8`` is how the package's operators are meant to follow one another, ``moe_layer_mx`` the same on weights kept
+in 4 bits; a model with another order of steps calls them one by one. The reference's harness runs the products alone, on random rows (reference bench.py:196-268).
 """
 from __future__ import annotations
 
 import torch
 
-from ._tensors import tracked
+from ._tensors import MXTensor, mx_columns, tracked
 from .autograd import FP8DelayedScaling, FP8WeightCache, grouped_linear_fp8
 from .moe import combine_tokens, dispatch_tokens, plan_dispatch, route_experts
+from .mx import dispatch_mx, grouped_gemm_mx_bias_act, quantize_mx
 from .product import _rows16, grouped_gemm_fp8_bias_act
 from .quant import quantize_fp8_tensorwise
 
@@ -66,4 +67,38 @@ def moe_layer_fp8(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, w_d
     qh, sh, _ = quantize_fp8_tensorwise(h, "e4m3", row_align=_LINE)
     qd, sd = _weight(w_down, caches[1])
     y = grouped_gemm_fp8_bias_act(qh, qd, sh, sd, plan.group_offs, bias_down)
+    return combine_tokens(y, plan, weights, residual)
+
+
+def moe_layer_mx(x: torch.Tensor, logits: torch.Tensor, w_up: MXTensor, w_down: MXTensor, top_k: int, *,
+                 bias_up: torch.Tensor | None = None, bias_down: torch.Tensor | None = None,
+                 activation: str | None = "swiglu", slope: float = 1.0, limit: float | None = None, shift: float = 0.0,
+                 residual: torch.Tensor | None = None, routing: dict | None = None, fmt: str = "e4m3") -> torch.Tensor:
+    """``residual + sum_j weight_j * expert_j(x)`` of every token, [T, H] bf16, for inference on microscaled weights.
+
+    w_up, w_down: e2m1, the values of [E, N, H] and [E, H, I] (``quantize_mx(w, row_align=128)``; neighbouring rows of w_up
+    are gate and value for "swiglu"); H and I multiples of 32. ``fmt``: what the activations are quantized to before each
+    product, "e4m3" or "e2m1". The rest as for ``moe_layer_fp8``.
+
+    A token's blocks are its own, so no scale is shared by a batch: a token's result does not depend on what it is batched
+    with, but for the order of fp32 sums in another kernel. It has no gradients and refuses an input that asks for one."""
+    if x.dim() != 2 or x.dtype != torch.bfloat16:
+        raise TypeError("x must be a bf16 [T, H] tensor")
+    if mx_columns(w_up, "w_up")[0] != 1 or mx_columns(w_down, "w_down")[0] != 1 or w_up.q.dim() != 3 or w_down.q.dim() != 3:
+        raise TypeError("w_up and w_down must hold e2m1 values [E, N, H] and [E, H, I]")
+    experts, hidden = w_up.q.shape[0], 2 * w_up.q.shape[2]
+    if x.shape[1] != hidden:
+        raise ValueError(f"x has {x.shape[1]} features, w_up {hidden}")
+    if logits.dim() != 2 or logits.shape[0] != x.shape[0] or logits.shape[1] != experts:
+        raise ValueError(f"logits must be [{x.shape[0]}, {experts}]")
+    inner = w_up.q.shape[1] // (2 if activation == "swiglu" else 1)
+    if tuple(w_down.q.shape) != (experts, hidden, inner // 2) or inner % 32:
+        raise ValueError("w_up and w_down hold the same experts, [E, N, H] and [E, H, I], I a multiple of 32")
+    if tracked(x, logits, bias_up, bias_down, residual):
+        raise RuntimeError("moe_layer_mx has no gradients: call it under torch.no_grad()")
+    weights, chosen = route_experts(logits, top_k, **(routing or {}))
+    plan = plan_dispatch(chosen, experts)
+    rows = dispatch_mx(quantize_mx(x, fmt), plan)
+    h = grouped_gemm_mx_bias_act(rows, w_up, plan.group_offs, bias_up, activation, slope=slope, limit=limit, shift=shift)
+    y = grouped_gemm_mx_bias_act(quantize_mx(h, fmt, _LINE), w_down, plan.group_offs, bias_down)
     return combine_tokens(y, plan, weights, residual)

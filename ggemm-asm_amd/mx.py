@@ -2,6 +2,7 @@
 of two, the values are e2m1 (4 bits) or e4m3 (8 bits).
 
 * ``quantize_mx`` / ``dequantize_mx``  -- rows to their blocks and back: weights in 4 bits, activation checkpoints in 8
+* ``dispatch_mx``                      -- tokens' blocks into expert order
 * ``grouped_gemm_mx_bias_act``         -- the grouped product of e2m1 weights with e2m1 or e4m3 activations, with bias,
   activation and residual in its epilogue
 
@@ -17,7 +18,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._tensors import MX_BLOCK as BLOCK, MXTensor, mx_columns as _columns, on_gpu as _on_gpu, row_stride as _stride, tracked
+from ._tensors import MX_BLOCK as BLOCK, MXTensor, mx_columns, on_gpu as _on_gpu, row_stride as _stride, tracked
+from .moe import DispatchPlan, dispatch_tokens
 from .product import _act, _check_offs, _rows16
 from .quant import _IN, _padded_empty
 from .vark import _validate_offsets
@@ -85,7 +87,7 @@ def dequantize_mx(t: MXTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
     if dtype not in _IN:
         raise TypeError(f"dtype must be bfloat16 or float32, got {dtype}")
     q, scales = t
-    code, cols = _columns(t, "t")
+    code, cols = mx_columns(t, "t")
     if q.dim() < 2:
         raise ValueError("t must have at least 2 dimensions (rows x columns)")
     _on_gpu(q, "the restoration")
@@ -130,6 +132,22 @@ def _product_rows(t: torch.Tensor, row: int, past: bool):
     return t, rs, gs
 
 
+def dispatch_mx(t: MXTensor, plan: DispatchPlan) -> MXTensor:
+    """The tokens' rows of t ([T, K]) in expert order, as ``dispatch_tokens`` copies them: [T * k, K], laid out as the grouped
+    product reads them best. Rows of no expert are zero."""
+    mx_columns(t, "t")
+    q, scales = t
+    if q.dim() != 2 or q.shape[1] == 0:
+        raise ValueError("t must be a [T, K] tensor, K positive")
+    _on_gpu(q, "the dispatch")
+    blocks = scales.shape[1]
+    row = -(-blocks // 16) * 16                                  # copied whole, 16 bytes at a time
+    if q.shape[0]:
+        scales, stride, _ = _product_rows(scales, row, row > blocks)
+        scales = scales.as_strided((q.shape[0], row), (stride, 1))
+    return MXTensor(dispatch_tokens(q, plan, row_align=128), dispatch_tokens(scales, plan, row_align=16)[:, :blocks])
+
+
 def grouped_gemm_mx_bias_act(a: MXTensor, b: MXTensor, group_offs: torch.Tensor, bias: torch.Tensor | None = None,
                              activation: str | None = None, residual: torch.Tensor | None = None, *, slope: float = 1.0,
                              limit: float | None = None, shift: float = 0.0, zero_tail: bool = False,
@@ -145,8 +163,8 @@ def grouped_gemm_mx_bias_act(a: MXTensor, b: MXTensor, group_offs: torch.Tensor,
     and of scales start on multiples of 16 bytes and rows of scales can be read up to a multiple of 16: weights from
     elsewhere are laid out so once. ``tile``: rows of the output tiles (16, 32, 64, 128 or 256), 0 for the library's choice.
     An operator of inference: it has no gradients and refuses a bias or residual that asks for one."""
-    code, K = _columns(a, "a")
-    b_code, Kb = _columns(b, "b")
+    code, K = mx_columns(a, "a")
+    b_code, Kb = mx_columns(b, "b")
     if b_code != 1:
         raise TypeError("b must hold e2m1 values (uint8)")
     aq, bq = a.q, b.q
