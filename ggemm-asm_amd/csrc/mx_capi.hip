@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
@@ -110,17 +111,18 @@ int64_t tiles_of(int64_t M, int64_t g, int N, int bm, int bn) { return (M / bm +
 // to 16 rows to a group in the mean and 160 tiles of 32 x 128. Measured (us, 32-row tiles -> it; weights not in a
 // cache): N = 5760, K = 2880, e4m3: 1 row of 1 expert 10.2 -> 6.3, 16 of 2 10.7 -> 9.5, 4 of 4 13.0 -> 13.4 (stays),
 // 64 of 32 55.8 -> 70.0 (stays); 2 of 2, N = K = 2880 9.7 -> 5.9; 2 of 1, N = K = 4096 11.6 -> 6.1.
-// The others by an estimate in us, c + rounds (e + s K / 1000), where a round is as many tiles as the chip holds at once.
-// The numbers are a fit to 32 (e4m3) and 26 launches (e2m1) of 32 to 32768 rows, 1 to 32 groups, N 512 to 5760, K 512 to
-// 4096: single times are off by up to 0.5 to 1.35, the choice by 3.5 % and 1.2 % in the mean, 22 % and 17 % at most.
+// The others by an estimate in us, c + rounds (e + s K / 1000), where a round is as many tiles as the chip holds at once; where
+// workgroups walk over their tiles, the last round is a whole one.
+// The numbers are a fit to 32 launches of each format, of 32 to 35149 rows, 1 to 32 groups, N 512 to 5760, K 512 to 4096:
+// single times are off by up to 0.5 to 1.4, the choice by 3.0 % (e4m3) and 1.6 % (e2m1) in the mean, 19 % and 17 % at most.
 struct Fit {
   int rows, cols, per_cu;
   double c, e, s;
 };
-constexpr Fit kFits[2][4] = {{{32, 128, 2, 0.6, 3.8, 3.05}, {64, 128, 2, -1.7, 4.7, 4.36},
-                              {128, 128, 2, -6.3, 10.5, 5.55}, {256, 256, 1, -0.1, 8.0, 11.6}},
-                             {{32, 128, 2, 0.1, 4.4, 2.22}, {64, 128, 2, -3.9, 8.6, 2.04},
-                              {128, 128, 2, -8.7, 14.4, 3.03}, {256, 256, 1, -5.0, 14.0, 6.51}}};
+constexpr Fit kFits[2][4] = {{{32, 128, 2, 0.7, 3.9, 3.08}, {64, 128, 2, -1.8, 4.9, 4.42},
+                              {128, 128, 2, -7.0, 11.6, 5.48}, {256, 256, 1, -0.5, 9.1, 10.4}},
+                             {{32, 128, 2, 0.0, 4.7, 2.31}, {64, 128, 2, -4.6, 9.5, 2.09},
+                              {128, 128, 2, -8.9, 14.0, 3.09}, {256, 256, 1, -0.3, 9.3, 5.72}}};
 int choose(int fmt, int G, int N, int K, int64_t M, int cus) {
   const int64_t g = std::min<int64_t>(G, M);
   if (M <= 16 * g && g * ((N + 127) / 128) <= 5 * cus / 8) return 16;
@@ -128,7 +130,8 @@ int choose(int fmt, int G, int N, int K, int64_t M, int cus) {
   double least = 0;
   for (const Fit& f : kFits[fmt == GGEMM_MX_E2M1]) {
     const double tiles = std::max<double>(g, (double)M / f.rows + g / 2.0) * ((N + f.cols - 1) / f.cols);
-    const double t = f.c + std::max(1.0, tiles / (f.per_cu * cus)) * (f.e + f.s * K / 1000);
+    const double part = std::max(1.0, tiles / (f.per_cu * cus)), rounds = f.per_cu == 1 ? std::ceil(part) : part;
+    const double t = f.c + rounds * (f.e + f.s * K / 1000);
     if (best == 0 || t < least) best = f.rows, least = t;
   }
   return best;

@@ -138,17 +138,18 @@ struct Cfg {
   static constexpr int PA = ABytes / 1024 / W, PB = BBytes / 1024 / W;   // LDS-DMA instructions for each wave and stage
   static constexpr int SA = (BM + 63) / 64, SB = (BN + 63) / 64;   // of scales for the workgroup, 64 rows each
   static constexpr int ScaleOff = S * Slot, ScaleBytes = 1024 * (SA + SB);
-  static constexpr int LineOff = ScaleOff + 2 * ScaleBytes;     // where results are put together, Line bytes of 32 rows of each wave
-  static constexpr int Line = !kWalk ? 0 : LineOff + 4096 * W <= 160 * 1024 ? 128 : 64;
-  static constexpr int BiasOff = Line == 128 ? LineOff + 4096 * W : LineOff;   // a wave's columns of the bias; in its lines' place
-  static constexpr int BiasBytes = Line == 128 ? 1024 : 32 * Line;
-  static constexpr int LdsBytes = LineOff + 32 * Line * W + (Line == 128 ? 1024 * W : 0);
   static constexpr int MB = BM / WM / 32, NB = BN / WN / 32;    // 32-wide blocks of a wave
+  // Where results are put together, Line bytes of 32 rows of each wave, and a wave's columns of the bias (in the place of its
+  // lines where those are not whole). No Line where LDS has no room or a wave's rows are short.
+  static constexpr int LineOff = ScaleOff + 2 * ScaleBytes, Room = (kWalk ? 160 : 80) * 1024;
+  static constexpr int Line = NB % 2 ? 0 : LineOff + 5120 * W <= Room ? 128 : LineOff + 2048 * W <= Room ? 64 : 0;
+  static constexpr int BiasOff = Line == 128 ? LineOff + 4096 * W : LineOff, BiasBytes = Line == 128 ? 1024 : 2048;
+  static constexpr int LdsBytes = LineOff + 32 * Line * W + (Line == 128 ? 1024 * W : 0);
   static constexpr int BandN = 8;                               // column tiles of a band, row tiles walked inside
   static_assert(W % 2 == 0 && MB >= 1 && NB >= 1 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "waves");
   static_assert(ABytes % (1024 * W) == 0 && BBytes % (1024 * W) == 0, "uniform LDS-DMA split");
   static_assert(S >= 2 && (kWalk ? S == 2 : S <= Super + 1), "a buffer of scales is read out when its next chunk is asked for");
-  static_assert(LdsBytes <= (kWalk ? 160 : 80) * 1024, "LDS");
+  static_assert(LdsBytes <= Room, "LDS");
 };
 
 // Chunk c of row r, `row` bytes a stage, lies at c ^ swizzle: 16 rows' equal chunks on 16 different groups of banks. Rows that
@@ -190,9 +191,9 @@ __device__ __forceinline__ void by_half(int& x, int& y) {
 // 4 g .. 4 g + 3. Rows row0 .. of the launch (the first `rows` of them exist), columns n0 .. of group g's product. The halves
 // of a row's columns change places between lanes s and s + 32, so that a lane holds (and reads of a residual) 16 bytes at a
 // time. kLine = 0: it stores them as they are. Else they go through 32 kLine bytes of the wave's LDS (`lines`) and are stored
-// kLine bytes of a row to neighbouring lanes, which for 131072 x 5760 x 2880 takes 9 % less (e4m3, whole lines) and 4 %
-// (e2m1, halves, as LDS has no more room), and the bias lies in LDS too (`bias_at`, raw, this wave's columns): a load's
-// wait would drain the stores before it and the next tile's loads.
+// kLine bytes of a row to neighbouring lanes, and the bias lies in LDS too (`bias_at`, raw, this wave's columns): a load's
+// wait would drain the stores before it and the next tile's loads. 32768 x 2880 x 2880, e4m3: 329 us without, 255 so;
+// 131072 x 5760 x 2880, e2m1, swiglu: 1434 and 1307; 128-row tiles, 4096 x 5760 x 2880, e2m1, swiglu: 90 and 84.
 template <int kAct, int MB, int NB, int kLine>
 __device__ __forceinline__ void store(const v16f (&acc)[MB][NB], const epi::Args& e, uint16_t* out, int stride_out, int g,
                                       int N, int64_t row0, int rows, int n0, int lane, GG_LDS uint8_t* lines,
@@ -257,11 +258,11 @@ __device__ __forceinline__ void store(const v16f (&acc)[MB][NB], const epi::Args
   if constexpr (kLine != 0) {
     constexpr int kRow = kLine / (32 * kParts), kChunks = kLine / 16;   // blocks and chunks of a piece
     constexpr bool kOwn = kLine == 128;                        // the bias has a place of its own
-    static_assert(NB == 4 && NB % kRow == 0, "two columns of bias to a lane, whole pieces");
-    float own[2] = {0.f, 0.f};                                 // bias of columns `lane` and 64 + `lane`
+    static_assert(NB % 2 == 0 && NB % kRow == 0, "whole pieces");
+    float own[NB / 2] = {};                                    // bias of columns 64 k + `lane`
     if (!kOwn && e.bias != nullptr)
 #pragma unroll
-      for (int k = 0; k < 2; ++k)
+      for (int k = 0; k < NB / 2; ++k)
         own[k] = e.bias_f32 ? *(const GG_LDS float*)(bias_at + 4 * (64 * k + lane))
                             : __uint_as_float((uint32_t)*(const GG_LDS uint16_t*)(bias_at + 2 * (64 * k + lane)) << 16);
     auto read_bias = [&](int j, bool f32, v4f (&bias)[4]) {
@@ -281,7 +282,7 @@ __device__ __forceinline__ void store(const v16f (&acc)[MB][NB], const epi::Args
       if constexpr (!kOwn) {
         if (e.bias != nullptr) {
 #pragma unroll
-          for (int k = 0; k < 2; ++k) *(GG_LDS float*)(bias_at + 4 * (64 * k + lane)) = own[k];
+          for (int k = 0; k < NB / 2; ++k) *(GG_LDS float*)(bias_at + 4 * (64 * k + lane)) = own[k];
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
 #pragma unroll
