@@ -13,7 +13,7 @@ include/ggemm_persistent.h. Modules:
 * ``mx``         -- microscaled rows (4 and 8 bits) and the grouped product of 4-bit weights, over the C ABI
 * ``moe``        -- routing tokens to experts, their rows into expert order and back, over the C ABI
 * ``autograd``   -- the FP8 grouped linear layer (forward, dgrad, wgrad) as a torch autograd op
-* ``layer``      -- a whole MoE layer from router logits to the combined tokens
+* ``layer``      -- a whole MoE layer from router logits to the combined tokens, on fp8 or on 4-bit weights
 * ``harness``    -- code-object launch paths mirroring the reference's hipModule harness
 * ``inputs``     -- seeded generators for the measured configurations
 * ``build``      -- in-tree hipcc build of the library and the drop-in code objects

@@ -103,6 +103,7 @@ MX_EXPORTS = (
     "ggemm_mx_keep_product",
     "ggemm_mx_keep_tile_rows",
     "ggemm_mx_act_backward",
+    "ggemm_mx_act_workspace",
 )
 
 # GGEMM_VARK_ABI_VERSION of include/ggemm_vark.h that these bindings are written for. Some exports
@@ -235,8 +236,9 @@ def load():
     lib.ggemm_moe_plan_workspace.restype = ctypes.c_int64
     lib.ggemm_product_tile_rows.argtypes = [i32] * 9 + [i64, i32]
     lib.ggemm_product_tile_rows.restype = ctypes.c_int32
-    lib.ggemm_product_act_workspace.argtypes = [i64, i32, i32]
-    lib.ggemm_product_act_workspace.restype = ctypes.c_int64
+    for name in ("ggemm_product_act_workspace", "ggemm_mx_act_workspace"):
+        getattr(lib, name).argtypes = [i64, i32, i32]
+        getattr(lib, name).restype = ctypes.c_int64
     lib.ggemm_mx_tile_rows.argtypes = [i32] * 4 + [i64, i32]
     lib.ggemm_mx_tile_rows.restype = ctypes.c_int32
     lib.ggemm_mx_keep_tile_rows.argtypes = [i32] * 9 + [i64, i32]

@@ -29,7 +29,7 @@ def mx_columns(t: MXTensor, what: str) -> tuple[int, int]:
         code, cols = 1, 2 * q.shape[-1]
     else:
         raise TypeError(f"{what} must hold float8_e4m3fn values or uint8 pairs of e2m1, got {q.dtype}")
-    if scales.dtype != torch.uint8 or tuple(scales.shape) != tuple(q.shape[:-1]) + (-(-cols // MX_BLOCK),):
+    if scales.dtype != torch.uint8 or scales.shape != q.shape[:-1] + (-(-cols // MX_BLOCK),):
         raise ValueError(f"{what}'s scales must be uint8 {list(q.shape[:-1]) + [-(-cols // MX_BLOCK)]}")
     if scales.device != q.device:
         raise ValueError(f"{what}'s values and scales must be on the same device")

@@ -24,7 +24,9 @@ namespace ag {
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxGroups = 2047;
-constexpr int kPer = (kMaxGroups + 1) / kThreads;      // group offsets a thread holds
+// Group offsets a thread holds: one of up to 255 groups, else all that there may be. (5003 x 1424 of 7 groups: 14.7 us with one,
+// 16.4 with eight, and the second kernel 4.0 and 4.7.)
+constexpr int kPerFew = 1, kPerMost = (kMaxGroups + 1) / kThreads;
 
 struct Args {
   const uint16_t* dout;
@@ -48,13 +50,15 @@ struct Args {
 // Group g has rows start[g] .. start[g + 1] - 1 and units pre[g] .. pre[g + 1] - 1. Offsets are clamped to
 // [0, m_total] and to the largest one before them, so groups never overlap and there are at most
 // m_total / rows + G units whatever group_offs holds.
+template <int kPer>
 struct Table {
-  int start[kMaxGroups + 1];
-  int pre[kMaxGroups + 1];
+  int start[kThreads * kPer];
+  int pre[kThreads * kPer];
   int scan[2 * kWaves];
 };
 
-__device__ __forceinline__ void group_table(const Args& a, Table& t) {
+template <int kPer>
+__device__ __forceinline__ void group_table(const Args& a, Table<kPer>& t) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int o[kPer + 1], mx = 0;
 #pragma unroll
@@ -162,9 +166,9 @@ __device__ __forceinline__ float row_scale(uint32_t v) {
 }
 
 // grid: units x strips; kMx: z from its 8-bit checkpoint
-template <int kAct, bool kMx>
+template <int kAct, bool kMx, int kPer>
 __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
-  __shared__ Table t;
+  __shared__ Table<kPer> t;
   group_table(a, t);
   const int unit = (int)blockIdx.x / a.strips, strip = (int)blockIdx.x % a.strips;
   const int n = 8 * (strip * a.lanes + (int)threadIdx.x), no = kAct == epi::kSwiglu ? n / 2 : n;
@@ -246,8 +250,9 @@ __global__ __launch_bounds__(kThreads) void act_backward_kernel(Args a) {
 
 // dbias[g, n] over the group's units; grid (columns / 64, G): a wave takes 64 columns and every kWaves-th unit, eight
 // of them in flight, and the waves' sums are added in their order.
-static __global__ __launch_bounds__(kThreads) void bias_sum_kernel(Args a) {
-  __shared__ Table t;
+template <int kPer>
+__global__ __launch_bounds__(kThreads) void bias_sum_kernel(Args a) {
+  __shared__ Table<kPer> t;
   __shared__ float s_sum[kThreads];
   group_table(a, t);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;

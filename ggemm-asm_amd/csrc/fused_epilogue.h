@@ -117,7 +117,8 @@ __device__ __forceinline__ int pack(float a, float b) {
 }
 
 // z of a row's 16 columns x 2 in four lanes 16 apart, eight each, as MX: the scale byte of the 32 columns and the lane's
-// values of either half, four bytes each.
+// values of either half, four bytes each. Two exchanges of lanes and a conversion for two values: 5003 x 2048 x 1424 with gelu
+// and a residual takes 38.8 us so and 37.4-39.3 with z in bf16, which writes 10 MB more.
 __device__ __forceinline__ uint32_t quantize32(const v4f& a, const v4f& b, int (&q)[2]) {
   uint32_t m = 0;
 #pragma unroll

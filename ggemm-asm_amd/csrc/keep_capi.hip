@@ -42,6 +42,11 @@ int32_t ggemm_mx_keep_tile_rows(int32_t G, int32_t N, int32_t K, int32_t stride_
   return rows[(int)choose(x, e, act, num_cus).kernel];
 }
 
+int64_t ggemm_mx_act_workspace(int64_t M_total, int32_t G, int32_t N) {
+  if (M_total < 0 || M_total > nt::kMaxRow || G <= 0 || G > ag::kMaxGroups || N <= 0) return 0;
+  return units_of(M_total, G, N, true) * N;
+}
+
 int ggemm_mx_act_backward(const void* dout, const void* q, const uint8_t* scales, const int64_t* group_offs, int32_t G,
                           int32_t N, int32_t stride_dout, int32_t stride_q, int64_t scale_row, int64_t scale_block,
                           int32_t act, float slope, float limit, float shift, int64_t M_total, void* dpre,

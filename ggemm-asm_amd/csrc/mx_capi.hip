@@ -65,6 +65,7 @@ int over_rows(mxq::Args a, int dtype, F launch) {
 
 // ------------------------------------------------------------------------------ the product
 
+// Slots of a stage: as many as LDS has room for, but three for what the small tiles gain by (two workgroups to a CU).
 template <bool kA8>
 using Tile256 = mx::Cfg<kA8, 256, 256, 4, 2, kA8 ? 128 : 256, 2, true>;
 template <bool kA8>

@@ -44,7 +44,7 @@ int32_t ggemm_product_tile_rows(int32_t G, int32_t N, int32_t K, int32_t stride_
 
 int64_t ggemm_product_act_workspace(int64_t M_total, int32_t G, int32_t N) {
   if (M_total < 0 || M_total > nt::kMaxRow || G <= 0 || G > ag::kMaxGroups || N <= 0) return 0;
-  return units_of(M_total, G, N) * N;
+  return units_of(M_total, G, N, false) * N;
 }
 
 int ggemm_product_act_backward(const void* dout, const void* pre, const int64_t* group_offs, int32_t G, int32_t N,

@@ -206,42 +206,51 @@ int launch_product(nt::Args x, const epi::Args& e, int act, int cus, hipStream_t
 }
 
 // Rows of a unit of the gradient: few enough that the units fill the chip, 64 at most (131072 x 5760: 256 rows 810 us, 64
-// 795: more rounds of workgroups even out), but for launches of more units than a grid takes.
+// 795: more rounds of workgroups even out), but for launches of more units than a grid takes. Of 8-bit z, eight rows of which
+// a thread has in flight at once, eight at least: 5003 x 1424 14.6 us, 16.4 with sixteen.
 constexpr int64_t kMaxUnits = 1 << 22;
 int strips_of(int N) { return (N / 8 + ag::kThreads - 1) / ag::kThreads; }
-int unit_rows(int64_t M, int N) {
+int unit_rows(int64_t M, int N, int least) {
   const int strips = strips_of(N);
   int64_t rows = 64;
-  while (rows > 16 && M / rows * strips < 2048) rows /= 2;
+  while (rows > least && M / rows * strips < 2048) rows /= 2;
   while (M / rows * strips > kMaxUnits) rows *= 2;
   return (int)rows;
 }
-int64_t units_of(int64_t M, int G, int N) { return std::max<int64_t>(1, M / unit_rows(M, N) + std::min<int64_t>(G, M)); }
+constexpr int least_rows(bool mx) { return mx ? 8 : 16; }
+int64_t units_of(int64_t M, int G, int N, bool mx) {
+  return std::max<int64_t>(1, M / unit_rows(M, N, least_rows(mx)) + std::min<int64_t>(G, M));
+}
 
 // Both launches of the gradient on checked arguments; kMx: z from its 8-bit checkpoint.
 template <bool kMx>
 int launch_act_backward(ag::Args a, int act, hipStream_t stream) {
   const int strips = strips_of(a.N);
-  const int64_t units = units_of(a.m_total, a.G, a.N);
+  const int64_t units = units_of(a.m_total, a.G, a.N, kMx);
   if (units * strips > 2 * kMaxUnits) return GGEMM_E_SHAPE;
-  a.rows = unit_rows(a.m_total, a.N);
+  a.rows = unit_rows(a.m_total, a.N, least_rows(kMx));
   a.units = (int)units;
   a.strips = strips;
   a.lanes = ((a.N / 8 + strips - 1) / strips + 3) / 4 * 4;      // whole blocks of 32 columns
+  const bool few = a.G < ag::kThreads * ag::kPerFew;             // and the last offset
+  const dim3 grid((uint32_t)(units * strips)), sums((uint32_t)((a.N + 63) / 64), (uint32_t)a.G);
   if (a.m_total > 0 && (a.dpre || a.dbias)) {
     const int rc = with_act(act, [&](auto code) {
       constexpr int kAct = decltype(code)::value;
       if constexpr (kMx && kAct == epi::kNone)
         return (int)GGEMM_E_FORMAT;                          // refused before: nothing is read
+      else if (few)
+        hipLaunchKernelGGL((ag::act_backward_kernel<kAct, kMx, ag::kPerFew>), grid, dim3(ag::kThreads), 0, stream, a);
       else
-        hipLaunchKernelGGL((ag::act_backward_kernel<kAct, kMx>), dim3((uint32_t)(units * strips)), dim3(ag::kThreads), 0,
-                           stream, a);
+        hipLaunchKernelGGL((ag::act_backward_kernel<kAct, kMx, ag::kPerMost>), grid, dim3(ag::kThreads), 0, stream, a);
       return (int)hipGetLastError();
     });
     if (rc) return rc;
   }
-  if (a.dbias)
-    hipLaunchKernelGGL(ag::bias_sum_kernel, dim3((uint32_t)((a.N + 63) / 64), (uint32_t)a.G), dim3(ag::kThreads), 0, stream, a);
+  if (a.dbias && few)
+    hipLaunchKernelGGL(ag::bias_sum_kernel<ag::kPerFew>, sums, dim3(ag::kThreads), 0, stream, a);
+  else if (a.dbias)
+    hipLaunchKernelGGL(ag::bias_sum_kernel<ag::kPerMost>, sums, dim3(ag::kThreads), 0, stream, a);
   return (int)hipGetLastError();
 }
 

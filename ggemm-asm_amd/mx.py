@@ -65,10 +65,13 @@ def quantize_mx(x: torch.Tensor, fmt: str = "e2m1", row_align: int | None = None
     dt, width = (torch.float8_e4m3fn, cols) if code == 0 else (torch.uint8, cols // 2)
     q = _padded_empty(x.shape[:-1] + (width,), row_align, dt, dev)
     blocks = -(-cols // BLOCK)
-    scales = torch.empty(x.shape[:-1] + (-(-blocks // 16) * 16,), dtype=torch.uint8, device=dev)[..., :blocks]
+    pitch = -(-blocks // 16) * 16
+    scales = x.new_empty(x.shape[:-1] + (pitch,), dtype=torch.uint8)
+    if pitch != blocks:
+        scales = scales.narrow(-1, 0, blocks)
     if rows:
         _lib.launch("ggemm_mx_quantize", dev, cols, x2.data_ptr(), _IN[x.dtype], rows, cols, _stride(x2), code, q.data_ptr(),
-                    q.stride(-2) if rows > 1 else width, scales.data_ptr(), scales.stride(-2) if rows > 1 else blocks)
+                    q.stride(-2) if rows > 1 else width, scales.data_ptr(), pitch)
     return MXTensor(q, scales)
 
 
@@ -95,7 +98,7 @@ def dequantize_mx(t: MXTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Ten
         raise ValueError(f"the last dimension must stand for a multiple of 16 values, got {cols}")
     q2 = _even_rows(q, 4 if code else 8)
     s2 = scales if scales.dim() == 2 else scales.reshape(-1, scales.shape[-1])
-    out = torch.empty(q.shape[:-1] + (cols,), dtype=dtype, device=q.device)
+    out = q.new_empty(q.shape[:-1] + (cols,), dtype=dtype)
     rows = q2.shape[0]
     if rows:
         _lib.launch("ggemm_mx_dequantize", q.device, cols, q2.data_ptr(), code, rows, cols, _stride(q2), s2.data_ptr(),
@@ -195,7 +198,7 @@ def grouped_gemm_mx_bias_act(a: MXTensor, b: MXTensor, group_offs: torch.Tensor,
         raise RuntimeError("grouped_gemm_mx_bias_act has no gradients: call it under torch.no_grad()")
     if validate:
         _validate_offsets(group_offs, M, mx=False)
-    out = torch.empty((M, width), dtype=torch.bfloat16, device=dev)
+    out = aq.new_empty((M, width), dtype=torch.bfloat16)
     if M == 0:
         return out
     group_offs = group_offs.contiguous()

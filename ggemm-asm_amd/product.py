@@ -8,6 +8,8 @@ bench.py:238-247). Every launch goes through libggemm_vark.so on torch's current
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -203,6 +205,12 @@ def _kept_rows(preact: MXTensor, M: int, N: int, dev):
     return q, preact.scales
 
 
+@functools.lru_cache(maxsize=256)                    # a size, no memory: the call is a twelfth of the whole one's time
+def _workspace(mx: bool, M: int, G: int, N: int) -> int:
+    lib = _lib.load()
+    return (lib.ggemm_mx_act_workspace if mx else lib.ggemm_product_act_workspace)(M, G, N)
+
+
 def bias_act_backward(dout: torch.Tensor, preact: torch.Tensor | MXTensor | None, group_offs: torch.Tensor,
                       activation: str | None = None, *, slope: float = 1.0, limit: float | None = None,
                       shift: float = 0.0, bias_grad: bool = True):
@@ -227,7 +235,7 @@ def bias_act_backward(dout: torch.Tensor, preact: torch.Tensor | MXTensor | None
     kept = None
     if activation is not None and isinstance(preact, MXTensor):
         kept = _kept_rows(preact, M, N, dev)
-        dpre = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        dpre = dout.new_empty((M, N))
     elif activation is not None:
         if preact is None or preact.dtype != torch.bfloat16 or tuple(preact.shape) != (M, N) or preact.device != dev:
             raise ValueError(f"preact must be bf16 [{M}, {N}] on dout's device")
@@ -237,10 +245,9 @@ def bias_act_backward(dout: torch.Tensor, preact: torch.Tensor | MXTensor | None
         preact, dpre = None, None
     G = group_offs.numel() - 1
     src = _rows16(dout)
-    dbias = torch.empty((G, N), dtype=torch.float32, device=dev) if bias_grad else None
+    dbias = dout.new_empty((G, N), dtype=torch.float32) if bias_grad else None
     if M and (bias_grad or dpre is not None):
-        ws = torch.empty(_lib.load().ggemm_product_act_workspace(M, G, N), dtype=torch.float32, device=dev) \
-            if bias_grad else None
+        ws = dout.new_empty(_workspace(kept is not None, M, G, N), dtype=torch.float32) if bias_grad else None
         if kept is not None:
             q, scales = kept
             _lib.launch("ggemm_mx_act_backward", dev, G | N | _stride(src) | _stride(q), src.data_ptr(), q.data_ptr(),

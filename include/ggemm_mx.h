@@ -77,11 +77,15 @@ int32_t ggemm_mx_keep_tile_rows(int32_t G, int32_t N, int32_t K, int32_t stride_
 
 /* ggemm_product_act_backward (ggemm_product.h) from such a z: q and scales as above, or of any strides (scale of row r and
  * block b at scales[r * scale_row + b * scale_block]); stride_q a multiple of 8, q 8-byte aligned. The gradient is
- * that of the values that were kept; a block with scale 255 gives NaN. Workspace: ggemm_product_act_workspace. */
+ * that of the values that were kept; a block with scale 255 gives NaN. With dbias, workspace:
+ * ggemm_mx_act_workspace(...) floats, 16-byte aligned. */
 int ggemm_mx_act_backward(const void* dout, const void* q, const uint8_t* scales, const int64_t* group_offs, int32_t G,
                           int32_t N, int32_t stride_dout, int32_t stride_q, int64_t scale_row, int64_t scale_block,
                           int32_t act, float slope, float limit, float shift, int64_t M_total, void* dpre,
                           int32_t stride_dpre, float* dbias, float* workspace, void* stream);
+
+/* Floats of workspace that ggemm_mx_act_backward needs, whatever group_offs holds. */
+int64_t ggemm_mx_act_workspace(int64_t M_total, int32_t G, int32_t N);
 
 #ifdef __cplusplus
 }
