@@ -283,7 +283,8 @@ def grouped_linear_fp8(x: torch.Tensor, w: torch.Tensor, group_offs: torch.Tenso
     ``weight_cache`` the weight's fp8 copy is reused while the weight is unchanged. With ``scaling``
     (one FP8DelayedScaling per layer) x, w and dy take delayed scaling (module docstring). bias: bf16 / fp32 [G, N],
     with a gradient of its type; ``activation`` and its options as for ``grouped_gemm_fp8_bias_act`` ("swiglu" halves
-    the width). ``checkpoint="mxfp8"`` keeps what the activation's gradient reads in 8 bits instead of 16."""
+    the width). ``checkpoint="mxfp8"`` keeps what the activation's gradient reads in 8 bits instead of 16
+    (without an activation there is nothing to keep)."""
     if checkpoint not in (None, MX8):
         raise ValueError(f"checkpoint must be None or {MX8!r}, got {checkpoint!r}")
     if main_grad is not None:

@@ -162,6 +162,29 @@ def test_gradient(pkg, M, N, lens, activation, options, by_block):
     assert torch.equal(pkg.bias_act_backward(dout, kept, dev_offs, activation, bias_grad=False, **options)[0], dpre)
 
 
+@pytest.mark.parametrize("G", [254, 255, 256, 2047])
+@pytest.mark.parametrize("kept", [True, False])
+def test_gradient_of_many_groups(pkg, G, kept):
+    """Around the number of groups that a thread's one offset is enough for; ones of no rows, decreasing and negative offsets."""
+    gen = torch.Generator().manual_seed(G)
+    M, N = 700, 48
+    z = pkg.quantize_mx(torch.randn((M, N), generator=gen).cuda(), "e4m3")
+    restored = pkg.dequantize_mx(z)
+    dout = torch.randn((M, N), generator=gen).to(torch.bfloat16).cuda()
+    offs = torch.randint(0, M + 1, (G + 1,), generator=gen).sort()[0]
+    for spoil in (False, True):
+        if spoil:
+            offs[G // 3], offs[G // 2], offs[-1] = -5, 0, M - 3
+        dpre, dbias = pkg.bias_act_backward(dout, z if kept else restored, offs.cuda(), "silu")
+        seen = offs.clamp(0, M).cummax(0)[0].tolist()
+        ref, ref_bias, _ = orx.backward(dout.cpu(), restored.cpu(), seen, "silu")
+        factor = restored.cpu().double().abs() + 1
+        terms = dout.cpu().double().abs() * factor
+        assert ((dpre.cpu().double() - ref).abs() <= 1.01 * BF * ref.abs() + 32 * 2.0 ** -23 * terms + 1e-30).all()
+        count = torch.tensor([b - a for a, b in zip(seen, seen[1:])], dtype=torch.float64)[:, None]
+        assert ((dbias.cpu().double() - ref_bias).abs() <= (32 + count) * 2.0 ** -23 * sum_of(terms, seen)).all()
+
+
 def test_gradient_of_views_and_nan_blocks(pkg):
     kept, gen = _random_kept(pkg, 90, 96, 3)
     wide = torch.full((90, 120), 0xFF, dtype=torch.uint8, device="cuda")

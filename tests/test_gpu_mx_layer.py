@@ -27,7 +27,7 @@ def _layer(pkg, T, E, H, I, activation, seed, logits=None):
     return x, logits, pkg.quantize_mx(wu, row_align=128), pkg.quantize_mx(wd, row_align=128), bu, bd, res
 
 
-@pytest.mark.parametrize("T,E,k,H,I", [(1, 4, 2, 64, 32), (5, 8, 3, 160, 96), (77, 4, 4, 2880, 64), (700, 32, 4, 512, 736),
+@pytest.mark.parametrize("T,E,k,H,I", [(1, 4, 2, 64, 32), (5, 8, 3, 160, 96), (77, 4, 4, 2880, 64), (700, 32, 4, 512, 736), (4200, 3, 2, 64, 64),
                                        (3000, 3, 2, 128, 2880)])
 @pytest.mark.parametrize("activation,options", [("swiglu", GATE), ("swiglu", {}), ("gelu", {}), (None, {})])
 @pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])

@@ -93,6 +93,14 @@ def test_keep_validation(pkg, kw, rc):
     assert _keep(pkg.load_library(), **kw) == rc
 
 
+def test_kept_gradient_workspace(pkg):
+    """A row of sums to every unit: units of 8 to 64 rows, a group's last one shorter."""
+    f = pkg.load_library().ggemm_mx_act_workspace
+    for M, G, N, rows in ((1, 1, 16, 8), (5003, 7, 1424, 8), (131072, 32, 5760, 64), (40000, 2047, 2048, 16)):
+        assert f(M, G, N) == (M // rows + min(G, M)) * N
+    assert f(0, 3, 64) == 64 and f(-1, 3, 64) == f(5, 0, 64) == f(5, 2048, 64) == 0
+
+
 def _back(lib, **kw):
     a = dict(dout=FAKE, q=FAKE, s=FAKE, offs=FAKE, G=4, N=64, sd=64, sq=64, sr=2, sb=1, act=1, slope=1.0, limit=7.0, shift=0.0,
              M=100, dpre=FAKE, sdp=64, db=FAKE, ws=FAKE)
