@@ -21,7 +21,8 @@
 // Tiles (mx_capi.hip): 256 x 256 by eight waves of 64 x 128, two stages of 64 or 48 KB, one workgroup to a CU that walks over its
 // tiles, the next one's first stages in flight during an epilogue. Waves of 128 x 128 would read a quarter less of LDS, but
 // with all 256 accumulation registers taken the compiler moves them back and forth (11 ms for the 1.6 of then); 256 x 192 and
-// 256 x 128 tiles take 7 and 11 % more. 128, 64 and 32 rows x 128 columns by four waves, two workgroups to a CU, for launches with fewer rows.
+// 256 x 128 tiles take 7 and 11 % more. 128, 64 and 32 rows x 128 columns by four waves, two workgroups to a CU, for launches
+// with fewer rows.
 //
 // The large ones are bound by power and by the epilogue, which no product runs beside: 131072 x 5760 x 2880 with swiglu takes
 // 1307 us with e2m1 rows, 3.33 PFLOP/s (a library's plain fp4 product of 16384^3 reaches 3.41, instructions alone on random
@@ -300,7 +301,8 @@ __device__ __forceinline__ void store(const v16f (&acc)[MB][NB], const epi::Args
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
       // rows that do not exist are out of the buffer's range, and so are columns by their offset
-      const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(out + row0 * stride_out + oj, 0, 2 * max(rows, 0) * stride_out, kRsrcWord3);
+      const auto rsrc =
+          __builtin_amdgcn_make_buffer_rsrc(out + row0 * stride_out + oj, 0, 2 * max(rows, 0) * stride_out, kRsrcWord3);
       const int to = 8 * c < width - oj ? 2 * (lane / kChunks * stride_out + 8 * c) : (int)kOob;
 #pragma unroll
       for (int i = 0; i < MB; ++i) {

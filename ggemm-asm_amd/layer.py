@@ -1,7 +1,8 @@
 """A whole MoE layer: routing, dispatch, the experts' two FP8 products and the combination.
 
 ``moe_layer_fp8`` is how the package's operators are meant to follow one another, ``moe_layer_mx`` the same on weights kept
-in 4 bits; a model with another order of steps calls them one by one. The reference's harness runs the products alone, on random rows (reference bench.py:196-268).
+in 4 bits; a model with another order of steps calls them one by one. The reference's harness runs the products alone, on
+random rows (reference bench.py:196-268).
 """
 from __future__ import annotations
 
