@@ -269,6 +269,11 @@ class GroupedLinearActFP8(torch.autograd.Function):
         return (dx, dw, None if db is None else db.to(ctx.bias_dtype)) + (None,) * 7
 
 
+def check_checkpoint(checkpoint):
+    if checkpoint not in (None, MX8):
+        raise ValueError(f"checkpoint must be None or {MX8!r}, got {checkpoint!r}")
+
+
 def grouped_linear_fp8(x: torch.Tensor, w: torch.Tensor, group_offs: torch.Tensor,
                        main_grad: torch.Tensor | None = None,
                        weight_cache: FP8WeightCache | None = None,
@@ -285,8 +290,7 @@ def grouped_linear_fp8(x: torch.Tensor, w: torch.Tensor, group_offs: torch.Tenso
     with a gradient of its type; ``activation`` and its options as for ``grouped_gemm_fp8_bias_act`` ("swiglu" halves
     the width). ``checkpoint="mxfp8"`` keeps what the activation's gradient reads in 8 bits instead of 16
     (without an activation there is nothing to keep)."""
-    if checkpoint not in (None, MX8):
-        raise ValueError(f"checkpoint must be None or {MX8!r}, got {checkpoint!r}")
+    check_checkpoint(checkpoint)
     if main_grad is not None:
         if main_grad.dtype != torch.float32 or tuple(main_grad.shape) != (w.shape[0], w.shape[2], w.shape[1]):
             raise ValueError(f"main_grad must be fp32 [G, K, N] = {[w.shape[0], w.shape[2], w.shape[1]]}")

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from ._tensors import MXTensor, mx_columns, tracked
-from .autograd import FP8DelayedScaling, FP8WeightCache, grouped_linear_fp8
+from .autograd import FP8DelayedScaling, FP8WeightCache, check_checkpoint, grouped_linear_fp8
 from .moe import combine_tokens, dispatch_tokens, plan_dispatch, route_experts
 from .mx import dispatch_mx, grouped_gemm_mx_bias_act, quantize_mx
 from .product import _rows16, grouped_gemm_fp8_bias_act
@@ -50,6 +50,7 @@ def moe_layer_fp8(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, w_d
         raise ValueError(f"logits must be [{x.shape[0]}, {w_up.shape[0]}]")
     if w_down.shape[0] != w_up.shape[0] or w_down.shape[1] != x.shape[1]:
         raise ValueError("w_up and w_down hold the same experts, [E, N, H] and [E, H, I]")
+    check_checkpoint(checkpoint)
     weights, experts = route_experts(logits, top_k, **(routing or {}))
     plan = plan_dispatch(experts, w_up.shape[0])
     gate = {"slope": slope, "limit": limit, "shift": shift}

@@ -159,6 +159,15 @@ def test_refusals(pkg):
         pkg.grouped_gemm_mx_bias_act(pkg.MXTensor(q, s), b, offs)
 
 
+@pytest.mark.parametrize("grad", [True, False])
+def test_layer_refuses_an_unknown_checkpoint(pkg, grad):
+    """Before anything else, on the path that keeps none too."""
+    x = torch.zeros((2, 64), dtype=torch.bfloat16)
+    w = torch.zeros((4, 64, 64), dtype=torch.bfloat16, requires_grad=grad)
+    with pytest.raises(ValueError, match="checkpoint"):
+        pkg.moe_layer_fp8(x, torch.zeros((2, 4)), w, w, 1, activation="silu", checkpoint="mxfp4")
+
+
 # --------------------------------------------------------------------------- the oracle
 
 @pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
