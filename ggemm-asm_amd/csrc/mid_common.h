@@ -19,7 +19,7 @@ constexpr uint32_t kOob = 0x7fff0000u;   // buffer offset past every num_records
 // Tile of workgroup b: the hardware deals workgroups round robin over the 8 XCDs; runs of kXcdRun
 // consecutive tiles go to one XCD, whose L2 then holds the operand rows that they share. The grid is
 // a multiple of 8 kXcdRun.
-__device__ __forceinline__ int tile_of_block(int b) {
+__host__ __device__ __forceinline__ constexpr int tile_of_block(int b) {
   const int run = kXcds * kXcdRun;
   const int r = b % run;
   return b - r + (r % kXcds) * kXcdRun + r / kXcds;

@@ -151,7 +151,7 @@ int launch(const mx::Args& a, const epi::Args& e, int tile, int cus, hipStream_t
   auto run = [&](auto cfg) {
     using C = decltype(cfg);
     const uint32_t blocks = tiles(C::BM, C::BN);
-    const uint32_t grid = C::kWalk && a.K > C::KS ? std::min<uint32_t>(blocks, cus) : blocks;
+    const uint32_t grid = C::kWalk && a.K > C::KS ? mx::walk_grid((int)blocks, cus) : blocks;
     hipLaunchKernelGGL((mx_product_kernel<kAct, kA8, C>), dim3(grid), dim3(C::NT), 0, stream, a, e, (int)grid, (int)blocks);
   };
   if (tile == 16) {

@@ -351,8 +351,15 @@ __device__ __forceinline__ void store(const v16f (&acc)[MB][NB], const epi::Args
   }
 }
 
-// grid: workgroups of the launch; blocks: what it would have with one for each tile. A grid of fewer needs tiles of two
-// stages at least: loads are asked for two stages ahead, which may not reach past the next tile.
+// Workgroups of a launch whose tiles are walked over, of `blocks` with one for each: as many as CUs, but a multiple of the XCDs,
+// so that the tiles of block, block + grid, .. rise (tile_of_block) and a walk may end at the first that is not there.
+__host__ __device__ constexpr int walk_grid(int blocks, int cus) {
+  const int even = cus < kXcds ? kXcds : cus - cus % kXcds;
+  return blocks < even ? blocks : even;
+}
+
+// grid: workgroups of the launch; blocks: what it would have with one for each tile. A grid of fewer (walk_grid) needs tiles of
+// two stages at least: loads are asked for two stages ahead, which may not reach past the next tile.
 template <int kAct, bool kA8, typename C>
 __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, const epi::Args& e, int grid, int blocks) {
   const int tid = threadIdx.x, lane = tid & 63;
@@ -562,7 +569,7 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
     store<kAct, C::MB, C::NB, C::Line>(acc, e, a.out, a.stride_out, tile.g, a.N, tile.row0 + 32 * C::MB * wm,
                               tile.rows - 32 * C::MB * wm, tile.n0 + 32 * C::NB * wn, lane,
                                        lines, bias_at);
-    if (next.rows == 0) break;
+    if (next.rows == 0) break;                                 // nor are those that follow: tiles rise along a walk
     tile = next;
     fetch_bias(tile);
     block += grid;

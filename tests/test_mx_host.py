@@ -3,6 +3,7 @@ kernel, and the oracle against other ways to say the same."""
 import math
 import os
 import re
+import subprocess
 
 import pytest
 import torch
@@ -124,6 +125,45 @@ def test_choice_of_a_kernel(pkg):
         assert [mx.tile_rows(fmt, 32, 5760, 2880, m) for m in (1, 256, 2048, 131072)] == [16, 32, 128, 256]
         assert all(mx.tile_rows(fmt, G, N, K, M) in mx.TILES[1:] for G in (1, 64, 2047) for N in (16, 5760) for K in (32, 8192)
                    for M in (1, 100, 10 ** 6))
+
+
+WALK = """
+#include <cstdio>
+#include <cstdlib>
+#include <vector>
+#include "mx_gemm.h"
+int main(int argc, char** argv) {
+  for (int i = 1; i + 1 < argc; i += 2) {
+    const int cus = std::atoi(argv[i]), tiles = std::atoi(argv[i + 1]);
+    const int run = ggemm::kXcds * ggemm::mid::kXcdRun, blocks = (tiles + run - 1) / run * run;
+    const int grid = ggemm::mx::walk_grid(blocks, cus);
+    std::vector<int> seen(tiles);
+    for (int first = 0; first < grid; ++first)
+      for (int b = first; b < blocks; b += grid) {
+        const int t = ggemm::mid::tile_of_block(b);
+        if (t >= tiles) break;
+        ++seen[t];
+      }
+    int once = 0;
+    for (int n : seen) once += n == 1;
+    std::printf("%d\\n", grid >= 1 && once == tiles);
+  }
+}
+"""
+
+
+def test_walks_take_every_tile_on_any_number_of_cus(pkg, tmp_path):
+    """The walk of the 256-row tiles in gemm_body: block, block + grid, .., up to the first that has no tile."""
+    from ggemm_asm_amd import build
+    if not os.path.exists(build.hipcc()):
+        pytest.skip("hipcc not available")
+    source, program = tmp_path / "walk.hip", tmp_path / "walk"
+    source.write_text(WALK)
+    subprocess.run([build.hipcc(), "-std=c++17", "--cuda-host-only", f"--offload-arch={build.ARCH}", "-I", build.CSRC, str(source),
+                    "-o", str(program)], check=True, capture_output=True)
+    cases = [(cus, tiles) for cus in (1, 7, 8, 32, 38, 64, 128, 228, 252, 256, 304) for tiles in (1, 255, 256, 257, 300, 700, 5000)]
+    got = subprocess.run([str(program), *(str(v) for case in cases for v in case)], check=True, capture_output=True, text=True)
+    assert [case for case, ok in zip(cases, got.stdout.split()) if ok != "1"] == [] and len(got.stdout.split()) == len(cases)
 
 
 # --------------------------------------------------------------------------- the torch ops
