@@ -23,10 +23,9 @@ inline int64_t mid_tiles(int rows, int G, int N, int64_t M_total) {
 // tiles, 16 more than 10 %: 13 groups, 5788 rows, N = K = 2880 75 us, 51 on the wide tiles; 15, 7007, N = 2560, K
 // = 5760 112, 85. With this rule 27 and 9 are, and 7 lose a gain of 20 % or more. For up to four groups it lost
 // as often as it gained.
-// extra: us that a large tile's epilogue takes with nothing beside it.
-inline bool rows128_faster(int N, double M, double g, double stages, double mem, bool wide, int cus, double extra) {
+// extra: us that a large tile's epilogue takes with nothing beside it; tn: the large tiles' columns.
+inline bool rows128_faster(int N, double M, double g, double stages, double mem, bool wide, int tn, int cus, double extra) {
   constexpr int kRun = ggemm::mid::kXcdRun;
-  const int tn = wide ? 320 : ggemm::wide_tiles(N, false) ? 384 : 320;
   double mid = 0, big = 0;
   for (const bool even : {true, false}) {
     auto tiles = [&](double h, double w) {
@@ -56,21 +55,21 @@ inline bool rows128_faster(int N, double M, double g, double stages, double mem,
 // 32: 256 rows 149 -> 95 (64), 3072 rows 148 -> 118 (128), 6144 rows 162, mid 182 (stays); N = K = 2880,
 // G = 4: 512 rows 38 -> 14, 8192 rows 83 -> 75, 16384 rows 132, mid 153 (stays); N = 2048, K = 1424, G =
 // 7: 512 rows 25 -> 9, 5003 rows 28, mid 31 (stays); N = 512, K = 1024, G = 8: 100000 rows 92 -> 77.
-// Products with an epilogue give two more numbers: extra, as above, and how far below the 128-row tiles' estimate that
-// of 64 rows has to be (product_capi.hip).
+// Products with an epilogue give more: extra, as above, how far below the 128-row tiles' estimate that of 64 rows has to be
+// (product_launch.h), and whether z is kept in 8 bits, with which the 512-thread kernel's tiles are 384 wide (persistent_entry).
 inline int mid_preferred(int G, int N, int K, int scm, int64_t M_total, bool wide, int cus, double extra = 0,
-                         double below = 0.97) {
+                         double below = 0.97, bool kept8 = false) {
   if (G > ggemm::mid::kMaxGroups || M_total <= 0 || mid_tiles(64, G, N, M_total) > (1 << 22)) return 0;
   if ((int64_t)scm * 2 * 64 >= (int64_t)ggemm::nt::kOob) return 0;   // a wave's rows of C: 32-bit offsets
   const double M = (double)M_total, g = G < M ? G : M;
   const double stages = (K + 127) / 128 + 2;                          // two more for the tile's ends
   const double mem = (M * K + g * N * K + 2 * M * N) / 5.1e6;
   auto tiles = [&](double h, double w) { return std::max(g, M / h + g / 2) * std::ceil(N / w); };
+  const int tn = !wide && (kept8 || ggemm::wide_tiles(N, false)) ? 384 : 320;
   double big;
   if (wide) {
-    big = 4 + std::ceil(tiles(256, 320) / cus) * (stages * 1.85 + extra);
+    big = 4 + std::ceil(tiles(256, tn) / cus) * (stages * 1.85 + extra);
   } else {
-    const int tn = ggemm::wide_tiles(N, false) ? 384 : 320;
     big = 4 + std::ceil(tiles(192, tn) / cus) * (stages * (tn == 384 ? 1.75 : 1.58) + extra) + 0.2 * mem;
   }
   const double f64 = tiles(64, 128) / (2 * cus), f128 = tiles(128, 128) / (2 * cus);
@@ -78,7 +77,7 @@ inline int mid_preferred(int G, int N, int K, int scm, int64_t M_total, bool wid
   const double c128 = 4 + std::max(1.0, f128) * stages * (0.64 + 0.42 * std::min(1.0, f128)) + 0.3 * mem;
   if (std::min(c64, c128) >= 0.92 * big) return 0;   // near the line the estimate is a few per cent off
   if (c64 < below * c128) return 64;
-  return g <= 4 || rows128_faster(N, M, g, (K + 127) / 128, mem, wide, cus, extra) ? 128 : 0;
+  return g <= 4 || rows128_faster(N, M, g, (K + 127) / 128, mem, wide, tn, cus, extra) ? 128 : 0;
 }
 
 }  // namespace host

@@ -147,7 +147,9 @@ bool few_preferred(const nt::Args& a, int64_t g, int64_t cus) {
 // kept, while the mid tiles' runs beside other workgroups' products; and 64 rows have to be 10 % better. Of 70 drawn
 // launches (1 to 40 groups, 16 to 131072 rows, features 64 to 5760) with bias, swiglu, swiglu and z, gelu and residual,
 // the choice was 1.012, 1.009, 1.008 and 1.016 times the best of the three kernels in the mean, 1.028, 1.020, 1.044 and
-// 1.023 by the plain product's numbers.
+// 1.023 by the plain product's numbers. With z in 8 bits the 512-thread kernel's tiles are 384 columns wide and cost 6 us each:
+// of 140 drawn launches, 110 of them near the line, the choice was 1.016 times the best (1.019 by 12 us and bf16 z's tiles);
+// 14998 rows of 8 groups, 1040 x 3696, swiglu 73 us (101 on 128-row tiles).
 Choice choose(const nt::Args& a, const epi::Args& e, int act, int cus) {
   const int64_t run = ggemm::kXcds * ggemm::mid::kXcdRun, g = std::min<int64_t>(a.G, a.m_total);
   auto runs = [&](int64_t tiles) { return (tiles + run - 1) / run * run; };
@@ -157,7 +159,8 @@ Choice choose(const nt::Args& a, const epi::Args& e, int act, int cus) {
     return {narrow ? Kernel::kFew16 : Kernel::kFew32, 0, runs(row_tiles * ((a.N + bn - 1) / bn))};
   }
   const int wide = wide_mode(a, e, act);
-  const int mid = mid_preferred(a.G, a.N, a.K, a.stride_cm, a.m_total, wide != 0, cus, e.pre || e.q8 ? 12 : 3, 0.9);
+  const int extra = e.q8 && !wide ? 6 : e.pre || e.q8 ? 12 : 3;
+  const int mid = mid_preferred(a.G, a.N, a.K, a.stride_cm, a.m_total, wide != 0, cus, extra, 0.9, e.q8 != nullptr);
   if (mid) return {mid == 64 ? Kernel::kMid64 : Kernel::kMid128, 0, runs(mid_tiles(mid, a.G, a.N, a.m_total))};
   return {wide ? Kernel::kWide : Kernel::k512, wide, 0};
 }
