@@ -72,6 +72,14 @@ def moe_layer_fp8(x: torch.Tensor, logits: torch.Tensor, w_up: torch.Tensor, w_d
     return combine_tokens(y, plan, weights, residual)
 
 
+def _copied_first(rows: int, features: int) -> bool:
+    """Whether the copied rows are quantized, one launch fewer, or the tokens' blocks copied, a quarter (e2m1) or half of the
+    bytes. The crossing lies at 2^25 values of the copied rows, whatever their features, top_k and format. Us so and by
+    dispatch_mx, e4m3, top 4: 512 features 65536 rows 32 and 34, 131072 61 and 43; 2880 features 8192 rows 25 and 38, 16384 45 and
+    39; 8192 features 4096 rows 33 and 34, 8192 62 and 34. Top 1: 65536 rows of 512 41 and 42, 4096 of 8192 40 and 36."""
+    return rows * features <= 1 << 25
+
+
 def moe_layer_mx(x: torch.Tensor, logits: torch.Tensor, w_up: MXTensor, w_down: MXTensor, top_k: int, *,
                  bias_up: torch.Tensor | None = None, bias_down: torch.Tensor | None = None,
                  activation: str | None = "swiglu", slope: float = 1.0, limit: float | None = None, shift: float = 0.0,
@@ -100,9 +108,7 @@ def moe_layer_mx(x: torch.Tensor, logits: torch.Tensor, w_up: MXTensor, w_down: 
         raise RuntimeError("moe_layer_mx has no gradients: call it under torch.no_grad()")
     weights, chosen = route_experts(logits, top_k, **(routing or {}))
     plan = plan_dispatch(chosen, experts)
-    # few rows: one launch fewer; many: a quarter (e2m1) or half of the bytes to copy top_k times. Of 2880 values, top 4: 4096
-    # rows 38 us by dispatch_mx, 24 so; 16384 rows 44 and 47; 131072 rows 159 and 323
-    if plan.slots.numel() <= 8192:
+    if _copied_first(plan.slots.numel(), hidden):
         rows = quantize_mx(dispatch_tokens(x, plan), fmt, _LINE)
     else:
         rows = dispatch_mx(quantize_mx(x, fmt), plan)

@@ -154,3 +154,22 @@ def test_refusals(pkg):
     for bad in (pkg.MXTensor(wu.q, wu.scales), pkg.MXTensor(wu.q[0, :6], wu.scales[0, :6, :1])):
         with pytest.raises(ValueError):
             pkg.dispatch_mx(bad, pkg.plan_dispatch(torch.zeros((6, 1), dtype=torch.int32, device="cuda"), 4))
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+def test_both_orders_of_copying_and_quantizing(pkg, fmt, monkeypatch):
+    """Rows enough that the tokens' blocks are copied, tokens that go nowhere among them: the bits of the other order."""
+    T, E, k, H = 3000, 8, 4, 2880
+    logits = torch.randn((T, E), generator=torch.Generator().manual_seed(7))
+    logits[1::97] = -math.inf
+    x, logits, wu, wd, bu, bd, res = _layer(pkg, T, E, H, 64, "swiglu", 7, logits.cuda())
+    x[1::97] = math.nan
+    assert not pkg.layer._copied_first(T * k, H)
+
+    def run():
+        return pkg.moe_layer_mx(x, logits, wu, wd, k, bias_up=bu, bias_down=bd, residual=res, fmt=fmt, **GATE)
+
+    out = run()
+    assert torch.isfinite(out).all() and torch.equal(out[1::97], res[1::97])
+    monkeypatch.setattr(pkg.layer, "_copied_first", lambda *_: True)
+    assert torch.equal(out, run())
