@@ -14,7 +14,7 @@ import pytest
 import torch
 
 from oracle import mx_oracle as omx, product_oracle as orx
-from test_gpu_product import GATE, KERNELS, SHAPES, _inputs, _strided
+from test_gpu_product import GATE, KERNELS, SHAPES, _check, _inputs, _strided
 
 pytestmark = pytest.mark.gpu
 
@@ -305,3 +305,83 @@ def test_captured(pkg):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(c, e) for c, e in zip(captured, step()))
+
+
+# units of 16, 32 and 64 rows: a thread goes through its eight rows in flight more than once, the last time with fewer
+LONG = [(12000, 16, [3001, 0, 1, 8990, 5]), (25000, 32, [7, 24950, 13]), (50000, 64, [20003, 1, 29989])]
+
+
+@pytest.mark.parametrize("M,rows,lens", LONG)
+@pytest.mark.parametrize("activation,options", [("silu", {}), ("swiglu", GATE)])
+def test_gradient_of_long_units(pkg, M, rows, lens, activation, options):
+    """dpre the bits of the bf16 path. The sums against 64 bits: a term is off by 32 ulps of its factors, a sum of n terms by
+    n 2^-24 of their magnitudes."""
+    N, G = 5760, len(lens)
+    assert pkg.load_library().ggemm_mx_act_workspace(M, G, N) == (M // rows + G) * N
+    gen = torch.Generator(device="cuda").manual_seed(M)
+    kept = pkg.quantize_mx(torch.randn((M, N), generator=gen, device="cuda") * 3, "e4m3")
+    wide = torch.empty((kept.scales.shape[1], M), dtype=torch.uint8, device="cuda")
+    kept = pkg.MXTensor(kept.q, wide.copy_(kept.scales.t()).t())
+    width = N // 2 if activation == "swiglu" else N
+    dout = torch.randn((M, width), generator=gen, device="cuda").to(torch.bfloat16)
+    offs = [0]
+    for n in lens:
+        offs.append(offs[-1] + n)
+    dev_offs = torch.tensor(offs).cuda()
+    dpre, dbias = pkg.bias_act_backward(dout, kept, dev_offs, activation, **options)
+    restored = pkg.dequantize_mx(kept)
+    assert torch.equal(dpre, pkg.bias_act_backward(dout, restored, dev_offs, activation, **options)[0])
+    assert not dpre[offs[-1]:].any()
+    for g, (lo, hi) in enumerate(zip(offs, offs[1:])):
+        z, d = restored[lo:hi].double(), dout[lo:hi].double()
+        d = d.repeat_interleave(2, 1) if activation == "swiglu" else d
+        terms = d * orx.act_grad(z, activation, **options)
+        assert ((dpre[lo:hi].double() - terms).abs() <= 1.01 * BF * terms.abs() + 32 * 2.0 ** -23 * d.abs() * _factor(z, activation, options) + 1e-30).all()
+        n = hi - lo
+        err = (2.0 ** -24 * n * terms.abs() + 32 * 2.0 ** -23 * d.abs() * _factor(z, activation, options)).sum(0)
+        assert ((dbias[g].double() - terms.sum(0)).abs() <= err).all()
+
+
+def _factor(z, activation, options):
+    """How large the factors are that a term is made of."""
+    z = z.abs() + 1
+    if activation != "swiglu":
+        return z
+    pair = torch.maximum(z[:, 0::2], z[:, 1::2]) + options.get("shift", 0.0)
+    return (pair * pair).repeat_interleave(2, 1) * options.get("slope", 1.0)
+
+
+# q and the gradient's rows past 2^32 bytes, by the tiles of 128, 192 and 256 rows; the last group's rows against the oracle
+@pytest.mark.parametrize("N,K,activation,options,residual,rows",
+                         [(5120, 128, "swiglu", GATE, False, 128), (5136, 1088, "gelu", {}, True, 192), (5120, 1088, "swiglu", GATE, False, 256)])
+def test_kept_rows_past_32_bits(pkg, N, K, activation, options, residual, rows):
+    M, last = 900000, 300
+    width = N // 2 if activation == "swiglu" else N
+    code = {"gelu": 2, "swiglu": 3}[activation]
+    assert pkg.load_library().ggemm_mx_keep_tile_rows(2, N, K, K, K, width, N, code, int(residual), M, 256) == rows
+    a, b, sa, sb, _, gen = _inputs(last, N, K, [0, last], 3)
+    full = torch.zeros((M, K), dtype=torch.uint8, device="cuda")
+    full[-last:] = a.view(torch.uint8).cuda()
+    bias = torch.randn((2, N), generator=gen)
+    tail = torch.randn((last, width), generator=gen).to(torch.bfloat16)
+    res = None
+    if residual:
+        res = torch.zeros((M, width), dtype=torch.bfloat16, device="cuda")
+        res[-last:] = tail.cuda()
+    offs = torch.tensor([0, M - last, M]).cuda()
+    out, kept = pkg.grouped_gemm_fp8_bias_act(full.view(a.dtype), b.cuda(), torch.tensor(sa).cuda(), torch.tensor(sb).cuda(), offs,
+                                              bias.cuda(), activation, res, keep_preact="mxfp8", **options)
+    del full, res
+    z, ref, size = orx.product(a, b, sa * sb, [0, 0, last], bias, activation, tail if residual else None, **options)
+    part = pkg.MXTensor(kept.q[-last:], kept.scales[-last:])
+    _check_kept(pkg.MXTensor(part.q.cpu(), part.scales.cpu()), z, size)
+    _check(out[-last:].cpu().double(), None, z, ref, size, activation, options, tail.double().abs() if residual else torch.zeros_like(ref))
+    # every row before has the bias of its group alone: the same bytes all over
+    assert (kept.q[:-last].view(torch.uint8) == kept.q[0].view(torch.uint8)).all() and (kept.scales[:-last] == kept.scales[0]).all()
+    dout = torch.zeros_like(out)
+    dout[-last:] = torch.randn((last, width), generator=gen).to(torch.bfloat16).cuda()
+    dpre, dbias = pkg.bias_act_backward(dout, kept, offs, activation, **options)
+    few, few_bias = pkg.bias_act_backward(dout[-last:], part, torch.tensor([0, 0, last]).cuda(), activation, **options)
+    assert torch.equal(dpre[-last:], few) and not dpre[:-last].any() and not dbias[0].any()
+    # the same terms in units of other lengths: each sum off by n 2^-24 of their magnitudes, known from their rounding to bf16
+    assert ((dbias[1].double() - few_bias[1].double()).abs() <= 2 * last * 2.0 ** -24 * (1 + BF) * few.double().abs().sum(0)).all()
