@@ -348,3 +348,55 @@ def test_past_32_bit_offsets(pkg):
         for g, lo in ((0, 0), (599, 20)):
             z, ref, size = omx.product(a64[lo:lo + 20], omx.decode(q[g:g + 1], s[g:g + 1]), "e2m1", [0, 20], None, None, None)
             _check(out[lo:lo + 20].double(), z, ref, size, None, {}, torch.zeros_like(ref))
+
+
+# more tiles of 256 rows than CUs, so that workgroups walk over them: K of two and of three stages of either format, the last one
+# whole, half full or of one block
+@pytest.mark.parametrize("K", [160, 256, 288, 384, 512, 544, 768])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_walks_of_few_stages(pkg, fmt, K):
+    M, N, lens = 20000, 2896, [256, 19001, 0, 700]
+    a, b, offs, gen = _case(M, N, K, lens, fmt, K)
+    da, db = (pkg.MXTensor(_laid_out(q, 0), _laid_out(s, 0)) for q, s in (a, b))
+    bias = torch.randn((len(lens), N), generator=gen).cuda()
+    out = pkg.grouped_gemm_mx_bias_act(da, db, torch.tensor(offs).cuda(), bias, zero_tail=True, tile=256)
+    z, ref, size = omx.product(omx.decode(*da), omx.decode(*db), fmt, offs, bias, None, None)
+    _check(out.double(), z, ref, size, None, {}, torch.zeros_like(ref))
+    assert not out[offs[-1]:].any()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("activation,options,dtype,residual", [("gelu", {}, torch.float32, True), ("silu", {}, None, True),
+                                                               ("swiglu", GATE, torch.float32, True), (None, {}, torch.float32, False)])
+def test_walks_with_every_operand(pkg, fmt, activation, options, dtype, residual):
+    """A later tile's bias comes into the place of the last one's (for e2m1 of its results too) and its residual is read while the
+    next stages are in flight."""
+    M, N, K, lens = LARGE[1]
+    a, b, offs, gen = _case(M, N, K, lens, fmt, 21)
+    da, db = (pkg.MXTensor(_laid_out(q, 0), _laid_out(s, 0)) for q, s in (a, b))
+    bias = None if dtype is None else torch.randn((len(lens), N), generator=gen).to(dtype).cuda()
+    res = torch.randn((M, N // 2 if activation == "swiglu" else N), generator=gen).bfloat16().cuda() if residual else None
+    out = pkg.grouped_gemm_mx_bias_act(da, db, torch.tensor(offs).cuda(), bias, activation, res, zero_tail=True, tile=256, **options)
+    z, ref, size = omx.product(omx.decode(*da), omx.decode(*db), fmt, offs, bias, activation, res, **options)
+    _check(out.double(), z, ref, size, activation, options, torch.zeros_like(ref) if res is None else res.double().abs())
+    assert not out[offs[-1]:].any()
+
+
+def test_rows_past_32_bit_offsets(pkg):
+    """Rows of a (e4m3), of the residual and of the result past 2^32 bytes, by every tile."""
+    M, N, K, last = 900000, 2560, 4800, 300
+    a, b, _, gen = _case(last, N, K, [0, last], "e4m3", 16)
+    q = torch.zeros((M, K), dtype=torch.uint8, device="cuda")
+    s = torch.full((M, 160), 127, dtype=torch.uint8, device="cuda")[:, :K // 32]
+    q[-last:], s[-last:] = a[0].view(torch.uint8).cuda(), a[1].cuda()
+    tail = torch.randn((last, N), generator=gen).bfloat16()
+    res = torch.zeros((M, N), dtype=torch.bfloat16, device="cuda")
+    res[-last:] = tail.cuda()
+    bias = torch.randn((2, N), generator=gen)
+    db = pkg.MXTensor(_laid_out(b[0], 0), _laid_out(b[1], 0))
+    z, ref, size = omx.product(omx.decode(*a), omx.decode(*b), "e4m3", [0, 0, last], bias, None, tail)
+    for tile in (16, 32, 64, 128, 256):
+        out = pkg.grouped_gemm_mx_bias_act(pkg.MXTensor(q.view(torch.float8_e4m3fn), s), db, torch.tensor([0, M - last, M]).cuda(), bias.cuda(),
+                                           None, res, tile=tile)
+        _check(out[-last:].cpu().double(), z, ref, size, None, {}, tail.double().abs())
+        assert (out[:-last] == bias[0].bfloat16().cuda()).all()
