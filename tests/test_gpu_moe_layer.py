@@ -126,3 +126,14 @@ def test_example_trains(pkg, monkeypatch):
                                       "--inner", "64", "--steps", "4"])
     losses = moe_layer.main()
     assert losses[-1] < losses[0]
+
+
+@pytest.mark.parametrize("hidden,inner", [(144, 64), (64, 144), (160, 96)])
+def test_example_runs_at_any_size_of_the_layer(pkg, monkeypatch, capsys, hidden, inner):
+    """Multiples of 16 that are none of 32 too, which 4-bit weights do not take."""
+    monkeypatch.syspath_prepend(os.path.join(ROOT, "examples"))
+    import moe_layer
+    monkeypatch.setattr(sys, "argv", ["moe_layer.py", "--tokens", "50", "--experts", "4", "--top-k", "2", "--hidden", str(hidden),
+                                      "--inner", str(inner), "--steps", "1"])
+    moe_layer.main()
+    assert ("weights in 4 bits, " in capsys.readouterr().out) == (hidden % 32 == inner % 32 == 0)
