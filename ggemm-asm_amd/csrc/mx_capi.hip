@@ -183,7 +183,7 @@ int validate(const mx::Args& a, const epi::Args& e, int fmt, int act, int bias_d
   const int64_t chunk = (int64_t)(a.K + 511) / 512 * 16, bytes_a = fmt == GGEMM_MX_E4M3 ? a.K : a.K / 2;
   const int64_t sa = strides[0], sas = strides[1], sbg = strides[2], sbn = strides[3], sbsg = strides[4], sbsn = strides[5];
   if (sa < bytes_a || sas < chunk || sbn < a.K / 2 || sbsn < chunk) return GGEMM_E_STRIDE;
-  if (a.G > 1 && (sbg < (a.N - 1) * sbn + a.K / 2 || sbsg < a.N * sbsn)) return GGEMM_E_STRIDE;
+  if (a.G > 1 && (sbg < (a.N - 1) * sbn + a.K / 2 || sbsg < (a.N - 1) * sbsn + chunk)) return GGEMM_E_STRIDE;
   for (int64_t s : strides)
     if (s % 16) return GGEMM_E_STRIDE;
   // 32-bit buffer offsets of a tile's 256 rows

@@ -400,3 +400,17 @@ def test_rows_past_32_bit_offsets(pkg):
                                            None, res, tile=tile)
         _check(out[-last:].cpu().double(), z, ref, size, None, {}, tail.double().abs())
         assert (out[:-last] == bias[0].bfloat16().cuda()).all()
+
+
+@pytest.mark.parametrize("tile", [16, 32, 64, 128, 256])
+def test_groups_that_follow_the_last_row_at_once(pkg, tile):
+    """Scales of a group whose rows are 64 bytes apart, the next group 16 bytes after the last one: read where they are."""
+    a, b, offs, _ = _case(40, 48, 480, [25, 15], "e4m3", 22)
+    da, db = (pkg.MXTensor(_laid_out(q, 0), _laid_out(s, 0)) for q, s in (a, b))
+    pitch, group = 64, 47 * 64 + 16
+    buffer = torch.full((2 * group,), 255, dtype=torch.uint8, device="cuda")
+    tight = buffer.as_strided((2, 48, 15), (group, pitch, 1))
+    tight.copy_(db.scales)
+    dev_offs = torch.tensor(offs).cuda()
+    want = pkg.grouped_gemm_mx_bias_act(da, db, dev_offs, tile=tile)
+    assert torch.equal(want, pkg.grouped_gemm_mx_bias_act(da, pkg.MXTensor(db.q, tight), dev_offs, tile=tile))

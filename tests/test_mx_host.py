@@ -77,6 +77,14 @@ def test_product_validation(pkg, kw, rc):
     assert _product(pkg.load_library(), **kw) == rc
 
 
+@pytest.mark.parametrize("kw,ok", [(dict(sbsn=32, sbsg=63 * 32 + 16), True), (dict(sbsn=32, sbsg=63 * 32), False),
+                                   (dict(sbn=48, sbg=63 * 48 + 32), True), (dict(sbn=48, sbg=63 * 48 + 16), False)])
+def test_product_takes_groups_that_follow_the_last_row_at_once(pkg, kw, ok):
+    """A group's last row of scales need not be as far from the next group as rows from each other, as for values."""
+    rc = _product(pkg.load_library(), **kw, M=0)
+    assert (rc != -3) is ok
+
+
 def _keep(lib, **kw):
     a = dict(a=FAKE, b=FAKE, out=FAKE, q=FAKE, s=FAKE, sa=FAKE, sb=FAKE, bias=FAKE, bdt=0, res=FAKE, offs=FAKE, G=4, N=64, K=32,
              sam=32, sbg=2048, sbn=32, so=64, sq=64, blk=100, sr=64, act=1, slope=1.0, limit=7.0, shift=0.0, M=100, tail=0)
