@@ -32,8 +32,8 @@ it before every build).
 """
 from __future__ import annotations
 
+import argparse
 import os
-import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 OUT = os.path.join(HERE, "vark_wide_asm.inc")
@@ -1610,4 +1610,6 @@ def main(path=OUT):
 
 
 if __name__ == "__main__":
-    print(f"{main(sys.argv[1] if len(sys.argv) > 1 else OUT)} instructions and labels")
+    ap = argparse.ArgumentParser(description="Writes vark_wide_asm.inc.")
+    ap.add_argument("path", nargs="?", default=OUT)
+    print(f"{main(ap.parse_args().path)} instructions and labels")

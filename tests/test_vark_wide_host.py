@@ -26,6 +26,8 @@ layout and for LDS bank conflicts.
 import importlib.util
 import os
 import re
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -919,3 +921,8 @@ def test_epilogue_joint_region_ordering(cfg, wave):
         if blk + 2 < c.bm:
             nxt = writes[4 * (blk + 2)]
             assert any(x[0] == "barrier" and r[-1][2] < x[2] < nxt[2] for x in seq)
+
+
+def test_the_generator_takes_no_option_for_a_path(tmp_path):
+    r = subprocess.run([sys.executable, os.path.abspath(GEN.__file__), "--help"], cwd=tmp_path, capture_output=True, text=True)
+    assert r.returncode == 0 and "usage" in r.stdout and os.listdir(tmp_path) == []
