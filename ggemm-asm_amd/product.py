@@ -149,7 +149,8 @@ def grouped_gemm_fp8_bias_act(a: torch.Tensor, b: torch.Tensor, a_scale: torch.T
     on the host first (a sync).
 
     Differentiable by bias and residual (``grouped_linear_fp8`` is by the activations and weights too); the value before
-    the activation is then kept for the bias' gradient, and a ``preact`` that is returned carries no gradient itself."""
+    the activation is then kept for the bias' gradient, in 8 bits with ``keep_preact="mxfp8"``, else in bf16, and the
+    gradient is taken at what is kept. A ``preact`` that is returned carries no gradient itself."""
     if a.dim() != 2 or b.dim() != 3:
         raise ValueError("a must be 2-D [M, K] and b 3-D [G, N, K]")
     if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
