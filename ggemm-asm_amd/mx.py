@@ -175,7 +175,7 @@ def grouped_gemm_mx_bias_act(a: MXTensor, b: MXTensor, group_offs: torch.Tensor,
         raise ValueError("a must be 2-D [M, K] and b 3-D [G, N, K]")
     dev = aq.device
     _on_gpu(aq, "the product")
-    _check_offs(group_offs, dev)
+    group_offs = _check_offs(group_offs, dev)
     M, (G, N) = aq.shape[0], bq.shape[:2]
     if G != group_offs.numel() - 1:
         raise ValueError(f"b holds {G} groups, group_offs {group_offs.numel() - 1}")
@@ -201,7 +201,6 @@ def grouped_gemm_mx_bias_act(a: MXTensor, b: MXTensor, group_offs: torch.Tensor,
     out = aq.new_empty((M, width), dtype=torch.bfloat16)
     if M == 0:
         return out
-    group_offs = group_offs.contiguous()
     if bias is not None:
         bias = bias.contiguous()
         if bias.data_ptr() % 16:

@@ -130,6 +130,7 @@ def grouped_gemm_fp8_tensorwise(a: torch.Tensor, b: torch.Tensor, a_scale: torch
         raise ValueError(f"kernel must be one of {sorted(KERNELS)}, got {kernel!r}")
     if M_total == 0:
         return out
+    group_offs = group_offs.contiguous()
     sam, (sbg, sbn, _), (scm, scn) = a.stride(0), b.stride(), out.stride()
     _lib.launch("ggemm_persistent_fp8_kernel", dev, G | N | K | sam | sbg | sbn | scm | scn, a.data_ptr(),
                 b.data_ptr(), out.data_ptr(), a_scale.data_ptr(), b_scale.data_ptr(), group_offs.data_ptr(), G, N, K,

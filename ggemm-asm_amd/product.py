@@ -42,10 +42,12 @@ def tile_rows(G: int, N: int, K: int, M: int, activation: str | None = None, *, 
 
 
 def _check_offs(group_offs, dev):
+    """The offsets as the kernels read them, one behind the other (a copy where they are not)."""
     if group_offs.dtype != torch.int64 or group_offs.dim() != 1 or not 2 <= group_offs.numel() <= MAX_GROUPS + 1:
         raise ValueError(f"group_offs must be int64 [G+1] with G <= {MAX_GROUPS}")
     if group_offs.device != dev:
         raise ValueError("all tensors must be on the same device")
+    return group_offs.contiguous()
 
 
 def _rows16(t: torch.Tensor) -> torch.Tensor:
@@ -157,7 +159,7 @@ def grouped_gemm_fp8_bias_act(a: torch.Tensor, b: torch.Tensor, a_scale: torch.T
         raise TypeError(f"a and b must be float8_e4m3fn, got {a.dtype} and {b.dtype}")
     dev = a.device
     _on_gpu(a, "the product")
-    _check_offs(group_offs, dev)
+    group_offs = _check_offs(group_offs, dev)
     (M, K), (G, N, Kb) = a.shape, b.shape
     if G != group_offs.numel() - 1:
         raise ValueError(f"b holds {G} groups, group_offs {group_offs.numel() - 1}")
@@ -228,7 +230,7 @@ def bias_act_backward(dout: torch.Tensor, preact: torch.Tensor | MXTensor | None
         raise TypeError("dout must be a bf16 [M, N] tensor")
     dev = dout.device
     _on_gpu(dout, "the gradient")
-    _check_offs(group_offs, dev)
+    group_offs = _check_offs(group_offs, dev)
     M = dout.shape[0]
     N = dout.shape[1] * (2 if activation == "swiglu" else 1)
     if N % 16 or N == 0:

@@ -242,6 +242,7 @@ def quantize_mxfp8_grouped(x: torch.Tensor, group_offs: torch.Tensor, fmt: str =
     if group_offs.device != x.device:
         raise ValueError("group_offs must be on x's device")
     M, N = x.shape
+    group_offs = group_offs.contiguous()
     G = group_offs.numel() - 1
     rows_out = padded_rows(M, G)
     code, dt = _OUT[fmt]

@@ -96,6 +96,7 @@ def grouped_gemm_fp8_tensorwise_variable_k(lhs: torch.Tensor, rhs: torch.Tensor,
     for s in (lhs_scale, rhs_scale):
         if s.dtype != torch.float32 or s.numel() != 1 or s.device != lhs.device:
             raise ValueError("scales must be single-element fp32 tensors on the input device")
+    group_offs = group_offs.contiguous()
     G = group_offs.numel() - 1
     M_total, OUT_M = lhs.shape
     OUT_N = rhs.shape[1]
@@ -142,6 +143,7 @@ def weight_grad_fp8(dy: torch.Tensor, x: torch.Tensor, dy_scale: torch.Tensor, x
     for s in (dy_scale, x_scale):
         if s.dtype != torch.float32 or s.numel() != 1 or s.device != dy.device:
             raise ValueError("scales must be single-element fp32 tensors on the input device")
+    group_offs = group_offs.contiguous()
     G = group_offs.numel() - 1
     M_total, N = dy.shape
     out = torch.empty((G, N, x.shape[1]), dtype=torch.bfloat16, device=dy.device)
@@ -173,6 +175,7 @@ def grouped_gemm_mxfp8_variable_k(lhs: torch.Tensor, rhs: torch.Tensor, lhs_scal
             raise ValueError(f"MX scales must be [{nblk}, width] with unit column stride")
         if s.device != lhs.device:
             raise ValueError("scales must be on the input device")
+    group_offs = group_offs.contiguous()
     G = group_offs.numel() - 1
     out = _check_out(out, G, OUT_M, OUT_N, lhs.device)
     if validate:
