@@ -8,7 +8,8 @@
 // adds up per group in unit order: no atomics, so the sums do not depend on what ran first. 131072 x 5760 with
 // swiglu: 761 us, 5.0 TB/s, and 16 for the second kernel.
 //
-// With z in 8 bits (kMx) a quarter less is read and written in all: 629 us, 4.8 TB/s, where the bf16 form takes 761. A
+// With z in 8 bits (kMx) a quarter less is read and written in all: 629 us, 4.8 TB/s, where the bf16 form takes 761. Its waves
+// wait for memory 0.62 of their cycles and yet it stays under the 6.1 TB/s that the quantizer streams; why is not found. A
 // row's eight values are 8 bytes, half of what the bf16 form loads, so eight rows are in flight and not four (700 us
 // against 686 with the scales read alike), and scales are read two rows to a lane (row_scales). 16 columns to a thread,
 // one load each of z and dout, store in halves of lines: 870 us, 1228 past the caches.
@@ -146,9 +147,8 @@ __device__ __forceinline__ void grad8(const float (&z)[8], const v4i& d8, const 
 }
 
 // The scales of eight rows and a block of columns, in the four lanes that hold its columns: lane k has those of rows 2 k
-// and 2 k + 1, low byte first. A byte a row and lane takes 16 us
-// more of 645 (131072 x 5760, swiglu; silu on 2880 columns: 47 of 415): by blocks, as the
-// product leaves them, a wave's bytes of a row lie in 16 lines.
+// and 2 k + 1, low byte first. A byte a row and lane takes 16 us more of 645 (131072 x 5760, swiglu; silu on 2880 columns: 47
+// of 415): by blocks, as the product leaves them, a wave's bytes of a row lie in 16 lines.
 __device__ __forceinline__ uint32_t row_scales(const Args& a, int64_t r, int64_t r1, int n) {
   const uint8_t* s = a.scales + (int64_t)(n / 32) * a.scale_block;
   const int64_t k = r + 2 * (threadIdx.x & 3);

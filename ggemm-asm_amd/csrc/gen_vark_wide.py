@@ -1263,8 +1263,8 @@ class GenK(Gen):
 # columns of z, and 80 of the result, in rows padded to an odd number of 16-byte chunks, and stores them as chunks.
 # Per SIMD and tile the activation is 160 pairs of 13 vector operations and an exp2 and a reciprocal at a quarter of
 # the rate each, about 12 thousand cycles beside the tile's 90 thousand, and nothing overlaps them: one wave holds
-# the SIMD's registers. 131072 rows x 5760 x 2880 take 1827 us so, 2028 with z kept; the plain product on the same box 1767.
-# On another one, in turn: 1700 the plain product, 1710 with swiglu, 1890-1930 with z in bf16 and 1900-1930 in 8 bits: half
+# the SIMD's registers. 131072 rows x 5760 x 2880 take 1827 us so, 2028 with z kept; the plain product in turn with them 1767.
+# On another card, in turn: 1700 the plain product, 1710 with swiglu, 1890-1930 with z in bf16 and 1900-1930 in 8 bits: half
 # the bytes of z, paid for by its maxima and conversions (its stores past the caches or through them: no difference).
 ZPITCH, OPITCH = 336, 176            # bytes of a staged row of z (160 bf16) and of the result (80)
 OREGION = 32 * ZPITCH                # a wave's staged result, after its z; 16 KiB together

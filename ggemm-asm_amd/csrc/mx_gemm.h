@@ -26,7 +26,8 @@
 //
 // The large ones are bound by power and by the epilogue, which no product runs beside: 131072 x 5760 x 2880 with swiglu takes
 // 1307 us with e2m1 rows, 3.33 PFLOP/s (a library's plain fp4 product of 16384^3 reaches 3.41, instructions alone on random
-// operands 6.26; matrix units busy 0.48 of the time at 1.66 GHz), and 1886 us, 2.31, with e4m3 (instructions alone 3.79). Random
+// operands 6.26; matrix units busy 0.48 of the time at 1.66 GHz), and 1886 us, 2.31, with e4m3 (instructions alone 3.79), 1.1 times
+// what fp8 weights take (1700-1750): with e4m3 rows 4 bits pay up to some ten thousand rows, where weights are read. Random
 // codes as operands, whose sums toggle more: 1555 and 2105 us, without the results' stores 1310 and 1818. The small ones
 // read weights: 256 rows of 32 experts, e4m3, 56 us, 5.0 TB/s.
 #pragma once
@@ -203,8 +204,9 @@ __device__ __forceinline__ void by_half(int& x, int& y) {
 // of a row's columns change places between lanes s and s + 32, so that a lane holds (and reads of a residual) 16 bytes at a
 // time. kLine = 0: it stores them as they are. Else they go through 32 kLine bytes of the wave's LDS (`lines`) and are stored
 // kLine bytes of a row to neighbouring lanes, and the bias lies in LDS too (`bias_at`, raw, this wave's columns): a load's
-// wait would drain the stores before it and the next tile's loads. 32768 x 2880 x 2880, e4m3: 329 us without, 255 so;
-// 131072 x 5760 x 2880, e2m1, swiglu: 1434 and 1307; 128-row tiles, 4096 x 5760 x 2880, e2m1, swiglu: 90 and 84.
+// wait would drain the stores before it and the next tile's loads. 32768 x 2880 x 2880, e4m3, with a
+// bias: 343-350 us without, 259-263 so, even and skewed groups alike; 131072 x 5760 x 2880, e2m1, swiglu: 1434 and 1307;
+// 128-row tiles, 4096 x 5760 x 2880, e2m1, swiglu: 90 and 84.
 template <int kAct, int MB, int NB, int kLine>
 __device__ __forceinline__ void store(const v16f (&acc)[MB][NB], const epi::Args& e, uint16_t* out, int stride_out, int g,
                                       int N, int64_t row0, int rows, int n0, int lane, GG_LDS uint8_t* lines,
@@ -323,7 +325,7 @@ __device__ __forceinline__ void store(const v16f (&acc)[MB][NB], const epi::Args
         for (int q = 0; q < kChunks / 2; ++q) {
           const int r = 64 / kChunks * q + lane / kChunks;
           const v4i v = *(const GG_LDS v4i*)(lines + kLine * r + 16 * (c ^ (r & (kChunks - 1))));
-          // whole lines past the caches: (e4m3) 32768 x 2880 x 2880 294 -> 261 us; halves through them
+          // whole lines past the caches, 33 us of what the epilogue gains at 32768 x 2880 x 2880 (e4m3); halves through them
           __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(mid::v4u32, v), rsrc,
                                                  to + 2 * (32 * i + 64 / kChunks * q) * stride_out, 0, kLine == 128 ? 2 : 0);
         }
@@ -567,8 +569,7 @@ __device__ __forceinline__ void gemm_body(const Args& a, GG_LDS uint8_t* lds, co
     nxt = nxt + 1 == C::S ? 0 : nxt + 1;
     if (st != 0) continue;
     store<kAct, C::MB, C::NB, C::Line>(acc, e, a.out, a.stride_out, tile.g, a.N, tile.row0 + 32 * C::MB * wm,
-                              tile.rows - 32 * C::MB * wm, tile.n0 + 32 * C::NB * wn, lane,
-                                       lines, bias_at);
+                                       tile.rows - 32 * C::MB * wm, tile.n0 + 32 * C::NB * wn, lane, lines, bias_at);
     if (next.rows == 0) break;                                 // nor are those that follow: tiles rise along a walk
     tile = next;
     fetch_bias(tile);
