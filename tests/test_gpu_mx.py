@@ -414,3 +414,28 @@ def test_groups_that_follow_the_last_row_at_once(pkg, tile):
     dev_offs = torch.tensor(offs).cuda()
     want = pkg.grouped_gemm_mx_bias_act(da, db, dev_offs, tile=tile)
     assert torch.equal(want, pkg.grouped_gemm_mx_bias_act(da, pkg.MXTensor(db.q, tight), dev_offs, tile=tile))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tile", [16, 32, 64, 128, 256])
+def test_scales_at_the_ends_of_their_range(pkg, fmt, tile):
+    """Every power that a scale can hold on one side, and on the other one that brings the product back; zeros under the largest
+    scales stay zeros, and products below fp32 vanish."""
+    M, N, K = 32, 32, 64
+    for s in (0, 1, 2, 40, 127, 200, 253, 254):
+        for d in (-3, 0, 4):
+            t = 254 - s + d
+            if not 0 <= t <= 254:
+                continue
+            a, b, offs, gen = _case(M, N, K, [M], fmt, 300 + s)
+            a[1].fill_(s), b[1].fill_(t)
+            out = pkg.grouped_gemm_mx_bias_act(pkg.MXTensor(_laid_out(a[0], 0), _laid_out(a[1], 0)),
+                                               pkg.MXTensor(_laid_out(b[0], 0), _laid_out(b[1], 0)), torch.tensor(offs).cuda(), tile=tile)
+            z, ref, size = omx.product(omx.decode(*a), omx.decode(*b), fmt, offs, None, None, None)
+            _check(out.cpu().double(), z, ref, size, None, {}, torch.zeros_like(ref))
+    zero = torch.zeros_like(a[0].view(torch.uint8)).view(a[0].dtype)
+    for q, s in ((zero, 254), (a[0], 0)):
+        a[1].fill_(s), b[1].fill_(s)
+        out = pkg.grouped_gemm_mx_bias_act(pkg.MXTensor(_laid_out(q, 0), _laid_out(a[1], 0)),
+                                           pkg.MXTensor(_laid_out(b[0], 0), _laid_out(b[1], 0)), torch.tensor(offs).cuda(), tile=tile)
+        assert not out.any()
